@@ -12,8 +12,11 @@ from .api import (  # noqa: F401
     GenSparseMatrixBinFile,
     InitSparseMatrixA_API,
     InitSparseMatrixA_API_NoReorder,
+    PagedBatch,
     SpMM_SplitK_API,
+    attention_workspace_bytes,
     build_library,
+    cache_accept,
     comm_alloc_buffer,
     comm_close_peer_buffer,
     comm_create,
@@ -28,11 +31,13 @@ from .api import (  # noqa: F401
     launch_count,
     library,
     load_sparse_matrix_bin_files,
+    prompt_attention,
     read_output_sizes,
     read_rank_lists,
     read_sparse_matrix_bin_files,
     release_scratch,
     release_stream_scratch,
+    rotary_append,
     set_launch_overlap,
     set_plan,
     splitk_reduction,
@@ -41,6 +46,8 @@ from .api import (  # noqa: F401
     spmm_splitk_strided,
     spmm_splitk_allreduce,
     spmm_splitk_no_alloc,
+    tree_attention,
     write_rank_lists,
 )
+from .rotary import rotary_frequencies  # noqa: F401
 from . import synthetic  # noqa: F401

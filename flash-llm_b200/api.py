@@ -9,6 +9,7 @@ from __future__ import annotations
 import ctypes as C
 import os
 import subprocess
+from dataclasses import dataclass
 
 import numpy as np
 
@@ -98,6 +99,21 @@ def library() -> C.CDLL:
     L.FlashLLM_SpMM_SplitK_AllReduce.argtypes = [C.c_void_p] * 6 + [C.c_int] * 3 + [C.c_void_p, C.c_int, C.c_void_p, C.c_int]
     L.FlashLLM_SplitK_Reduction.restype = C.c_int
     L.FlashLLM_SplitK_Reduction.argtypes = [C.c_void_p, C.c_void_p, C.c_void_p, C.c_int, C.c_int, C.c_int]
+    cache = [C.c_void_p] * 2 + [C.c_int] * 2  # K_cache, V_cache, pages, page_size
+    batch = [C.c_void_p] * 3 + [C.c_int] * 3  # cu_tokens, context, page_table, table_width, sequences, tokens
+    L.FlashLLM_RotaryAppend.restype = C.c_int
+    L.FlashLLM_RotaryAppend.argtypes = ([C.c_void_p, C.c_void_p, C.c_int, C.c_void_p, C.c_int] + cache + batch + [C.c_int] * 3
+                                        + [C.c_void_p, C.c_int, C.c_int, C.c_float, C.c_void_p])
+    L.FlashLLM_TreeAttention.restype = C.c_int
+    L.FlashLLM_TreeAttention.argtypes = ([C.c_void_p, C.c_void_p, C.c_int] + cache + batch + [C.c_int] * 3 + [C.c_void_p] * 2
+                                         + [C.c_float] * 2 + [C.c_void_p] * 3)
+    L.FlashLLM_PromptAttention.restype = C.c_int
+    L.FlashLLM_PromptAttention.argtypes = ([C.c_void_p, C.c_void_p, C.c_int] + cache + batch + [C.c_int] * 3 + [C.c_void_p]
+                                           + [C.c_float] * 2 + [C.c_void_p] * 3)
+    L.FlashLLM_Attention_WorkspaceBytes.restype = C.c_ulonglong
+    L.FlashLLM_Attention_WorkspaceBytes.argtypes = [C.c_int]
+    L.FlashLLM_CacheAccept.restype = C.c_int
+    L.FlashLLM_CacheAccept.argtypes = ([C.c_void_p] * 3 + [C.c_int] * 3 + batch + [C.c_int] * 2 + [C.c_void_p] * 2 + [C.c_int])
     L.FlashLLM_ReleaseScratch.restype = C.c_int
     L.FlashLLM_ReleaseScratch.argtypes = []
     L.FlashLLM_ReleaseStreamScratch.restype = C.c_int
@@ -285,6 +301,84 @@ def spmm_splitk_no_alloc(stream: int, Compressed_A: int, TileOffsets: int, B: in
     code = library().FlashLLM_SpMM_SplitK_NoAlloc(stream, Compressed_A, TileOffsets, B, C_out, M, N, K, Split_K)
     if code:
         _check(code, f"SpMM_SplitK_NoAlloc(M={M}, N={N}, K={K}, Split_K={Split_K})")
+
+
+# ----------------------------------------------------------------------------- a paged key/value cache and its attention
+
+@dataclass(frozen=True)
+class PagedBatch:
+    """A cache and the batch a call works on, as integer device pointers and sizes: ``K_cache`` and ``V_cache`` are fp16
+    ``[pages][kv_heads][page_size][head_dim]`` (``layers`` of them one behind another for :func:`cache_accept`), sequence b owns
+    rows ``cu_tokens[b]`` up to ``cu_tokens[b + 1]`` of the ``tokens`` rows, and ``context[b]`` of its positions, which lie in the
+    pages ``page_table[b * table_width + ...]``, are filled before the call (int32 device arrays)."""
+    K_cache: int
+    V_cache: int
+    pages: int
+    page_size: int
+    kv_heads: int
+    head_dim: int
+    cu_tokens: int
+    context: int
+    page_table: int
+    table_width: int
+    sequences: int
+    tokens: int
+    layers: int = 1
+
+    def _cache(self):
+        return self.K_cache, self.V_cache, self.pages, self.page_size
+
+    def _batch(self):
+        return self.cu_tokens, self.context, self.page_table, self.table_width, self.sequences, self.tokens
+
+
+def rotary_append(stream: int, QKV: int, ld_qkv: int, Q: int, ld_q: int, batch: PagedBatch, heads: int,
+                  frequencies: int | None = None, rotary_dim: int = 0, interleaved: bool = False, magnitude: float = 1.0,
+                  positions: int | None = None) -> None:
+    """Turned queries of ``QKV[tokens][ld_qkv]`` (query, key and value heads) to ``Q[tokens][ld_q]``, turned keys and values
+    into the cache.  ``frequencies`` are ``rotary_dim / 2`` device doubles (see :func:`rotary_frequencies`); ``rotary_dim`` 0
+    turns nothing."""
+    code = library().FlashLLM_RotaryAppend(stream, QKV, ld_qkv, Q, ld_q, *batch._cache(), *batch._batch(), heads, batch.kv_heads,
+                                           batch.head_dim, frequencies, rotary_dim, int(interleaved), magnitude, positions)
+    if code:
+        _check(code, f"RotaryAppend(heads={heads}, rotary_dim={rotary_dim}, ld_qkv={ld_qkv}, ld_q={ld_q}, {batch})")
+
+
+def attention_workspace_bytes(head_dim: int) -> int:
+    """Bytes of the workspace that :func:`tree_attention` and :func:`prompt_attention` take on the current device."""
+    return int(library().FlashLLM_Attention_WorkspaceBytes(head_dim))
+
+
+def tree_attention(stream: int, Q: int, ld_q: int, batch: PagedBatch, heads: int, tree_mask: int, Out: int, workspace: int,
+                   scale: float | None = None, cap: float = 0.0, slopes: int | None = None, positions: int | None = None) -> None:
+    """Attention of up to 64 drafted tokens of each sequence over its cache, ``Out[tokens][heads * head_dim]``: row n sees the
+    context and the new tokens of its sequence whose bit ``tree_mask[n]`` (64 bits) has.  Scores are ``scale`` q . k (1 /
+    sqrt(head_dim) unless given), capped by ``cap * tanh(. / cap)`` where ``cap`` > 0, plus ``slopes[head]`` times the
+    distance."""
+    code = library().FlashLLM_TreeAttention(stream, Q, ld_q, *batch._cache(), *batch._batch(), heads, batch.kv_heads,
+                                            batch.head_dim, tree_mask, positions, batch.head_dim ** -0.5 if scale is None else scale,
+                                            cap, slopes, Out, workspace)
+    if code:
+        _check(code, f"TreeAttention(heads={heads}, ld_q={ld_q}, scale={scale}, cap={cap}, {batch})")
+
+
+def prompt_attention(stream: int, Q: int, ld_q: int, batch: PagedBatch, heads: int, Out: int, workspace: int,
+                     prefix: int | None = None, scale: float | None = None, cap: float = 0.0, slopes: int | None = None) -> None:
+    """The same for prompts and single tokens: row n sees its sequence up to itself and the first ``prefix[b]`` positions."""
+    code = library().FlashLLM_PromptAttention(stream, Q, ld_q, *batch._cache(), *batch._batch(), heads, batch.kv_heads,
+                                              batch.head_dim, prefix, batch.head_dim ** -0.5 if scale is None else scale, cap, slopes,
+                                              Out, workspace)
+    if code:
+        _check(code, f"PromptAttention(heads={heads}, ld_q={ld_q}, scale={scale}, cap={cap}, {batch})")
+
+
+def cache_accept(stream: int, batch: PagedBatch, accepted: int, accepted_lengths: int, accepted_width: int) -> None:
+    """Keys and values of each sequence's new token ``accepted[b][i]`` move to position ``context[b] + i``, in all layers."""
+    code = library().FlashLLM_CacheAccept(stream, batch.K_cache, batch.V_cache, batch.layers, batch.pages, batch.page_size,
+                                          *batch._batch(), batch.kv_heads, batch.head_dim, accepted, accepted_lengths,
+                                          accepted_width)
+    if code:
+        _check(code, f"CacheAccept(accepted_width={accepted_width}, {batch})")
 
 
 # ----------------------------------------------------------------------------- fused row-parallel SpMM + all-reduce

@@ -1,0 +1,190 @@
+// Host side of the operators around a paged key/value cache: argument checks and launches.
+#include <cuda.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+
+#include <cmath>
+
+#include "../../include/SpMM_API.cuh"
+#include "attention_kernel_sm100.cuh"
+#include "cache_kernels_sm100.cuh"
+#include "launch.h"
+#include "tiled_csl_host.h"
+
+namespace flashllm {
+
+static bool aligned16(const void* p)
+{
+    return (reinterpret_cast<uintptr_t>(p) & 15u) == 0;
+}
+
+// What every operator's cache and batch have to be.
+static bool describe_batch(CacheBatch* batch, const void* K_cache, const void* V_cache, int pages, int page_size,
+                           const int* cu_tokens, const int* context, const int* page_table, int table_width, int sequences,
+                           int tokens, int kv_heads, int head_dim)
+{
+    if (K_cache == nullptr || V_cache == nullptr || cu_tokens == nullptr || context == nullptr || page_table == nullptr
+        || !aligned16(K_cache) || !aligned16(V_cache) || pages < 1 || kv_heads < 1 || (head_dim != 64 && head_dim != 128)
+        || page_size < 16 || (page_size & (page_size - 1)) != 0 || table_width < 1 || sequences < 0
+        || sequences > kMaxSequences || tokens < 0)
+        return false;
+    // Positions, and the pages of all heads, are counted in ints; a tile may reach 127 positions behind the last.
+    if (static_cast<long long>(table_width) * page_size > 0x7fffffffll - 256
+        || static_cast<long long>(pages) * kv_heads > 0x7fffffffll - 1)
+        return false;
+    batch->cu_tokens   = cu_tokens;
+    batch->context     = context;
+    batch->page_table  = page_table;
+    batch->sequences   = sequences;
+    batch->tokens      = tokens;
+    batch->table_width = table_width;
+    batch->pages       = pages;
+    batch->page_shift  = __builtin_ctz(static_cast<unsigned>(page_size));
+    batch->kv_heads    = kv_heads;
+    return true;
+}
+
+static bool rows_fit(const void* matrix, int ld, int heads, int head_dim)
+{
+    return matrix != nullptr && aligned16(matrix) && ld % 8 == 0 && ld >= static_cast<long long>(heads) * head_dim;
+}
+
+static cudaError_t launch_rotary(cudaStream_t stream, const RotaryParams& p, int head_dim, bool interleaved)
+{
+    auto launch = [&](auto kernel) {
+        return launch_in_stream_order(kernel, dim3(p.batch.tokens), dim3(kRotaryThreads), 0, stream, 1, p);
+    };
+    if (head_dim == 64)
+        return interleaved ? launch(rotary_append_kernel<64, true>) : launch(rotary_append_kernel<64, false>);
+    return interleaved ? launch(rotary_append_kernel<128, true>) : launch(rotary_append_kernel<128, false>);
+}
+
+// The checks that tree and prompt attention share, and the launch.
+static cudaError_t attend(cudaStream_t stream, AttentionParams p, const void* Q, int ld_q, const void* K_cache,
+                          const void* V_cache, int pages, int page_size, const int* cu_tokens, const int* context,
+                          const int* page_table, int table_width, int sequences, int tokens, int heads, int kv_heads,
+                          int head_dim, float scale, float cap, const float* slopes, void* Out)
+{
+    if (!describe_batch(&p.batch, K_cache, V_cache, pages, page_size, cu_tokens, context, page_table, table_width, sequences, tokens,
+                        kv_heads, head_dim)
+        || heads < 1 || heads % kv_heads != 0 || static_cast<long long>(heads) * head_dim > (1 << 24) || !rows_fit(Q, ld_q, heads, head_dim)
+        || Out == nullptr || !aligned16(Out) || !(scale > 0.0f) || !std::isfinite(scale) || !(cap >= 0.0f) || !std::isfinite(cap)
+        || static_cast<long long>(tokens) * heads > 0x7fffffffll - 256)
+        return cudaErrorInvalidValue;
+    if (tokens == 0 || sequences == 0)
+        return cudaSuccess;
+    if (const int err = device_status_pointer(&p.batch.status))
+        return static_cast<cudaError_t>(err);
+    p.q       = static_cast<const half*>(Q);
+    p.out     = static_cast<half*>(Out);
+    p.k_cache = static_cast<const half*>(K_cache);
+    p.v_cache = static_cast<const half*>(V_cache);
+    p.slopes  = slopes;
+    p.ld_q    = ld_q;
+    p.heads   = heads;
+    p.scale   = scale;
+    p.cap     = cap;
+    const int  warps = kAttentionThreads / 32;
+    const dim3 grid(tokens, (heads + warps - 1) / warps);
+    return head_dim == 64 ? launch_in_stream_order(attention_kernel<64>, grid, dim3(kAttentionThreads), 0, stream, 1, p)
+                          : launch_in_stream_order(attention_kernel<128>, grid, dim3(kAttentionThreads), 0, stream, 1, p);
+}
+
+}  // namespace flashllm
+
+using namespace flashllm;
+
+extern "C" {
+
+int FlashLLM_RotaryAppend(void* stream, const void* QKV, int ld_qkv, void* Q, int ld_q, void* K_cache, void* V_cache, int pages,
+                          int page_size, const int* cu_tokens, const int* context, const int* page_table, int table_width,
+                          int sequences, int tokens, int heads, int kv_heads, int head_dim, const double* frequencies,
+                          int rotary_dim, int interleaved, float magnitude, const int* positions)
+{
+    RotaryParams p{};
+    if (!describe_batch(&p.batch, K_cache, V_cache, pages, page_size, cu_tokens, context, page_table, table_width, sequences, tokens,
+                        kv_heads, head_dim)
+        || heads < 1 || static_cast<long long>(heads) * head_dim > (1 << 24) || static_cast<long long>(kv_heads) * head_dim > (1 << 24)
+        || !rows_fit(QKV, ld_qkv, heads + 2 * kv_heads, head_dim) || !rows_fit(Q, ld_q, heads, head_dim) || rotary_dim < 0
+        || rotary_dim > head_dim || rotary_dim % 16 != 0 || (rotary_dim > 0 && frequencies == nullptr) || !std::isfinite(magnitude))
+        return static_cast<int>(cudaErrorInvalidValue);
+    if (tokens == 0 || sequences == 0)
+        return 0;
+    if (const int err = device_status_pointer(&p.batch.status))
+        return err;
+    p.qkv         = static_cast<const half*>(QKV);
+    p.q           = static_cast<half*>(Q);
+    p.k_cache     = static_cast<half*>(K_cache);
+    p.v_cache     = static_cast<half*>(V_cache);
+    p.frequencies = frequencies;
+    p.positions   = positions;
+    p.ld_qkv      = ld_qkv;
+    p.ld_q        = ld_q;
+    p.heads       = heads;
+    p.rotary_dim  = rotary_dim;
+    p.magnitude   = magnitude;
+    return static_cast<int>(launch_rotary(static_cast<cudaStream_t>(stream), p, head_dim, interleaved != 0));
+}
+
+unsigned long long FlashLLM_Attention_WorkspaceBytes(int head_dim)
+{
+    return head_dim == 64 || head_dim == 128 ? 16 : 0;
+}
+
+int FlashLLM_TreeAttention(void* stream, const void* Q, int ld_q, const void* K_cache, const void* V_cache, int pages,
+                           int page_size, const int* cu_tokens, const int* context, const int* page_table, int table_width,
+                           int sequences, int tokens, int heads, int kv_heads, int head_dim, const unsigned long long* tree_mask,
+                           const int* positions, float scale, float cap, const float* slopes, void* Out, void* workspace)
+{
+    if (tree_mask == nullptr || (slopes != nullptr && positions == nullptr) || workspace == nullptr || !aligned16(workspace))
+        return static_cast<int>(cudaErrorInvalidValue);
+    AttentionParams p{};
+    p.tree_mask = tree_mask;
+    p.positions = positions;
+    return static_cast<int>(attend(static_cast<cudaStream_t>(stream), p, Q, ld_q, K_cache, V_cache, pages, page_size, cu_tokens,
+                                   context, page_table, table_width, sequences, tokens, heads, kv_heads, head_dim, scale, cap,
+                                   slopes, Out));
+}
+
+int FlashLLM_PromptAttention(void* stream, const void* Q, int ld_q, const void* K_cache, const void* V_cache, int pages,
+                             int page_size, const int* cu_tokens, const int* context, const int* page_table, int table_width,
+                             int sequences, int tokens, int heads, int kv_heads, int head_dim, const int* prefix, float scale,
+                             float cap, const float* slopes, void* Out, void* workspace)
+{
+    if (workspace == nullptr || !aligned16(workspace))
+        return static_cast<int>(cudaErrorInvalidValue);
+    AttentionParams p{};
+    p.prefix = prefix;
+    return static_cast<int>(attend(static_cast<cudaStream_t>(stream), p, Q, ld_q, K_cache, V_cache, pages, page_size, cu_tokens,
+                                   context, page_table, table_width, sequences, tokens, heads, kv_heads, head_dim, scale, cap,
+                                   slopes, Out));
+}
+
+int FlashLLM_CacheAccept(void* stream, void* K_cache, void* V_cache, int layers, int pages, int page_size, const int* cu_tokens,
+                         const int* context, const int* page_table, int table_width, int sequences, int tokens, int kv_heads,
+                         int head_dim, const int* accepted, const int* accepted_lengths, int accepted_width)
+{
+    AcceptParams p{};
+    if (!describe_batch(&p.batch, K_cache, V_cache, pages, page_size, cu_tokens, context, page_table, table_width, sequences, tokens,
+                        kv_heads, head_dim)
+        || layers < 1 || layers > 65535 || kv_heads > 65535 || accepted == nullptr || accepted_lengths == nullptr || accepted_width < 1
+        || accepted_width > kMaxDrafted)
+        return static_cast<int>(cudaErrorInvalidValue);
+    if (tokens == 0 || sequences == 0)
+        return 0;
+    if (const int err = device_status_pointer(&p.batch.status))
+        return err;
+    p.k_cache          = static_cast<half*>(K_cache);
+    p.v_cache          = static_cast<half*>(V_cache);
+    p.accepted         = accepted;
+    p.accepted_lengths = accepted_lengths;
+    p.accepted_width   = accepted_width;
+    p.layer_elems      = static_cast<long long>(pages) * kv_heads * page_size * head_dim;
+    const dim3 grid(sequences, kv_heads, layers);
+    auto       launch = [&](auto kernel) {
+        return launch_in_stream_order(kernel, grid, dim3(kAcceptThreads), 0, static_cast<cudaStream_t>(stream), 1, p);
+    };
+    return static_cast<int>(head_dim == 64 ? launch(cache_accept_kernel<64>) : launch(cache_accept_kernel<128>));
+}
+
+}  // extern "C"

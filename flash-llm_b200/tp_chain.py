@@ -4,8 +4,10 @@ FFN2 SpMM -> all-reduce, the way the reference's FasterTransformer integration s
 QKV and FFN1, row-parallel out-proj and FFN2, one NCCL all-reduce of [N][H] after each row-parallel matmul,
 ft.patch ParallelGpt decoder layers).
 
-The chain has no attention, LayerNorm, bias or residual: the out-proj input is the V third of the QKV output, which
-is what attention returns for a single-position context.  All four matmuls are `Y[N][M] = X[N][K] @ W[M][K]^T` with
+The chain has no LayerNorm, bias or residual.  Between QKV and out-proj it runs the attention it is given
+(`CachedAttention`: rotary positions, the append to a paged cache, attention of a drafted tree or of prompts); without
+one the out-proj input is the V third of the QKV output, which is what attention returns for a single-position
+context.  All four matmuls are `Y[N][M] = X[N][K] @ W[M][K]^T` with
 W tiled-CSL encoded, i.e. SpMM_SplitK_API calls; everything else here is plumbing (slicing, the collective, ReLU).
 
 The matmul and the collective are injected, so that the same chain runs
@@ -64,21 +66,26 @@ def shard_weights(shape: ChainShape, rank: int, w_qkv: torch.Tensor, w_out: torc
 def run_chain(shape: ChainShape, x: torch.Tensor, matmul: Callable[..., torch.Tensor],
               all_reduce: Callable[[torch.Tensor], torch.Tensor] | None = None,
               matmul_reduced: Callable[[str, torch.Tensor], torch.Tensor] | None = None,
-              strided: bool = False) -> torch.Tensor:
+              strided: bool = False, attention: Callable[[torch.Tensor], torch.Tensor] | None = None) -> torch.Tensor:
     """One rank's pass over the layer.  `matmul(name, X[N][K], relu=False) -> Y[N][M]` multiplies by that rank's shard
     `name` (and applies ReLU to the result when asked: FFN1 is column-parallel, so its activation needs no partner).
     The two row-parallel layers need the sum over the ranks: either `all_reduce(t)` is applied to their outputs, or
     `matmul_reduced(name, X)` does the matmul and the sum in one step (the fused SpMM + all-reduce of the library).
     `strided`: the matmul takes a slice of the QKV output as it lies, instead of a copy of it (the copy's launch between the
     two matmuls took 6 us of a hidden-9216 layer's 215 and of a hidden-1536 layer's 46).
+    `attention(Y[N][3H/g]) -> [N][H/g]` takes this rank's Q, K and V features to the out-proj input (`CachedAttention`);
+    without one that input is the V third.
     Returns the layer output [N][H] (same on every rank)."""
     if matmul_reduced is None:
         matmul_reduced = lambda name, t: all_reduce(matmul(name, t))  # noqa: E731
     h = shape.hidden // shape.world
     y_qkv = matmul("qkv", x)                               # [N][3H/g]: this rank's Q, K, V features
-    v = y_qkv[:, 2 * h:3 * h]                              # single-position attention returns V
-    if not strided:
-        v = v.contiguous()
+    if attention is not None:
+        v = attention(y_qkv)
+    else:
+        v = y_qkv[:, 2 * h:3 * h]                          # single-position attention returns V
+        if not strided:
+            v = v.contiguous()
     attn = matmul_reduced("out_proj", v)                   # [N][H], partial sums over the K slices added up
     y1 = matmul("ffn1", attn, relu=True)                   # [N][F/g]
     return matmul_reduced("ffn2", y1)                      # [N][H]
@@ -100,14 +107,49 @@ def fp32_all_reduce(dist=None) -> Callable[[torch.Tensor], torch.Tensor]:
 
 
 def reference_chain(shape: ChainShape, x: torch.Tensor, w_qkv: torch.Tensor, w_out: torch.Tensor,
-                    w_ffn1: torch.Tensor, w_ffn2: torch.Tensor) -> torch.Tensor:
-    """The unsharded layer on the host in fp32, rounding to fp16 where the kernels store fp16 (every matmul output)."""
+                    w_ffn1: torch.Tensor, w_ffn2: torch.Tensor,
+                    attention: Callable[[torch.Tensor], torch.Tensor] | None = None) -> torch.Tensor:
+    """The unsharded layer on the host in fp32, rounding to fp16 where the kernels store fp16 (every matmul output, and what
+    `attention(Y[N][3H]) -> [N][H]` returns, if one is given)."""
     H = shape.hidden
     r16 = lambda t: t.to(torch.float16).float()  # noqa: E731
     y_qkv = r16(x.float() @ w_qkv.float().T)
-    attn = r16(y_qkv[:, 2 * H:3 * H] @ w_out.float().T)
+    v = y_qkv[:, 2 * H:3 * H] if attention is None else r16(attention(y_qkv))
+    attn = r16(v @ w_out.float().T)
     y1 = torch.relu(r16(attn @ w_ffn1.float().T))
     return r16(y1 @ w_ffn2.float().T)
+
+
+@dataclass
+class CachedAttention:
+    """The attention of one layer's heads on this rank over their paged cache (fp16 `[pages][heads][page_size][head_dim]`):
+    rotary positions and the append of the batch's rows, then attention of drafted trees (`tree_mask`, with `positions` = depth +
+    context for the angles and distances) or, without masks, of prompts and single tokens.  cu_tokens, context and page_table
+    describe the batch (int32; see torch_op); the caller advances `context` between steps, and accepts a drafted path with
+    torch.ops.flashllm.cache_accept first.  `frequencies` None: no rotary positions."""
+
+    k_cache: torch.Tensor
+    v_cache: torch.Tensor
+    cu_tokens: torch.Tensor
+    context: torch.Tensor
+    page_table: torch.Tensor
+    tree_mask: torch.Tensor | None = None
+    positions: torch.Tensor | None = None
+    prefix: torch.Tensor | None = None
+    frequencies: torch.Tensor | None = None
+    interleaved: bool = False
+    magnitude: float = 1.0
+    cap: float = 0.0
+    slopes: torch.Tensor | None = None
+
+    def __call__(self, y_qkv: torch.Tensor) -> torch.Tensor:
+        from . import torch_op  # noqa: F401  (registers torch.ops.flashllm)
+        ops = torch.ops.flashllm
+        batch = (self.k_cache, self.v_cache, self.cu_tokens, self.context, self.page_table)
+        q = ops.rotary_append(y_qkv, *batch, self.frequencies, self.interleaved, self.magnitude, self.positions)
+        if self.tree_mask is not None:
+            return ops.tree_attention(q, *batch, self.tree_mask, None, self.cap, self.slopes, self.positions)
+        return ops.prompt_attention(q, *batch, self.prefix, None, self.cap, self.slopes)
 
 
 class DeviceChain:
@@ -160,11 +202,12 @@ class DeviceChain:
         return call
 
     def step(self, x: torch.Tensor, all_reduce: Callable[[torch.Tensor], torch.Tensor] | None = None,
-             comm=None) -> torch.Tensor:
-        """One pass; with `comm` (see PeerGroup) the row-parallel layers use the fused SpMM + all-reduce."""
+             comm=None, attention: Callable[[torch.Tensor], torch.Tensor] | None = None) -> torch.Tensor:
+        """One pass; with `comm` (see PeerGroup) the row-parallel layers use the fused SpMM + all-reduce, with `attention`
+        (see CachedAttention) the layer attends to its cache."""
         if comm is not None:
-            return run_chain(self.shape, x, self.matmul, matmul_reduced=self.matmul_reduced(comm))
-        return run_chain(self.shape, x, self.matmul, all_reduce, strided=True)
+            return run_chain(self.shape, x, self.matmul, matmul_reduced=self.matmul_reduced(comm), attention=attention)
+        return run_chain(self.shape, x, self.matmul, all_reduce, strided=True, attention=attention)
 
 
 class PeerGroup:

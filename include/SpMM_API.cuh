@@ -300,6 +300,141 @@ int FlashLLM_SpMM_SplitK_NoAlloc(void*       stream,
  * C[i] = fp16(sum_s float(Workspace[s*M*N + i])). */
 int FlashLLM_SplitK_Reduction(void* stream, void* C, const void* Reduction_Workspace, int M, int N, int Split_K);
 
+/* ------------------------------------------------------------------------------------------------------------
+ * A paged key/value cache and the attention that reads it: what stands between the QKV projection and the attention
+ * output projection of a decoder layer (no counterpart in the reference library, whose caller runs FasterTransformer's
+ * attention there).
+ *
+ * K_cache and V_cache are fp16 [pages][kv_heads][page_size][head_dim] on 16-byte boundaries, head_dim 64 or 128, page_size
+ * a power of two from 16 on.  Position j of sequence b lives in place j % page_size of page
+ * page_table[b * table_width + j / page_size].  A batch is `sequences` (at most 4096) sequences whose new tokens lie one
+ * behind another in `tokens` rows: sequence b owns rows cu_tokens[b] up to cu_tokens[b + 1] (cu_tokens has sequences + 1
+ * entries), and its first row stands at position context[b] of its cache: so many positions are in the cache already.  Rows
+ * behind the last sequence are neither read nor written.  All index arrays are int32 device arrays and are read by the
+ * kernels, so a captured call may be replayed with other lengths and pages in them.
+ *
+ * Results are cudaError_t values; bad sizes or pointers return cudaErrorInvalidValue.  What the host cannot see sets bit 64 of
+ * the status word (FlashLLM_ConsumeStatus): a page id outside the cache (its keys and values read as zeros, writes to it are
+ * left out), or a sequence that does not fit into its row of the page table (its attention output is zero, it is not written
+ * to the cache).  No two sequences may share a page that a call writes to.
+ * ---------------------------------------------------------------------------------------------------------- */
+
+/* Rotary positions and the append.  QKV [tokens][ld_qkv] holds the query heads, the key heads and the value heads of each row
+ * (head_dim each), as a QKV projection leaves them; the turned queries go to Q [tokens][ld_q] (which may be QKV itself, with
+ * the same row length), turned keys and the values into the cache at position context + the row's place in its sequence.
+ * Of each head the first rotary_dim elements (a multiple of 16, 0: none, the call is an append) are turned in pairs
+ * (i, i + rotary_dim / 2), with interleaved != 0 (2 i, 2 i + 1), by the angle position * frequencies[i] (radians, device
+ * doubles) and scaled by `magnitude`.  `positions` (int32 [tokens], or nullptr) replaces the row's place in the cache in the
+ * angle: the depth of a drafted token is not its place. */
+int FlashLLM_RotaryAppend(void*         stream,
+                          const void*   QKV,
+                          int           ld_qkv,
+                          void*         Q,
+                          int           ld_q,
+                          void*         K_cache,
+                          void*         V_cache,
+                          int           pages,
+                          int           page_size,
+                          const int*    cu_tokens,
+                          const int*    context,
+                          const int*    page_table,
+                          int           table_width,
+                          int           sequences,
+                          int           tokens,
+                          int           heads,
+                          int           kv_heads,
+                          int           head_dim,
+                          const double* frequencies,
+                          int           rotary_dim,
+                          int           interleaved,
+                          float         magnitude,
+                          const int*    positions);
+
+/* Attention of drafted tokens: Out[n][h] = sum over the keys j that row n sees of softmax_j(s_nj) V[j], with
+ * s_nj = scale * Q[n][h] . K[j], then cap * tanh(s / cap) where cap > 0, then + slopes[h] * (position of j - position of n)
+ * where slopes (device floats, [heads]) are given; zero for a row that sees no key.  Query head h reads key/value head
+ * h / (heads / kv_heads).  The batch's own keys are in the cache already (FlashLLM_RotaryAppend).  A row sees the context of its
+ * sequence and those of its sequence's first 64 new tokens whose bit tree_mask[n] has (its ancestors and itself, usually).
+ * `positions` (int32 [tokens]) are needed with slopes only: the distance is between them, for keys of the context to their
+ * place.  Q is [tokens][ld_q], Out [tokens][heads * head_dim]; scale > 0.  `workspace`: FlashLLM_Attention_WorkspaceBytes on a
+ * 16-byte boundary, its contents before and after the call of no use to anybody; calls that may overlap on the GPU need one
+ * each. */
+int FlashLLM_TreeAttention(void*                     stream,
+                           const void*               Q,
+                           int                       ld_q,
+                           const void*               K_cache,
+                           const void*               V_cache,
+                           int                       pages,
+                           int                       page_size,
+                           const int*                cu_tokens,
+                           const int*                context,
+                           const int*                page_table,
+                           int                       table_width,
+                           int                       sequences,
+                           int                       tokens,
+                           int                       heads,
+                           int                       kv_heads,
+                           int                       head_dim,
+                           const unsigned long long* tree_mask,
+                           const int*                positions,
+                           float                     scale,
+                           float                     cap,
+                           const float*              slopes,
+                           void*                     Out,
+                           void*                     workspace);
+
+/* Attention of prompts, of pieces of prompts, and, with one row per sequence, of single tokens: as above, but a row sees the
+ * context, its sequence's new tokens up to itself and, where `prefix` (int32 [sequences]) is given, the first prefix[b]
+ * positions of its sequence whether they lie before or behind it.  Positions are places in the cache.  Sequences do not see one
+ * another. */
+int FlashLLM_PromptAttention(void*        stream,
+                             const void*  Q,
+                             int          ld_q,
+                             const void*  K_cache,
+                             const void*  V_cache,
+                             int          pages,
+                             int          page_size,
+                             const int*   cu_tokens,
+                             const int*   context,
+                             const int*   page_table,
+                             int          table_width,
+                             int          sequences,
+                             int          tokens,
+                             int          heads,
+                             int          kv_heads,
+                             int          head_dim,
+                             const int*   prefix,
+                             float        scale,
+                             float        cap,
+                             const float* slopes,
+                             void*        Out,
+                             void*        workspace);
+
+/* Bytes of `workspace` for the two calls above on the current device; 0 for an unsupported head_dim. */
+unsigned long long FlashLLM_Attention_WorkspaceBytes(int head_dim);
+
+/* Accepts a path of a drafted tree: keys and values of sequence b's new token accepted[b * accepted_width + i] (its row in the
+ * sequence) move to position context[b] + i, for i < accepted_lengths[b] (0 .. accepted_width, at most 64).  `layers` caches lie
+ * one behind another from K_cache and V_cache on, and all of them are moved by the one launch.  Tokens may be named in any
+ * order.  A token that the sequence does not have, or a length out of range, sets bit 64 and moves nothing. */
+int FlashLLM_CacheAccept(void*      stream,
+                         void*      K_cache,
+                         void*      V_cache,
+                         int        layers,
+                         int        pages,
+                         int        page_size,
+                         const int* cu_tokens,
+                         const int* context,
+                         const int* page_table,
+                         int        table_width,
+                         int        sequences,
+                         int        tokens,
+                         int        kv_heads,
+                         int        head_dim,
+                         const int* accepted,
+                         const int* accepted_lengths,
+                         int        accepted_width);
+
 /* Launch overlap (no counterpart in the reference).  Every kernel of this library is launched with programmatic stream
  * serialisation: its CTAs may start and set up while the previous kernel of the stream is still draining, and wait for the
  * end of everything enqueued before them before they touch any data.  With enable != 0 SpMM kernels stream Compressed_A and
@@ -359,10 +494,11 @@ void FlashLLM_SetPlan(const int* fields, int count);
 int FlashLLM_GetPlan(int M, int N, int K, int Split_K, int* out, int count);
 
 /* Reads and clears the device-side status word of the current device (synchronises the device).  0 = no kernel of
- * this library gave up on a bounded wait or met a malformed TileOffsets since the last call.  Bits: 1 a bounded wait
+ * this library gave up on a bounded wait or met a malformed TileOffsets or page table since the last call.  Bits: 1 a bounded wait
  * inside a kernel ran out, 2 malformed TileOffsets (nothing stored for that tile row), 8 device encoder: offsets do not
- * match the matrix, 16 misaligned shared memory, 32 fused all-reduce: a GPU of the group did not deliver in time.  A
- * give-up belongs to the launch it happened in: later calls run normally whether or not the word is read. */
+ * match the matrix, 16 misaligned shared memory, 32 fused all-reduce: a GPU of the group did not deliver in time, 64 a page
+ * id, a length or an accepted token out of range (see the paged cache above).  A give-up belongs to the launch it happened in: later calls
+ * run normally whether or not the word is read. */
 unsigned int FlashLLM_ConsumeStatus(void);
 
 /* Number of kernels this library has launched from this process (all devices). */
