@@ -3,6 +3,7 @@
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
+#include <atomic>
 #include <cmath>
 
 #include "../../include/SpMM_API.cuh"
@@ -59,16 +60,92 @@ static cudaError_t launch_rotary(cudaStream_t stream, const RotaryParams& p, int
     return interleaved ? launch(rotary_append_kernel<128, true>) : launch(rotary_append_kernel<128, false>);
 }
 
+using EncodeTiledFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
+                                   const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                                   CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+static EncodeTiledFn encode_tiled()
+{
+    static const EncodeTiledFn function = []() -> EncodeTiledFn {
+        void*                           fn = nullptr;
+        cudaDriverEntryPointQueryResult found;
+        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &fn, cudaEnableDefault, &found) != cudaSuccess
+            || found != cudaDriverEntryPointSuccess)
+            return nullptr;
+        return reinterpret_cast<EncodeTiledFn>(fn);
+    }();
+    return function;
+}
+
+// Multiprocessors of the current device, and with them the shared-memory limits of the attention kernels raised: once per
+// device.
+static cudaError_t multiprocessors(int* count)
+{
+    constexpr int           kMaxDevices = 64;
+    static std::atomic<int> known[kMaxDevices];
+    int                     device = 0;
+    cudaError_t             err    = cudaGetDevice(&device);
+    if (err != cudaSuccess)
+        return err;
+    if (device < 0 || device >= kMaxDevices)
+        return cudaErrorInvalidDevice;
+    *count = known[device].load(std::memory_order_acquire);
+    if (*count > 0)
+        return cudaSuccess;
+    err = cudaDeviceGetAttribute(count, cudaDevAttrMultiProcessorCount, device);
+    if (err == cudaSuccess)
+        err = cudaFuncSetAttribute(attention_kernel<64>, cudaFuncAttributeMaxDynamicSharedMemorySize, attn_smem_bytes(64));
+    if (err == cudaSuccess)
+        err = cudaFuncSetAttribute(attention_kernel<128>, cudaFuncAttributeMaxDynamicSharedMemorySize, attn_smem_bytes(128));
+    if (err == cudaSuccess)
+        known[device].store(*count, std::memory_order_release);
+    return err;
+}
+
+// A cache tensor as (head_dim, page_size, pages * kv_heads), copied in boxes of 64 columns and the rows of a page, 128 at most.
+static bool encode_cache(CUtensorMap* map, const half* cache, const CacheBatch& batch, int head_dim)
+{
+    const EncodeTiledFn encode = encode_tiled();
+    if (encode == nullptr)
+        return false;
+    const cuuint64_t page = cuuint64_t(1) << batch.page_shift, row = static_cast<cuuint64_t>(head_dim) * 2;
+    const cuuint64_t dims[3]    = {static_cast<cuuint64_t>(head_dim), page, static_cast<cuuint64_t>(batch.pages) * batch.kv_heads};
+    const cuuint64_t strides[2] = {row, page * row};
+    const cuuint32_t box[3]     = {64, static_cast<cuuint32_t>(page < kAttnKeys ? page : kAttnKeys), 1};
+    const cuuint32_t ones[3]    = {1, 1, 1};
+    return encode(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, const_cast<half*>(cache), dims, strides, box, ones,
+                  CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE)
+           == CUDA_SUCCESS;
+}
+
+template<int HEAD_DIM>
+static cudaError_t launch_attention(cudaStream_t stream, const AttentionParams& p)
+{
+    int         sms = 0;
+    cudaError_t err = multiprocessors(&sms);
+    if (err != cudaSuccess)
+        return err;
+    CUtensorMap map_k, map_v;
+    if (!encode_cache(&map_k, p.k_cache, p.batch, HEAD_DIM) || !encode_cache(&map_v, p.v_cache, p.batch, HEAD_DIM))
+        return cudaErrorInvalidValue;
+    err = launch_in_stream_order(attention_kernel<HEAD_DIM>, dim3(sms), dim3(kAttnThreads), attn_smem_bytes(HEAD_DIM), stream, 1, map_k,
+                                 map_v, p);
+    if (err != cudaSuccess)
+        return err;
+    return launch_in_stream_order(attention_join_kernel<HEAD_DIM>, dim3(sms, kAttnItemRows / 32), dim3(256), 0, stream, 1, p, sms);
+}
+
 // The checks that tree and prompt attention share, and the launch.
 static cudaError_t attend(cudaStream_t stream, AttentionParams p, const void* Q, int ld_q, const void* K_cache,
                           const void* V_cache, int pages, int page_size, const int* cu_tokens, const int* context,
                           const int* page_table, int table_width, int sequences, int tokens, int heads, int kv_heads,
-                          int head_dim, float scale, float cap, const float* slopes, void* Out)
+                          int head_dim, float scale, float cap, const float* slopes, void* Out, void* workspace)
 {
     if (!describe_batch(&p.batch, K_cache, V_cache, pages, page_size, cu_tokens, context, page_table, table_width, sequences, tokens,
                         kv_heads, head_dim)
         || heads < 1 || heads % kv_heads != 0 || static_cast<long long>(heads) * head_dim > (1 << 24) || !rows_fit(Q, ld_q, heads, head_dim)
-        || Out == nullptr || !aligned16(Out) || !(scale > 0.0f) || !std::isfinite(scale) || !(cap >= 0.0f) || !std::isfinite(cap)
+        || workspace == nullptr || !aligned16(workspace) || Out == nullptr || !aligned16(Out) || !(scale > 0.0f) || !std::isfinite(scale) || !(cap >= 0.0f) || !std::isfinite(cap)
         || static_cast<long long>(tokens) * heads > 0x7fffffffll - 256)
         return cudaErrorInvalidValue;
     if (tokens == 0 || sequences == 0)
@@ -84,10 +161,9 @@ static cudaError_t attend(cudaStream_t stream, AttentionParams p, const void* Q,
     p.heads   = heads;
     p.scale   = scale;
     p.cap     = cap;
-    const int  warps = kAttentionThreads / 32;
-    const dim3 grid(tokens, (heads + warps - 1) / warps);
-    return head_dim == 64 ? launch_in_stream_order(attention_kernel<64>, grid, dim3(kAttentionThreads), 0, stream, 1, p)
-                          : launch_in_stream_order(attention_kernel<128>, grid, dim3(kAttentionThreads), 0, stream, 1, p);
+    p.workspace = static_cast<unsigned char*>(workspace);
+    p.share     = heads / kv_heads;
+    return head_dim == 64 ? launch_attention<64>(stream, p) : launch_attention<128>(stream, p);
 }
 
 }  // namespace flashllm
@@ -128,7 +204,10 @@ int FlashLLM_RotaryAppend(void* stream, const void* QKV, int ld_qkv, void* Q, in
 
 unsigned long long FlashLLM_Attention_WorkspaceBytes(int head_dim)
 {
-    return head_dim == 64 || head_dim == 128 ? 16 : 0;
+    int sms = 0;
+    if ((head_dim != 64 && head_dim != 128) || multiprocessors(&sms) != cudaSuccess)
+        return 0;
+    return attn_workspace_bytes(sms, head_dim);
 }
 
 int FlashLLM_TreeAttention(void* stream, const void* Q, int ld_q, const void* K_cache, const void* V_cache, int pages,
@@ -136,14 +215,14 @@ int FlashLLM_TreeAttention(void* stream, const void* Q, int ld_q, const void* K_
                            int sequences, int tokens, int heads, int kv_heads, int head_dim, const unsigned long long* tree_mask,
                            const int* positions, float scale, float cap, const float* slopes, void* Out, void* workspace)
 {
-    if (tree_mask == nullptr || (slopes != nullptr && positions == nullptr) || workspace == nullptr || !aligned16(workspace))
+    if (tree_mask == nullptr || (slopes != nullptr && positions == nullptr))
         return static_cast<int>(cudaErrorInvalidValue);
     AttentionParams p{};
     p.tree_mask = tree_mask;
     p.positions = positions;
     return static_cast<int>(attend(static_cast<cudaStream_t>(stream), p, Q, ld_q, K_cache, V_cache, pages, page_size, cu_tokens,
                                    context, page_table, table_width, sequences, tokens, heads, kv_heads, head_dim, scale, cap,
-                                   slopes, Out));
+                                   slopes, Out, workspace));
 }
 
 int FlashLLM_PromptAttention(void* stream, const void* Q, int ld_q, const void* K_cache, const void* V_cache, int pages,
@@ -151,13 +230,11 @@ int FlashLLM_PromptAttention(void* stream, const void* Q, int ld_q, const void* 
                              int sequences, int tokens, int heads, int kv_heads, int head_dim, const int* prefix, float scale,
                              float cap, const float* slopes, void* Out, void* workspace)
 {
-    if (workspace == nullptr || !aligned16(workspace))
-        return static_cast<int>(cudaErrorInvalidValue);
     AttentionParams p{};
     p.prefix = prefix;
     return static_cast<int>(attend(static_cast<cudaStream_t>(stream), p, Q, ld_q, K_cache, V_cache, pages, page_size, cu_tokens,
                                    context, page_table, table_width, sequences, tokens, heads, kv_heads, head_dim, scale, cap,
-                                   slopes, Out));
+                                   slopes, Out, workspace));
 }
 
 int FlashLLM_CacheAccept(void* stream, void* K_cache, void* V_cache, int layers, int pages, int page_size, const int* cu_tokens,

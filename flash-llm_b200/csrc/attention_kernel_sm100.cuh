@@ -5,8 +5,22 @@
 //
 // What token i of a sequence (rows first + i, place context + i in the cache) sees: the whole context, and of the batch's own
 // tokens either those up to itself and those of the prefix (prompts), or those whose bit its mask has (trees).
+//
+// One pass over the keys in tiles of 128 with the running maximum and sum of a softmax: S = Q K^T on the tensor cores, P =
+// exp(S - maximum) in registers, one thread per row, rounded to fp16 (the type of the other operand of its product; 2^-11 of a
+// weight) and back to tensor memory, O += P V from there.  The query heads that share a key/value head are rows of one tile:
+// row r of a sequence's (tokens x share) rows is token r / share, head r % share of the group.
+//
+// An item is 256 such rows of one sequence and one key/value head.  Its two tiles of rows are two groups of softmax warps that
+// take turns on the tensor core; an item of at most 128 rows (single tokens, drafted trees) is the same tile for both groups,
+// each takes every other tile of keys, and the two results are joined at the end.  The work of a call is the linear sequence
+// of all items' tiles of keys, dealt out evenly over one CTA per SM whatever the sequences' lengths; an item that is cut leaves
+// partial sums in the workspace, which attention_join_kernel adds up in key order.
 #pragma once
+#include <math_constants.h>
+
 #include "cache_batch.cuh"
+#include "tiling.h"
 
 namespace flashllm {
 
@@ -20,95 +34,1013 @@ struct AttentionParams {
     const int*                positions;  // [tokens] positions of tree tokens, for the distance
     const int*                prefix;     // [sequences] keys that all tokens of a prompt see, or nullptr
     const float*              slopes;     // [heads], or nullptr
+    unsigned char*            workspace;
     long long                 ld_q;
     int                       heads;
+    int                       share;  // query heads per key/value head
     float                     scale;
     float                     cap;  // 0: none
 };
 
-constexpr int kAttentionThreads = 128;
+constexpr int kAttnKeys      = 128;  // keys per tile
+constexpr int kAttnRows      = 128;  // rows per tile: one per lane of tensor memory
+constexpr int kAttnItemRows  = 2 * kAttnRows;
+constexpr int kAttnMmaWarp   = 8;  // warps 0..3 and 4..7: the two groups of rows
+constexpr int kAttnLoadWarp  = 9;
+constexpr int kAttnCleanWarp = 10;  // and 11
+constexpr int kAttnThreads   = 12 * 32;
+constexpr int kAttnTmemCols  = 512;
+constexpr int kAttnSegments  = 8;  // segments that shared memory holds at a time
+// Registers of a thread: the softmax warps keep a row of 128 scores, 256 x 208 + 128 x 88 = 384 x 168.
+constexpr int kAttnSoftmaxRegisters = 208, kAttnOtherRegisters = 88;
 
-// One warp per row and head, key by key: a running maximum, the sum and the output in 32 bits.
-template<int HEAD_DIM>
-__global__ void __launch_bounds__(kAttentionThreads) attention_kernel(const AttentionParams p)
+constexpr unsigned long long kAttnWaitLimitNs = 200ull * 1000 * 1000;
+
+// Tiles of keys (and as many of values) in shared memory at a time.
+__host__ __device__ constexpr int attn_stages(int head_dim)
 {
-    constexpr int     kPairs = HEAD_DIM / 64;  // half2 per lane
-    const CacheBatch& c      = p.batch;
-    const int         n = blockIdx.x, lane = threadIdx.x & 31;
-    const int         head = blockIdx.y * (kAttentionThreads / 32) + (threadIdx.x >> 5);
-    ptx::grid_dependency_wait();
-    ptx::grid_launch_dependents();
-    if (head >= p.heads)
-        return;
-    int owner = -1;
-    for (int b = lane; b < c.sequences; b += 32) {
-        const int begin = c.cu_tokens[b];
-        if (begin >= 0 && begin <= n && n < c.cu_tokens[b + 1])
-            owner = b;
+    return head_dim == 128 ? 2 : 4;
+}
+
+__host__ __device__ constexpr int attn_tile_bytes(int head_dim)
+{
+    return kAttnKeys * head_dim * 2;
+}
+
+// The part of an item that one CTA takes in one go.
+struct AttnSegment {
+    int  b;
+    int  first, count, context, prefix;  // of the sequence: first row, rows, position of the first row, keys that all see
+    int  head;     // key/value head
+    int  row0;     // first row of the item in the sequence's rows (tokens x share)
+    int  rows;     // rows of the item, at most kAttnItemRows
+    int  keys;     // keys that any row of the item sees: none at or behind this
+    int  open[2];  // keys that every row of a group sees: the first tile that needs a mask ends behind them
+    int  tiles;    // of keys, the whole item
+    int  begin;    // first tile of the segment
+    int  end;      // behind its last; 0: no more segments
+    int  tiles0;   // pair: tiles of keys that the first tile of rows needs
+    bool pair;     // two tiles of rows; otherwise both groups share the one
+
+    // Tiles of keys that a group goes through, and the i-th of them.
+    __device__ __forceinline__ int count_of(int group) const
+    {
+        if (pair)
+            return group == 0 ? max(min(end, tiles0) - begin, 0) : end - begin;
+        return (end - begin + 1 - group) / 2;
     }
-    owner = __reduce_max_sync(0xffffffffu, owner);
-    if (owner < 0)
-        return;
-    const Sequence s       = load_sequence(c, owner);
-    const int      i       = n - s.first;
-    const int      kv_head = head / (p.heads / c.kv_heads);
-    half2*         out     = reinterpret_cast<half2*>(p.out + (static_cast<long long>(n) * p.heads + head) * HEAD_DIM);
-    const half2*   q       = reinterpret_cast<const half2*>(p.q + n * p.ld_q + static_cast<long long>(head) * HEAD_DIM);
-    float2         x[kPairs], o[kPairs];
-#pragma unroll
-    for (int k = 0; k < kPairs; ++k) {
-        x[k] = __half22float2(q[lane + 32 * k]);
-        o[k] = make_float2(0.0f, 0.0f);
+    __device__ __forceinline__ int tile(int group, int i) const
+    {
+        return pair ? begin + i : begin + group + 2 * i;
     }
-    const unsigned long long mask = p.tree_mask ? p.tree_mask[n] : 0ull;
-    int                      end  = s.count > 0 ? s.context + s.count : 0;
-    int                      seen = s.context + i + 1;  // keys that are seen because of their place
-    if (p.tree_mask) {
-        seen = s.context;
-        end  = min(end, s.context + kMaxDrafted);
-    }
-    else if (p.prefix)
-        seen = max(seen, p.prefix[owner]);
-    const float slope = p.slopes ? p.slopes[head] : 0.0f;
-    const int   place = p.tree_mask && p.slopes ? p.positions[n] : s.context + i;
-    float       top = -INFINITY, sum = 0.0f;
-    for (int j = 0; j < end; ++j) {
-        const int drafted = j - s.context;
-        if (j >= seen && !(p.tree_mask && (mask >> drafted & 1)))
-            continue;
-        const long long row   = cache_row(c, owner, j, kv_head);
-        const half2*    k_row = reinterpret_cast<const half2*>(p.k_cache + row * HEAD_DIM);
-        const half2*    v_row = reinterpret_cast<const half2*>(p.v_cache + row * HEAD_DIM);
-        float           dot   = 0.0f;
-#pragma unroll
-        for (int k = 0; k < kPairs; ++k) {
-            const float2 y = row < 0 ? make_float2(0.0f, 0.0f) : __half22float2(k_row[lane + 32 * k]);
-            dot += x[k].x * y.x + x[k].y * y.y;
+};
+
+// Dynamic shared memory: two tiles of Q, the stages, and what AttnShared holds.
+struct AttnShared {
+    unsigned long long k_full[4], k_empty[4], v_full[4], v_clean[4], v_empty[4];
+    unsigned long long s_full[2], p_full[2], o_done[2], q_full[2], segment_full[kAttnSegments];
+    uint32_t           tmem;
+    volatile uint32_t  abort_flag;
+    int                start_sequence, start_rows, start_head, start_tile;
+    long long          start_units;
+    // Written by the loader, which is ahead of everybody, by at most the stages and one: a segment's values cannot be loaded
+    // before those of the one so many tiles earlier have been multiplied, and its place here is taken again only after
+    // kAttnSegments more.
+    AttnSegment        segment[kAttnSegments];
+    float              top[2][kAttnRows], sum[2][kAttnRows];
+    uint32_t           not_finite[kAttnSegments][3][4];  // keys of an item's last three tiles whose values are not finite
+    int                drafted[2][kMaxDrafted];          // positions of drafted tokens, by group
+    unsigned int       tiles[kMaxSequences];             // of all items of a sequence's first key/value head
+};
+
+__host__ __device__ constexpr int attn_smem_bytes(int head_dim)
+{
+    return (2 + 2 * attn_stages(head_dim)) * attn_tile_bytes(head_dim) + static_cast<int>(sizeof(AttnShared)) + 1024;
+}
+
+// The workspace: for each CTA two slots, the segment that continues an item that another CTA began, and the one that begins an
+// item that another CTA continues.
+constexpr unsigned kPartNone = 0, kPartBegins = 1, kPartContinues = 2, kPartEnds = 3;
+
+struct AttnPart {
+    unsigned kind;
+    int      first;  // first row of the sequence in the batch
+    int      row0;   // first row of the item in the sequence
+    int      rows;   // rows of the item
+    int      head;   // key/value head
+    int      pad[3];
+};
+
+__host__ __device__ constexpr size_t attn_stats_offset(int ctas)
+{
+    return size_t(2) * ctas * sizeof(AttnPart);
+}
+
+__host__ __device__ constexpr size_t attn_sums_offset(int ctas)
+{
+    return attn_stats_offset(ctas) + size_t(2) * ctas * kAttnItemRows * sizeof(float2);
+}
+
+// Sums lie as [slot][tile of rows][head_dim / 4][row] float4: a warp's rows are neighbours.
+__host__ __device__ constexpr size_t attn_workspace_bytes(int ctas, int head_dim)
+{
+    return attn_sums_offset(ctas) + size_t(2) * ctas * kAttnItemRows * head_dim * sizeof(float);
+}
+
+__device__ __forceinline__ bool attn_wait(const unsigned long long* barrier, uint32_t parity, AttnShared& sh, unsigned int* status)
+{
+    const uint32_t bar = ptx::smem_u32(barrier);
+    if (ptx::mbar_try_wait(bar, parity))
+        return true;
+    uint64_t t0 = 0;
+    for (uint32_t it = 1;; ++it) {
+        if (ptx::mbar_try_wait(bar, parity))
+            return true;
+        if ((it & 63u) == 0u) {
+            if (sh.abort_flag)
+                return false;
+            const uint64_t now = ptx::globaltimer_ns();
+            if (t0 == 0)
+                t0 = now;
+            else if (now - t0 > kAttnWaitLimitNs) {
+                sh.abort_flag = 1u;
+                atomicOr(status, kStatusWaitExpired);
+                return false;
+            }
         }
+    }
+}
+
+// ---------------------------------------------------------------- the work of a call
+
+// One sequence as the rows of its items see it.
+struct AttnSequence {
+    Sequence s;
+    int      prefix;  // keys of the sequence that all of its rows see, beyond the context
+    int      rows;    // count * share
+};
+
+__device__ __forceinline__ AttnSequence attn_sequence(const AttentionParams& p, int b)
+{
+    AttnSequence a;
+    a.s      = load_sequence(p.batch, b);
+    a.prefix = p.prefix ? min(p.prefix[b], a.s.context + a.s.count) : 0;
+    a.rows   = a.s.count * p.share;
+    return a;
+}
+
+// Keys that rows before `row_end` (of the sequence's rows) see at most: no row sees the key of that index or one behind it.
+__device__ __forceinline__ int attn_keys(const AttentionParams& p, const AttnSequence& a, int row_end)
+{
+    if (p.tree_mask)
+        return a.s.context + min(a.s.count, kMaxDrafted);
+    return max(a.s.context + (row_end - 1) / p.share + 1, a.prefix);
+}
+
+// Keys that all rows from `row` on see.
+__device__ __forceinline__ int attn_open_keys(const AttentionParams& p, const AttnSequence& a, int row)
+{
+    return p.tree_mask ? a.s.context : max(a.s.context + row / p.share + 1, a.prefix);
+}
+
+__device__ __forceinline__ int attn_tiles(int keys)
+{
+    return (keys + kAttnKeys - 1) / kAttnKeys;
+}
+
+// Walks a CTA's share of the linear sequence of tiles, order (sequence, rows, key/value head, keys).
+struct AttnCursor {
+    AttnSequence a;
+    AttnSegment  seg;
+    long long    left;
+    int          next_tile;
+
+    __device__ __forceinline__ void enter_rows(const AttentionParams& p)
+    {
+        const int end  = min(seg.row0 + kAttnItemRows, a.rows);
+        seg.rows       = end - seg.row0;
+        seg.pair       = seg.rows > kAttnRows;
+        seg.keys       = attn_keys(p, a, end);
+        seg.tiles      = attn_tiles(seg.keys);
+        seg.tiles0     = seg.pair ? attn_tiles(attn_keys(p, a, seg.row0 + kAttnRows)) : seg.tiles;
+        seg.open[0]    = attn_open_keys(p, a, seg.row0);
+        seg.open[1]    = seg.pair ? attn_open_keys(p, a, seg.row0 + kAttnRows) : seg.open[0];
+    }
+    __device__ __forceinline__ void enter_sequence(const AttentionParams& p)
+    {
+        for (;; ++seg.b) {
+            if (seg.b >= p.batch.sequences) {  // only if somebody writes the arrays during the call
+                left = 0;
+                return;
+            }
+            a = attn_sequence(p, seg.b);
+            if (a.rows > 0)
+                break;
+        }
+        seg.first   = a.s.first;
+        seg.count   = a.s.count;
+        seg.context = a.s.context;
+        seg.prefix  = a.prefix;
+        enter_rows(p);
+    }
+    __device__ __forceinline__ AttnCursor(const AttentionParams& p, const AttnShared& sh)
+    {
+        left      = sh.start_units;
+        seg.b     = sh.start_sequence;
+        seg.row0  = sh.start_rows;
+        seg.head  = sh.start_head;
+        next_tile = sh.start_tile;
+        if (left > 0)
+            enter_sequence(p);
+    }
+    // The next segment; its `end` is 0 at the end of the share.
+    __device__ __forceinline__ void next(const AttentionParams& p)
+    {
+        if (left > 0 && next_tile >= seg.tiles) {
+            next_tile = 0;
+            if (++seg.head == p.batch.kv_heads) {
+                seg.head = 0;
+                seg.row0 += kAttnItemRows;
+                if (seg.row0 >= a.rows) {
+                    seg.row0 = 0;
+                    ++seg.b;
+                    enter_sequence(p);
+                }
+                else
+                    enter_rows(p);
+            }
+        }
+        seg.begin = next_tile;
+        seg.end   = left > 0 ? static_cast<int>(min(static_cast<long long>(seg.tiles), next_tile + left)) : 0;
+        left -= seg.end - seg.begin;
+        next_tile = seg.end;
+    }
+};
+
+// The segment of that number, once the loader has written it; nullptr at the end and when the CTA gives up.
+__device__ __forceinline__ const AttnSegment* attn_segment(AttnShared& sh, int number, unsigned int* status)
+{
+    const int place = number % kAttnSegments;
+    if (!attn_wait(&sh.segment_full[place], number / kAttnSegments & 1, sh, status) || sh.segment[place].end == 0)
+        return nullptr;
+    return &sh.segment[place];
+}
+
+constexpr unsigned kAttnSeveralItems = 0xffffffffu, kAttnLostRows = 0xfffffffeu;  // in place of a sequence's tiles
+
+// Where this CTA's share begins and how long it is; all threads, ends with a barrier.  The rows of a sequence that does not fit
+// into the page table are cleared here, by one CTA.
+__device__ __forceinline__ void attn_plan(const AttentionParams& p, AttnShared& sh, int head_dim)
+{
+    const int B = p.batch.sequences, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    for (int b = threadIdx.x; b < B; b += kAttnThreads) {
+        const AttnSequence a = attn_sequence(p, b);
+        sh.tiles[b]          = a.s.lost > 0            ? kAttnLostRows
+                               : a.rows == 0            ? 0u
+                               : a.rows > kAttnItemRows ? kAttnSeveralItems
+                                                        : attn_tiles(attn_keys(p, a, a.rows));
+    }
+    __syncthreads();
+    for (int b = warp; b < B; b += kAttnThreads / 32) {
+        if (sh.tiles[b] < kAttnLostRows)
+            continue;
+        const AttnSequence a    = attn_sequence(p, b);
+        unsigned           mine = 0;
+        if (a.s.lost > 0 && b % gridDim.x == blockIdx.x) {
+            const long long row = static_cast<long long>(p.heads) * head_dim;
+            for (long long i = lane * 8; i < a.s.lost * row; i += 32 * 8)
+                *reinterpret_cast<uint4*>(p.out + a.s.first * row + i) = make_uint4(0, 0, 0, 0);
+        }
+        for (long long r = lane * kAttnItemRows; r < a.rows; r += 32 * kAttnItemRows)
+            mine += attn_tiles(attn_keys(p, a, static_cast<int>(min(r + kAttnItemRows, static_cast<long long>(a.rows)))));
+        mine = __reduce_add_sync(0xffffffffu, mine);
+        __syncwarp();
+        if (lane == 0)
+            sh.tiles[b] = mine;
+    }
+    __syncthreads();
+    if (warp == 0) {
+        long long total = 0;
+        for (int b = lane; b < B; b += 32)
+            total += sh.tiles[b];
 #pragma unroll
         for (int d = 16; d > 0; d >>= 1)
-            dot += __shfl_xor_sync(0xffffffffu, dot, d);
-        dot *= p.scale;
-        if (p.cap > 0.0f)
-            dot = p.cap * tanhf(dot / p.cap);
-        if (p.slopes)
-            dot += slope * static_cast<float>((p.tree_mask && drafted >= 0 ? p.positions[s.first + drafted] : j) - place);
-        const float new_top = fmaxf(top, dot);
-        const float keep    = new_top == -INFINITY ? 1.0f : expf(top - new_top);
-        const float weight  = new_top == -INFINITY ? 0.0f : expf(dot - new_top);
-        top                 = new_top;
-        sum                 = sum * keep + weight;
+            total += __shfl_xor_sync(0xffffffffu, total, d);
+        const int       heads = p.batch.kv_heads;
+        const long long units = total * heads;
+        const long long ctas  = min(units, static_cast<long long>(gridDim.x));  // none of them without a tile
+        const long long cta   = blockIdx.x;
+        const long long u0    = cta < ctas ? units * cta / ctas : 0, u1 = cta < ctas ? units * (cta + 1) / ctas : 0;
+        // The sequence that holds unit u0: the first whose running sum passes it.
+        int       b = 0, row0 = 0;
+        long long before = 0;
+        if (u1 > u0) {
+            for (int base = 0;; base += 32) {
+                long long mine = base + lane < B ? static_cast<long long>(sh.tiles[base + lane]) * heads : 0, upto = mine;
 #pragma unroll
-        for (int k = 0; k < kPairs; ++k) {
-            const float2 y = row < 0 ? make_float2(0.0f, 0.0f) : __half22float2(v_row[lane + 32 * k]);
-            o[k].x         = o[k].x * keep + weight * y.x;
-            o[k].y         = o[k].y * keep + weight * y.y;
+                for (int d = 1; d < 32; d <<= 1) {
+                    const long long other = __shfl_up_sync(0xffffffffu, upto, d);
+                    if (lane >= d)
+                        upto += other;
+                }
+                const unsigned past = __ballot_sync(0xffffffffu, before + upto > u0);
+                if (past) {
+                    const int l = __ffs(past) - 1;
+                    b           = base + l;
+                    before += __shfl_sync(0xffffffffu, upto - mine, l);
+                    break;
+                }
+                before += __shfl_sync(0xffffffffu, upto, 31);
+            }
+            const AttnSequence a = attn_sequence(p, b);
+            for (long long base = 0;; base += 32 * kAttnItemRows) {  // ... and of its items the first
+                const long long r    = base + lane * kAttnItemRows;
+                long long       mine = 0;
+                if (r < a.rows)
+                    mine = static_cast<long long>(heads)
+                           * attn_tiles(attn_keys(p, a, static_cast<int>(min(r + kAttnItemRows, static_cast<long long>(a.rows)))));
+                long long upto = mine;
+#pragma unroll
+                for (int d = 1; d < 32; d <<= 1) {
+                    const long long other = __shfl_up_sync(0xffffffffu, upto, d);
+                    if (lane >= d)
+                        upto += other;
+                }
+                const unsigned past = __ballot_sync(0xffffffffu, before + upto > u0);
+                if (past || base + 32 * kAttnItemRows >= a.rows) {
+                    const int l = past ? __ffs(past) - 1 : 0;
+                    row0        = static_cast<int>(base) + l * kAttnItemRows;
+                    before += __shfl_sync(0xffffffffu, upto - mine, l);
+                    break;
+                }
+                before += __shfl_sync(0xffffffffu, upto, 31);
+            }
+            if (lane == 0) {
+                const int tiles   = max(1, attn_tiles(attn_keys(p, a, min(row0 + kAttnItemRows, a.rows))));
+                sh.start_sequence = b;
+                sh.start_rows     = row0;
+                sh.start_head     = static_cast<int>((u0 - before) / tiles);
+                sh.start_tile     = static_cast<int>((u0 - before) % tiles);
+            }
+        }
+        if (lane == 0)
+            sh.start_units = u1 - u0;
+    }
+    __syncthreads();
+}
+
+// ---------------------------------------------------------------- masks
+
+// What a row sees.
+struct AttnRow {
+    int                limit;   // all keys before this one
+    int                drafts;  // ... and, for trees, key drafts + i where bit i is set
+    unsigned long long bits;
+
+    __device__ __forceinline__ bool sees(int key) const
+    {
+        const int i = key - drafts;
+        return key < limit || (i >= 0 && i < kMaxDrafted && (bits >> i & 1));
+    }
+    // Bit c: the row sees key `key0` + c.
+    __device__ __forceinline__ uint32_t word(int key0) const
+    {
+        const int n = limit - key0;
+        uint32_t  w = n >= 32 ? 0xffffffffu : n > 0 ? (1u << n) - 1u : 0u;
+        const int d = drafts - key0;
+        if (d >= 0 && d < 32)
+            w |= static_cast<uint32_t>(bits << d);
+        else if (d < 0 && d > -kMaxDrafted)
+            w |= static_cast<uint32_t>(bits >> -d);
+        return w;
+    }
+};
+
+__device__ __forceinline__ AttnRow attn_row(const AttentionParams& p, const AttnSegment& seg, int row, bool valid)
+{
+    AttnRow r;
+    r.limit  = 0;
+    r.drafts = seg.context;
+    r.bits   = 0;
+    if (!valid)
+        return r;
+    const int token = row / p.share;
+    if (p.tree_mask) {
+        r.limit = seg.context;
+        r.bits  = p.tree_mask[seg.first + token];
+        if (seg.count < kMaxDrafted)
+            r.bits &= (1ull << seg.count) - 1;
+    }
+    else
+        r.limit = max(seg.context + token + 1, seg.prefix);
+    return r;
+}
+
+// ---------------------------------------------------------------- the kernel
+
+__device__ __forceinline__ bool half_not_finite(uint32_t h)
+{
+    return (h & 0x7c00u) == 0x7c00u;
+}
+
+// Adds to o[c], element column + c of a row's output, the values that are not finite of keys that the row sees (the products
+// took zeros in their place: a weight of zero times infinity is not zero).
+template<int HEAD_DIM>
+__device__ __forceinline__ void attn_add_not_finite(const AttentionParams& p, const AttnSegment& seg, const AttnRow& row,
+                                                    const uint32_t (&list)[3][4], int column, float (&o)[32])
+{
+#pragma unroll 1
+    for (int i = 0; i < 12; ++i)
+#pragma unroll 1
+        for (uint32_t w = list[i / 4][i % 4]; w != 0; w &= w - 1) {
+            const int key = (seg.tiles - 1 - i / 4) * kAttnKeys + 32 * (i % 4) + __ffs(w) - 1;
+            if (!row.sees(key))
+                continue;
+            const long long at = cache_row(p.batch, seg.b, key, seg.head);
+            if (at < 0)
+                continue;
+            const half* v = p.v_cache + at * HEAD_DIM + column;
+#pragma unroll
+            for (int c = 0; c < 32; ++c)
+                if (half_not_finite(__half_as_ushort(v[c])))
+                    o[c] += __half2float(v[c]);
+        }
+}
+
+template<int HEAD_DIM>
+__global__ void __launch_bounds__(kAttnThreads, 1)
+attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const AttentionParams p)
+{
+    constexpr int      kStages    = attn_stages(HEAD_DIM);
+    constexpr int      kTileBytes = attn_tile_bytes(HEAD_DIM);
+    constexpr int      kBlock     = kAttnKeys * 128;  // bytes of 64 columns of a tile
+    constexpr int      kBlocks    = HEAD_DIM / 64;
+    constexpr uint32_t kS = 0, kO = 256;  // tensor memory: scores (weights in their first half) and outputs, 128 columns a group
+    extern __shared__ unsigned char smem_raw[];
+    const uint32_t raw  = ptx::smem_u32(smem_raw);
+    const uint32_t base = (raw + 1023u) & ~1023u;
+    unsigned char* const smem = smem_raw + (base - raw);
+    const uint32_t       q_base = base, k_base = base + 2 * kTileBytes, v_base = k_base + kStages * kTileBytes;
+    AttnShared&          sh     = *reinterpret_cast<AttnShared*>(smem + (2 + 2 * kStages) * kTileBytes);
+    unsigned int* const  status = p.batch.status;
+    const int            warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < 4; ++i) {
+            ptx::mbar_init(ptx::smem_u32(&sh.k_full[i]), 1);
+            ptx::mbar_init(ptx::smem_u32(&sh.k_empty[i]), 1);
+            ptx::mbar_init(ptx::smem_u32(&sh.v_full[i]), 1);
+            ptx::mbar_init(ptx::smem_u32(&sh.v_clean[i]), 64);
+            ptx::mbar_init(ptx::smem_u32(&sh.v_empty[i]), 1);
+        }
+        for (int i = 0; i < 2; ++i) {
+            ptx::mbar_init(ptx::smem_u32(&sh.s_full[i]), 1);
+            ptx::mbar_init(ptx::smem_u32(&sh.p_full[i]), 4);
+            ptx::mbar_init(ptx::smem_u32(&sh.o_done[i]), 1);
+            ptx::mbar_init(ptx::smem_u32(&sh.q_full[i]), 4);
+        }
+        for (int i = 0; i < kAttnSegments; ++i)
+            ptx::mbar_init(ptx::smem_u32(&sh.segment_full[i]), 1);
+        sh.abort_flag = 0u;
+        ptx::fence_mbar_init();
+        ptx::prefetch_tensormap(&map_k);
+        ptx::prefetch_tensormap(&map_v);
+    }
+    if (warp == kAttnMmaWarp) {
+        ptx::tmem_alloc(ptx::smem_u32(&sh.tmem), kAttnTmemCols);
+        ptx::tmem_relinquish();
+    }
+    ptx::grid_dependency_wait();
+    ptx::tc_fence_before_sync();
+    attn_plan(p, sh, HEAD_DIM);
+    ptx::tc_fence_after_sync();
+    const uint32_t tmem = sh.tmem;
+    if (threadIdx.x == 0)
+        ptx::grid_launch_dependents();
+
+    if (warp < kAttnMmaWarp)
+        ptx::take_registers<kAttnSoftmaxRegisters>();
+    else
+        ptx::give_registers<kAttnOtherRegisters>();
+
+    if (warp < kAttnMmaWarp) {
+        // ================================================================ softmax: one thread per row
+        const int      group = warp >> 2, thread = threadIdx.x & 127;
+        const uint32_t lanes = static_cast<uint32_t>(warp & 3) << 21;  // this warp's lanes of tensor memory
+        const uint32_t s_tmem = tmem + kS + group * 128 + lanes, o_tmem = tmem + kO + group * 128 + lanes;
+        const bool     plain  = p.cap == 0.0f && p.slopes == nullptr;
+        const float    factor = plain ? p.scale * CUDART_L2E_F : 1.0f;  // scores times this are in units of log 2
+        const float    cap_in = p.cap > 0.0f ? 2.0f * CUDART_L2E_F * p.scale / p.cap : 0.0f;  // e^(2 s / cap) = 2^(cap_in q.k)
+        uint32_t       s_parity = 0, o_count = 0;  // phases of s_full, products of P and V so far
+        AttnPart* const parts = reinterpret_cast<AttnPart*>(p.workspace) + 2 * blockIdx.x;
+        bool            ok = true, written[2] = {false, false};
+        for (int number = 0;; ++number) {
+            const AttnSegment* const current = attn_segment(sh, number, status);
+            // All or none: the barriers below count every thread of the two groups.
+            if (ptx::named_barrier_any(1, 256, current == nullptr || !ok))
+                break;
+            ptx::tc_fence_after_sync();
+            const AttnSegment& seg = *current;
+            const int  in_item = (seg.pair ? group * kAttnRows : 0) + thread;  // row of the item, and of the sequence
+            const int  row_id  = seg.row0 + in_item;
+            const bool valid   = in_item < seg.rows;
+            const bool busy    = (in_item & ~31) < seg.rows;  // the warp has a row
+            const int  token = valid ? row_id / p.share : 0, head = seg.head * p.share + (valid ? row_id % p.share : 0);
+            if (seg.pair || group == 0) {  // this group's tile of Q
+                const uint4* src = reinterpret_cast<const uint4*>(p.q + (seg.first + token) * p.ld_q + static_cast<long long>(head) * HEAD_DIM);
+                unsigned char* dst = smem + (seg.pair ? group * kTileBytes : 0) + thread * 128;
+                if (valid) {
+#pragma unroll
+                    for (int c = 0; c < HEAD_DIM / 8; ++c)
+                        *reinterpret_cast<uint4*>(dst + (c / 8) * kBlock + (((c % 8) ^ (thread & 7)) << 4)) = src[c];
+                }
+                ptx::fence_proxy_async_smem();
+                __syncwarp();
+                if (lane == 0)
+                    ptx::mbar_arrive(ptx::smem_u32(&sh.q_full[seg.pair ? group : 0]));
+            }
+            const AttnRow row   = attn_row(p, seg, row_id, valid);
+            const int     open  = seg.open[group];
+            const int     tiles = seg.count_of(group);
+            float         slope = 0.0f;
+            int           place = 0;
+            if (p.slopes) {
+                slope = p.slopes[head] * CUDART_L2E_F;
+                place = valid && p.tree_mask ? p.positions[seg.first + token] : seg.context + token;
+                if (p.tree_mask) {
+                    if (thread < min(seg.count, kMaxDrafted))
+                        sh.drafted[group][thread] = p.positions[seg.first + thread];
+                    ptx::named_barrier_sync(2 + group, 128);  // the group's threads, of which none reads the last segment's any more
+                }
+            }
+            float top = -CUDART_INF_F, sum = 0.0f;
+            const int key_begin = seg.tile(group, 0) * kAttnKeys, key_step = (seg.pair ? 1 : 2) * kAttnKeys;
+            for (int i = 0; ok && i < tiles; ++i) {
+                const int key0 = key_begin + i * key_step;
+                ok             = attn_wait(&sh.s_full[group], s_parity, sh, status);
+                s_parity ^= 1u;
+                if (!__all_sync(0xffffffffu, ok)) {
+                    ok = false;
+                    break;
+                }
+                ptx::tc_fence_after_sync();
+                if (busy) {
+                    float s[kAttnKeys];
+                    {
+                        uint32_t(&raw_s)[kAttnKeys] = reinterpret_cast<uint32_t(&)[kAttnKeys]>(s);
+#pragma unroll
+                        for (int c = 0; c < kAttnKeys; c += 32)
+                            ptx::tmem_ld_x32(s_tmem + c, raw_s + c);
+                        ptx::tmem_wait_ld();
+#pragma unroll
+                        for (int c = 0; c < kAttnKeys; ++c)
+                            asm volatile("" : "+r"(raw_s[c]));  // not read before the wait
+                    }
+                    if (!plain) {
+                        if (p.cap > 0.0f) {
+                            // cap tanh(x) = cap - 2 cap / (1 + e^2x), times log2 e
+                            const float c1 = p.cap * CUDART_L2E_F, c2 = -2.0f * c1;
+#pragma unroll
+                            for (int c = 0; c < kAttnKeys; ++c)
+                                s[c] = fmaf(c2, ptx::rcp_approx(1.0f + ptx::exp2_approx(s[c] * cap_in)), c1);
+                        }
+                        else {
+                            const float f = p.scale * CUDART_L2E_F;
+#pragma unroll
+                            for (int c = 0; c < kAttnKeys; ++c)
+                                s[c] *= f;
+                        }
+                        if (p.slopes) {
+                            if (p.tree_mask && key0 + kAttnKeys > open) {
+#pragma unroll
+                                for (int c = 0; c < kAttnKeys; ++c) {
+                                    const int i_draft = key0 + c - open;
+                                    const int where   = i_draft >= 0 && i_draft < kMaxDrafted ? sh.drafted[group][i_draft] : key0 + c;
+                                    s[c]              = fmaf(slope, static_cast<float>(where - place), s[c]);
+                                }
+                            }
+                            else {
+                                const float away = static_cast<float>(key0 - place);
+#pragma unroll
+                                for (int c = 0; c < kAttnKeys; ++c)
+                                    s[c] = fmaf(slope, away + static_cast<float>(c), s[c]);
+                            }
+                        }
+                    }
+                    if (key0 + kAttnKeys > open) {
+#pragma unroll
+                        for (int k = 0; k < kAttnKeys / 32; ++k) {
+                            const uint32_t seen = row.word(key0 + 32 * k);
+#pragma unroll
+                            for (int c = 0; c < 32; ++c)
+                                s[32 * k + c] = seen >> c & 1u ? s[32 * k + c] : -CUDART_INF_F;
+                        }
+                    }
+                    float m[4] = {s[0], s[1], s[2], s[3]};
+#pragma unroll
+                    for (int c = 4; c < kAttnKeys; ++c)
+                        m[c & 3] = fmaxf(m[c & 3], s[c]);
+                    const float new_top = fmaxf(top, fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3])));
+                    if (i == 0)
+                        top = new_top;
+                    else if (__any_sync(0xffffffffu, valid && (new_top - top) * factor > 8.0f)) {  // rows of nobody have no say
+                        // The maximum that the weights are taken against moves only when it has grown by more than 2^8, which
+                        // 32-bit sums and fp16 weights have room for: rarely after the first tiles.
+                        const float keep = new_top == top ? 1.0f : ptx::exp2_approx((top - new_top) * factor);
+                        top              = new_top;
+                        sum *= keep;
+                        ok = attn_wait(&sh.o_done[group], (o_count - 1) & 1u, sh, status);
+                        if (!__all_sync(0xffffffffu, ok)) {
+                            ok = false;
+                            break;
+                        }
+                        ptx::tc_fence_after_sync();
+#pragma unroll 1
+                        for (int c = 0; c < HEAD_DIM; c += 32) {
+                            uint32_t o[32];
+                            ptx::tmem_ld_x32(o_tmem + c, o);
+                            ptx::tmem_wait_ld();
+#pragma unroll
+                            for (int k = 0; k < 32; ++k) {
+                                asm volatile("" : "+r"(o[k]));
+                                o[k] = __float_as_uint(__uint_as_float(o[k]) * keep);
+                            }
+                            ptx::tmem_st_x32(o_tmem + c, o);
+                        }
+                    }
+                    const float minus = top == -CUDART_INF_F ? 0.0f : -top * factor;
+                    float       part[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                    for (int c = 0; c < kAttnKeys; c += 32) {
+                        uint32_t w[16];
+#pragma unroll
+                        for (int k = 0; k < 32; k += 2) {
+                            const float x = ptx::exp2_approx(fmaf(s[c + k], factor, minus));
+                            const float y = ptx::exp2_approx(fmaf(s[c + k + 1], factor, minus));
+                            part[k & 3] += x;
+                            part[k + 1 & 3] += y;
+                            const half2 h = __floats2half2_rn(x, y);
+                            w[k / 2]      = *reinterpret_cast<const uint32_t*>(&h);
+                        }
+                        ptx::tmem_st_x16(s_tmem + c / 2, w);
+                    }
+                    sum += (part[0] + part[1]) + (part[2] + part[3]);
+                    ptx::tmem_wait_st();
+                }
+                ++o_count;
+                ptx::tc_fence_before_sync();
+                __syncwarp();
+                if (lane == 0)
+                    ptx::mbar_arrive(ptx::smem_u32(&sh.p_full[group]));
+            }
+            if (ok && tiles > 0)
+                ok = attn_wait(&sh.o_done[group], (o_count - 1) & 1u, sh, status);
+            ptx::tc_fence_after_sync();
+
+            // ---- the end of the segment: this row's columns, whole or a part
+            int   column0 = 0, column1 = HEAD_DIM;
+            float keep[2] = {1.0f, 0.0f};  // on this group's output, on the other group's
+            bool  join    = false;
+            if (!seg.pair) {  // the other group's sums of the same row
+                sh.top[group][thread] = tiles > 0 ? top : -CUDART_INF_F;
+                sh.sum[group][thread] = tiles > 0 ? sum : 0.0f;
+                ptx::tc_fence_before_sync();
+                ptx::named_barrier_sync(1, 256);
+                ptx::tc_fence_after_sync();
+                const float top0 = sh.top[0][thread], top1 = sh.top[1][thread];
+                const float both = fmaxf(top0, top1);
+                const float f0   = top0 == both ? 1.0f : ptx::exp2_approx((top0 - both) * factor);
+                const float f1   = top1 == both ? 1.0f : ptx::exp2_approx((top1 - both) * factor);
+                sum              = sh.sum[0][thread] * f0 + sh.sum[1][thread] * f1;
+                top              = both;
+                keep[0]          = group == 0 ? f0 : f1;
+                keep[1]          = group == 0 ? f1 : f0;
+                join             = seg.count_of(1) > 0;
+                if (!join) {  // group 0 has it all
+                    keep[0] = group == 0 ? 1.0f : 0.0f;
+                    keep[1] = group == 0 ? 0.0f : 1.0f;
+                }
+                column0 = group * (HEAD_DIM / 2);
+                column1 = column0 + HEAD_DIM / 2;
+            }
+            ok = ok && sh.abort_flag == 0u;
+            const bool     whole = seg.begin == 0 && seg.end == seg.tiles;
+            const unsigned kind  = whole ? kPartNone : seg.begin == 0 ? kPartBegins : seg.end == seg.tiles ? kPartEnds : kPartContinues;
+            const int      slot  = kind == kPartBegins ? 1 : 0;
+            if (ok && busy) {
+                const uint32_t(&list)[3][4] = sh.not_finite[number % kAttnSegments];
+                uint32_t any = 0;
+#pragma unroll
+                for (int k = 0; k < 12; ++k)
+                    any |= (&list[0][0])[k];
+                const float inverse  = sum == 0.0f ? 0.0f : 1.0f / sum;
+                const int   tile_row = seg.pair ? group : 0;
+                float4*     sums     = reinterpret_cast<float4*>(p.workspace + attn_sums_offset(gridDim.x))
+                               + (static_cast<size_t>(2 * blockIdx.x + slot) * 2 + tile_row) * (HEAD_DIM / 4) * kAttnRows + thread;
+                half* out = p.out + (static_cast<long long>(seg.first + token) * p.heads + head) * HEAD_DIM;
+#pragma unroll 1
+                for (int c = column0; c < column1; c += 32) {
+                    float    o[32];
+                    uint32_t mine[32], other[32];
+                    if (tiles > 0 && (seg.pair || join || group == 0)) {
+                        ptx::tmem_ld_x32(o_tmem + c, mine);
+                        if (join)
+                            ptx::tmem_ld_x32(tmem + kO + (group ^ 1) * 128 + lanes + c, other);
+                        ptx::tmem_wait_ld();
+#pragma unroll
+                        for (int k = 0; k < 32; ++k) {
+                            asm volatile("" : "+r"(mine[k]));
+                            o[k] = __uint_as_float(mine[k]) * keep[0];
+                            if (join) {
+                                asm volatile("" : "+r"(other[k]));
+                                o[k] = fmaf(__uint_as_float(other[k]), keep[1], o[k]);
+                            }
+                        }
+                    }
+                    else if (!seg.pair) {  // one tile of keys in all: group 0 multiplied it
+                        ptx::tmem_ld_x32(tmem + kO + lanes + c, other);
+                        ptx::tmem_wait_ld();
+#pragma unroll
+                        for (int k = 0; k < 32; ++k) {
+                            asm volatile("" : "+r"(other[k]));
+                            o[k] = __uint_as_float(other[k]);
+                        }
+                    }
+                    else {
+#pragma unroll
+                        for (int k = 0; k < 32; ++k)
+                            o[k] = 0.0f;
+                    }
+                    if (any)
+                        attn_add_not_finite<HEAD_DIM>(p, seg, row, list, c, o);
+                    if (valid && whole) {
+#pragma unroll
+                        for (int k = 0; k < 32; k += 8) {
+                            uint32_t w[4];
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) {  // a row that sees no key: what its sums hold are zeros
+                                const half2 h = __floats2half2_rn(o[k + 2 * e] * inverse, o[k + 2 * e + 1] * inverse);
+                                w[e]          = *reinterpret_cast<const uint32_t*>(&h);
+                            }
+                            *reinterpret_cast<uint4*>(out + c + k) = make_uint4(w[0], w[1], w[2], w[3]);
+                        }
+                    }
+                    else if (valid) {
+#pragma unroll
+                        for (int k = 0; k < 32; k += 4)
+                            sums[(c + k) / 4 * kAttnRows] = make_float4(o[k], o[k + 1], o[k + 2], o[k + 3]);
+                    }
+                    __syncwarp();
+                }
+                if (!whole && valid && column0 == 0)
+                    reinterpret_cast<float2*>(p.workspace + attn_stats_offset(gridDim.x))[static_cast<size_t>(2 * blockIdx.x + slot) * kAttnItemRows
+                                                                                          + tile_row * kAttnRows + thread] =
+                        make_float2(top * factor, sum);
+            }
+            if (kind != kPartNone) {
+                written[slot] = true;
+                if (threadIdx.x == 0)
+                    parts[slot] = AttnPart{ok ? kind : kPartNone, seg.first, seg.row0, seg.rows, seg.head, {0, 0, 0}};
+            }
+            // The barrier before the next segment: both groups are done with both outputs, with Q, and with the joined sums' room.
+            ptx::tc_fence_before_sync();
+        }
+        if (threadIdx.x == 0) {
+            for (int slot = 0; slot < 2; ++slot)
+                if (!written[slot])
+                    parts[slot].kind = kPartNone;
         }
     }
-    const float inverse = sum == 0.0f ? 0.0f : 1.0f / sum;
+    else if (warp == kAttnMmaWarp) {
+        // ================================================================ products: one thread issues them all
+        if (lane == 0) {
+            const uint32_t idesc_s = ptx::umma_idesc_f16_f32(kAttnRows, kAttnKeys);
+            const uint32_t idesc_o = ptx::umma_idesc_f16_f32(kAttnRows, HEAD_DIM) | ptx::kUmmaBNMajor;
+            uint32_t       loaded  = 0;  // tiles of keys before this segment
+            uint32_t       q_parity[2] = {0, 0}, p_parity[2] = {0, 0};
+            bool           ok = true;
+            const AttnSegment* current = nullptr;
+            auto               scores  = [&](int group, int tile, bool last_user) {
+                const AttnSegment& seg = *current;
+                const uint32_t     n = loaded + static_cast<uint32_t>(tile - seg.begin), stage = n % kStages;
+                if (!attn_wait(&sh.k_full[stage], n / kStages & 1u, sh, status))
+                    return false;
+                ptx::tc_fence_after_sync();
+                const uint64_t q = ptx::umma_desc_kmajor_sw128(q_base + (seg.pair ? group * kTileBytes : 0));
+                const uint64_t k = ptx::umma_desc_kmajor_sw128(k_base + stage * kTileBytes);
 #pragma unroll
-    for (int k = 0; k < kPairs; ++k)
-        out[lane + 32 * k] = sum == 0.0f ? __floats2half2_rn(0.0f, 0.0f) : __floats2half2_rn(o[k].x * inverse, o[k].y * inverse);
+                for (int step = 0; step < HEAD_DIM / 16; ++step) {
+                    const uint64_t at = (step / 4) * (kBlock >> 4) + (step % 4) * 2;
+                    ptx::umma_f16_ss(tmem + kS + group * 128, q + at, k + at, idesc_s, step > 0);
+                }
+                if (last_user)
+                    ptx::umma_commit(ptx::smem_u32(&sh.k_empty[stage]));
+                ptx::umma_commit(ptx::smem_u32(&sh.s_full[group]));
+                return true;
+            };
+            for (int number = 0; ok && (current = attn_segment(sh, number, status)) != nullptr; ++number) {
+                const AttnSegment& seg      = *current;
+                const int          tiles[2] = {seg.count_of(0), seg.count_of(1)};
+                for (int group = 0; ok && group < 2; ++group) {
+                    if (seg.pair || group == 0) {
+                        ok = attn_wait(&sh.q_full[group], q_parity[group], sh, status);
+                        q_parity[group] ^= 1u;
+                    }
+                    if (ok && tiles[group] > 0)
+                        ok = scores(group, seg.tile(group, 0), !seg.pair || group == 1);
+                }
+                const int most = max(tiles[0], tiles[1]);
+                for (int i = 0; ok && i < most; ++i)
+                    for (int group = 0; ok && group < 2; ++group) {
+                        if (i >= tiles[group])
+                            continue;
+                        const uint32_t n = loaded + static_cast<uint32_t>(seg.tile(group, i) - seg.begin), stage = n % kStages;
+                        ok = attn_wait(&sh.v_clean[stage], n / kStages & 1u, sh, status)
+                             && attn_wait(&sh.p_full[group], p_parity[group], sh, status);
+                        p_parity[group] ^= 1u;
+                        if (!ok)
+                            break;
+                        ptx::tc_fence_after_sync();
+                        const uint64_t v = ptx::umma_desc_nmajor_sw128(v_base + stage * kTileBytes, kBlock);
+#pragma unroll
+                        for (int step = 0; step < kAttnKeys / 16; ++step)
+                            ptx::umma_f16_ts(tmem + kO + group * 128, tmem + kS + group * 128 + step * 8, v + step * (2048 >> 4), idesc_o,
+                                             i > 0 || step > 0);
+                        if (!seg.pair || group == 1)
+                            ptx::umma_commit(ptx::smem_u32(&sh.v_empty[stage]));
+                        ptx::umma_commit(ptx::smem_u32(&sh.o_done[group]));
+                        if (i + 1 < tiles[group])
+                            ok = scores(group, seg.tile(group, i + 1), !seg.pair || group == 1);
+                    }
+                loaded += seg.end - seg.begin;
+            }
+        }
+        __syncwarp();
+    }
+    else if (warp == kAttnLoadWarp) {
+        // ================================================================ tiles of keys and values, one tensor copy per page and 64 columns
+        const CacheBatch& c        = p.batch;
+        const int         page     = 1 << c.page_shift;
+        const int         box      = min(page, kAttnKeys);  // rows of a copy
+        const int         pieces   = kAttnKeys / box;
+        const int         piece    = lane / kBlocks, block = lane % kBlocks;
+        const bool        active   = piece < pieces;
+        const uint32_t    offset   = block * kBlock + piece * box * 128;
+        AttnCursor        cursor(p, sh);
+        const AttnSegment& seg     = cursor.seg;
+        uint32_t          n        = 0;
+        bool              ok       = true;
+        for (int number = 0; ok; ++number) {
+            cursor.next(p);
+            if (lane == 0) {
+                sh.segment[number % kAttnSegments] = seg;
+                ptx::mbar_arrive(ptx::smem_u32(&sh.segment_full[number % kAttnSegments]));
+            }
+            if (seg.end == 0)
+                break;
+            const int* table = c.page_table + static_cast<long long>(seg.b) * c.table_width;
+            for (int t = seg.begin; ok && t < seg.end; ++t, ++n) {
+                const int key   = t * kAttnKeys + piece * box;
+                int       z     = c.pages * c.kv_heads;  // behind the cache: reads as zeros
+                if (active && key < seg.keys) {
+                    const int id = table[key >> c.page_shift];
+                    if (static_cast<unsigned>(id) < static_cast<unsigned>(c.pages))
+                        z = id * c.kv_heads + seg.head;
+                    else
+                        atomicOr(status, kStatusBadCache);
+                }
+                const uint32_t stage = n % kStages, parity = (n / kStages & 1u) ^ 1u;
+                for (int which = 0; which < 2; ++which) {
+                    ok = attn_wait(which ? &sh.v_empty[stage] : &sh.k_empty[stage], parity, sh, status);
+                    if (!__all_sync(0xffffffffu, ok)) {
+                        ok = false;
+                        break;
+                    }
+                    const uint32_t bar = ptx::smem_u32(which ? &sh.v_full[stage] : &sh.k_full[stage]);
+                    if (lane == 0)
+                        ptx::mbar_arrive_expect_tx(bar, kTileBytes);
+                    __syncwarp();
+                    if (active)
+                        ptx::tma_load_3d((which ? v_base : k_base) + stage * kTileBytes + offset, which ? &map_v : &map_k, block * 64,
+                                         key & (page - 1), z, bar);
+                }
+            }
+        }
+    }
+    else {
+        // ================================================================ values that no product may see: behind the last key, not finite
+        const int t64  = threadIdx.x - kAttnCleanWarp * 32;
+        uint32_t  n    = 0;
+        bool      ok   = true;
+        for (int number = 0;; ++number) {
+            const AttnSegment* const current = attn_segment(sh, number, status);
+            uint32_t(&list)[3][4] = sh.not_finite[number % kAttnSegments];
+            if (t64 < 12)
+                (&list[0][0])[t64] = 0u;
+            if (ptx::named_barrier_any(4, 64, current == nullptr || !ok))  // all or none
+                break;
+            const AttnSegment& seg  = *current;
+            const int          open = seg.open[0];
+            for (int t = seg.begin; t < seg.end; ++t, ++n) {
+                const uint32_t stage = n % kStages;
+                ok                   = attn_wait(&sh.v_full[stage], n / kStages & 1u, sh, status);
+                if (!ok)
+                    break;
+                if ((t + 1) * kAttnKeys > open) {
+                    for (int r = t64; r < kAttnKeys; r += 64) {
+                        const int key = t * kAttnKeys + r;
+                        uint4*    v   = reinterpret_cast<uint4*>(smem + (2 + kStages) * kTileBytes + stage * kTileBytes + r * 128);
+                        bool      bad = false;
+                        for (int x = 0; x < HEAD_DIM / 8; ++x) {
+                            uint4& at = v[(x / 8) * (kBlock / 16) + ((x + r) & 7)];  // any order of chunks: banks
+                            uint4  w  = key < seg.keys ? at : make_uint4(0, 0, 0, 0);
+                            auto   spoilt = [](uint32_t u) { return ((u & 0x7fff7fffu) + 0x04000400u) & 0x80008000u; };
+                            if (key >= seg.keys)
+                                at = w;
+                            else if (spoilt(w.x) | spoilt(w.y) | spoilt(w.z) | spoilt(w.w)) {
+                                bad        = true;
+                                auto clean = [&](uint32_t u) {
+                                    return (half_not_finite(u) ? 0u : u & 0xffffu) | (half_not_finite(u >> 16) ? 0u : u & 0xffff0000u);
+                                };
+                                at = make_uint4(clean(w.x), clean(w.y), clean(w.z), clean(w.w));
+                            }
+                        }
+                        if (bad && seg.tiles - 1 - t < 3)
+                            atomicOr(&list[seg.tiles - 1 - t][r / 32], 1u << r % 32);
+                    }
+                    ptx::fence_proxy_async_smem();
+                }
+                ptx::mbar_arrive(ptx::smem_u32(&sh.v_clean[stage]));
+            }
+        }
+    }
+
+    if (sh.abort_flag) {  // copies and products already issued get a bounded chance to end before the CTA may exit
+        const uint64_t t0 = ptx::globaltimer_ns();
+        while (ptx::globaltimer_ns() - t0 < 2000000ull) {}
+    }
+    ptx::tc_fence_before_sync();
+    __syncthreads();
+    if (warp == kAttnMmaWarp)
+        ptx::tmem_dealloc(tmem, kAttnTmemCols);
+}
+
+// Adds up the parts of the item that CTA blockIdx.x of the attention ended but did not begin, in key order, for 32 rows and all
+// columns of it.
+template<int HEAD_DIM>
+__global__ void __launch_bounds__(256) attention_join_kernel(const AttentionParams p, int ctas)
+{
+    ptx::grid_dependency_wait();
+    ptx::grid_launch_dependents();
+    const AttnPart* const parts = reinterpret_cast<const AttnPart*>(p.workspace);
+    const float2* const   stats = reinterpret_cast<const float2*>(p.workspace + attn_stats_offset(ctas));
+    const float4* const   sums  = reinterpret_cast<const float4*>(p.workspace + attn_sums_offset(ctas));
+    const int             cta = blockIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const AttnPart        last = parts[2 * cta];
+    const int             row  = blockIdx.y * 32 + lane;  // of the item
+    if (last.kind != kPartEnds || static_cast<int>(blockIdx.y) * 32 >= last.rows)
+        return;
+    // The CTA whose segment began the item.
+    int begin = cta - 1;
+    while (begin >= 0 && parts[2 * begin].kind == kPartContinues)
+        --begin;
+    if (begin < 0 || parts[2 * begin + 1].kind != kPartBegins)
+        return;  // a CTA gave up
+    auto  slot = [&](int c) { return static_cast<size_t>(2 * c + (c == begin ? 1 : 0)); };
+    float top  = -CUDART_INF_F;
+    for (int c = begin; c <= cta; ++c)
+        top = fmaxf(top, stats[slot(c) * kAttnItemRows + row].x);
+    constexpr int kPer = HEAD_DIM / 4 / 8;  // float4 columns of a warp
+    float4        o[kPer];
+    float         sum = 0.0f;
+#pragma unroll
+    for (int k = 0; k < kPer; ++k)
+        o[k] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    for (int c = begin; c <= cta; ++c) {
+        const float2 stat = stats[slot(c) * kAttnItemRows + row];
+        const float  keep = stat.x == top ? 1.0f : ptx::exp2_approx(stat.x - top);
+        sum += stat.y * keep;
+        const float4* src = sums + ((slot(c) * 2 + row / kAttnRows) * (HEAD_DIM / 4) + warp * kPer) * kAttnRows + row % kAttnRows;
+#pragma unroll
+        for (int k = 0; k < kPer; ++k) {
+            const float4 v = src[k * kAttnRows];
+            o[k].x         = fmaf(v.x, keep, o[k].x);
+            o[k].y         = fmaf(v.y, keep, o[k].y);
+            o[k].z         = fmaf(v.z, keep, o[k].z);
+            o[k].w         = fmaf(v.w, keep, o[k].w);
+        }
+    }
+    if (row >= last.rows)
+        return;
+    const float inverse = sum == 0.0f ? 0.0f : 1.0f / sum;
+    const int   r       = last.row0 + row;
+    half* out = p.out + (static_cast<long long>(last.first + r / p.share) * p.heads + last.head * p.share + r % p.share) * HEAD_DIM
+                + warp * kPer * 4;
+#pragma unroll
+    for (int k = 0; k < kPer; ++k) {
+        const half2 a = __floats2half2_rn(o[k].x * inverse, o[k].y * inverse), b = __floats2half2_rn(o[k].z * inverse, o[k].w * inverse);
+        *reinterpret_cast<uint2*>(out + 4 * k) = make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b));
+    }
 }
 
 }  // namespace flashllm

@@ -36,8 +36,9 @@ struct CacheBatch {
 // Sequence b's rows and first position, made to fit the batch and the page table whatever the arrays hold.
 struct Sequence {
     int first;    // first row
-    int count;    // rows
+    int count;    // rows; 0 for a sequence that does not fit
     int context;  // position of the first row
+    int lost;     // rows of a sequence that does not fit
 };
 
 __device__ __forceinline__ long long table_positions(const CacheBatch& c)
@@ -52,9 +53,11 @@ __device__ __forceinline__ Sequence load_sequence(const CacheBatch& c, int b)
     s.first   = min(max(begin, 0), c.tokens);
     s.count   = min(max(end, s.first), c.tokens) - s.first;
     s.context = context;
+    s.lost    = 0;
     if (context < 0 || static_cast<long long>(context) + s.count > table_positions(c)) {
         if (s.count > 0)
             atomicOr(c.status, kStatusBadCache);
+        s.lost    = s.count;
         s.count   = 0;
         s.context = 0;
     }

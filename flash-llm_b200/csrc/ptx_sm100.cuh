@@ -216,6 +216,20 @@ umma_f16_ss(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, u
         : "memory");
 }
 
+// D[tmem] (+)= A[tmem] * B[smem]: A holds fp16 pairs, one row per lane, two neighbouring K elements per column.
+__device__ __forceinline__ void
+umma_f16_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc, uint32_t accumulate)
+{
+    asm volatile(
+        "{\n"
+        ".reg .pred p;\n"
+        "setp.ne.b32 p, %4, 0;\n"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n"
+        "}\n" ::"r"(d_tmem),
+        "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+
 // One 128x64 tile of A times one [N x 64] slab of B: the four K=16 MMAs, the commit that hands the A stage back, an
 // optional second commit (B batch finished), and -- issued first so that its shared-memory round trip overlaps the
 // MMA issue -- a probe of the barriers the NEXT tile needs.  All in one asm block because the probe's predicate must
@@ -322,6 +336,21 @@ __device__ __forceinline__ void tmem_ld_x8(uint32_t taddr, uint32_t (&r)[8])
                  : "memory");
 }
 
+// ... 32 consecutive columns.
+__device__ __forceinline__ void tmem_ld_x32(uint32_t taddr, uint32_t* r)
+{
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+                 "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]),
+                   "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]),
+                   "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]),
+                   "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
+                   "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]),
+                   "=r"(r[30]), "=r"(r[31])
+                 : "r"(taddr)
+                 : "memory");
+}
+
 __device__ __forceinline__ void tmem_wait_ld()
 {
     asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
@@ -333,6 +362,30 @@ __device__ __forceinline__ void tmem_st_x8(uint32_t taddr, const float (&v)[8])
     asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"r"(taddr),
                  "r"(__float_as_uint(v[0])), "r"(__float_as_uint(v[1])), "r"(__float_as_uint(v[2])), "r"(__float_as_uint(v[3])),
                  "r"(__float_as_uint(v[4])), "r"(__float_as_uint(v[5])), "r"(__float_as_uint(v[6])), "r"(__float_as_uint(v[7]))
+                 : "memory");
+}
+
+// ... 16 columns of raw words.
+__device__ __forceinline__ void tmem_st_x16(uint32_t taddr, const uint32_t* r)
+{
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+                 "%16};" ::"r"(taddr),
+                 "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+                 "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+                 : "memory");
+}
+
+// ... 32 columns of raw words.
+__device__ __forceinline__ void tmem_st_x32(uint32_t taddr, const uint32_t* r)
+{
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, "
+                 "%17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};" ::"r"(taddr),
+                 "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]),
+                 "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]),
+                 "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]),
+                 "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]),
+                 "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]),
+                 "r"(r[30]), "r"(r[31])
                  : "memory");
 }
 
@@ -354,6 +407,22 @@ __device__ __forceinline__ uint64_t umma_desc_kmajor_sw128(uint32_t addr)
     d |= static_cast<uint64_t>(2) << 61;                 // layout: 128-byte swizzle
     return d;
 }
+
+// ... of a B operand that lies N-major: rows of 64 fp16 along N (128 bytes, the 128-byte swizzle in groups of 8 rows), one row
+// per K; `addr` plus 2048 bytes per 16-wide K step, the next 64 columns of N `block_bytes` further on.
+__device__ __forceinline__ uint64_t umma_desc_nmajor_sw128(uint32_t addr, uint32_t block_bytes)
+{
+    uint64_t d = 0;
+    d |= static_cast<uint64_t>((addr & 0x3FFFFu) >> 4);
+    d |= static_cast<uint64_t>(block_bytes >> 4) << 16;  // leading byte offset: next 64 columns
+    d |= static_cast<uint64_t>(1024 >> 4) << 32;         // stride byte offset: next 8 rows of K
+    d |= static_cast<uint64_t>(1) << 46;
+    d |= static_cast<uint64_t>(2) << 61;
+    return d;
+}
+
+// Bit of the instruction descriptor that says so.
+constexpr uint32_t kUmmaBNMajor = 1u << 16;
 
 // Instruction descriptor for kind::f16: fp16 A and B (both K-major), fp32 D, M x N tile.
 __device__ __forceinline__ uint32_t umma_idesc_f16_f32(uint32_t m, uint32_t n)
@@ -454,9 +523,55 @@ __device__ __forceinline__ float4 ld_dsmem_v4_f32(uint32_t addr)
     return v;
 }
 
+// 2^x within 2^-22 of itself; subnormal results are zero.
+__device__ __forceinline__ float exp2_approx(float x)
+{
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+// 1/x within 1 ulp.
+__device__ __forceinline__ float rcp_approx(float x)
+{
+    float y;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
 __device__ __forceinline__ void named_barrier_sync(uint32_t id, uint32_t threads)
 {
     asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory");
+}
+
+// ... which tells all of them whether any of them said so.
+__device__ __forceinline__ bool named_barrier_any(uint32_t id, uint32_t threads, bool mine)
+{
+    uint32_t any;
+    asm volatile(
+        "{\n"
+        ".reg .pred p, q;\n"
+        "setp.ne.u32 p, %3, 0;\n"
+        "barrier.cta.red.or.pred q, %1, %2, p;\n"
+        "selp.u32 %0, 1, 0, q;\n"
+        "}\n"
+        : "=r"(any)
+        : "r"(id), "r"(threads), "r"(mine ? 1u : 0u)
+        : "memory");
+    return any != 0;
+}
+
+// Moves registers between the warpgroups of a CTA: the sum must stay within what the CTA was launched with.
+template<int REGISTERS>
+__device__ __forceinline__ void take_registers()
+{
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(REGISTERS));
+}
+
+template<int REGISTERS>
+__device__ __forceinline__ void give_registers()
+{
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(REGISTERS));
 }
 
 }  // namespace ptx
