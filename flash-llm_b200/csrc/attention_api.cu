@@ -93,10 +93,14 @@ static cudaError_t multiprocessors(int* count)
     if (*count > 0)
         return cudaSuccess;
     err = cudaDeviceGetAttribute(count, cudaDevAttrMultiProcessorCount, device);
-    if (err == cudaSuccess)
-        err = cudaFuncSetAttribute(attention_kernel<64>, cudaFuncAttributeMaxDynamicSharedMemorySize, attn_smem_bytes(64));
-    if (err == cudaSuccess)
-        err = cudaFuncSetAttribute(attention_kernel<128>, cudaFuncAttributeMaxDynamicSharedMemorySize, attn_smem_bytes(128));
+    auto raise = [&](auto kernel, int bytes) {
+        if (err == cudaSuccess)
+            err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    };
+    raise(attention_kernel<64, true>, attn_smem_bytes(64));
+    raise(attention_kernel<64, false>, attn_smem_bytes(64));
+    raise(attention_kernel<128, true>, attn_smem_bytes(128));
+    raise(attention_kernel<128, false>, attn_smem_bytes(128));
     if (err == cudaSuccess)
         known[device].store(*count, std::memory_order_release);
     return err;
@@ -129,7 +133,8 @@ static cudaError_t launch_attention(cudaStream_t stream, const AttentionParams& 
     CUtensorMap map_k, map_v;
     if (!encode_cache(&map_k, p.k_cache, p.batch, HEAD_DIM) || !encode_cache(&map_v, p.v_cache, p.batch, HEAD_DIM))
         return cudaErrorInvalidValue;
-    err = launch_in_stream_order(attention_kernel<HEAD_DIM>, dim3(sms), dim3(kAttnThreads), attn_smem_bytes(HEAD_DIM), stream, 1, map_k,
+    const bool plain = p.cap == 0.0f && p.slopes == nullptr;
+    err = launch_in_stream_order(plain ? attention_kernel<HEAD_DIM, true> : attention_kernel<HEAD_DIM, false>, dim3(sms), dim3(kAttnThreads), attn_smem_bytes(HEAD_DIM), stream, 1, map_k,
                                  map_v, p);
     if (err != cudaSuccess)
         return err;

@@ -13,7 +13,9 @@
 //
 // An item is 256 such rows of one sequence and one key/value head.  Its two tiles of rows are two groups of softmax warps that
 // take turns on the tensor core; an item of at most 128 rows (single tokens, drafted trees) is the same tile for both groups,
-// each takes every other tile of keys, and the two results are joined at the end.  The work of a call is the linear sequence
+// each takes every other tile of keys, and the two results are joined at the end.  An item of at most 32 rows, which would leave
+// one warp of four with all the work, lies in the tile four times: every warp has all rows and a quarter of the tile's keys
+// (weights of zero for the others), and the joined results are eight.  The work of a call is the linear sequence
 // of all items' tiles of keys, dealt out evenly over one CTA per SM whatever the sequences' lengths; an item that is cut leaves
 // partial sums in the workspace, which attention_join_kernel adds up in key order.
 #pragma once
@@ -50,6 +52,8 @@ constexpr int kAttnLoadWarp  = 9;
 constexpr int kAttnCleanWarp = 10;  // and 11
 constexpr int kAttnThreads   = 12 * 32;
 constexpr int kAttnTmemCols  = 512;
+constexpr int kAttnFewRows   = 32;
+constexpr int kAttnKnown     = 512;  // sequences whose sizes are kept in shared memory from the plan on
 constexpr int kAttnSegments  = 8;  // segments that shared memory holds at a time
 // Registers of a thread: the softmax warps keep a row of 128 scores, 256 x 208 + 128 x 88 = 384 x 168.
 constexpr int kAttnSoftmaxRegisters = 208, kAttnOtherRegisters = 88;
@@ -81,6 +85,7 @@ struct AttnSegment {
     int  end;      // behind its last; 0: no more segments
     int  tiles0;   // pair: tiles of keys that the first tile of rows needs
     bool pair;     // two tiles of rows; otherwise both groups share the one
+    bool fourfold;  // at most 32 rows: four copies of them in the tile
 
     // Tiles of keys that a group goes through, and the i-th of them.
     __device__ __forceinline__ int count_of(int group) const
@@ -98,7 +103,7 @@ struct AttnSegment {
 // Dynamic shared memory: two tiles of Q, the stages, and what AttnShared holds.
 struct AttnShared {
     unsigned long long k_full[4], k_empty[4], v_full[4], v_clean[4], v_empty[4];
-    unsigned long long s_full[2], p_full[2], o_done[2], q_full[2], segment_full[kAttnSegments];
+    unsigned long long s_full[2], p_full[2][2], o_done[2], q_full[2], segment_full[kAttnSegments];
     uint32_t           tmem;
     volatile uint32_t  abort_flag;
     int                start_sequence, start_rows, start_head, start_tile;
@@ -111,6 +116,7 @@ struct AttnShared {
     uint32_t           not_finite[kAttnSegments][3][4];  // keys of an item's last three tiles whose values are not finite
     int                drafted[2][kMaxDrafted];          // positions of drafted tokens, by group
     unsigned int       tiles[kMaxSequences];             // of all items of a sequence's first key/value head
+    int4               known[kAttnKnown];                // first row, rows, context and prefix of the first sequences
 };
 
 __host__ __device__ constexpr int attn_smem_bytes(int head_dim)
@@ -189,6 +195,15 @@ __device__ __forceinline__ AttnSequence attn_sequence(const AttentionParams& p, 
     return a;
 }
 
+// ... what the plan has kept of it.
+__device__ __forceinline__ AttnSequence attn_sequence(const AttentionParams& p, const AttnShared& sh, int b)
+{
+    if (b >= kAttnKnown)
+        return attn_sequence(p, b);
+    const int4 known = sh.known[b];
+    return AttnSequence{{known.x, known.y, known.z, 0}, known.w, known.y * p.share};
+}
+
 // Keys that rows before `row_end` (of the sequence's rows) see at most: no row sees the key of that index or one behind it.
 __device__ __forceinline__ int attn_keys(const AttentionParams& p, const AttnSequence& a, int row_end)
 {
@@ -220,20 +235,21 @@ struct AttnCursor {
         const int end  = min(seg.row0 + kAttnItemRows, a.rows);
         seg.rows       = end - seg.row0;
         seg.pair       = seg.rows > kAttnRows;
+        seg.fourfold   = seg.rows <= kAttnFewRows;
         seg.keys       = attn_keys(p, a, end);
         seg.tiles      = attn_tiles(seg.keys);
         seg.tiles0     = seg.pair ? attn_tiles(attn_keys(p, a, seg.row0 + kAttnRows)) : seg.tiles;
         seg.open[0]    = attn_open_keys(p, a, seg.row0);
         seg.open[1]    = seg.pair ? attn_open_keys(p, a, seg.row0 + kAttnRows) : seg.open[0];
     }
-    __device__ __forceinline__ void enter_sequence(const AttentionParams& p)
+    __device__ __forceinline__ void enter_sequence(const AttentionParams& p, const AttnShared& sh)
     {
         for (;; ++seg.b) {
             if (seg.b >= p.batch.sequences) {  // only if somebody writes the arrays during the call
                 left = 0;
                 return;
             }
-            a = attn_sequence(p, seg.b);
+            a = attn_sequence(p, sh, seg.b);
             if (a.rows > 0)
                 break;
         }
@@ -251,10 +267,10 @@ struct AttnCursor {
         seg.head  = sh.start_head;
         next_tile = sh.start_tile;
         if (left > 0)
-            enter_sequence(p);
+            enter_sequence(p, sh);
     }
     // The next segment; its `end` is 0 at the end of the share.
-    __device__ __forceinline__ void next(const AttentionParams& p)
+    __device__ __forceinline__ void next(const AttentionParams& p, const AttnShared& sh)
     {
         if (left > 0 && next_tile >= seg.tiles) {
             next_tile = 0;
@@ -264,7 +280,7 @@ struct AttnCursor {
                 if (seg.row0 >= a.rows) {
                     seg.row0 = 0;
                     ++seg.b;
-                    enter_sequence(p);
+                    enter_sequence(p, sh);
                 }
                 else
                     enter_rows(p);
@@ -295,6 +311,8 @@ __device__ __forceinline__ void attn_plan(const AttentionParams& p, AttnShared& 
     const int B = p.batch.sequences, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     for (int b = threadIdx.x; b < B; b += kAttnThreads) {
         const AttnSequence a = attn_sequence(p, b);
+        if (b < kAttnKnown)
+            sh.known[b] = make_int4(a.s.first, a.s.count, a.s.context, a.prefix);
         sh.tiles[b]          = a.s.lost > 0            ? kAttnLostRows
                                : a.rows == 0            ? 0u
                                : a.rows > kAttnItemRows ? kAttnSeveralItems
@@ -352,7 +370,7 @@ __device__ __forceinline__ void attn_plan(const AttentionParams& p, AttnShared& 
                 }
                 before += __shfl_sync(0xffffffffu, upto, 31);
             }
-            const AttnSequence a = attn_sequence(p, b);
+            const AttnSequence a = attn_sequence(p, sh, b);
             for (long long base = 0;; base += 32 * kAttnItemRows) {  // ... and of its items the first
                 const long long r    = base + lane * kAttnItemRows;
                 long long       mine = 0;
@@ -438,6 +456,12 @@ __device__ __forceinline__ AttnRow attn_row(const AttentionParams& p, const Attn
 
 // ---------------------------------------------------------------- the kernel
 
+// Where 16 bytes of a row lie in a tile in shared memory: blocks of 64 columns, the 128-byte swizzle.
+__device__ __forceinline__ int attn_chunk(int row, int chunk)
+{
+    return chunk / 8 * (kAttnKeys * 128) + row * 128 + ((chunk % 8 ^ (row & 7)) << 4);
+}
+
 __device__ __forceinline__ bool half_not_finite(uint32_t h)
 {
     return (h & 0x7c00u) == 0x7c00u;
@@ -445,9 +469,9 @@ __device__ __forceinline__ bool half_not_finite(uint32_t h)
 
 // Adds to o[c], element column + c of a row's output, the values that are not finite of keys that the row sees (the products
 // took zeros in their place: a weight of zero times infinity is not zero).
-template<int HEAD_DIM>
+template<int HEAD_DIM, int COLUMNS>
 __device__ __forceinline__ void attn_add_not_finite(const AttentionParams& p, const AttnSegment& seg, const AttnRow& row,
-                                                    const uint32_t (&list)[3][4], int column, float (&o)[32])
+                                                    const uint32_t (&list)[3][4], int column, float (&o)[COLUMNS])
 {
 #pragma unroll 1
     for (int i = 0; i < 12; ++i)
@@ -461,13 +485,182 @@ __device__ __forceinline__ void attn_add_not_finite(const AttentionParams& p, co
                 continue;
             const half* v = p.v_cache + at * HEAD_DIM + column;
 #pragma unroll
-            for (int c = 0; c < 32; ++c)
+            for (int c = 0; c < COLUMNS; ++c)
                 if (half_not_finite(__half_as_ushort(v[c])))
                     o[c] += __half2float(v[c]);
         }
 }
 
-template<int HEAD_DIM>
+// What a softmax thread keeps of its row from tile to tile, and what the transformation of its scores takes.
+struct AttnState {
+    float top, sum;      // the maximum that weights are taken against (of q.k, or of scores times log2 e), their sum
+    float factor;        // what turns the scores at hand into powers of two
+    float scale, cap;    // of scores in units of log 2; cap 0: none
+    float slope;         // likewise
+    int   place;         // the row's position
+    const int* drafted;  // positions of drafted tokens in shared memory, or nullptr
+    bool  valid;         // the row is somebody's
+};
+
+// tanh on [-1, 1] to 2.4e-7: x times a polynomial in x^2, fitted to it for the smallest largest error.
+__device__ __forceinline__ float2 attn_tanh_small(float2 x)
+{
+    const float2 y = ptx::mul_x2(x, x);
+    float2       t = make_float2(-0.002839469350874424f, -0.002839469350874424f);
+    t              = ptx::fma_x2(t, y, make_float2(0.016114192083477974f, 0.016114192083477974f));
+    t              = ptx::fma_x2(t, y, make_float2(-0.05097287520766258f, -0.05097287520766258f));
+    t              = ptx::fma_x2(t, y, make_float2(0.13253526389598846f, 0.13253526389598846f));
+    t              = ptx::fma_x2(t, y, make_float2(-0.3332400321960449f, -0.3332400321960449f));
+    t              = ptx::fma_x2(t, y, make_float2(0.9999968409538269f, 0.9999968409538269f));
+    return ptx::mul_x2(x, t);
+}
+
+// One tile of scores of one row, columns `column` up to column + COLUMNS of 128: from tensor memory to weights there.  The tile's
+// first key is `key0`; keys before `open` are seen by all rows.  `rescale(keep)` multiplies the row's output by `keep`, and is
+// called by whole warps.  `part_done(half)` tells that the weights of that half of the tile are in place.
+template<bool PLAIN, int COLUMNS, typename Rescale, typename PartDone>
+__device__ __forceinline__ void attn_softmax(AttnState& st, const AttnRow& row, uint32_t s_tmem, int column, int key0, int open,
+                                             bool first, Rescale&& rescale, PartDone&& part_done)
+{
+    float s[COLUMNS];
+    {
+        uint32_t(&raw)[COLUMNS] = reinterpret_cast<uint32_t(&)[COLUMNS]>(s);
+#pragma unroll
+        for (int c = 0; c < COLUMNS; c += 32)
+            ptx::tmem_ld_x32(s_tmem + column + c, raw + c);
+        ptx::tmem_wait_ld();
+#pragma unroll
+        for (int c = 0; c < COLUMNS; ++c)
+            asm volatile("" : "+r"(raw[c]));  // not read before the wait
+    }
+    const bool masked = key0 + kAttnKeys > open;
+    if constexpr (!PLAIN) {
+        if (st.cap > 0.0f) {
+            // Scores are mostly small against the cap: then a polynomial, half the cost of two approximations by the special
+            // function unit, which the weights need too.
+            float2 largest = make_float2(0.0f, 0.0f);
+#pragma unroll
+            for (int c = 0; c < COLUMNS; c += 4) {
+                largest.x = ptx::max3_nan(largest.x, fabsf(s[c]), fabsf(s[c + 1]));
+                largest.y = ptx::max3_nan(largest.y, fabsf(s[c + 2]), fabsf(s[c + 3]));
+            }
+            const float in = st.scale / st.cap;  // the cap is in units of log 2, as the scale is
+            if (__all_sync(0xffffffffu, !st.valid || fmaxf(largest.x, largest.y) * in <= 1.0f)) {
+#pragma unroll
+                for (int c = 0; c < COLUMNS; c += 2) {
+                    const float2 t = ptx::mul_x2(attn_tanh_small(ptx::mul_x2(make_float2(s[c], s[c + 1]), make_float2(in, in))),
+                                                 make_float2(st.cap, st.cap));
+                    s[c]           = t.x;
+                    s[c + 1]       = t.y;
+                }
+            }
+            else {
+                const float twice = 2.0f * CUDART_L2E_F * in;  // tanh x = 1 - 2 / (1 + e^2x)
+#pragma unroll
+                for (int c = 0; c < COLUMNS; ++c)
+                    s[c] = fmaf(-2.0f * st.cap, ptx::rcp_approx(1.0f + ptx::exp2_approx(s[c] * twice)), st.cap);
+            }
+        }
+        else {
+#pragma unroll
+            for (int c = 0; c < COLUMNS; c += 2) {
+                const float2 t = ptx::mul_x2(make_float2(s[c], s[c + 1]), make_float2(st.scale, st.scale));
+                s[c]           = t.x;
+                s[c + 1]       = t.y;
+            }
+        }
+        if (st.drafted != nullptr && masked) {
+#pragma unroll
+            for (int c = 0; c < COLUMNS; ++c) {
+                const int key   = key0 + column + c, i = key - open;
+                const int where = i >= 0 && i < kMaxDrafted ? st.drafted[i] : key;
+                s[c]            = fmaf(st.slope, static_cast<float>(where - st.place), s[c]);
+            }
+        }
+        else {
+            const float  away  = st.slope * static_cast<float>(key0 + column - st.place);
+            const float2 slope = make_float2(st.slope, st.slope), base = make_float2(away, away);
+#pragma unroll
+            for (int c = 0; c < COLUMNS; c += 2) {
+                const float2 far = ptx::fma_x2(slope, make_float2(static_cast<float>(c), static_cast<float>(c + 1)), base);
+                const float2 t   = ptx::add_x2(make_float2(s[c], s[c + 1]), far);
+                s[c]             = t.x;
+                s[c + 1]         = t.y;
+            }
+        }
+    }
+    if (masked) {
+#pragma unroll
+        for (int k = 0; k < COLUMNS / 32; ++k) {
+            const uint32_t seen = row.word(key0 + column + 32 * k);
+#pragma unroll
+            for (int c = 0; c < 32; ++c)
+                s[32 * k + c] = seen >> c & 1u ? s[32 * k + c] : -CUDART_INF_F;
+        }
+    }
+    float m[4] = {s[0], s[1], s[2], s[3]};
+#pragma unroll
+    for (int c = 4; c < COLUMNS - 4; c += 8)
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+            m[k] = ptx::max3_nan(m[k], s[c + k], s[c + 4 + k]);
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+        m[k] = ptx::max3_nan(m[k], s[COLUMNS - 4 + k], m[k]);
+    float new_top = ptx::max3_nan(ptx::max3_nan(m[0], m[1], m[2]), m[3], st.top);
+    if (!(new_top < CUDART_INF_F)) {  // a score that is no number, or infinity less itself: neither has the row's output a number
+        st.sum  = CUDART_NAN_F;
+        new_top = st.top;
+    }
+    if (first)
+        st.top = new_top;
+    else if (__any_sync(0xffffffffu, st.valid && (new_top - st.top) * st.factor > 8.0f)) {  // rows of nobody have no say
+        // The maximum that the weights are taken against moves only when it has grown by more than 2^8, which 32-bit sums and
+        // fp16 weights have room for: rarely after the first tiles.
+        const float keep = new_top == st.top ? 1.0f : ptx::exp2_approx((st.top - new_top) * st.factor);
+        st.top           = new_top;
+        st.sum *= keep;
+        rescale(keep);
+    }
+    const float  minus   = st.top == -CUDART_INF_F ? 0.0f : -st.top * st.factor;
+    float2       part[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
+    if constexpr (COLUMNS < kAttnKeys) {  // the other copies' keys
+        const uint32_t zeros[16] = {0};
+#pragma unroll
+        for (int c = 0; c < kAttnKeys; c += 32)
+            if (c != column)
+                ptx::tmem_st_x16(s_tmem + c / 2, zeros);
+    }
+#pragma unroll
+    for (int c = 0; c < COLUMNS; c += 32) {
+        uint32_t w[16];
+#pragma unroll
+        for (int k = 0; k < 16; ++k) {
+            float2 x = make_float2(s[c + 2 * k], s[c + 2 * k + 1]);
+            if constexpr (PLAIN)
+                x = ptx::fma_x2(x, make_float2(st.factor, st.factor), make_float2(minus, minus));
+            else
+                x = ptx::add_x2(x, make_float2(minus, minus));
+            x             = make_float2(ptx::exp2_approx(x.x), ptx::exp2_approx(x.y));
+            part[k & 1]   = ptx::add_x2(part[k & 1], x);
+            const half2 h = __floats2half2_rn(x.x, x.y);
+            w[k]          = *reinterpret_cast<const uint32_t*>(&h);
+        }
+        ptx::tmem_st_x16(s_tmem + (column + c) / 2, w);
+        if (COLUMNS < kAttnKeys || c % 64 == 32) {
+            ptx::tmem_wait_st();
+            ptx::tc_fence_before_sync();
+            __syncwarp();
+            if (COLUMNS < kAttnKeys)
+                part_done(0);
+            part_done(COLUMNS < kAttnKeys ? 1 : c / 64);
+        }
+    }
+    st.sum += (part[0].x + part[1].x) + (part[0].y + part[1].y);
+}
+
+// PLAIN: neither cap nor slopes.
+template<int HEAD_DIM, bool PLAIN>
 __global__ void __launch_bounds__(kAttnThreads, 1)
 attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const AttentionParams p)
 {
@@ -475,6 +668,7 @@ attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
     constexpr int      kTileBytes = attn_tile_bytes(HEAD_DIM);
     constexpr int      kBlock     = kAttnKeys * 128;  // bytes of 64 columns of a tile
     constexpr int      kBlocks    = HEAD_DIM / 64;
+    constexpr int      kRowChunks = HEAD_DIM / 8;  // of 16 bytes in a row of Q or of the output
     constexpr uint32_t kS = 0, kO = 256;  // tensor memory: scores (weights in their first half) and outputs, 128 columns a group
     extern __shared__ unsigned char smem_raw[];
     const uint32_t raw  = ptx::smem_u32(smem_raw);
@@ -495,7 +689,8 @@ attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
         }
         for (int i = 0; i < 2; ++i) {
             ptx::mbar_init(ptx::smem_u32(&sh.s_full[i]), 1);
-            ptx::mbar_init(ptx::smem_u32(&sh.p_full[i]), 4);
+            ptx::mbar_init(ptx::smem_u32(&sh.p_full[i][0]), 4);
+            ptx::mbar_init(ptx::smem_u32(&sh.p_full[i][1]), 4);
             ptx::mbar_init(ptx::smem_u32(&sh.o_done[i]), 1);
             ptx::mbar_init(ptx::smem_u32(&sh.q_full[i]), 4);
         }
@@ -525,13 +720,10 @@ attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
 
     if (warp < kAttnMmaWarp) {
         // ================================================================ softmax: one thread per row
-        const int      group = warp >> 2, thread = threadIdx.x & 127;
-        const uint32_t lanes = static_cast<uint32_t>(warp & 3) << 21;  // this warp's lanes of tensor memory
-        const uint32_t s_tmem = tmem + kS + group * 128 + lanes, o_tmem = tmem + kO + group * 128 + lanes;
-        const bool     plain  = p.cap == 0.0f && p.slopes == nullptr;
-        const float    factor = plain ? p.scale * CUDART_L2E_F : 1.0f;  // scores times this are in units of log 2
-        const float    cap_in = p.cap > 0.0f ? 2.0f * CUDART_L2E_F * p.scale / p.cap : 0.0f;  // e^(2 s / cap) = 2^(cap_in q.k)
-        uint32_t       s_parity = 0, o_count = 0;  // phases of s_full, products of P and V so far
+        const int       group = warp >> 2, thread = threadIdx.x & 127;
+        const uint32_t  lanes = static_cast<uint32_t>(warp & 3) << 21;  // this warp's lanes of tensor memory
+        const uint32_t  s_tmem = tmem + kS + group * 128 + lanes, o_tmem = tmem + kO + group * 128 + lanes;
+        uint32_t        s_parity = 0, o_count = 0;  // phases of s_full, products of weights and values so far
         AttnPart* const parts = reinterpret_cast<AttnPart*>(p.workspace) + 2 * blockIdx.x;
         bool            ok = true, written[2] = {false, false};
         for (int number = 0;; ++number) {
@@ -540,263 +732,236 @@ attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
             if (ptx::named_barrier_any(1, 256, current == nullptr || !ok))
                 break;
             ptx::tc_fence_after_sync();
-            const AttnSegment& seg = *current;
-            const int  in_item = (seg.pair ? group * kAttnRows : 0) + thread;  // row of the item, and of the sequence
-            const int  row_id  = seg.row0 + in_item;
-            const bool valid   = in_item < seg.rows;
-            const bool busy    = (in_item & ~31) < seg.rows;  // the warp has a row
-            const int  token = valid ? row_id / p.share : 0, head = seg.head * p.share + (valid ? row_id % p.share : 0);
-            if (seg.pair || group == 0) {  // this group's tile of Q
-                const uint4* src = reinterpret_cast<const uint4*>(p.q + (seg.first + token) * p.ld_q + static_cast<long long>(head) * HEAD_DIM);
-                unsigned char* dst = smem + (seg.pair ? group * kTileBytes : 0) + thread * 128;
-                if (valid) {
+            const AttnSegment& seg     = *current;
+            const bool         pair = seg.pair, fourfold = seg.fourfold;
+            const int          in_item = pair ? group * kAttnRows + thread : fourfold ? lane : thread;  // row of the item
+            const int          row_id  = seg.row0 + in_item;                                          // ... of the sequence
+            const bool         valid   = in_item < seg.rows;
+            const bool         busy    = (in_item & ~31) < seg.rows;  // the warp has a row
+            const int          token   = valid ? row_id / p.share : 0;
+            const int          head    = seg.head * p.share + (valid ? row_id - token * p.share : 0);
+            const long long    in_row  = static_cast<long long>(head) * HEAD_DIM;
+            const AttnRow      row     = attn_row(p, seg, row_id, valid);
+            if (pair || group == 0) {  // this group's tile of Q: a warp's rows, whole rows at a time
+                const long long from = valid ? (seg.first + token) * p.ld_q + in_row : -1;
+                unsigned char*  dst  = smem + (pair ? group * kTileBytes : 0) + (thread & ~31) * 128;
+                uint4           v[kRowChunks];
 #pragma unroll
-                    for (int c = 0; c < HEAD_DIM / 8; ++c)
-                        *reinterpret_cast<uint4*>(dst + (c / 8) * kBlock + (((c % 8) ^ (thread & 7)) << 4)) = src[c];
+                for (int k = 0; k < kRowChunks; ++k) {
+                    const long long at = __shfl_sync(0xffffffffu, from, k * (32 / kRowChunks) + lane / kRowChunks);
+                    v[k]               = ptx::ldg_v4_if(p.q + at + lane % kRowChunks * 8, at >= 0);
                 }
+#pragma unroll
+                for (int k = 0; k < kRowChunks; ++k)
+                    *reinterpret_cast<uint4*>(dst + attn_chunk(k * (32 / kRowChunks) + lane / kRowChunks, lane % kRowChunks)) = v[k];
                 ptx::fence_proxy_async_smem();
                 __syncwarp();
                 if (lane == 0)
-                    ptx::mbar_arrive(ptx::smem_u32(&sh.q_full[seg.pair ? group : 0]));
+                    ptx::mbar_arrive(ptx::smem_u32(&sh.q_full[pair ? group : 0]));
             }
-            const AttnRow row   = attn_row(p, seg, row_id, valid);
-            const int     open  = seg.open[group];
-            const int     tiles = seg.count_of(group);
-            float         slope = 0.0f;
-            int           place = 0;
-            if (p.slopes) {
-                slope = p.slopes[head] * CUDART_L2E_F;
-                place = valid && p.tree_mask ? p.positions[seg.first + token] : seg.context + token;
-                if (p.tree_mask) {
-                    if (thread < min(seg.count, kMaxDrafted))
-                        sh.drafted[group][thread] = p.positions[seg.first + thread];
-                    ptx::named_barrier_sync(2 + group, 128);  // the group's threads, of which none reads the last segment's any more
+            const int open  = seg.open[group];
+            const int tiles = seg.count_of(group);
+            AttnState st{};
+            st.top    = -CUDART_INF_F;
+            st.valid  = valid;
+            st.factor = PLAIN ? p.scale * CUDART_L2E_F : 1.0f;
+            if constexpr (!PLAIN) {
+                st.scale = p.scale * CUDART_L2E_F;
+                st.cap   = p.cap * CUDART_L2E_F;
+                st.place = seg.context + token;
+                if (p.slopes) {
+                    st.slope = p.slopes[head] * CUDART_L2E_F;
+                    if (p.tree_mask) {
+                        st.place   = valid ? p.positions[seg.first + token] : 0;
+                        st.drafted = sh.drafted[group];
+                        if (thread < min(seg.count, kMaxDrafted))
+                            sh.drafted[group][thread] = p.positions[seg.first + thread];
+                        ptx::named_barrier_sync(2 + group, 128);  // the group's threads, none of which reads the last segment's any more
+                    }
                 }
             }
-            float top = -CUDART_INF_F, sum = 0.0f;
-            const int key_begin = seg.tile(group, 0) * kAttnKeys, key_step = (seg.pair ? 1 : 2) * kAttnKeys;
-            for (int i = 0; ok && i < tiles; ++i) {
+            auto rescale = [&](float keep) {
+                ok = attn_wait(&sh.o_done[group], (o_count - 1) & 1u, sh, status);  // the product before has ended
+                ptx::tc_fence_after_sync();
+#pragma unroll 1
+                for (int c = 0; c < HEAD_DIM; c += 32) {
+                    uint32_t o[32];
+                    ptx::tmem_ld_x32(o_tmem + c, o);
+                    ptx::tmem_wait_ld();
+#pragma unroll
+                    for (int k = 0; k < 32; ++k) {
+                        asm volatile("" : "+r"(o[k]));
+                        o[k] = __float_as_uint(__uint_as_float(o[k]) * keep);
+                    }
+                    ptx::tmem_st_x32(o_tmem + c, o);
+                }
+            };
+            auto part_done = [&](int half_tile) {  // the product with the first 64 values may begin before the rest is there
+                if (lane == 0)
+                    ptx::mbar_arrive(ptx::smem_u32(&sh.p_full[group][half_tile]));
+            };
+            const int key_begin = seg.tile(group, 0) * kAttnKeys, key_step = (pair ? 1 : 2) * kAttnKeys;
+            for (int i = 0; i < tiles; ++i) {
                 const int key0 = key_begin + i * key_step;
-                ok             = attn_wait(&sh.s_full[group], s_parity, sh, status);
+                ok             = attn_wait(&sh.s_full[group], s_parity, sh, status) && ok;
                 s_parity ^= 1u;
                 if (!__all_sync(0xffffffffu, ok)) {
                     ok = false;
                     break;
                 }
                 ptx::tc_fence_after_sync();
-                if (busy) {
-                    float s[kAttnKeys];
-                    {
-                        uint32_t(&raw_s)[kAttnKeys] = reinterpret_cast<uint32_t(&)[kAttnKeys]>(s);
-#pragma unroll
-                        for (int c = 0; c < kAttnKeys; c += 32)
-                            ptx::tmem_ld_x32(s_tmem + c, raw_s + c);
-                        ptx::tmem_wait_ld();
-#pragma unroll
-                        for (int c = 0; c < kAttnKeys; ++c)
-                            asm volatile("" : "+r"(raw_s[c]));  // not read before the wait
-                    }
-                    if (!plain) {
-                        if (p.cap > 0.0f) {
-                            // cap tanh(x) = cap - 2 cap / (1 + e^2x), times log2 e
-                            const float c1 = p.cap * CUDART_L2E_F, c2 = -2.0f * c1;
-#pragma unroll
-                            for (int c = 0; c < kAttnKeys; ++c)
-                                s[c] = fmaf(c2, ptx::rcp_approx(1.0f + ptx::exp2_approx(s[c] * cap_in)), c1);
-                        }
-                        else {
-                            const float f = p.scale * CUDART_L2E_F;
-#pragma unroll
-                            for (int c = 0; c < kAttnKeys; ++c)
-                                s[c] *= f;
-                        }
-                        if (p.slopes) {
-                            if (p.tree_mask && key0 + kAttnKeys > open) {
-#pragma unroll
-                                for (int c = 0; c < kAttnKeys; ++c) {
-                                    const int i_draft = key0 + c - open;
-                                    const int where   = i_draft >= 0 && i_draft < kMaxDrafted ? sh.drafted[group][i_draft] : key0 + c;
-                                    s[c]              = fmaf(slope, static_cast<float>(where - place), s[c]);
-                                }
-                            }
-                            else {
-                                const float away = static_cast<float>(key0 - place);
-#pragma unroll
-                                for (int c = 0; c < kAttnKeys; ++c)
-                                    s[c] = fmaf(slope, away + static_cast<float>(c), s[c]);
-                            }
-                        }
-                    }
-                    if (key0 + kAttnKeys > open) {
-#pragma unroll
-                        for (int k = 0; k < kAttnKeys / 32; ++k) {
-                            const uint32_t seen = row.word(key0 + 32 * k);
-#pragma unroll
-                            for (int c = 0; c < 32; ++c)
-                                s[32 * k + c] = seen >> c & 1u ? s[32 * k + c] : -CUDART_INF_F;
-                        }
-                    }
-                    float m[4] = {s[0], s[1], s[2], s[3]};
-#pragma unroll
-                    for (int c = 4; c < kAttnKeys; ++c)
-                        m[c & 3] = fmaxf(m[c & 3], s[c]);
-                    const float new_top = fmaxf(top, fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3])));
-                    if (i == 0)
-                        top = new_top;
-                    else if (__any_sync(0xffffffffu, valid && (new_top - top) * factor > 8.0f)) {  // rows of nobody have no say
-                        // The maximum that the weights are taken against moves only when it has grown by more than 2^8, which
-                        // 32-bit sums and fp16 weights have room for: rarely after the first tiles.
-                        const float keep = new_top == top ? 1.0f : ptx::exp2_approx((top - new_top) * factor);
-                        top              = new_top;
-                        sum *= keep;
-                        ok = attn_wait(&sh.o_done[group], (o_count - 1) & 1u, sh, status);
-                        if (!__all_sync(0xffffffffu, ok)) {
-                            ok = false;
-                            break;
-                        }
-                        ptx::tc_fence_after_sync();
-#pragma unroll 1
-                        for (int c = 0; c < HEAD_DIM; c += 32) {
-                            uint32_t o[32];
-                            ptx::tmem_ld_x32(o_tmem + c, o);
-                            ptx::tmem_wait_ld();
-#pragma unroll
-                            for (int k = 0; k < 32; ++k) {
-                                asm volatile("" : "+r"(o[k]));
-                                o[k] = __float_as_uint(__uint_as_float(o[k]) * keep);
-                            }
-                            ptx::tmem_st_x32(o_tmem + c, o);
-                        }
-                    }
-                    const float minus = top == -CUDART_INF_F ? 0.0f : -top * factor;
-                    float       part[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-                    for (int c = 0; c < kAttnKeys; c += 32) {
-                        uint32_t w[16];
-#pragma unroll
-                        for (int k = 0; k < 32; k += 2) {
-                            const float x = ptx::exp2_approx(fmaf(s[c + k], factor, minus));
-                            const float y = ptx::exp2_approx(fmaf(s[c + k + 1], factor, minus));
-                            part[k & 3] += x;
-                            part[k + 1 & 3] += y;
-                            const half2 h = __floats2half2_rn(x, y);
-                            w[k / 2]      = *reinterpret_cast<const uint32_t*>(&h);
-                        }
-                        ptx::tmem_st_x16(s_tmem + c / 2, w);
-                    }
-                    sum += (part[0] + part[1]) + (part[2] + part[3]);
-                    ptx::tmem_wait_st();
+                if (fourfold)
+                    attn_softmax<PLAIN, 32>(st, row, s_tmem, thread & ~31, key0, open, i == 0, rescale, part_done);
+                else if (busy)
+                    attn_softmax<PLAIN, kAttnKeys>(st, row, s_tmem, 0, key0, open, i == 0, rescale, part_done);
+                else {
+                    part_done(0);
+                    part_done(1);
                 }
                 ++o_count;
-                ptx::tc_fence_before_sync();
-                __syncwarp();
-                if (lane == 0)
-                    ptx::mbar_arrive(ptx::smem_u32(&sh.p_full[group]));
             }
             if (ok && tiles > 0)
                 ok = attn_wait(&sh.o_done[group], (o_count - 1) & 1u, sh, status);
             ptx::tc_fence_after_sync();
 
-            // ---- the end of the segment: this row's columns, whole or a part
+            // ---- the end of the segment: what is added up to a row lies in up to eight places, 2 groups x 4 copies
             int   column0 = 0, column1 = HEAD_DIM;
-            float keep[2] = {1.0f, 0.0f};  // on this group's output, on the other group's
-            bool  join    = false;
-            if (!seg.pair) {  // the other group's sums of the same row
-                sh.top[group][thread] = tiles > 0 ? top : -CUDART_INF_F;
-                sh.sum[group][thread] = tiles > 0 ? sum : 0.0f;
+            float keep = 1.0f, keep_other = 0.0f;  // on this group's output of this lane, on the other group's
+            bool  join = false;
+            if (!pair) {
+                sh.top[group][thread] = st.top;
+                sh.sum[group][thread] = st.sum;
                 ptx::tc_fence_before_sync();
-                ptx::named_barrier_sync(1, 256);
+                ok = !ptx::named_barrier_any(1, 256, !ok);
                 ptx::tc_fence_after_sync();
-                const float top0 = sh.top[0][thread], top1 = sh.top[1][thread];
-                const float both = fmaxf(top0, top1);
-                const float f0   = top0 == both ? 1.0f : ptx::exp2_approx((top0 - both) * factor);
-                const float f1   = top1 == both ? 1.0f : ptx::exp2_approx((top1 - both) * factor);
-                sum              = sh.sum[0][thread] * f0 + sh.sum[1][thread] * f1;
-                top              = both;
-                keep[0]          = group == 0 ? f0 : f1;
-                keep[1]          = group == 0 ? f1 : f0;
-                join             = seg.count_of(1) > 0;
-                if (!join) {  // group 0 has it all
-                    keep[0] = group == 0 ? 1.0f : 0.0f;
-                    keep[1] = group == 0 ? 0.0f : 1.0f;
-                }
-                column0 = group * (HEAD_DIM / 2);
-                column1 = column0 + HEAD_DIM / 2;
+                const int step   = fourfold ? 32 : kAttnRows;
+                float     newtop = -CUDART_INF_F, newsum = 0.0f;
+                for (int r = fourfold ? lane : thread; r < kAttnRows; r += step)
+                    newtop = fmaxf(newtop, fmaxf(sh.top[0][r], sh.top[1][r]));
+                auto weight = [&](float top) { return top == newtop ? 1.0f : ptx::exp2_approx((top - newtop) * st.factor); };
+                for (int r = fourfold ? lane : thread; r < kAttnRows; r += step)
+                    newsum += sh.sum[0][r] * weight(sh.top[0][r]) + sh.sum[1][r] * weight(sh.top[1][r]);
+                keep       = weight(st.top);
+                keep_other = weight(sh.top[group ^ 1][thread]);
+                join       = seg.count_of(1) > 0;
+                st.top     = newtop;
+                st.sum     = newsum;
+                column0    = group * (HEAD_DIM / 2);
+                column1    = column0 + HEAD_DIM / 2;
             }
             ok = ok && sh.abort_flag == 0u;
-            const bool     whole = seg.begin == 0 && seg.end == seg.tiles;
-            const unsigned kind  = whole ? kPartNone : seg.begin == 0 ? kPartBegins : seg.end == seg.tiles ? kPartEnds : kPartContinues;
-            const int      slot  = kind == kPartBegins ? 1 : 0;
-            if (ok && busy) {
-                const uint32_t(&list)[3][4] = sh.not_finite[number % kAttnSegments];
-                uint32_t any = 0;
+            const bool      whole = seg.begin == 0 && seg.end == seg.tiles;
+            const unsigned  kind  = whole ? kPartNone : seg.begin == 0 ? kPartBegins : seg.end == seg.tiles ? kPartEnds : kPartContinues;
+            const int       slot  = kind == kPartBegins ? 1 : 0;
+            const int       tile_row = pair ? group : 0;
+            const long long to       = static_cast<long long>(seg.first + token) * p.heads * HEAD_DIM + in_row;
+            float4* const   sums     = reinterpret_cast<float4*>(p.workspace + attn_sums_offset(gridDim.x))
+                                 + (static_cast<size_t>(2 * blockIdx.x + slot) * 2 + tile_row) * (HEAD_DIM / 4) * kAttnRows;
+            const uint32_t(&list)[3][4] = sh.not_finite[number % kAttnSegments];
+            const float inverse         = st.sum == 0.0f ? 0.0f : 1.0f / st.sum;
+            uint32_t    any             = 0;
 #pragma unroll
-                for (int k = 0; k < 12; ++k)
-                    any |= (&list[0][0])[k];
-                const float inverse  = sum == 0.0f ? 0.0f : 1.0f / sum;
-                const int   tile_row = seg.pair ? group : 0;
-                float4*     sums     = reinterpret_cast<float4*>(p.workspace + attn_sums_offset(gridDim.x))
-                               + (static_cast<size_t>(2 * blockIdx.x + slot) * 2 + tile_row) * (HEAD_DIM / 4) * kAttnRows + thread;
-                half* out = p.out + (static_cast<long long>(seg.first + token) * p.heads + head) * HEAD_DIM;
+            for (int k = 0; k < 12; ++k)
+                any |= (&list[0][0])[k];
+            // An accumulator that no product has written is not read: this group's without a tile of its own, where the groups
+            // share the rows the second group's with a single tile.
+            const bool mine_there = pair ? tiles > 0 : group == 0 || join, other_there = !pair && (group == 1 || join);
+            // 16 columns of this lane's row, both groups' where they share it
+            auto outputs = [&](int c, float(&o)[16]) {
+                uint32_t x[16];
+#pragma unroll
+                for (int k = 0; k < 16; ++k)
+                    o[k] = 0.0f;
+                if (mine_there) {
+                    ptx::tmem_ld_x16(o_tmem + c, x);
+                    ptx::tmem_wait_ld();
+#pragma unroll
+                    for (int k = 0; k < 16; ++k) {
+                        asm volatile("" : "+r"(x[k]));
+                        o[k] = __uint_as_float(x[k]) * keep;
+                    }
+                }
+                if (other_there) {
+                    ptx::tmem_ld_x16(tmem + kO + (group ^ 1) * 128 + lanes + c, x);
+                    ptx::tmem_wait_ld();
+#pragma unroll
+                    for (int k = 0; k < 16; ++k) {
+                        asm volatile("" : "+r"(x[k]));
+                        o[k] = fmaf(__uint_as_float(x[k]), keep_other, o[k]);
+                    }
+                }
+            };
+            if (fourfold) {
+                float4* const staged = reinterpret_cast<float4*>(smem + group * kTileBytes);  // [columns / 4][lane], in Q's place
 #pragma unroll 1
-                for (int c = column0; c < column1; c += 32) {
-                    float    o[32];
-                    uint32_t mine[32], other[32];
-                    if (tiles > 0 && (seg.pair || join || group == 0)) {
-                        ptx::tmem_ld_x32(o_tmem + c, mine);
-                        if (join)
-                            ptx::tmem_ld_x32(tmem + kO + (group ^ 1) * 128 + lanes + c, other);
-                        ptx::tmem_wait_ld();
+                for (int c = column0; c < column1; c += 16) {
+                    float o[16];
+                    outputs(c, o);
 #pragma unroll
-                        for (int k = 0; k < 32; ++k) {
-                            asm volatile("" : "+r"(mine[k]));
-                            o[k] = __uint_as_float(mine[k]) * keep[0];
-                            if (join) {
-                                asm volatile("" : "+r"(other[k]));
-                                o[k] = fmaf(__uint_as_float(other[k]), keep[1], o[k]);
-                            }
-                        }
-                    }
-                    else if (!seg.pair) {  // one tile of keys in all: group 0 multiplied it
-                        ptx::tmem_ld_x32(tmem + kO + lanes + c, other);
-                        ptx::tmem_wait_ld();
+                    for (int k = 0; k < 16; k += 4)
+                        staged[(c - column0 + k) / 4 * kAttnRows + thread] = make_float4(o[k], o[k + 1], o[k + 2], o[k + 3]);
+                }
+                ptx::named_barrier_sync(2 + group, 128);
 #pragma unroll
-                        for (int k = 0; k < 32; ++k) {
-                            asm volatile("" : "+r"(other[k]));
-                            o[k] = __uint_as_float(other[k]);
-                        }
-                    }
-                    else {
-#pragma unroll
-                        for (int k = 0; k < 32; ++k)
-                            o[k] = 0.0f;
-                    }
+                for (int k = 0; k < HEAD_DIM / 32; ++k) {
+                    const int    at = (warp & 3) + 4 * k, column = column0 + 4 * at;
+                    const float4 a = staged[at * kAttnRows + lane], b = staged[at * kAttnRows + lane + 32],
+                                 c = staged[at * kAttnRows + lane + 64], d = staged[at * kAttnRows + lane + 96];
+                    float o[4] = {(a.x + b.x) + (c.x + d.x), (a.y + b.y) + (c.y + d.y), (a.z + b.z) + (c.z + d.z), (a.w + b.w) + (c.w + d.w)};
                     if (any)
-                        attn_add_not_finite<HEAD_DIM>(p, seg, row, list, c, o);
+                        attn_add_not_finite<HEAD_DIM, 4>(p, seg, row, list, column, o);
+                    if (valid && ok && whole) {
+                        const half2 x = __floats2half2_rn(o[0] * inverse, o[1] * inverse), y = __floats2half2_rn(o[2] * inverse, o[3] * inverse);
+                        *reinterpret_cast<uint2*>(p.out + to + column) =
+                            make_uint2(*reinterpret_cast<const uint32_t*>(&x), *reinterpret_cast<const uint32_t*>(&y));
+                    }
+                    else if (valid && ok)
+                        sums[column / 4 * kAttnRows + lane] = make_float4(o[0], o[1], o[2], o[3]);
+                }
+            }
+            else if (ok && busy) {
+                unsigned char* const staged = smem + tile_row * kTileBytes + (thread & ~31) * 128;  // this warp's rows, in Q's place
+#pragma unroll 1
+                for (int c = column0; c < column1; c += 16) {
+                    float o[16];
+                    outputs(c, o);
+                    if (any)
+                        attn_add_not_finite<HEAD_DIM, 16>(p, seg, row, list, c, o);
                     if (valid && whole) {
 #pragma unroll
-                        for (int k = 0; k < 32; k += 8) {
+                        for (int k = 0; k < 16; k += 8) {
                             uint32_t w[4];
 #pragma unroll
                             for (int e = 0; e < 4; ++e) {  // a row that sees no key: what its sums hold are zeros
                                 const half2 h = __floats2half2_rn(o[k + 2 * e] * inverse, o[k + 2 * e + 1] * inverse);
                                 w[e]          = *reinterpret_cast<const uint32_t*>(&h);
                             }
-                            *reinterpret_cast<uint4*>(out + c + k) = make_uint4(w[0], w[1], w[2], w[3]);
+                            *reinterpret_cast<uint4*>(staged + attn_chunk(lane, (c + k) / 8)) = make_uint4(w[0], w[1], w[2], w[3]);
                         }
                     }
                     else if (valid) {
 #pragma unroll
-                        for (int k = 0; k < 32; k += 4)
-                            sums[(c + k) / 4 * kAttnRows] = make_float4(o[k], o[k + 1], o[k + 2], o[k + 3]);
+                        for (int k = 0; k < 16; k += 4)
+                            sums[(c + k) / 4 * kAttnRows + thread] = make_float4(o[k], o[k + 1], o[k + 2], o[k + 3]);
                     }
                     __syncwarp();
                 }
-                if (!whole && valid && column0 == 0)
-                    reinterpret_cast<float2*>(p.workspace + attn_stats_offset(gridDim.x))[static_cast<size_t>(2 * blockIdx.x + slot) * kAttnItemRows
-                                                                                          + tile_row * kAttnRows + thread] =
-                        make_float2(top * factor, sum);
+                if (whole) {  // whole rows at a time
+                    const int       chunks = (column1 - column0) / 8, shift = __ffs(chunks) - 1;
+                    const long long mine   = valid ? to : -1;
+#pragma unroll 4
+                    for (int k = 0; k < chunks; ++k) {
+                        const int       r  = (32 * k + lane) >> shift, chunk = column0 / 8 + (lane & (chunks - 1));
+                        const long long at = __shfl_sync(0xffffffffu, mine, r);
+                        if (at >= 0)
+                            *reinterpret_cast<uint4*>(p.out + at + chunk * 8) = *reinterpret_cast<const uint4*>(staged + attn_chunk(r, chunk));
+                    }
+                }
             }
+            if (ok && !whole && valid && column0 == 0 && (!fourfold || thread < 32))
+                reinterpret_cast<float2*>(p.workspace + attn_stats_offset(gridDim.x))[static_cast<size_t>(2 * blockIdx.x + slot) * kAttnItemRows
+                                                                                      + tile_row * kAttnRows + thread] =
+                    make_float2(st.top * st.factor, st.sum);
             if (kind != kPartNone) {
                 written[slot] = true;
                 if (threadIdx.x == 0)
@@ -855,17 +1020,22 @@ attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
                         if (i >= tiles[group])
                             continue;
                         const uint32_t n = loaded + static_cast<uint32_t>(seg.tile(group, i) - seg.begin), stage = n % kStages;
-                        ok = attn_wait(&sh.v_clean[stage], n / kStages & 1u, sh, status)
-                             && attn_wait(&sh.p_full[group], p_parity[group], sh, status);
-                        p_parity[group] ^= 1u;
+                        const uint64_t v = ptx::umma_desc_nmajor_sw128(v_base + stage * kTileBytes, kBlock);
+                        ok               = attn_wait(&sh.v_clean[stage], n / kStages & 1u, sh, status);
+#pragma unroll
+                        for (int half_tile = 0; half_tile < 2; ++half_tile) {
+                            ok = ok && attn_wait(&sh.p_full[group][half_tile], p_parity[group], sh, status);
+                            if (!ok)
+                                break;
+                            ptx::tc_fence_after_sync();
+#pragma unroll
+                            for (int step = 4 * half_tile; step < 4 * half_tile + 4; ++step)
+                                ptx::umma_f16_ts(tmem + kO + group * 128, tmem + kS + group * 128 + step * 8, v + step * (2048 >> 4),
+                                                 idesc_o, i > 0 || step > 0);
+                        }
                         if (!ok)
                             break;
-                        ptx::tc_fence_after_sync();
-                        const uint64_t v = ptx::umma_desc_nmajor_sw128(v_base + stage * kTileBytes, kBlock);
-#pragma unroll
-                        for (int step = 0; step < kAttnKeys / 16; ++step)
-                            ptx::umma_f16_ts(tmem + kO + group * 128, tmem + kS + group * 128 + step * 8, v + step * (2048 >> 4), idesc_o,
-                                             i > 0 || step > 0);
+                        p_parity[group] ^= 1u;
                         if (!seg.pair || group == 1)
                             ptx::umma_commit(ptx::smem_u32(&sh.v_empty[stage]));
                         ptx::umma_commit(ptx::smem_u32(&sh.o_done[group]));
@@ -891,13 +1061,20 @@ attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
         uint32_t          n        = 0;
         bool              ok       = true;
         for (int number = 0; ok; ++number) {
-            cursor.next(p);
+            cursor.next(p, sh);
             if (lane == 0) {
                 sh.segment[number % kAttnSegments] = seg;
                 ptx::mbar_arrive(ptx::smem_u32(&sh.segment_full[number % kAttnSegments]));
             }
             if (seg.end == 0)
                 break;
+            // The rows of Q on their way to L2 before the keys and values that they would otherwise queue behind.
+            for (int r = lane; r < seg.rows; r += 32) {
+                const int   token = (seg.row0 + r) / p.share, head = seg.head * p.share + (seg.row0 + r) % p.share;
+                const half* q     = p.q + (seg.first + token) * p.ld_q + static_cast<long long>(head) * HEAD_DIM;
+                for (int c = 0; c < HEAD_DIM; c += 64)
+                    ptx::prefetch_l2(q + c);
+            }
             const int* table = c.page_table + static_cast<long long>(seg.b) * c.table_width;
             for (int t = seg.begin; ok && t < seg.end; ++t, ++n) {
                 const int key   = t * kAttnKeys + piece * box;

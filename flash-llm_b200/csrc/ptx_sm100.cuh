@@ -336,6 +336,17 @@ __device__ __forceinline__ void tmem_ld_x8(uint32_t taddr, uint32_t (&r)[8])
                  : "memory");
 }
 
+// ... 16 consecutive columns.
+__device__ __forceinline__ void tmem_ld_x16(uint32_t taddr, uint32_t* r)
+{
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, "
+                 "[%16];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+                   "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+                 : "r"(taddr)
+                 : "memory");
+}
+
 // ... 32 consecutive columns.
 __device__ __forceinline__ void tmem_ld_x32(uint32_t taddr, uint32_t* r)
 {
@@ -529,6 +540,78 @@ __device__ __forceinline__ float exp2_approx(float x)
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
+}
+
+// Two 32-bit operations in one instruction, each rounded to nearest.
+__device__ __forceinline__ float2 fma_x2(float2 a, float2 b, float2 c)
+{
+    float2 d;
+    asm("{\n"
+        ".reg .b64 a, b, c, d;\n"
+        "mov.b64 a, {%2, %3};\n"
+        "mov.b64 b, {%4, %5};\n"
+        "mov.b64 c, {%6, %7};\n"
+        "fma.rn.f32x2 d, a, b, c;\n"
+        "mov.b64 {%0, %1}, d;\n"
+        "}\n"
+        : "=f"(d.x), "=f"(d.y)
+        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+    return d;
+}
+
+__device__ __forceinline__ float2 add_x2(float2 a, float2 b)
+{
+    float2 d;
+    asm("{\n"
+        ".reg .b64 a, b, d;\n"
+        "mov.b64 a, {%2, %3};\n"
+        "mov.b64 b, {%4, %5};\n"
+        "add.rn.f32x2 d, a, b;\n"
+        "mov.b64 {%0, %1}, d;\n"
+        "}\n"
+        : "=f"(d.x), "=f"(d.y)
+        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return d;
+}
+
+__device__ __forceinline__ float2 mul_x2(float2 a, float2 b)
+{
+    float2 d;
+    asm("{\n"
+        ".reg .b64 a, b, d;\n"
+        "mov.b64 a, {%2, %3};\n"
+        "mov.b64 b, {%4, %5};\n"
+        "mul.rn.f32x2 d, a, b;\n"
+        "mov.b64 {%0, %1}, d;\n"
+        "}\n"
+        : "=f"(d.x), "=f"(d.y)
+        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return d;
+}
+
+// The largest of three; NaN if one of them is.
+__device__ __forceinline__ float max3_nan(float a, float b, float c)
+{
+    float d;
+    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
+
+// 16 bytes where the predicate holds, zeros elsewhere.  Loads written one behind another are issued one behind another, ahead of
+// the first use.
+__device__ __forceinline__ uint4 ldg_v4_if(const void* p, bool there)
+{
+    uint4 v = make_uint4(0, 0, 0, 0);
+    asm volatile(
+        "{\n"
+        ".reg .pred p;\n"
+        "setp.ne.u32 p, %5, 0;\n"
+        "@p ld.global.v4.u32 {%0, %1, %2, %3}, [%4];\n"
+        "}\n"
+        : "+r"(v.x), "+r"(v.y), "+r"(v.z), "+r"(v.w)
+        : "l"(p), "r"(there ? 1u : 0u)
+        : "memory");
+    return v;
 }
 
 // 1/x within 1 ulp.
