@@ -123,6 +123,23 @@ static bool encode_cache(CUtensorMap* map, const half* cache, const CacheBatch& 
            == CUDA_SUCCESS;
 }
 
+// The queries as (head_dim, heads, tokens), copied in boxes of 64 columns, the heads of a group and as many tokens as `rows` hold.
+static bool encode_rows(CUtensorMap* map, const AttentionParams& p, int head_dim, int rows)
+{
+    const EncodeTiledFn encode = encode_tiled();
+    if (encode == nullptr)
+        return false;
+    const cuuint64_t dims[3]    = {static_cast<cuuint64_t>(head_dim), static_cast<cuuint64_t>(p.heads),
+                                   static_cast<cuuint64_t>(p.batch.tokens)};
+    const cuuint64_t strides[2] = {static_cast<cuuint64_t>(head_dim) * 2, static_cast<cuuint64_t>(p.ld_q) * 2};
+    const cuuint32_t box[3]     = {64, static_cast<cuuint32_t>(p.share), static_cast<cuuint32_t>(rows / p.share)};
+    const cuuint32_t ones[3]    = {1, 1, 1};
+    return encode(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, const_cast<half*>(p.q), dims, strides, box, ones,
+                  CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE)
+           == CUDA_SUCCESS;
+}
+
 template<int HEAD_DIM>
 static cudaError_t launch_attention(cudaStream_t stream, const AttentionParams& p)
 {
@@ -130,15 +147,16 @@ static cudaError_t launch_attention(cudaStream_t stream, const AttentionParams& 
     cudaError_t err = multiprocessors(&sms);
     if (err != cudaSuccess)
         return err;
-    CUtensorMap map_k, map_v;
-    if (!encode_cache(&map_k, p.k_cache, p.batch, HEAD_DIM) || !encode_cache(&map_v, p.v_cache, p.batch, HEAD_DIM))
+    CUtensorMap map_q, map_q_few, map_k, map_v;
+    if (!encode_rows(&map_q, p, HEAD_DIM, p.tile_rows) || !encode_rows(&map_q_few, p, HEAD_DIM, p.few_rows > 0 ? p.few_rows : p.tile_rows)
+        || !encode_cache(&map_k, p.k_cache, p.batch, HEAD_DIM) || !encode_cache(&map_v, p.v_cache, p.batch, HEAD_DIM))
         return cudaErrorInvalidValue;
     const bool plain = p.cap == 0.0f && p.slopes == nullptr;
-    err = launch_in_stream_order(plain ? attention_kernel<HEAD_DIM, true> : attention_kernel<HEAD_DIM, false>, dim3(sms), dim3(kAttnThreads), attn_smem_bytes(HEAD_DIM), stream, 1, map_k,
-                                 map_v, p);
+    err = launch_in_stream_order(plain ? attention_kernel<HEAD_DIM, true> : attention_kernel<HEAD_DIM, false>, dim3(sms), dim3(kAttnThreads), attn_smem_bytes(HEAD_DIM), stream, 1, map_q,
+                                 map_q_few, map_k, map_v, p);
     if (err != cudaSuccess)
         return err;
-    return launch_in_stream_order(attention_join_kernel<HEAD_DIM>, dim3(sms, kAttnItemRows / 32), dim3(256), 0, stream, 1, p, sms);
+    return launch_in_stream_order(attention_join_kernel<HEAD_DIM>, dim3(sms, kAttnSlotRows / 32), dim3(256), 0, stream, 1, p, sms);
 }
 
 // The checks that tree and prompt attention share, and the launch.
@@ -149,7 +167,7 @@ static cudaError_t attend(cudaStream_t stream, AttentionParams p, const void* Q,
 {
     if (!describe_batch(&p.batch, K_cache, V_cache, pages, page_size, cu_tokens, context, page_table, table_width, sequences, tokens,
                         kv_heads, head_dim)
-        || heads < 1 || heads % kv_heads != 0 || static_cast<long long>(heads) * head_dim > (1 << 24) || !rows_fit(Q, ld_q, heads, head_dim)
+        || heads < 1 || heads % kv_heads != 0 || heads / kv_heads > kAttnRows || static_cast<long long>(heads) * head_dim > (1 << 24) || !rows_fit(Q, ld_q, heads, head_dim)
         || workspace == nullptr || !aligned16(workspace) || Out == nullptr || !aligned16(Out) || !(scale > 0.0f) || !std::isfinite(scale) || !(cap >= 0.0f) || !std::isfinite(cap)
         || static_cast<long long>(tokens) * heads > 0x7fffffffll - 256)
         return cudaErrorInvalidValue;
@@ -168,6 +186,11 @@ static cudaError_t attend(cudaStream_t stream, AttentionParams p, const void* Q,
     p.cap     = cap;
     p.workspace = static_cast<unsigned char*>(workspace);
     p.share     = heads / kv_heads;
+    p.tile_rows = kAttnRows / p.share * p.share;
+    p.few_rows  = 32 / p.share * p.share;
+    while ((1 << p.share_shift) < p.share)
+        ++p.share_shift;
+    p.share_magic = static_cast<unsigned>(((1ull << 32) * ((1ull << p.share_shift) - p.share)) / p.share + 1);
     return head_dim == 64 ? launch_attention<64>(stream, p) : launch_attention<128>(stream, p);
 }
 

@@ -9,10 +9,11 @@
 // One pass over the keys in tiles of 128 with the running maximum and sum of a softmax: S = Q K^T on the tensor cores, P =
 // exp(S - maximum) in registers, one thread per row, rounded to fp16 (the type of the other operand of its product; 2^-11 of a
 // weight) and back to tensor memory, O += P V from there.  The query heads that share a key/value head are rows of one tile:
-// row r of a sequence's (tokens x share) rows is token r / share, head r % share of the group.
+// row r of a sequence's (tokens x share) rows is token r / share, head r % share of the group.  A tile holds the rows of as many
+// whole tokens as its 128 have room for: one tensor copy brings 64 columns of them.
 //
-// An item is 256 such rows of one sequence and one key/value head.  Its two tiles of rows are two groups of softmax warps that
-// take turns on the tensor core; an item of at most 128 rows (single tokens, drafted trees) is the same tile for both groups,
+// An item is two such tiles of one sequence and one key/value head.  Its two tiles of rows are two groups of softmax warps that
+// take turns on the tensor core; an item of one tile (single tokens, drafted trees) is the same tile for both groups,
 // each takes every other tile of keys, and the two results are joined at the end.  An item of at most 32 rows, which would leave
 // one warp of four with all the work, lies in the tile four times: every warp has all rows and a quarter of the tile's keys
 // (weights of zero for the others), and the joined results are eight.  The work of a call is the linear sequence
@@ -20,6 +21,8 @@
 // partial sums in the workspace, which attention_join_kernel adds up in key order.
 #pragma once
 #include <math_constants.h>
+
+#include <type_traits>
 
 #include "cache_batch.cuh"
 #include "tiling.h"
@@ -39,20 +42,29 @@ struct AttentionParams {
     unsigned char*            workspace;
     long long                 ld_q;
     int                       heads;
-    int                       share;  // query heads per key/value head
+    int                       share;  // query heads per key/value head, and what divides by it: (mulhi(n, magic) + n) >> shift
+    unsigned                  share_magic;
+    int                       share_shift;
+    int                       tile_rows;  // rows of a tile: whole tokens, at most 128
+    int                       few_rows;   // ... at most 32; 0 where not one fits
     float                     scale;
     float                     cap;  // 0: none
 };
 
+// Token of a row of a sequence's (tokens x share) rows.
+__device__ __forceinline__ int attn_token(const AttentionParams& p, int row)
+{
+    return static_cast<int>((__umulhi(static_cast<unsigned>(row), p.share_magic) + static_cast<unsigned>(row)) >> p.share_shift);
+}
+
 constexpr int kAttnKeys      = 128;  // keys per tile
 constexpr int kAttnRows      = 128;  // rows per tile: one per lane of tensor memory
-constexpr int kAttnItemRows  = 2 * kAttnRows;
+constexpr int kAttnSlotRows  = 2 * kAttnRows;  // rows that the workspace has room for in a part of an item
 constexpr int kAttnMmaWarp   = 8;  // warps 0..3 and 4..7: the two groups of rows
 constexpr int kAttnLoadWarp  = 9;
-constexpr int kAttnCleanWarp = 10;  // and 11
+constexpr int kAttnHelpWarp  = 10;  // and 11
 constexpr int kAttnThreads   = 12 * 32;
 constexpr int kAttnTmemCols  = 512;
-constexpr int kAttnFewRows   = 32;
 constexpr int kAttnKnown     = 512;  // sequences whose sizes are kept in shared memory from the plan on
 constexpr int kAttnSegments  = 8;  // segments that shared memory holds at a time
 // Registers of a thread: the softmax warps keep a row of 128 scores, 256 x 208 + 128 x 88 = 384 x 168.
@@ -77,7 +89,7 @@ struct AttnSegment {
     int  first, count, context, prefix;  // of the sequence: first row, rows, position of the first row, keys that all see
     int  head;     // key/value head
     int  row0;     // first row of the item in the sequence's rows (tokens x share)
-    int  rows;     // rows of the item, at most kAttnItemRows
+    int  rows;     // rows of the item
     int  keys;     // keys that any row of the item sees: none at or behind this
     int  open[2];  // keys that every row of a group sees: the first tile that needs a mask ends behind them
     int  tiles;    // of keys, the whole item
@@ -85,7 +97,7 @@ struct AttnSegment {
     int  end;      // behind its last; 0: no more segments
     int  tiles0;   // pair: tiles of keys that the first tile of rows needs
     bool pair;     // two tiles of rows; otherwise both groups share the one
-    bool fourfold;  // at most 32 rows: four copies of them in the tile
+    bool fourfold;  // few rows: four copies of them in the tile
 
     // Tiles of keys that a group goes through, and the i-th of them.
     __device__ __forceinline__ int count_of(int group) const
@@ -103,19 +115,23 @@ struct AttnSegment {
 // Dynamic shared memory: two tiles of Q, the stages, and what AttnShared holds.
 struct AttnShared {
     unsigned long long k_full[4], k_empty[4], v_full[4], v_clean[4], v_empty[4];
-    unsigned long long s_full[2], p_full[2][2], o_done[2], q_full[2], segment_full[kAttnSegments];
+    unsigned long long s_full[2], p_full[2][2], o_done[2], q_full[2], q_empty[2], segment_full[kAttnSegments];
     uint32_t           tmem;
     volatile uint32_t  abort_flag;
-    int                start_sequence, start_rows, start_head, start_tile;
+    int                start_sequence, start_rows, start_head, start_unit;
     long long          start_units;
     // Written by the loader, which is ahead of everybody, by at most the stages and one: a segment's values cannot be loaded
     // before those of the one so many tiles earlier have been multiplied, and its place here is taken again only after
     // kAttnSegments more.
     AttnSegment        segment[kAttnSegments];
     float              top[2][kAttnRows], sum[2][kAttnRows];
+    uint32_t           any_not_finite[kAttnSegments];
     uint32_t           not_finite[kAttnSegments][3][4];  // keys of an item's last three tiles whose values are not finite
     int                drafted[2][kMaxDrafted];          // positions of drafted tokens, by group
-    unsigned int       tiles[kMaxSequences];             // of all items of a sequence's first key/value head
+    union {
+        unsigned int units[kMaxSequences];  // of all items of a sequence's first key/value head; the plan's alone
+        float4       staged[2][512];        // by group: outputs on their way out
+    };
     int4               known[kAttnKnown];                // first row, rows, context and prefix of the first sequences
 };
 
@@ -144,37 +160,42 @@ __host__ __device__ constexpr size_t attn_stats_offset(int ctas)
 
 __host__ __device__ constexpr size_t attn_sums_offset(int ctas)
 {
-    return attn_stats_offset(ctas) + size_t(2) * ctas * kAttnItemRows * sizeof(float2);
+    return attn_stats_offset(ctas) + size_t(2) * ctas * kAttnSlotRows * sizeof(float2);
 }
 
 // Sums lie as [slot][tile of rows][head_dim / 4][row] float4: a warp's rows are neighbours.
 __host__ __device__ constexpr size_t attn_workspace_bytes(int ctas, int head_dim)
 {
-    return attn_sums_offset(ctas) + size_t(2) * ctas * kAttnItemRows * head_dim * sizeof(float);
+    return attn_sums_offset(ctas) + size_t(2) * ctas * kAttnSlotRows * head_dim * sizeof(float);
 }
 
-__device__ __forceinline__ bool attn_wait(const unsigned long long* barrier, uint32_t parity, AttnShared& sh, unsigned int* status)
+__device__ __forceinline__ bool attn_wait_longer(uint32_t bar, uint32_t parity, volatile uint32_t* abort_flag, unsigned int* status)
 {
-    const uint32_t bar = ptx::smem_u32(barrier);
-    if (ptx::mbar_try_wait(bar, parity))
-        return true;
     uint64_t t0 = 0;
+#pragma unroll 1
     for (uint32_t it = 1;; ++it) {
         if (ptx::mbar_try_wait(bar, parity))
             return true;
         if ((it & 63u) == 0u) {
-            if (sh.abort_flag)
+            if (*abort_flag)
                 return false;
             const uint64_t now = ptx::globaltimer_ns();
             if (t0 == 0)
                 t0 = now;
             else if (now - t0 > kAttnWaitLimitNs) {
-                sh.abort_flag = 1u;
+                *abort_flag = 1u;
                 atomicOr(status, kStatusWaitExpired);
                 return false;
             }
         }
     }
+}
+
+// A bounded wait; false once the CTA gives up.
+__device__ __forceinline__ bool attn_wait(const unsigned long long* barrier, uint32_t parity, AttnShared& sh, unsigned int* status)
+{
+    const uint32_t bar = ptx::smem_u32(barrier);
+    return ptx::mbar_try_wait(bar, parity) || attn_wait_longer(bar, parity, &sh.abort_flag, status);
 }
 
 // ---------------------------------------------------------------- the work of a call
@@ -209,13 +230,13 @@ __device__ __forceinline__ int attn_keys(const AttentionParams& p, const AttnSeq
 {
     if (p.tree_mask)
         return a.s.context + min(a.s.count, kMaxDrafted);
-    return max(a.s.context + (row_end - 1) / p.share + 1, a.prefix);
+    return max(a.s.context + attn_token(p, row_end - 1) + 1, a.prefix);
 }
 
 // Keys that all rows from `row` on see.
 __device__ __forceinline__ int attn_open_keys(const AttentionParams& p, const AttnSequence& a, int row)
 {
-    return p.tree_mask ? a.s.context : max(a.s.context + row / p.share + 1, a.prefix);
+    return p.tree_mask ? a.s.context : max(a.s.context + attn_token(p, row) + 1, a.prefix);
 }
 
 __device__ __forceinline__ int attn_tiles(int keys)
@@ -223,24 +244,34 @@ __device__ __forceinline__ int attn_tiles(int keys)
     return (keys + kAttnKeys - 1) / kAttnKeys;
 }
 
-// Walks a CTA's share of the linear sequence of tiles, order (sequence, rows, key/value head, keys).
+// Beginning an item, and ending it, takes about as long as kAttnItemUnits tiles of keys: an item counts as so many units more
+// than it has tiles when the work is dealt out.  A CTA has at least kAttnLeastUnits of them: two tiles, one for each group, cost
+// little more than one, and an item that is not cut needs no joining.
+constexpr int kAttnItemUnits = 2, kAttnLeastUnits = 4;
+
+__device__ __forceinline__ int attn_units(int tiles)
+{
+    return tiles + kAttnItemUnits;
+}
+
+// Walks a CTA's share of the linear sequence of units, order (sequence, rows, key/value head, keys).
 struct AttnCursor {
     AttnSequence a;
     AttnSegment  seg;
     long long    left;
-    int          next_tile;
+    int          next_unit;  // of the item
 
     __device__ __forceinline__ void enter_rows(const AttentionParams& p)
     {
-        const int end  = min(seg.row0 + kAttnItemRows, a.rows);
+        const int end  = min(seg.row0 + 2 * p.tile_rows, a.rows);
         seg.rows       = end - seg.row0;
-        seg.pair       = seg.rows > kAttnRows;
-        seg.fourfold   = seg.rows <= kAttnFewRows;
+        seg.pair       = seg.rows > p.tile_rows;
+        seg.fourfold   = seg.rows <= p.few_rows;
         seg.keys       = attn_keys(p, a, end);
         seg.tiles      = attn_tiles(seg.keys);
-        seg.tiles0     = seg.pair ? attn_tiles(attn_keys(p, a, seg.row0 + kAttnRows)) : seg.tiles;
+        seg.tiles0     = seg.pair ? attn_tiles(attn_keys(p, a, seg.row0 + p.tile_rows)) : seg.tiles;
         seg.open[0]    = attn_open_keys(p, a, seg.row0);
-        seg.open[1]    = seg.pair ? attn_open_keys(p, a, seg.row0 + kAttnRows) : seg.open[0];
+        seg.open[1]    = seg.pair ? attn_open_keys(p, a, seg.row0 + p.tile_rows) : seg.open[0];
     }
     __device__ __forceinline__ void enter_sequence(const AttentionParams& p, const AttnShared& sh)
     {
@@ -265,31 +296,37 @@ struct AttnCursor {
         seg.b     = sh.start_sequence;
         seg.row0  = sh.start_rows;
         seg.head  = sh.start_head;
-        next_tile = sh.start_tile;
+        next_unit = sh.start_unit;
         if (left > 0)
             enter_sequence(p, sh);
     }
-    // The next segment; its `end` is 0 at the end of the share.
+    // The next segment that has a tile; its `end` is 0 at the end of the share.
     __device__ __forceinline__ void next(const AttentionParams& p, const AttnShared& sh)
     {
-        if (left > 0 && next_tile >= seg.tiles) {
-            next_tile = 0;
-            if (++seg.head == p.batch.kv_heads) {
-                seg.head = 0;
-                seg.row0 += kAttnItemRows;
-                if (seg.row0 >= a.rows) {
-                    seg.row0 = 0;
-                    ++seg.b;
-                    enter_sequence(p, sh);
+        do {
+            if (left > 0 && next_unit >= attn_units(seg.tiles)) {
+                next_unit = 0;
+                if (++seg.head == p.batch.kv_heads) {
+                    seg.head = 0;
+                    seg.row0 += 2 * p.tile_rows;
+                    if (seg.row0 >= a.rows) {
+                        seg.row0 = 0;
+                        ++seg.b;
+                        enter_sequence(p, sh);
+                    }
+                    else
+                        enter_rows(p);
                 }
-                else
-                    enter_rows(p);
             }
-        }
-        seg.begin = next_tile;
-        seg.end   = left > 0 ? static_cast<int>(min(static_cast<long long>(seg.tiles), next_tile + left)) : 0;
-        left -= seg.end - seg.begin;
-        next_tile = seg.end;
+            seg.begin = seg.end = 0;
+            if (left <= 0)
+                return;
+            const int upto = static_cast<int>(min(static_cast<long long>(attn_units(seg.tiles)), next_unit + left));
+            seg.begin      = max(next_unit - kAttnItemUnits, 0);
+            seg.end        = max(upto - kAttnItemUnits, 0);
+            left -= upto - next_unit;
+            next_unit = upto;
+        } while (seg.end == seg.begin);
     }
 };
 
@@ -302,59 +339,70 @@ __device__ __forceinline__ const AttnSegment* attn_segment(AttnShared& sh, int n
     return &sh.segment[place];
 }
 
-constexpr unsigned kAttnSeveralItems = 0xffffffffu, kAttnLostRows = 0xfffffffeu;  // in place of a sequence's tiles
+constexpr unsigned kAttnSeveralItems = 0xffffffffu, kAttnLostRows = 0xfffffffeu;  // in place of a sequence's units
 
 // Where this CTA's share begins and how long it is; all threads, ends with a barrier.  The rows of a sequence that does not fit
 // into the page table are cleared here, by one CTA.
 __device__ __forceinline__ void attn_plan(const AttentionParams& p, AttnShared& sh, int head_dim)
 {
     const int B = p.batch.sequences, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int item_rows = 2 * p.tile_rows;
+#pragma unroll 1
     for (int b = threadIdx.x; b < B; b += kAttnThreads) {
         const AttnSequence a = attn_sequence(p, b);
         if (b < kAttnKnown)
             sh.known[b] = make_int4(a.s.first, a.s.count, a.s.context, a.prefix);
-        sh.tiles[b]          = a.s.lost > 0            ? kAttnLostRows
+        sh.units[b]          = a.s.lost > 0            ? kAttnLostRows
                                : a.rows == 0            ? 0u
-                               : a.rows > kAttnItemRows ? kAttnSeveralItems
-                                                        : attn_tiles(attn_keys(p, a, a.rows));
+                               : a.rows > item_rows ? kAttnSeveralItems
+                                                        : attn_units(attn_tiles(attn_keys(p, a, a.rows)));
     }
     __syncthreads();
+#pragma unroll 1
     for (int b = warp; b < B; b += kAttnThreads / 32) {
-        if (sh.tiles[b] < kAttnLostRows)
+        if (sh.units[b] < kAttnLostRows)
             continue;
         const AttnSequence a    = attn_sequence(p, b);
         unsigned           mine = 0;
         if (a.s.lost > 0 && b % gridDim.x == blockIdx.x) {
             const long long row = static_cast<long long>(p.heads) * head_dim;
+#pragma unroll 1
             for (long long i = lane * 8; i < a.s.lost * row; i += 32 * 8)
                 *reinterpret_cast<uint4*>(p.out + a.s.first * row + i) = make_uint4(0, 0, 0, 0);
         }
-        for (long long r = lane * kAttnItemRows; r < a.rows; r += 32 * kAttnItemRows)
-            mine += attn_tiles(attn_keys(p, a, static_cast<int>(min(r + kAttnItemRows, static_cast<long long>(a.rows)))));
+#pragma unroll 1
+        for (long long r = lane * item_rows; r < a.rows; r += 32 * item_rows)
+            mine += attn_units(attn_tiles(attn_keys(p, a, static_cast<int>(min(r + item_rows, static_cast<long long>(a.rows))))));
         mine = __reduce_add_sync(0xffffffffu, mine);
         __syncwarp();
         if (lane == 0)
-            sh.tiles[b] = mine;
+            sh.units[b] = mine;
     }
     __syncthreads();
     if (warp == 0) {
         long long total = 0;
+#pragma unroll 1
         for (int b = lane; b < B; b += 32)
-            total += sh.tiles[b];
+            total += sh.units[b];
 #pragma unroll
         for (int d = 16; d > 0; d >>= 1)
             total += __shfl_xor_sync(0xffffffffu, total, d);
         const int       heads = p.batch.kv_heads;
         const long long units = total * heads;
-        const long long ctas  = min(units, static_cast<long long>(gridDim.x));  // none of them without a tile
-        const long long cta   = blockIdx.x;
-        const long long u0    = cta < ctas ? units * cta / ctas : 0, u1 = cta < ctas ? units * (cta + 1) / ctas : 0;
+        long long       share = 0;
+        if (units < 0x7fffffffll)
+            share = (static_cast<unsigned>(units) + gridDim.x - 1) / gridDim.x;
+        else
+            share = (units + gridDim.x - 1) / gridDim.x;
+        share              = max(share, static_cast<long long>(kAttnLeastUnits));
+        const long long u0 = min(units, share * blockIdx.x), u1 = min(units, u0 + share);
         // The sequence that holds unit u0: the first whose running sum passes it.
         int       b = 0, row0 = 0;
         long long before = 0;
         if (u1 > u0) {
+#pragma unroll 1
             for (int base = 0;; base += 32) {
-                long long mine = base + lane < B ? static_cast<long long>(sh.tiles[base + lane]) * heads : 0, upto = mine;
+                long long mine = base + lane < B ? static_cast<long long>(sh.units[base + lane]) * heads : 0, upto = mine;
 #pragma unroll
                 for (int d = 1; d < 32; d <<= 1) {
                     const long long other = __shfl_up_sync(0xffffffffu, upto, d);
@@ -371,12 +419,13 @@ __device__ __forceinline__ void attn_plan(const AttentionParams& p, AttnShared& 
                 before += __shfl_sync(0xffffffffu, upto, 31);
             }
             const AttnSequence a = attn_sequence(p, sh, b);
-            for (long long base = 0;; base += 32 * kAttnItemRows) {  // ... and of its items the first
-                const long long r    = base + lane * kAttnItemRows;
+#pragma unroll 1
+            for (long long base = 0;; base += 32 * item_rows) {  // ... and of its items the first
+                const long long r    = base + lane * item_rows;
                 long long       mine = 0;
                 if (r < a.rows)
                     mine = static_cast<long long>(heads)
-                           * attn_tiles(attn_keys(p, a, static_cast<int>(min(r + kAttnItemRows, static_cast<long long>(a.rows)))));
+                           * attn_units(attn_tiles(attn_keys(p, a, static_cast<int>(min(r + item_rows, static_cast<long long>(a.rows))))));
                 long long upto = mine;
 #pragma unroll
                 for (int d = 1; d < 32; d <<= 1) {
@@ -385,20 +434,21 @@ __device__ __forceinline__ void attn_plan(const AttentionParams& p, AttnShared& 
                         upto += other;
                 }
                 const unsigned past = __ballot_sync(0xffffffffu, before + upto > u0);
-                if (past || base + 32 * kAttnItemRows >= a.rows) {
+                if (past || base + 32 * item_rows >= a.rows) {
                     const int l = past ? __ffs(past) - 1 : 0;
-                    row0        = static_cast<int>(base) + l * kAttnItemRows;
+                    row0        = static_cast<int>(base) + l * item_rows;
                     before += __shfl_sync(0xffffffffu, upto - mine, l);
                     break;
                 }
                 before += __shfl_sync(0xffffffffu, upto, 31);
             }
             if (lane == 0) {
-                const int tiles   = max(1, attn_tiles(attn_keys(p, a, min(row0 + kAttnItemRows, a.rows))));
+                const unsigned item = attn_units(attn_tiles(attn_keys(p, a, min(row0 + item_rows, a.rows))));
                 sh.start_sequence = b;
                 sh.start_rows     = row0;
-                sh.start_head     = static_cast<int>((u0 - before) / tiles);
-                sh.start_tile     = static_cast<int>((u0 - before) % tiles);
+                const unsigned in = static_cast<unsigned>(u0 - before);  // of the item's units of all heads
+                sh.start_head     = static_cast<int>(in / item);
+                sh.start_unit     = static_cast<int>(in % item);
             }
         }
         if (lane == 0)
@@ -442,7 +492,7 @@ __device__ __forceinline__ AttnRow attn_row(const AttentionParams& p, const Attn
     r.bits   = 0;
     if (!valid)
         return r;
-    const int token = row / p.share;
+    const int token = attn_token(p, row);
     if (p.tree_mask) {
         r.limit = seg.context;
         r.bits  = p.tree_mask[seg.first + token];
@@ -455,12 +505,6 @@ __device__ __forceinline__ AttnRow attn_row(const AttentionParams& p, const Attn
 }
 
 // ---------------------------------------------------------------- the kernel
-
-// Where 16 bytes of a row lie in a tile in shared memory: blocks of 64 columns, the 128-byte swizzle.
-__device__ __forceinline__ int attn_chunk(int row, int chunk)
-{
-    return chunk / 8 * (kAttnKeys * 128) + row * 128 + ((chunk % 8 ^ (row & 7)) << 4);
-}
 
 __device__ __forceinline__ bool half_not_finite(uint32_t h)
 {
@@ -662,13 +706,13 @@ __device__ __forceinline__ void attn_softmax(AttnState& st, const AttnRow& row, 
 // PLAIN: neither cap nor slopes.
 template<int HEAD_DIM, bool PLAIN>
 __global__ void __launch_bounds__(kAttnThreads, 1)
-attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const AttentionParams p)
+attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_q_few,
+                 const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const AttentionParams p)
 {
     constexpr int      kStages    = attn_stages(HEAD_DIM);
     constexpr int      kTileBytes = attn_tile_bytes(HEAD_DIM);
     constexpr int      kBlock     = kAttnKeys * 128;  // bytes of 64 columns of a tile
     constexpr int      kBlocks    = HEAD_DIM / 64;
-    constexpr int      kRowChunks = HEAD_DIM / 8;  // of 16 bytes in a row of Q or of the output
     constexpr uint32_t kS = 0, kO = 256;  // tensor memory: scores (weights in their first half) and outputs, 128 columns a group
     extern __shared__ unsigned char smem_raw[];
     const uint32_t raw  = ptx::smem_u32(smem_raw);
@@ -680,6 +724,7 @@ attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
     const int            warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
     if (threadIdx.x == 0) {
+#pragma unroll 1
         for (int i = 0; i < 4; ++i) {
             ptx::mbar_init(ptx::smem_u32(&sh.k_full[i]), 1);
             ptx::mbar_init(ptx::smem_u32(&sh.k_empty[i]), 1);
@@ -687,17 +732,22 @@ attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
             ptx::mbar_init(ptx::smem_u32(&sh.v_clean[i]), 64);
             ptx::mbar_init(ptx::smem_u32(&sh.v_empty[i]), 1);
         }
+#pragma unroll 1
         for (int i = 0; i < 2; ++i) {
             ptx::mbar_init(ptx::smem_u32(&sh.s_full[i]), 1);
             ptx::mbar_init(ptx::smem_u32(&sh.p_full[i][0]), 4);
             ptx::mbar_init(ptx::smem_u32(&sh.p_full[i][1]), 4);
             ptx::mbar_init(ptx::smem_u32(&sh.o_done[i]), 1);
-            ptx::mbar_init(ptx::smem_u32(&sh.q_full[i]), 4);
+            ptx::mbar_init(ptx::smem_u32(&sh.q_full[i]), 1);
+            ptx::mbar_init(ptx::smem_u32(&sh.q_empty[i]), 1);
         }
+#pragma unroll 1
         for (int i = 0; i < kAttnSegments; ++i)
             ptx::mbar_init(ptx::smem_u32(&sh.segment_full[i]), 1);
         sh.abort_flag = 0u;
         ptx::fence_mbar_init();
+        ptx::prefetch_tensormap(&map_q);
+        ptx::prefetch_tensormap(&map_q_few);
         ptx::prefetch_tensormap(&map_k);
         ptx::prefetch_tensormap(&map_v);
     }
@@ -734,31 +784,15 @@ attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
             ptx::tc_fence_after_sync();
             const AttnSegment& seg     = *current;
             const bool         pair = seg.pair, fourfold = seg.fourfold;
-            const int          in_item = pair ? group * kAttnRows + thread : fourfold ? lane : thread;  // row of the item
-            const int          row_id  = seg.row0 + in_item;                                          // ... of the sequence
-            const bool         valid   = in_item < seg.rows;
-            const bool         busy    = (in_item & ~31) < seg.rows;  // the warp has a row
-            const int          token   = valid ? row_id / p.share : 0;
+            const int          in_tile = fourfold ? lane : thread, tile0 = pair ? group * p.tile_rows : 0;
+            const int          row_id  = seg.row0 + tile0 + in_tile;  // of the sequence
+            const int          rows    = min(seg.rows - tile0, p.tile_rows);
+            const bool         valid   = in_tile < rows;
+            const bool         busy    = (in_tile & ~31) < rows;  // the warp has a row
+            const int          token   = valid ? attn_token(p, row_id) : 0;
             const int          head    = seg.head * p.share + (valid ? row_id - token * p.share : 0);
             const long long    in_row  = static_cast<long long>(head) * HEAD_DIM;
             const AttnRow      row     = attn_row(p, seg, row_id, valid);
-            if (pair || group == 0) {  // this group's tile of Q: a warp's rows, whole rows at a time
-                const long long from = valid ? (seg.first + token) * p.ld_q + in_row : -1;
-                unsigned char*  dst  = smem + (pair ? group * kTileBytes : 0) + (thread & ~31) * 128;
-                uint4           v[kRowChunks];
-#pragma unroll
-                for (int k = 0; k < kRowChunks; ++k) {
-                    const long long at = __shfl_sync(0xffffffffu, from, k * (32 / kRowChunks) + lane / kRowChunks);
-                    v[k]               = ptx::ldg_v4_if(p.q + at + lane % kRowChunks * 8, at >= 0);
-                }
-#pragma unroll
-                for (int k = 0; k < kRowChunks; ++k)
-                    *reinterpret_cast<uint4*>(dst + attn_chunk(k * (32 / kRowChunks) + lane / kRowChunks, lane % kRowChunks)) = v[k];
-                ptx::fence_proxy_async_smem();
-                __syncwarp();
-                if (lane == 0)
-                    ptx::mbar_arrive(ptx::smem_u32(&sh.q_full[pair ? group : 0]));
-            }
             const int open  = seg.open[group];
             const int tiles = seg.count_of(group);
             AttnState st{};
@@ -836,9 +870,11 @@ attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
                 ptx::tc_fence_after_sync();
                 const int step   = fourfold ? 32 : kAttnRows;
                 float     newtop = -CUDART_INF_F, newsum = 0.0f;
+#pragma unroll 1
                 for (int r = fourfold ? lane : thread; r < kAttnRows; r += step)
                     newtop = fmaxf(newtop, fmaxf(sh.top[0][r], sh.top[1][r]));
                 auto weight = [&](float top) { return top == newtop ? 1.0f : ptx::exp2_approx((top - newtop) * st.factor); };
+#pragma unroll 1
                 for (int r = fourfold ? lane : thread; r < kAttnRows; r += step)
                     newsum += sh.sum[0][r] * weight(sh.top[0][r]) + sh.sum[1][r] * weight(sh.top[1][r]);
                 keep       = weight(st.top);
@@ -859,75 +895,104 @@ attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
                                  + (static_cast<size_t>(2 * blockIdx.x + slot) * 2 + tile_row) * (HEAD_DIM / 4) * kAttnRows;
             const uint32_t(&list)[3][4] = sh.not_finite[number % kAttnSegments];
             const float inverse         = st.sum == 0.0f ? 0.0f : 1.0f / st.sum;
-            uint32_t    any             = 0;
-#pragma unroll
-            for (int k = 0; k < 12; ++k)
-                any |= (&list[0][0])[k];
-            // An accumulator that no product has written is not read: this group's without a tile of its own, where the groups
+            const bool  any             = sh.any_not_finite[number % kAttnSegments] != 0;
+            // An accumulator that no product has written may hold anything: this group's without a tile of its own, where the groups
             // share the rows the second group's with a single tile.
             const bool mine_there = pair ? tiles > 0 : group == 0 || join, other_there = !pair && (group == 1 || join);
             // 16 columns of this lane's row, both groups' where they share it
             auto outputs = [&](int c, float(&o)[16]) {
-                uint32_t x[16];
+                uint32_t x[16], y[16];
+                ptx::tmem_ld_x16(o_tmem + c, x);
+                if (!pair)
+                    ptx::tmem_ld_x16(tmem + kO + (group ^ 1) * 128 + lanes + c, y);
+                ptx::tmem_wait_ld();
 #pragma unroll
-                for (int k = 0; k < 16; ++k)
-                    o[k] = 0.0f;
-                if (mine_there) {
-                    ptx::tmem_ld_x16(o_tmem + c, x);
-                    ptx::tmem_wait_ld();
-#pragma unroll
-                    for (int k = 0; k < 16; ++k) {
-                        asm volatile("" : "+r"(x[k]));
-                        o[k] = __uint_as_float(x[k]) * keep;
-                    }
-                }
-                if (other_there) {
-                    ptx::tmem_ld_x16(tmem + kO + (group ^ 1) * 128 + lanes + c, x);
-                    ptx::tmem_wait_ld();
-#pragma unroll
-                    for (int k = 0; k < 16; ++k) {
-                        asm volatile("" : "+r"(x[k]));
-                        o[k] = fmaf(__uint_as_float(x[k]), keep_other, o[k]);
-                    }
+                for (int k = 0; k < 16; ++k) {
+                    asm volatile("" : "+r"(x[k]), "+r"(y[k]));
+                    o[k] = mine_there ? __uint_as_float(x[k]) * keep : 0.0f;
+                    o[k] = other_there ? fmaf(__uint_as_float(y[k]), keep_other, o[k]) : o[k];
                 }
             };
             if (fourfold) {
-                float4* const staged = reinterpret_cast<float4*>(smem + group * kTileBytes);  // [columns / 4][lane], in Q's place
+                float4* const staged = sh.staged[group];  // [4 x 4 columns][lane]
 #pragma unroll 1
                 for (int c = column0; c < column1; c += 16) {
                     float o[16];
                     outputs(c, o);
 #pragma unroll
                     for (int k = 0; k < 16; k += 4)
-                        staged[(c - column0 + k) / 4 * kAttnRows + thread] = make_float4(o[k], o[k + 1], o[k + 2], o[k + 3]);
-                }
-                ptx::named_barrier_sync(2 + group, 128);
+                        staged[k / 4 * kAttnRows + thread] = make_float4(o[k], o[k + 1], o[k + 2], o[k + 3]);
+                    ptx::named_barrier_sync(2 + group, 128);
+                    const int     column = c + 4 * (warp & 3);
+                    const float4* four   = staged + (warp & 3) * kAttnRows + lane;
+                    float         sum4[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-                for (int k = 0; k < HEAD_DIM / 32; ++k) {
-                    const int    at = (warp & 3) + 4 * k, column = column0 + 4 * at;
-                    const float4 a = staged[at * kAttnRows + lane], b = staged[at * kAttnRows + lane + 32],
-                                 c = staged[at * kAttnRows + lane + 64], d = staged[at * kAttnRows + lane + 96];
-                    float o[4] = {(a.x + b.x) + (c.x + d.x), (a.y + b.y) + (c.y + d.y), (a.z + b.z) + (c.z + d.z), (a.w + b.w) + (c.w + d.w)};
+                    for (int copy = 0; copy < 4; ++copy) {
+                        const float4 v = four[32 * copy];
+                        sum4[0] += v.x, sum4[1] += v.y, sum4[2] += v.z, sum4[3] += v.w;
+                    }
                     if (any)
-                        attn_add_not_finite<HEAD_DIM, 4>(p, seg, row, list, column, o);
+                        attn_add_not_finite<HEAD_DIM, 4>(p, seg, row, list, column, sum4);
                     if (valid && ok && whole) {
-                        const half2 x = __floats2half2_rn(o[0] * inverse, o[1] * inverse), y = __floats2half2_rn(o[2] * inverse, o[3] * inverse);
+                        const half2 x = __floats2half2_rn(sum4[0] * inverse, sum4[1] * inverse),
+                                    y = __floats2half2_rn(sum4[2] * inverse, sum4[3] * inverse);
                         *reinterpret_cast<uint2*>(p.out + to + column) =
                             make_uint2(*reinterpret_cast<const uint32_t*>(&x), *reinterpret_cast<const uint32_t*>(&y));
                     }
                     else if (valid && ok)
-                        sums[column / 4 * kAttnRows + lane] = make_float4(o[0], o[1], o[2], o[3]);
+                        sums[column / 4 * kAttnRows + lane] = make_float4(sum4[0], sum4[1], sum4[2], sum4[3]);
+                    ptx::named_barrier_sync(2 + group, 128);
+                }
+            }
+            else if (ok && busy && pair && whole && !any) {
+                // 32 rows x 32 columns at a time through 2 KB of the warp's own, so that neighbouring lanes store neighbours
+                uint4* const    staged = reinterpret_cast<uint4*>(sh.staged[group]) + (warp & 3) * 128;
+                const long long mine   = valid ? to : -1;
+                const int       r      = lane / 4;
+                const long long at[4]  = {__shfl_sync(0xffffffffu, mine, r), __shfl_sync(0xffffffffu, mine, r + 8),
+                                          __shfl_sync(0xffffffffu, mine, r + 16), __shfl_sync(0xffffffffu, mine, r + 24)};
+#pragma unroll 1
+                for (int c = 0; c < HEAD_DIM; c += 32) {
+                    uint32_t x[32];
+                    ptx::tmem_ld_x32(o_tmem + c, x);
+                    ptx::tmem_wait_ld();
+#pragma unroll
+                    for (int k = 0; k < 32; ++k)
+                        asm volatile("" : "+r"(x[k]));
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        uint32_t w[4];
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const half2 h = __floats2half2_rn(__uint_as_float(x[8 * k + 2 * e]) * inverse,
+                                                              __uint_as_float(x[8 * k + 2 * e + 1]) * inverse);
+                            w[e]          = *reinterpret_cast<const uint32_t*>(&h);
+                        }
+                        staged[lane * 4 + (k ^ (lane >> 1 & 3))] = make_uint4(w[0], w[1], w[2], w[3]);
+                    }
+                    __syncwarp();
+                    uint4 v[4];
+#pragma unroll
+                    for (int k = 0; k < 4; ++k)
+                        v[k] = staged[(8 * k + r) * 4 + ((lane ^ (r >> 1)) & 3)];
+#pragma unroll
+                    for (int k = 0; k < 4; ++k)
+                        if (at[k] >= 0)
+                            *reinterpret_cast<uint4*>(p.out + at[k] + c + lane % 4 * 8) = v[k];
+                    __syncwarp();
                 }
             }
             else if (ok && busy) {
-                unsigned char* const staged = smem + tile_row * kTileBytes + (thread & ~31) * 128;  // this warp's rows, in Q's place
+                // 32 rows x 16 columns at a time through 1 KB of the warp's own, so that neighbouring lanes store neighbours
+                uint4* const    staged = reinterpret_cast<uint4*>(sh.staged[group]) + (warp & 3) * 64;
+                const long long mine   = valid ? to : -1;
 #pragma unroll 1
                 for (int c = column0; c < column1; c += 16) {
                     float o[16];
                     outputs(c, o);
                     if (any)
                         attn_add_not_finite<HEAD_DIM, 16>(p, seg, row, list, c, o);
-                    if (valid && whole) {
+                    if (whole) {
 #pragma unroll
                         for (int k = 0; k < 16; k += 8) {
                             uint32_t w[4];
@@ -936,7 +1001,16 @@ attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
                                 const half2 h = __floats2half2_rn(o[k + 2 * e] * inverse, o[k + 2 * e + 1] * inverse);
                                 w[e]          = *reinterpret_cast<const uint32_t*>(&h);
                             }
-                            *reinterpret_cast<uint4*>(staged + attn_chunk(lane, (c + k) / 8)) = make_uint4(w[0], w[1], w[2], w[3]);
+                            staged[lane * 2 + (k / 8 ^ (lane >> 2 & 1))] = make_uint4(w[0], w[1], w[2], w[3]);
+                        }
+                        __syncwarp();
+#pragma unroll
+                        for (int k = 0; k < 2; ++k) {
+                            const int       r  = 16 * k + lane / 2;
+                            const long long at = __shfl_sync(0xffffffffu, mine, r);
+                            const uint4     v  = staged[r * 2 + ((lane ^ r >> 2) & 1)];
+                            if (at >= 0)
+                                *reinterpret_cast<uint4*>(p.out + at + c + lane % 2 * 8) = v;
                         }
                     }
                     else if (valid) {
@@ -946,20 +1020,9 @@ attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
                     }
                     __syncwarp();
                 }
-                if (whole) {  // whole rows at a time
-                    const int       chunks = (column1 - column0) / 8, shift = __ffs(chunks) - 1;
-                    const long long mine   = valid ? to : -1;
-#pragma unroll 4
-                    for (int k = 0; k < chunks; ++k) {
-                        const int       r  = (32 * k + lane) >> shift, chunk = column0 / 8 + (lane & (chunks - 1));
-                        const long long at = __shfl_sync(0xffffffffu, mine, r);
-                        if (at >= 0)
-                            *reinterpret_cast<uint4*>(p.out + at + chunk * 8) = *reinterpret_cast<const uint4*>(staged + attn_chunk(r, chunk));
-                    }
-                }
             }
             if (ok && !whole && valid && column0 == 0 && (!fourfold || thread < 32))
-                reinterpret_cast<float2*>(p.workspace + attn_stats_offset(gridDim.x))[static_cast<size_t>(2 * blockIdx.x + slot) * kAttnItemRows
+                reinterpret_cast<float2*>(p.workspace + attn_stats_offset(gridDim.x))[static_cast<size_t>(2 * blockIdx.x + slot) * kAttnSlotRows
                                                                                       + tile_row * kAttnRows + thread] =
                     make_float2(st.top * st.factor, st.sum);
             if (kind != kPartNone) {
@@ -967,7 +1030,7 @@ attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
                 if (threadIdx.x == 0)
                     parts[slot] = AttnPart{ok ? kind : kPartNone, seg.first, seg.row0, seg.rows, seg.head, {0, 0, 0}};
             }
-            // The barrier before the next segment: both groups are done with both outputs, with Q, and with the joined sums' room.
+            // The barrier before the next segment: both groups are done with both outputs and with the joined sums' room.
             ptx::tc_fence_before_sync();
         }
         if (threadIdx.x == 0) {
@@ -981,68 +1044,89 @@ attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
         if (lane == 0) {
             const uint32_t idesc_s = ptx::umma_idesc_f16_f32(kAttnRows, kAttnKeys);
             const uint32_t idesc_o = ptx::umma_idesc_f16_f32(kAttnRows, HEAD_DIM) | ptx::kUmmaBNMajor;
+            const uint64_t q_desc = ptx::umma_desc_kmajor_sw128(q_base), k_desc = ptx::umma_desc_kmajor_sw128(k_base);
+            const uint64_t v_desc  = ptx::umma_desc_nmajor_sw128(v_base, kBlock);
             uint32_t       loaded  = 0;  // tiles of keys before this segment
-            uint32_t       q_parity[2] = {0, 0}, p_parity[2] = {0, 0};
+            uint32_t       q_parity0 = 0, q_parity1 = 0, p_parity0 = 0, p_parity1 = 0;
             bool           ok = true;
-            const AttnSegment* current = nullptr;
-            auto               scores  = [&](int group, int tile, bool last_user) {
-                const AttnSegment& seg = *current;
-                const uint32_t     n = loaded + static_cast<uint32_t>(tile - seg.begin), stage = n % kStages;
+            // What one group's next step takes, with everything but the group known to the compiler (a thread by itself pays
+            // for every instruction: an array in its place took the whole kernel from 840 to 970 us a prompt of 7000).
+            int  tiles0 = 0, tiles1 = 0;
+            bool pair = false;
+            auto stage_of = [&](int group, int i) { return loaded + static_cast<uint32_t>(pair ? i : group + 2 * i); };
+            auto scores   = [&](auto which, int i) {
+                constexpr int  group = decltype(which)::value;
+                const uint32_t n = stage_of(group, i), stage = n % kStages;
+                const uint64_t q = q_desc + (pair ? group * (kTileBytes >> 4) : 0), k = k_desc + stage * (kTileBytes >> 4);
+                const bool     last = i + 1 == (group == 0 ? tiles0 : tiles1);
                 if (!attn_wait(&sh.k_full[stage], n / kStages & 1u, sh, status))
                     return false;
                 ptx::tc_fence_after_sync();
-                const uint64_t q = ptx::umma_desc_kmajor_sw128(q_base + (seg.pair ? group * kTileBytes : 0));
-                const uint64_t k = ptx::umma_desc_kmajor_sw128(k_base + stage * kTileBytes);
 #pragma unroll
                 for (int step = 0; step < HEAD_DIM / 16; ++step) {
                     const uint64_t at = (step / 4) * (kBlock >> 4) + (step % 4) * 2;
                     ptx::umma_f16_ss(tmem + kS + group * 128, q + at, k + at, idesc_s, step > 0);
                 }
-                if (last_user)
-                    ptx::umma_commit(ptx::smem_u32(&sh.k_empty[stage]));
                 ptx::umma_commit(ptx::smem_u32(&sh.s_full[group]));
+                if (!pair || group == 1)  // the last to need this tile of keys
+                    ptx::umma_commit(ptx::smem_u32(&sh.k_empty[stage]));
+                // Q's room is free for the next segment's after the group's last scores; where the groups share it, after the last
+                // of both (the groups take turns: the second's if their numbers are even, else the first's).
+                if (last && (pair || (tiles0 == tiles1) == (group == 1)))
+                    ptx::umma_commit(ptx::smem_u32(&sh.q_empty[pair ? group : 0]));
                 return true;
             };
-            for (int number = 0; ok && (current = attn_segment(sh, number, status)) != nullptr; ++number) {
-                const AttnSegment& seg      = *current;
-                const int          tiles[2] = {seg.count_of(0), seg.count_of(1)};
-                for (int group = 0; ok && group < 2; ++group) {
-                    if (seg.pair || group == 0) {
-                        ok = attn_wait(&sh.q_full[group], q_parity[group], sh, status);
-                        q_parity[group] ^= 1u;
-                    }
-                    if (ok && tiles[group] > 0)
-                        ok = scores(group, seg.tile(group, 0), !seg.pair || group == 1);
+            auto products = [&](auto which, int i) {
+                constexpr int  group = decltype(which)::value;
+                const uint32_t n = stage_of(group, i), stage = n % kStages;
+                const uint64_t v = v_desc + stage * (kTileBytes >> 4);
+                uint32_t&      parity = group == 0 ? p_parity0 : p_parity1;
+                if (!attn_wait(&sh.v_clean[stage], n / kStages & 1u, sh, status))
+                    return false;
+#pragma unroll
+                for (int half_tile = 0; half_tile < 2; ++half_tile) {
+                    if (!attn_wait(&sh.p_full[group][half_tile], parity, sh, status))
+                        return false;
+                    ptx::tc_fence_after_sync();
+#pragma unroll
+                    for (int step = 4 * half_tile; step < 4 * half_tile + 4; ++step)
+                        ptx::umma_f16_ts(tmem + kO + group * 128, tmem + kS + group * 128 + step * 8, v + step * (2048 >> 4), idesc_o,
+                                         i > 0 || step > 0);
                 }
-                const int most = max(tiles[0], tiles[1]);
-                for (int i = 0; ok && i < most; ++i)
-                    for (int group = 0; ok && group < 2; ++group) {
-                        if (i >= tiles[group])
-                            continue;
-                        const uint32_t n = loaded + static_cast<uint32_t>(seg.tile(group, i) - seg.begin), stage = n % kStages;
-                        const uint64_t v = ptx::umma_desc_nmajor_sw128(v_base + stage * kTileBytes, kBlock);
-                        ok               = attn_wait(&sh.v_clean[stage], n / kStages & 1u, sh, status);
-#pragma unroll
-                        for (int half_tile = 0; half_tile < 2; ++half_tile) {
-                            ok = ok && attn_wait(&sh.p_full[group][half_tile], p_parity[group], sh, status);
-                            if (!ok)
-                                break;
-                            ptx::tc_fence_after_sync();
-#pragma unroll
-                            for (int step = 4 * half_tile; step < 4 * half_tile + 4; ++step)
-                                ptx::umma_f16_ts(tmem + kO + group * 128, tmem + kS + group * 128 + step * 8, v + step * (2048 >> 4),
-                                                 idesc_o, i > 0 || step > 0);
-                        }
-                        if (!ok)
-                            break;
-                        p_parity[group] ^= 1u;
-                        if (!seg.pair || group == 1)
-                            ptx::umma_commit(ptx::smem_u32(&sh.v_empty[stage]));
-                        ptx::umma_commit(ptx::smem_u32(&sh.o_done[group]));
-                        if (i + 1 < tiles[group])
-                            ok = scores(group, seg.tile(group, i + 1), !seg.pair || group == 1);
+                parity ^= 1u;
+                ptx::umma_commit(ptx::smem_u32(&sh.o_done[group]));
+                if (!pair || group == 1)
+                    ptx::umma_commit(ptx::smem_u32(&sh.v_empty[stage]));
+                return true;
+            };
+            constexpr std::integral_constant<int, 0> first{};
+            constexpr std::integral_constant<int, 1> second{};
+            const AttnSegment*                       current = nullptr;
+#pragma unroll 1
+            for (int number = 0; ok && (current = attn_segment(sh, number, status)) != nullptr; ++number) {
+                tiles0 = current->count_of(0);
+                tiles1 = current->count_of(1);
+                pair   = current->pair;
+                const int length = current->end - current->begin;
+                if (tiles0 > 0) {
+                    ok = attn_wait(&sh.q_full[0], q_parity0, sh, status) && scores(first, 0);
+                    q_parity0 ^= 1u;
+                }
+                if (ok && tiles1 > 0) {
+                    if (pair) {
+                        ok = attn_wait(&sh.q_full[1], q_parity1, sh, status);
+                        q_parity1 ^= 1u;
                     }
-                loaded += seg.end - seg.begin;
+                    ok = ok && scores(second, 0);
+                }
+#pragma unroll 1
+                for (int i = 0; ok && (i < tiles0 || i < tiles1); ++i) {
+                    if (i < tiles0)
+                        ok = products(first, i) && (i + 1 >= tiles0 || scores(first, i + 1));
+                    if (ok && i < tiles1)
+                        ok = products(second, i) && (i + 1 >= tiles1 || scores(second, i + 1));
+                }
+                loaded += length;
             }
         }
         __syncwarp();
@@ -1068,13 +1152,6 @@ attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
             }
             if (seg.end == 0)
                 break;
-            // The rows of Q on their way to L2 before the keys and values that they would otherwise queue behind.
-            for (int r = lane; r < seg.rows; r += 32) {
-                const int   token = (seg.row0 + r) / p.share, head = seg.head * p.share + (seg.row0 + r) % p.share;
-                const half* q     = p.q + (seg.first + token) * p.ld_q + static_cast<long long>(head) * HEAD_DIM;
-                for (int c = 0; c < HEAD_DIM; c += 64)
-                    ptx::prefetch_l2(q + c);
-            }
             const int* table = c.page_table + static_cast<long long>(seg.b) * c.table_width;
             for (int t = seg.begin; ok && t < seg.end; ++t, ++n) {
                 const int key   = t * kAttnKeys + piece * box;
@@ -1105,29 +1182,53 @@ attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
         }
     }
     else {
-        // ================================================================ values that no product may see: behind the last key, not finite
-        const int t64  = threadIdx.x - kAttnCleanWarp * 32;
-        uint32_t  n    = 0;
-        bool      ok   = true;
+        // ================================================================ rows of Q, and values that no product may see
+        const int t64         = threadIdx.x - kAttnHelpWarp * 32;
+        uint32_t  n           = 0, q_parity[2] = {1, 1};
+        bool      ok          = true;
         for (int number = 0;; ++number) {
             const AttnSegment* const current = attn_segment(sh, number, status);
             uint32_t(&list)[3][4] = sh.not_finite[number % kAttnSegments];
             if (t64 < 12)
                 (&list[0][0])[t64] = 0u;
+            if (t64 == 0)
+                sh.any_not_finite[number % kAttnSegments] = 0u;
             if (ptx::named_barrier_any(4, 64, current == nullptr || !ok))  // all or none
                 break;
             const AttnSegment& seg  = *current;
             const int          open = seg.open[0];
+            if (t64 == 0) {
+                const CUtensorMap* map   = seg.fourfold ? &map_q_few : &map_q;
+                const int          bytes = (seg.fourfold ? 4 * p.few_rows : p.tile_rows) * HEAD_DIM * 2;
+#pragma unroll
+                for (int tile = 0; tile < 2; ++tile) {
+                    if ((tile == 1 && !seg.pair) || seg.count_of(tile) == 0)
+                        continue;
+                    ok = ok && attn_wait(&sh.q_empty[tile], q_parity[tile], sh, status);
+                    q_parity[tile] ^= 1u;
+                    if (!ok)
+                        continue;
+                    const uint32_t bar   = ptx::smem_u32(&sh.q_full[tile]), dst = q_base + tile * kTileBytes;
+                    const int      token = seg.first + attn_token(p, seg.row0 + tile * p.tile_rows);
+                    ptx::mbar_arrive_expect_tx(bar, bytes);
+#pragma unroll
+                    for (int block = 0; block < kBlocks; ++block)
+                        for (int copy = 0; copy < (seg.fourfold ? 4 : 1); ++copy)
+                            ptx::tma_load_3d(dst + block * kBlock + copy * 32 * 128, map, block * 64, seg.head * p.share, token, bar);
+                }
+            }
             for (int t = seg.begin; t < seg.end; ++t, ++n) {
                 const uint32_t stage = n % kStages;
                 ok                   = attn_wait(&sh.v_full[stage], n / kStages & 1u, sh, status);
                 if (!ok)
                     break;
                 if ((t + 1) * kAttnKeys > open) {
+#pragma unroll 1
                     for (int r = t64; r < kAttnKeys; r += 64) {
                         const int key = t * kAttnKeys + r;
                         uint4*    v   = reinterpret_cast<uint4*>(smem + (2 + kStages) * kTileBytes + stage * kTileBytes + r * 128);
                         bool      bad = false;
+#pragma unroll 2
                         for (int x = 0; x < HEAD_DIM / 8; ++x) {
                             uint4& at = v[(x / 8) * (kBlock / 16) + ((x + r) & 7)];  // any order of chunks: banks
                             uint4  w  = key < seg.keys ? at : make_uint4(0, 0, 0, 0);
@@ -1142,8 +1243,10 @@ attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
                                 at = make_uint4(clean(w.x), clean(w.y), clean(w.z), clean(w.w));
                             }
                         }
-                        if (bad && seg.tiles - 1 - t < 3)
+                        if (bad && seg.tiles - 1 - t < 3) {
                             atomicOr(&list[seg.tiles - 1 - t][r / 32], 1u << r % 32);
+                            sh.any_not_finite[number % kAttnSegments] = 1u;
+                        }
                     }
                     ptx::fence_proxy_async_smem();
                 }
@@ -1174,8 +1277,10 @@ __global__ void __launch_bounds__(256) attention_join_kernel(const AttentionPara
     const float4* const   sums  = reinterpret_cast<const float4*>(p.workspace + attn_sums_offset(ctas));
     const int             cta = blockIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const AttnPart        last = parts[2 * cta];
-    const int             row  = blockIdx.y * 32 + lane;  // of the item
-    if (last.kind != kPartEnds || static_cast<int>(blockIdx.y) * 32 >= last.rows)
+    const int             place = blockIdx.y * 32 + lane;  // in a part: tile of rows, row of the tile
+    const int             row   = place / kAttnRows * p.tile_rows + place % kAttnRows;  // of the item
+    const bool            valid = place % kAttnRows < p.tile_rows && row < last.rows;
+    if (last.kind != kPartEnds || !__any_sync(0xffffffffu, valid))
         return;
     // The CTA whose segment began the item.
     int begin = cta - 1;
@@ -1186,7 +1291,7 @@ __global__ void __launch_bounds__(256) attention_join_kernel(const AttentionPara
     auto  slot = [&](int c) { return static_cast<size_t>(2 * c + (c == begin ? 1 : 0)); };
     float top  = -CUDART_INF_F;
     for (int c = begin; c <= cta; ++c)
-        top = fmaxf(top, stats[slot(c) * kAttnItemRows + row].x);
+        top = fmaxf(top, stats[slot(c) * kAttnSlotRows + place].x);
     constexpr int kPer = HEAD_DIM / 4 / 8;  // float4 columns of a warp
     float4        o[kPer];
     float         sum = 0.0f;
@@ -1194,10 +1299,10 @@ __global__ void __launch_bounds__(256) attention_join_kernel(const AttentionPara
     for (int k = 0; k < kPer; ++k)
         o[k] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
     for (int c = begin; c <= cta; ++c) {
-        const float2 stat = stats[slot(c) * kAttnItemRows + row];
+        const float2 stat = stats[slot(c) * kAttnSlotRows + place];
         const float  keep = stat.x == top ? 1.0f : ptx::exp2_approx(stat.x - top);
         sum += stat.y * keep;
-        const float4* src = sums + ((slot(c) * 2 + row / kAttnRows) * (HEAD_DIM / 4) + warp * kPer) * kAttnRows + row % kAttnRows;
+        const float4* src = sums + ((slot(c) * 2 + place / kAttnRows) * (HEAD_DIM / 4) + warp * kPer) * kAttnRows + place % kAttnRows;
 #pragma unroll
         for (int k = 0; k < kPer; ++k) {
             const float4 v = src[k * kAttnRows];
@@ -1207,11 +1312,11 @@ __global__ void __launch_bounds__(256) attention_join_kernel(const AttentionPara
             o[k].w         = fmaf(v.w, keep, o[k].w);
         }
     }
-    if (row >= last.rows)
+    if (!valid)
         return;
     const float inverse = sum == 0.0f ? 0.0f : 1.0f / sum;
     const int   r       = last.row0 + row;
-    half* out = p.out + (static_cast<long long>(last.first + r / p.share) * p.heads + last.head * p.share + r % p.share) * HEAD_DIM
+    half* out = p.out + (static_cast<long long>(last.first + attn_token(p, r)) * p.heads + last.head * p.share + r - attn_token(p, r) * p.share) * HEAD_DIM
                 + warp * kPer * 4;
 #pragma unroll
     for (int k = 0; k < kPer; ++k) {

@@ -597,23 +597,6 @@ __device__ __forceinline__ float max3_nan(float a, float b, float c)
     return d;
 }
 
-// 16 bytes where the predicate holds, zeros elsewhere.  Loads written one behind another are issued one behind another, ahead of
-// the first use.
-__device__ __forceinline__ uint4 ldg_v4_if(const void* p, bool there)
-{
-    uint4 v = make_uint4(0, 0, 0, 0);
-    asm volatile(
-        "{\n"
-        ".reg .pred p;\n"
-        "setp.ne.u32 p, %5, 0;\n"
-        "@p ld.global.v4.u32 {%0, %1, %2, %3}, [%4];\n"
-        "}\n"
-        : "+r"(v.x), "+r"(v.y), "+r"(v.z), "+r"(v.w)
-        : "l"(p), "r"(there ? 1u : 0u)
-        : "memory");
-    return v;
-}
-
 // 1/x within 1 ulp.
 __device__ __forceinline__ float rcp_approx(float x)
 {

@@ -51,7 +51,7 @@ def test_bad_arguments_of_each_operator_are_refused(lib):
                    dict(magnitude=math.inf), dict(magnitude=math.nan)):
         _refused(lib, lambda: lib.rotary_append(0, **{**append, **change}))
     attend = dict(Q=P, ld_q=512, batch=b, heads=4, Out=P, workspace=P)
-    for change in (dict(Q=None), dict(Q=P + 8), dict(ld_q=504), dict(ld_q=513), dict(heads=3), dict(heads=0), dict(Out=None), dict(Out=P + 4),
+    for change in (dict(Q=None), dict(Q=P + 8), dict(ld_q=504), dict(ld_q=513), dict(heads=3), dict(heads=0), dict(heads=258, ld_q=258 * 128), dict(Out=None), dict(Out=P + 4),
                    dict(workspace=None), dict(workspace=P + 8), dict(scale=0.0), dict(scale=-1.0), dict(scale=math.nan), dict(scale=math.inf),
                    dict(cap=-1.0), dict(cap=math.nan), dict(cap=math.inf)):
         _refused(lib, lambda: lib.prompt_attention(0, **{**attend, **change}))

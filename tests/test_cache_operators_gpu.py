@@ -150,7 +150,7 @@ PROMPTS = [
     ([0], [700], 8, 1, 64, 64, 0.0, False, [333]),
     ([5000], [3], 32, 8, 128, 512, 0.0, False, None),
     ([100 + 7 * i for i in range(70)], [1] * 70, 8, 2, 128, 64, 0.0, True, None),
-    ([31], [1], 130, 1, 64, 16, 0.0, False, None),  # more heads than a tile has rows
+    ([31, 5], [1, 9], 128, 1, 64, 16, 0.0, False, None),  # a token fills a tile of rows
     ([0, 3], [50, 90], 21, 3, 128, 32, 0.0, False, [-5, 1 << 30]),  # prefixes out of range: none, and all
 ]
 
