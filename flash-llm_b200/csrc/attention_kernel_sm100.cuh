@@ -540,7 +540,9 @@ struct AttnState {
     float top, sum;      // the maximum that weights are taken against (of q.k, or of scores times log2 e), their sum
     float factor;        // what turns the scores at hand into powers of two
     float scale, cap;    // of scores in units of log 2; cap 0: none
-    float slope;         // likewise
+    float cap_in;        // products times this are what the tanh takes
+    float slope;         // in units of log 2
+    bool  biased;        // by slopes
     int   place;         // the row's position
     const int* drafted;  // positions of drafted tokens in shared memory, or nullptr
     bool  valid;         // the row is somebody's
@@ -559,90 +561,12 @@ __device__ __forceinline__ float2 attn_tanh_small(float2 x)
     return ptx::mul_x2(x, t);
 }
 
-// One tile of scores of one row, columns `column` up to column + COLUMNS of 128: from tensor memory to weights there.  The tile's
-// first key is `key0`; keys before `open` are seen by all rows.  `rescale(keep)` multiplies the row's output by `keep`, and is
-// called by whole warps.  `part_done(half)` tells that the weights of that half of the tile are in place.
-template<bool PLAIN, int COLUMNS, typename Rescale, typename PartDone>
-__device__ __forceinline__ void attn_softmax(AttnState& st, const AttnRow& row, uint32_t s_tmem, int column, int key0, int open,
-                                             bool first, Rescale&& rescale, PartDone&& part_done)
+// The largest of a row's scores, NaN if one of them is.
+template<int COLUMNS>
+__device__ __forceinline__ float attn_largest(const float (&s)[COLUMNS], float m0)
 {
-    float s[COLUMNS];
-    {
-        uint32_t(&raw)[COLUMNS] = reinterpret_cast<uint32_t(&)[COLUMNS]>(s);
-#pragma unroll
-        for (int c = 0; c < COLUMNS; c += 32)
-            ptx::tmem_ld_x32(s_tmem + column + c, raw + c);
-        ptx::tmem_wait_ld();
-#pragma unroll
-        for (int c = 0; c < COLUMNS; ++c)
-            asm volatile("" : "+r"(raw[c]));  // not read before the wait
-    }
-    const bool masked = key0 + kAttnKeys > open;
-    if constexpr (!PLAIN) {
-        if (st.cap > 0.0f) {
-            // Scores are mostly small against the cap: then a polynomial, half the cost of two approximations by the special
-            // function unit, which the weights need too.
-            float2 largest = make_float2(0.0f, 0.0f);
-#pragma unroll
-            for (int c = 0; c < COLUMNS; c += 4) {
-                largest.x = ptx::max3_nan(largest.x, fabsf(s[c]), fabsf(s[c + 1]));
-                largest.y = ptx::max3_nan(largest.y, fabsf(s[c + 2]), fabsf(s[c + 3]));
-            }
-            const float in = st.scale / st.cap;  // the cap is in units of log 2, as the scale is
-            if (__all_sync(0xffffffffu, !st.valid || fmaxf(largest.x, largest.y) * in <= 1.0f)) {
-#pragma unroll
-                for (int c = 0; c < COLUMNS; c += 2) {
-                    const float2 t = ptx::mul_x2(attn_tanh_small(ptx::mul_x2(make_float2(s[c], s[c + 1]), make_float2(in, in))),
-                                                 make_float2(st.cap, st.cap));
-                    s[c]           = t.x;
-                    s[c + 1]       = t.y;
-                }
-            }
-            else {
-                const float twice = 2.0f * CUDART_L2E_F * in;  // tanh x = 1 - 2 / (1 + e^2x)
-#pragma unroll
-                for (int c = 0; c < COLUMNS; ++c)
-                    s[c] = fmaf(-2.0f * st.cap, ptx::rcp_approx(1.0f + ptx::exp2_approx(s[c] * twice)), st.cap);
-            }
-        }
-        else {
-#pragma unroll
-            for (int c = 0; c < COLUMNS; c += 2) {
-                const float2 t = ptx::mul_x2(make_float2(s[c], s[c + 1]), make_float2(st.scale, st.scale));
-                s[c]           = t.x;
-                s[c + 1]       = t.y;
-            }
-        }
-        if (st.drafted != nullptr && masked) {
-#pragma unroll
-            for (int c = 0; c < COLUMNS; ++c) {
-                const int key   = key0 + column + c, i = key - open;
-                const int where = i >= 0 && i < kMaxDrafted ? st.drafted[i] : key;
-                s[c]            = fmaf(st.slope, static_cast<float>(where - st.place), s[c]);
-            }
-        }
-        else {
-            const float  away  = st.slope * static_cast<float>(key0 + column - st.place);
-            const float2 slope = make_float2(st.slope, st.slope), base = make_float2(away, away);
-#pragma unroll
-            for (int c = 0; c < COLUMNS; c += 2) {
-                const float2 far = ptx::fma_x2(slope, make_float2(static_cast<float>(c), static_cast<float>(c + 1)), base);
-                const float2 t   = ptx::add_x2(make_float2(s[c], s[c + 1]), far);
-                s[c]             = t.x;
-                s[c + 1]         = t.y;
-            }
-        }
-    }
-    if (masked) {
-#pragma unroll
-        for (int k = 0; k < COLUMNS / 32; ++k) {
-            const uint32_t seen = row.word(key0 + column + 32 * k);
-#pragma unroll
-            for (int c = 0; c < 32; ++c)
-                s[32 * k + c] = seen >> c & 1u ? s[32 * k + c] : -CUDART_INF_F;
-        }
-    }
-    float m[4] = {s[0], s[1], s[2], s[3]};
+    float m[4] = {m0, s[1], s[2], s[3]};
+    m[0]       = ptx::max3_nan(m0, s[0], s[0]);
 #pragma unroll
     for (int c = 4; c < COLUMNS - 4; c += 8)
 #pragma unroll
@@ -651,7 +575,88 @@ __device__ __forceinline__ void attn_softmax(AttnState& st, const AttnRow& row, 
 #pragma unroll
     for (int k = 0; k < 4; ++k)
         m[k] = ptx::max3_nan(m[k], s[COLUMNS - 4 + k], m[k]);
-    float new_top = ptx::max3_nan(ptx::max3_nan(m[0], m[1], m[2]), m[3], st.top);
+    return ptx::max3_nan(ptx::max3_nan(m[0], m[1], m[2]), m[3], m[3]);
+}
+
+// 32 products of a row to scores in units of log 2, capped and biased: those with the keys from `key0` on.  `drafted`: keys at and
+// behind `open` may stand elsewhere than they lie.
+__device__ __forceinline__ void attn_transform(const AttnState& st, float (&s)[32], int key0, int open, bool drafted)
+{
+    if (st.cap > 0.0f) {
+        // Scores are mostly small against the cap: then a polynomial, a third of the cost of two approximations by the special
+        // function unit, which the weights need too.
+        float2 largest = make_float2(0.0f, 0.0f);
+#pragma unroll
+        for (int c = 0; c < 32; c += 4) {
+            largest.x = ptx::max3_nan(largest.x, fabsf(s[c]), fabsf(s[c + 1]));
+            largest.y = ptx::max3_nan(largest.y, fabsf(s[c + 2]), fabsf(s[c + 3]));
+        }
+        const float in = st.cap_in;
+        if (__all_sync(0xffffffffu, !st.valid || ptx::max3_nan(largest.x, largest.y, largest.y) * in <= 1.0f)) {
+#pragma unroll
+            for (int c = 0; c < 32; c += 2) {
+                const float2 t = ptx::mul_x2(attn_tanh_small(ptx::mul_x2(make_float2(s[c], s[c + 1]), make_float2(in, in))),
+                                             make_float2(st.cap, st.cap));
+                s[c]           = t.x;
+                s[c + 1]       = t.y;
+            }
+        }
+        else {
+            const float twice = 2.0f * CUDART_L2E_F * in;  // tanh x = 1 - 2 / (1 + e^2x)
+#pragma unroll
+            for (int c = 0; c < 32; ++c)
+                s[c] = fmaf(-2.0f * st.cap, ptx::rcp_approx(1.0f + ptx::exp2_approx(s[c] * twice)), st.cap);
+        }
+    }
+    else {
+#pragma unroll
+        for (int c = 0; c < 32; c += 2) {
+            const float2 t = ptx::mul_x2(make_float2(s[c], s[c + 1]), make_float2(st.scale, st.scale));
+            s[c]           = t.x;
+            s[c + 1]       = t.y;
+        }
+    }
+    if (!st.biased)
+        return;
+    if (drafted) {
+#pragma unroll
+        for (int c = 0; c < 32; ++c) {
+            const int key   = key0 + c, i = key - open;
+            const int where = i >= 0 && i < kMaxDrafted ? st.drafted[i] : key;
+            s[c]            = fmaf(st.slope, static_cast<float>(where - st.place), s[c]);
+        }
+    }
+    else {
+        const float  away  = st.slope * static_cast<float>(key0 - st.place);
+        const float2 slope = make_float2(st.slope, st.slope), base = make_float2(away, away);
+#pragma unroll
+        for (int c = 0; c < 32; c += 2) {
+            const float2 far = ptx::fma_x2(slope, make_float2(static_cast<float>(c), static_cast<float>(c + 1)), base);
+            const float2 t   = ptx::add_x2(make_float2(s[c], s[c + 1]), far);
+            s[c]             = t.x;
+            s[c + 1]         = t.y;
+        }
+    }
+}
+
+// Minus infinity for the keys, from `key0` on, that the row does not see.
+template<int COLUMNS>
+__device__ __forceinline__ void attn_mask(const AttnRow& row, float (&s)[COLUMNS], int key0)
+{
+#pragma unroll
+    for (int k = 0; k < COLUMNS / 32; ++k) {
+        const uint32_t seen = row.word(key0 + 32 * k);
+#pragma unroll
+        for (int c = 0; c < 32; ++c)
+            s[32 * k + c] = seen >> c & 1u ? s[32 * k + c] : -CUDART_INF_F;
+    }
+}
+
+// The maximum that weights are taken against, from the largest score of a tile.  `rescale(keep)` multiplies the row's output by
+// `keep`, and is called by whole warps.
+template<typename Rescale>
+__device__ __forceinline__ void attn_new_top(AttnState& st, float new_top, bool first, Rescale&& rescale)
+{
     if (!(new_top < CUDART_INF_F)) {  // a score that is no number, or infinity less itself: neither has the row's output a number
         st.sum  = CUDART_NAN_F;
         new_top = st.top;
@@ -659,45 +664,127 @@ __device__ __forceinline__ void attn_softmax(AttnState& st, const AttnRow& row, 
     if (first)
         st.top = new_top;
     else if (__any_sync(0xffffffffu, st.valid && (new_top - st.top) * st.factor > 8.0f)) {  // rows of nobody have no say
-        // The maximum that the weights are taken against moves only when it has grown by more than 2^8, which 32-bit sums and
-        // fp16 weights have room for: rarely after the first tiles.
+        // It moves only when it has grown by more than 2^8, which 32-bit sums and fp16 weights have room for: rarely after the
+        // first tiles.
         const float keep = new_top == st.top ? 1.0f : ptx::exp2_approx((st.top - new_top) * st.factor);
         st.top           = new_top;
         st.sum *= keep;
         rescale(keep);
     }
-    const float  minus   = st.top == -CUDART_INF_F ? 0.0f : -st.top * st.factor;
-    float2       part[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
-    if constexpr (COLUMNS < kAttnKeys) {  // the other copies' keys
-        const uint32_t zeros[16] = {0};
+}
+
+// 32 scores to weights, rounded to fp16 in pairs; `part` takes their sums before the rounding.
+template<bool PLAIN>
+__device__ __forceinline__ void attn_weights(const float* s, float factor, float minus, float2 (&part)[2], uint32_t (&w)[16])
+{
 #pragma unroll
-        for (int c = 0; c < kAttnKeys; c += 32)
+    for (int k = 0; k < 16; ++k) {
+        float2 x = make_float2(s[2 * k], s[2 * k + 1]);
+        if constexpr (PLAIN)
+            x = ptx::fma_x2(x, make_float2(factor, factor), make_float2(minus, minus));
+        else
+            x = ptx::add_x2(x, make_float2(minus, minus));
+        x             = make_float2(ptx::exp2_approx(x.x), ptx::exp2_approx(x.y));
+        part[k & 1]   = ptx::add_x2(part[k & 1], x);
+        const half2 h = __floats2half2_rn(x.x, x.y);
+        w[k]          = *reinterpret_cast<const uint32_t*>(&h);
+    }
+}
+
+template<int COLUMNS>
+__device__ __forceinline__ void attn_load_scores(uint32_t s_tmem, float (&s)[COLUMNS])
+{
+    uint32_t(&raw)[COLUMNS] = reinterpret_cast<uint32_t(&)[COLUMNS]>(s);
+#pragma unroll
+    for (int c = 0; c < COLUMNS; c += 32)
+        ptx::tmem_ld_x32(s_tmem + c, raw + c);
+    ptx::tmem_wait_ld();
+#pragma unroll
+    for (int c = 0; c < COLUMNS; ++c)
+        asm volatile("" : "+r"(raw[c]));  // not read before the wait
+}
+
+// One tile of scores of one row, from tensor memory to weights there: all 128 of them, or, where the row lies in the tile four
+// times, the 32 from `column` on and zeros for the others.  The tile's first key is `key0`; keys before `open` are seen by all
+// rows.  `part_done(half)` tells that the weights of that half of the tile are in place.
+template<bool PLAIN, bool FOURFOLD, typename Rescale, typename PartDone>
+__device__ __forceinline__ void attn_softmax(AttnState& st, const AttnRow& row, uint32_t s_tmem, int column, int key0, int open,
+                                             bool first, Rescale&& rescale, PartDone&& part_done)
+{
+    const bool masked  = key0 + kAttnKeys > open;
+    float2     part[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
+    auto       stored  = [&]() {
+        ptx::tmem_wait_st();
+        ptx::tc_fence_before_sync();
+        __syncwarp();
+    };
+    if constexpr (FOURFOLD) {
+        float s[32];
+        attn_load_scores(s_tmem + column, s);
+        if constexpr (!PLAIN)
+            attn_transform(st, s, key0 + column, open, masked && st.drafted != nullptr);
+        if (masked)
+            attn_mask(row, s, key0 + column);
+        attn_new_top(st, attn_largest(s, st.top), first, rescale);
+        const float    minus     = st.top == -CUDART_INF_F ? 0.0f : -st.top * st.factor;
+        const uint32_t zeros[16] = {0};
+        uint32_t       w[16];
+#pragma unroll
+        for (int c = 0; c < kAttnKeys; c += 32)  // the other copies' keys
             if (c != column)
                 ptx::tmem_st_x16(s_tmem + c / 2, zeros);
+        attn_weights<PLAIN>(s, st.factor, minus, part, w);
+        ptx::tmem_st_x16(s_tmem + column / 2, w);
+        stored();
+        part_done(0);
+        part_done(1);
     }
+    else if constexpr (PLAIN) {
+        float s[kAttnKeys];
+        attn_load_scores(s_tmem, s);
+        if (masked)
+            attn_mask(row, s, key0);
+        attn_new_top(st, attn_largest(s, st.top), first, rescale);
+        const float minus = st.top == -CUDART_INF_F ? 0.0f : -st.top * st.factor;
 #pragma unroll
-    for (int c = 0; c < COLUMNS; c += 32) {
-        uint32_t w[16];
-#pragma unroll
-        for (int k = 0; k < 16; ++k) {
-            float2 x = make_float2(s[c + 2 * k], s[c + 2 * k + 1]);
-            if constexpr (PLAIN)
-                x = ptx::fma_x2(x, make_float2(st.factor, st.factor), make_float2(minus, minus));
-            else
-                x = ptx::add_x2(x, make_float2(minus, minus));
-            x             = make_float2(ptx::exp2_approx(x.x), ptx::exp2_approx(x.y));
-            part[k & 1]   = ptx::add_x2(part[k & 1], x);
-            const half2 h = __floats2half2_rn(x.x, x.y);
-            w[k]          = *reinterpret_cast<const uint32_t*>(&h);
+        for (int c = 0; c < kAttnKeys; c += 32) {
+            uint32_t w[16];
+            attn_weights<PLAIN>(s + c, st.factor, minus, part, w);
+            ptx::tmem_st_x16(s_tmem + c / 2, w);
+            if (c % 64 == 32) {
+                stored();
+                part_done(c / 64);
+            }
         }
-        ptx::tmem_st_x16(s_tmem + (column + c) / 2, w);
-        if (COLUMNS < kAttnKeys || c % 64 == 32) {
-            ptx::tmem_wait_st();
-            ptx::tc_fence_before_sync();
-            __syncwarp();
-            if (COLUMNS < kAttnKeys)
-                part_done(0);
-            part_done(COLUMNS < kAttnKeys ? 1 : c / 64);
+    }
+    else {
+        // 32 columns at a time, the transformed scores back to tensor memory in between: with all 128 in registers the code of one
+        // tile did not fit the instruction cache (capped trees of 64 tokens 90 us, now @CAPNOW@).
+        float new_top = st.top;
+#pragma unroll 1
+        for (int c = 0; c < kAttnKeys; c += 32) {
+            float s[32];
+            attn_load_scores(s_tmem + c, s);
+            attn_transform(st, s, key0 + c, open, masked && st.drafted != nullptr);
+            if (masked)
+                attn_mask(row, s, key0 + c);
+            new_top = attn_largest(s, new_top);
+            ptx::tmem_st_x32(s_tmem + c, reinterpret_cast<const uint32_t*>(s));
+        }
+        ptx::tmem_wait_st();
+        attn_new_top(st, new_top, first, rescale);
+        const float minus = st.top == -CUDART_INF_F ? 0.0f : -st.top * st.factor;
+#pragma unroll 1
+        for (int c = 0; c < kAttnKeys; c += 32) {  // weights take the place of scores already read
+            float    s[32];
+            uint32_t w[16];
+            attn_load_scores(s_tmem + c, s);
+            attn_weights<PLAIN>(s, st.factor, minus, part, w);
+            ptx::tmem_st_x16(s_tmem + c / 2, w);
+            if (c % 64 == 32) {
+                stored();
+                part_done(c / 64);
+            }
         }
     }
     st.sum += (part[0].x + part[1].x) + (part[0].y + part[1].y);
@@ -801,10 +888,12 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
             st.factor = PLAIN ? p.scale * CUDART_L2E_F : 1.0f;
             if constexpr (!PLAIN) {
                 st.scale = p.scale * CUDART_L2E_F;
-                st.cap   = p.cap * CUDART_L2E_F;
+                st.cap    = p.cap * CUDART_L2E_F;
+                st.cap_in = p.cap > 0.0f ? p.scale / p.cap : 0.0f;
                 st.place = seg.context + token;
                 if (p.slopes) {
-                    st.slope = p.slopes[head] * CUDART_L2E_F;
+                    st.biased = true;
+                    st.slope  = p.slopes[head] * CUDART_L2E_F;
                     if (p.tree_mask) {
                         st.place   = valid ? p.positions[seg.first + token] : 0;
                         st.drafted = sh.drafted[group];
@@ -845,9 +934,9 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
                 }
                 ptx::tc_fence_after_sync();
                 if (fourfold)
-                    attn_softmax<PLAIN, 32>(st, row, s_tmem, thread & ~31, key0, open, i == 0, rescale, part_done);
+                    attn_softmax<PLAIN, true>(st, row, s_tmem, thread & ~31, key0, open, i == 0, rescale, part_done);
                 else if (busy)
-                    attn_softmax<PLAIN, kAttnKeys>(st, row, s_tmem, 0, key0, open, i == 0, rescale, part_done);
+                    attn_softmax<PLAIN, false>(st, row, s_tmem, 0, key0, open, i == 0, rescale, part_done);
                 else {
                     part_done(0);
                     part_done(1);
