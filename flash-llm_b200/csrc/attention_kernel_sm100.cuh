@@ -739,39 +739,25 @@ __device__ __forceinline__ void attn_softmax(AttnState& st, const AttnRow& row, 
         part_done(0);
         part_done(1);
     }
-    else if constexpr (PLAIN) {
-        float s[kAttnKeys];
-        attn_load_scores(s_tmem, s);
-        if (masked)
-            attn_mask(row, s, key0);
-        attn_new_top(st, attn_largest(s, st.top), first, rescale);
-        const float minus = st.top == -CUDART_INF_F ? 0.0f : -st.top * st.factor;
-#pragma unroll
-        for (int c = 0; c < kAttnKeys; c += 32) {
-            uint32_t w[16];
-            attn_weights<PLAIN>(s + c, st.factor, minus, part, w);
-            ptx::tmem_st_x16(s_tmem + c / 2, w);
-            if (c % 64 == 32) {
-                stored();
-                part_done(c / 64);
-            }
-        }
-    }
     else {
-        // 32 columns at a time, the transformed scores back to tensor memory in between: with all 128 in registers the code of one
-        // tile did not fit the instruction cache (capped trees of 64 tokens 90 us, now @CAPNOW@).
+        // 32 columns at a time, masked or transformed scores back to tensor memory in between: with all 128 in registers the code of
+        // one tile does not fit the instruction cache (capped trees of 64 tokens took 90 us instead of 77, ragged prompts 71
+        // instead of 60).
         float new_top = st.top;
 #pragma unroll 1
         for (int c = 0; c < kAttnKeys; c += 32) {
             float s[32];
             attn_load_scores(s_tmem + c, s);
-            attn_transform(st, s, key0 + c, open, masked && st.drafted != nullptr);
+            if constexpr (!PLAIN)
+                attn_transform(st, s, key0 + c, open, masked && st.drafted != nullptr);
             if (masked)
                 attn_mask(row, s, key0 + c);
             new_top = attn_largest(s, new_top);
-            ptx::tmem_st_x32(s_tmem + c, reinterpret_cast<const uint32_t*>(s));
+            if (!PLAIN || masked)
+                ptx::tmem_st_x32(s_tmem + c, reinterpret_cast<const uint32_t*>(s));
         }
-        ptx::tmem_wait_st();
+        if (!PLAIN || masked)
+            ptx::tmem_wait_st();
         attn_new_top(st, new_top, first, rescale);
         const float minus = st.top == -CUDART_INF_F ? 0.0f : -st.top * st.factor;
 #pragma unroll 1
@@ -1129,94 +1115,93 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
         }
     }
     else if (warp == kAttnMmaWarp) {
-        // ================================================================ products: one thread issues them all
-        if (lane == 0) {
-            const uint32_t idesc_s = ptx::umma_idesc_f16_f32(kAttnRows, kAttnKeys);
-            const uint32_t idesc_o = ptx::umma_idesc_f16_f32(kAttnRows, HEAD_DIM) | ptx::kUmmaBNMajor;
-            const uint64_t q_desc = ptx::umma_desc_kmajor_sw128(q_base), k_desc = ptx::umma_desc_kmajor_sw128(k_base);
-            const uint64_t v_desc  = ptx::umma_desc_nmajor_sw128(v_base, kBlock);
-            uint32_t       loaded  = 0;  // tiles of keys before this segment
-            uint32_t       q_parity0 = 0, q_parity1 = 0, p_parity0 = 0, p_parity1 = 0;
-            bool           ok = true;
-            // What one group's next step takes, with everything but the group known to the compiler (a thread by itself pays
-            // for every instruction: an array in its place took the whole kernel from 840 to 970 us a prompt of 7000).
-            int  tiles0 = 0, tiles1 = 0;
-            bool pair = false;
-            auto stage_of = [&](int group, int i) { return loaded + static_cast<uint32_t>(pair ? i : group + 2 * i); };
-            auto scores   = [&](auto which, int i) {
-                constexpr int  group = decltype(which)::value;
-                const uint32_t n = stage_of(group, i), stage = n % kStages;
-                const uint64_t q = q_desc + (pair ? group * (kTileBytes >> 4) : 0), k = k_desc + stage * (kTileBytes >> 4);
-                const bool     last = i + 1 == (group == 0 ? tiles0 : tiles1);
-                if (!attn_wait(&sh.k_full[stage], n / kStages & 1u, sh, status))
+        // ================================================================ products: one converged warp issues them all
+        const uint32_t idesc_s = ptx::umma_idesc_f16_f32(kAttnRows, kAttnKeys);
+        const uint32_t idesc_o = ptx::umma_idesc_f16_f32(kAttnRows, HEAD_DIM) | ptx::kUmmaBNMajor;
+        const uint64_t q_desc = ptx::umma_desc_kmajor_sw128(q_base), k_desc = ptx::umma_desc_kmajor_sw128(k_base);
+        const uint64_t v_desc  = ptx::umma_desc_nmajor_sw128(v_base, kBlock);
+        uint32_t       loaded  = 0;  // tiles of keys before this segment
+        uint32_t       q_parity0 = 0, q_parity1 = 0, p_parity0 = 0, p_parity1 = 0;
+        bool           ok = true;
+        // Everything but the group is known to the compiler, and all lanes come to the same answer.
+        int  tiles0 = 0, tiles1 = 0;
+        bool pair = false;
+        auto have     = [&](const unsigned long long* barrier, uint32_t parity) {
+            return __all_sync(0xffffffffu, attn_wait(barrier, parity, sh, status)) != 0;
+        };
+        auto stage_of = [&](int group, int i) { return loaded + static_cast<uint32_t>(pair ? i : group + 2 * i); };
+        auto scores   = [&](auto which, int i) {
+            constexpr int  group = decltype(which)::value;
+            const uint32_t n = stage_of(group, i), stage = n % kStages;
+            const uint64_t q = q_desc + (pair ? group * (kTileBytes >> 4) : 0), k = k_desc + stage * (kTileBytes >> 4);
+            const bool     last = i + 1 == (group == 0 ? tiles0 : tiles1);
+            if (!have(&sh.k_full[stage], n / kStages & 1u))
+                return false;
+            ptx::tc_fence_after_sync();
+#pragma unroll
+            for (int block = 0; block < kBlocks; ++block)
+                ptx::umma_f16_ss_x4_elect(tmem + kS + group * 128, q + block * (kBlock >> 4), k + block * (kBlock >> 4), idesc_s, block > 0);
+            ptx::umma_commit_elect(ptx::smem_u32(&sh.s_full[group]));
+            if (!pair || group == 1)  // the last to need this tile of keys
+                ptx::umma_commit_elect(ptx::smem_u32(&sh.k_empty[stage]));
+            // Q's room is free for the next segment's after the group's last scores; where the groups share it, after the last
+            // of both (the groups take turns: the second's if their numbers are even, else the first's).
+            if (last && (pair || (tiles0 == tiles1) == (group == 1)))
+                ptx::umma_commit_elect(ptx::smem_u32(&sh.q_empty[pair ? group : 0]));
+            return true;
+        };
+        auto products = [&](auto which, int i) {
+            constexpr int  group = decltype(which)::value;
+            const uint32_t n = stage_of(group, i), stage = n % kStages;
+            const uint64_t v = v_desc + stage * (kTileBytes >> 4);
+            uint32_t&      parity = group == 0 ? p_parity0 : p_parity1;
+            if (!have(&sh.v_clean[stage], n / kStages & 1u))
+                return false;
+#pragma unroll
+            for (int half_tile = 0; half_tile < 2; ++half_tile) {
+                if (!have(&sh.p_full[group][half_tile], parity))
                     return false;
                 ptx::tc_fence_after_sync();
-#pragma unroll
-                for (int step = 0; step < HEAD_DIM / 16; ++step) {
-                    const uint64_t at = (step / 4) * (kBlock >> 4) + (step % 4) * 2;
-                    ptx::umma_f16_ss(tmem + kS + group * 128, q + at, k + at, idesc_s, step > 0);
-                }
-                ptx::umma_commit(ptx::smem_u32(&sh.s_full[group]));
-                if (!pair || group == 1)  // the last to need this tile of keys
-                    ptx::umma_commit(ptx::smem_u32(&sh.k_empty[stage]));
-                // Q's room is free for the next segment's after the group's last scores; where the groups share it, after the last
-                // of both (the groups take turns: the second's if their numbers are even, else the first's).
-                if (last && (pair || (tiles0 == tiles1) == (group == 1)))
-                    ptx::umma_commit(ptx::smem_u32(&sh.q_empty[pair ? group : 0]));
-                return true;
-            };
-            auto products = [&](auto which, int i) {
-                constexpr int  group = decltype(which)::value;
-                const uint32_t n = stage_of(group, i), stage = n % kStages;
-                const uint64_t v = v_desc + stage * (kTileBytes >> 4);
-                uint32_t&      parity = group == 0 ? p_parity0 : p_parity1;
-                if (!attn_wait(&sh.v_clean[stage], n / kStages & 1u, sh, status))
-                    return false;
-#pragma unroll
-                for (int half_tile = 0; half_tile < 2; ++half_tile) {
-                    if (!attn_wait(&sh.p_full[group][half_tile], parity, sh, status))
-                        return false;
-                    ptx::tc_fence_after_sync();
-#pragma unroll
-                    for (int step = 4 * half_tile; step < 4 * half_tile + 4; ++step)
-                        ptx::umma_f16_ts(tmem + kO + group * 128, tmem + kS + group * 128 + step * 8, v + step * (2048 >> 4), idesc_o,
-                                         i > 0 || step > 0);
-                }
-                parity ^= 1u;
-                ptx::umma_commit(ptx::smem_u32(&sh.o_done[group]));
-                if (!pair || group == 1)
-                    ptx::umma_commit(ptx::smem_u32(&sh.v_empty[stage]));
-                return true;
-            };
-            constexpr std::integral_constant<int, 0> first{};
-            constexpr std::integral_constant<int, 1> second{};
-            const AttnSegment*                       current = nullptr;
-#pragma unroll 1
-            for (int number = 0; ok && (current = attn_segment(sh, number, status)) != nullptr; ++number) {
-                tiles0 = current->count_of(0);
-                tiles1 = current->count_of(1);
-                pair   = current->pair;
-                const int length = current->end - current->begin;
-                if (tiles0 > 0) {
-                    ok = attn_wait(&sh.q_full[0], q_parity0, sh, status) && scores(first, 0);
-                    q_parity0 ^= 1u;
-                }
-                if (ok && tiles1 > 0) {
-                    if (pair) {
-                        ok = attn_wait(&sh.q_full[1], q_parity1, sh, status);
-                        q_parity1 ^= 1u;
-                    }
-                    ok = ok && scores(second, 0);
-                }
-#pragma unroll 1
-                for (int i = 0; ok && (i < tiles0 || i < tiles1); ++i) {
-                    if (i < tiles0)
-                        ok = products(first, i) && (i + 1 >= tiles0 || scores(first, i + 1));
-                    if (ok && i < tiles1)
-                        ok = products(second, i) && (i + 1 >= tiles1 || scores(second, i + 1));
-                }
-                loaded += length;
+                ptx::umma_f16_ts_x4_elect(tmem + kO + group * 128, tmem + kS + group * 128 + half_tile * 32,
+                                          v + half_tile * (4 * 2048 >> 4), idesc_o, i > 0 || half_tile > 0);
             }
+            parity ^= 1u;
+            ptx::umma_commit_elect(ptx::smem_u32(&sh.o_done[group]));
+            if (!pair || group == 1)
+                ptx::umma_commit_elect(ptx::smem_u32(&sh.v_empty[stage]));
+            return true;
+        };
+        constexpr std::integral_constant<int, 0> first{};
+        constexpr std::integral_constant<int, 1> second{};
+        const AttnSegment*                       current = nullptr;
+#pragma unroll 1
+        for (int number = 0; ok; ++number) {
+            current = attn_segment(sh, number, status);
+            if (__any_sync(0xffffffffu, current == nullptr))
+                break;
+            tiles0 = current->count_of(0);
+            tiles1 = current->count_of(1);
+            pair   = current->pair;
+            const int length = current->end - current->begin;
+            if (tiles0 > 0) {
+                ok = have(&sh.q_full[0], q_parity0) && scores(first, 0);
+                q_parity0 ^= 1u;
+            }
+            if (ok && tiles1 > 0) {
+                if (pair) {
+                    ok = have(&sh.q_full[1], q_parity1);
+                    q_parity1 ^= 1u;
+                }
+                ok = ok && scores(second, 0);
+            }
+#pragma unroll 1
+            for (int i = 0; ok && (i < tiles0 || i < tiles1); ++i) {
+                if (i < tiles0)
+                    ok = products(first, i) && (i + 1 >= tiles0 || scores(first, i + 1));
+                if (ok && i < tiles1)
+                    ok = products(second, i) && (i + 1 >= tiles1 || scores(second, i + 1));
+            }
+            loaded += length;
         }
         __syncwarp();
     }

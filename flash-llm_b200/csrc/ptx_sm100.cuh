@@ -216,20 +216,6 @@ umma_f16_ss(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, u
         : "memory");
 }
 
-// D[tmem] (+)= A[tmem] * B[smem]: A holds fp16 pairs, one row per lane, two neighbouring K elements per column.
-__device__ __forceinline__ void
-umma_f16_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc, uint32_t accumulate)
-{
-    asm volatile(
-        "{\n"
-        ".reg .pred p;\n"
-        "setp.ne.b32 p, %4, 0;\n"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n"
-        "}\n" ::"r"(d_tmem),
-        "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate)
-        : "memory");
-}
-
 // One 128x64 tile of A times one [N x 64] slab of B: the four K=16 MMAs, the commit that hands the A stage back, an
 // optional second commit (B batch finished), and -- issued first so that its shared-memory round trip overlaps the
 // MMA issue -- a probe of the barriers the NEXT tile needs.  All in one asm block because the probe's predicate must
@@ -306,6 +292,60 @@ __device__ __forceinline__ void umma_tile_elect(uint32_t d_tmem, uint64_t a_desc
         "@pcb tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%6];\n"
         "}\n" ::"r"(d_tmem),
         "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate_first), "r"(commit_a_bar), "r"(commit_b_bar), "r"(do_commit_b)
+        : "memory");
+}
+
+// Four products of K = 16 each by one elected lane of a CONVERGED warp (operands in uniform registers: a thread by itself took half
+// as long again to issue them): A and B in shared memory, 64 K-major columns of the 128-byte swizzle.
+__device__ __forceinline__ void umma_f16_ss_x4_elect(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
+                                                     uint32_t accumulate_first)
+{
+    asm volatile(
+        "{\n"
+        ".reg .pred pacc, ptrue, pe;\n"
+        ".reg .b64 da, db;\n"
+        "setp.ne.b32 pacc, %4, 0;\n"
+        "setp.eq.b32 ptrue, 0, 0;\n"
+        "elect.sync _|pe, 0xffffffff;\n"
+        "@pe tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, pacc;\n"
+        "add.s64 da, %1, 2;\n"
+        "add.s64 db, %2, 2;\n"
+        "@pe tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %3, ptrue;\n"
+        "add.s64 da, %1, 4;\n"
+        "add.s64 db, %2, 4;\n"
+        "@pe tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %3, ptrue;\n"
+        "add.s64 da, %1, 6;\n"
+        "add.s64 db, %2, 6;\n"
+        "@pe tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %3, ptrue;\n"
+        "}\n" ::"r"(d_tmem),
+        "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate_first)
+        : "memory");
+}
+
+// ... A in tensor memory (8 columns per product), B N-major in shared memory (2048 bytes per product).
+__device__ __forceinline__ void umma_f16_ts_x4_elect(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc,
+                                                     uint32_t accumulate_first)
+{
+    asm volatile(
+        "{\n"
+        ".reg .pred pacc, ptrue, pe;\n"
+        ".reg .b64 db;\n"
+        ".reg .b32 ta;\n"
+        "setp.ne.b32 pacc, %4, 0;\n"
+        "setp.eq.b32 ptrue, 0, 0;\n"
+        "elect.sync _|pe, 0xffffffff;\n"
+        "@pe tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, pacc;\n"
+        "add.u32 ta, %1, 8;\n"
+        "add.s64 db, %2, 128;\n"
+        "@pe tcgen05.mma.cta_group::1.kind::f16 [%0], [ta], db, %3, ptrue;\n"
+        "add.u32 ta, %1, 16;\n"
+        "add.s64 db, %2, 256;\n"
+        "@pe tcgen05.mma.cta_group::1.kind::f16 [%0], [ta], db, %3, ptrue;\n"
+        "add.u32 ta, %1, 24;\n"
+        "add.s64 db, %2, 384;\n"
+        "@pe tcgen05.mma.cta_group::1.kind::f16 [%0], [ta], db, %3, ptrue;\n"
+        "}\n" ::"r"(d_tmem),
+        "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate_first)
         : "memory");
 }
 
