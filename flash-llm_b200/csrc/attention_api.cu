@@ -3,6 +3,7 @@
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
+#include <algorithm>
 #include <atomic>
 #include <cmath>
 
@@ -272,7 +273,7 @@ int FlashLLM_CacheAccept(void* stream, void* K_cache, void* V_cache, int layers,
     AcceptParams p{};
     if (!describe_batch(&p.batch, K_cache, V_cache, pages, page_size, cu_tokens, context, page_table, table_width, sequences, tokens,
                         kv_heads, head_dim)
-        || layers < 1 || layers > 65535 || kv_heads > 65535 || accepted == nullptr || accepted_lengths == nullptr || accepted_width < 1
+        || layers < 1 || static_cast<long long>(kv_heads) * layers > 0x7fffffffll || accepted == nullptr || accepted_lengths == nullptr || accepted_width < 1
         || accepted_width > kMaxDrafted)
         return static_cast<int>(cudaErrorInvalidValue);
     if (tokens == 0 || sequences == 0)
@@ -285,7 +286,10 @@ int FlashLLM_CacheAccept(void* stream, void* K_cache, void* V_cache, int layers,
     p.accepted_lengths = accepted_lengths;
     p.accepted_width   = accepted_width;
     p.layer_elems      = static_cast<long long>(pages) * kv_heads * page_size * head_dim;
-    const dim3 grid(sequences, kv_heads, layers);
+    p.layers           = layers;
+    // Some four CTAs for each multiprocessor, of a sequence's heads and layers at most as many as there are.
+    const long long heads = static_cast<long long>(kv_heads) * layers;
+    const dim3      grid(sequences, static_cast<unsigned>(std::min(heads, (4 * 148ll + sequences - 1) / sequences)));
     auto       launch = [&](auto kernel) {
         return launch_in_stream_order(kernel, grid, dim3(kAcceptThreads), 0, static_cast<cudaStream_t>(stream), 1, p);
     };

@@ -119,7 +119,7 @@ struct AttnShared {
     uint32_t           tmem;
     volatile uint32_t  abort_flag;
     int                start_sequence, start_rows, start_head, start_unit;
-    long long          start_units;
+    unsigned           start_units;
     // Written by the loader, which is ahead of everybody, by at most the stages and one: a segment's values cannot be loaded
     // before those of the one so many tiles earlier have been multiplied, and its place here is taken again only after
     // kAttnSegments more.
@@ -244,22 +244,29 @@ __device__ __forceinline__ int attn_tiles(int keys)
     return (keys + kAttnKeys - 1) / kAttnKeys;
 }
 
-// Beginning an item, and ending it, takes about as long as kAttnItemUnits tiles of keys: an item counts as so many units more
-// than it has tiles when the work is dealt out.  A CTA has at least kAttnLeastUnits of them: two tiles, one for each group, cost
-// little more than one, and an item that is not cut needs no joining.
-constexpr int kAttnItemUnits = 2, kAttnLeastUnits = 4;
-
-__device__ __forceinline__ int attn_units(int tiles)
+// Beginning an item, and ending it, takes about as long as two of its tiles of keys, and as five where its groups share their rows
+// and join their sums (us a call with 2 / 3 / 4 for all: decoding of 64 sequences 128 / 124 / 122, prompts with a prefix 73 / 76 /
+// 79): an item counts as so many units more than it has tiles when the work is dealt out.  A CTA has at least four units more
+// than that: tiles for both groups cost little more than for one, and an item that is not cut needs no joining.
+__device__ __forceinline__ int attn_extra_units(const AttentionParams& p, int rows)
 {
-    return tiles + kAttnItemUnits;
+    return rows > p.tile_rows ? 2 : 5;
+}
+
+// Units of the item whose rows begin with row0 of the sequence's.
+__device__ __forceinline__ unsigned attn_units(const AttentionParams& p, const AttnSequence& a, int row0)
+{
+    const int end = min(row0 + 2 * p.tile_rows, a.rows);
+    return static_cast<unsigned>(attn_tiles(attn_keys(p, a, end)) + attn_extra_units(p, end - row0));
 }
 
 // Walks a CTA's share of the linear sequence of units, order (sequence, rows, key/value head, keys).
 struct AttnCursor {
     AttnSequence a;
     AttnSegment  seg;
-    long long    left;
+    unsigned     left;
     int          next_unit;  // of the item
+    int          extra;      // units of the item beyond its tiles
 
     __device__ __forceinline__ void enter_rows(const AttentionParams& p)
     {
@@ -267,6 +274,7 @@ struct AttnCursor {
         seg.rows       = end - seg.row0;
         seg.pair       = seg.rows > p.tile_rows;
         seg.fourfold   = seg.rows <= p.few_rows;
+        extra          = attn_extra_units(p, seg.rows);
         seg.keys       = attn_keys(p, a, end);
         seg.tiles      = attn_tiles(seg.keys);
         seg.tiles0     = seg.pair ? attn_tiles(attn_keys(p, a, seg.row0 + p.tile_rows)) : seg.tiles;
@@ -304,7 +312,7 @@ struct AttnCursor {
     __device__ __forceinline__ void next(const AttentionParams& p, const AttnShared& sh)
     {
         do {
-            if (left > 0 && next_unit >= attn_units(seg.tiles)) {
+            if (left > 0 && next_unit >= seg.tiles + extra) {
                 next_unit = 0;
                 if (++seg.head == p.batch.kv_heads) {
                     seg.head = 0;
@@ -319,11 +327,11 @@ struct AttnCursor {
                 }
             }
             seg.begin = seg.end = 0;
-            if (left <= 0)
+            if (left == 0)
                 return;
-            const int upto = static_cast<int>(min(static_cast<long long>(attn_units(seg.tiles)), next_unit + left));
-            seg.begin      = max(next_unit - kAttnItemUnits, 0);
-            seg.end        = max(upto - kAttnItemUnits, 0);
+            const int upto = static_cast<int>(min(static_cast<unsigned>(seg.tiles + extra), next_unit + left));
+            seg.begin      = max(next_unit - extra, 0);
+            seg.end        = max(upto - extra, 0);
             left -= upto - next_unit;
             next_unit = upto;
         } while (seg.end == seg.begin);
@@ -347,65 +355,63 @@ __device__ __forceinline__ void attn_plan(const AttentionParams& p, AttnShared& 
 {
     const int B = p.batch.sequences, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int item_rows = 2 * p.tile_rows;
+    bool      several   = false;
 #pragma unroll 1
     for (int b = threadIdx.x; b < B; b += kAttnThreads) {
         const AttnSequence a = attn_sequence(p, b);
         if (b < kAttnKnown)
             sh.known[b] = make_int4(a.s.first, a.s.count, a.s.context, a.prefix);
-        sh.units[b]          = a.s.lost > 0            ? kAttnLostRows
-                               : a.rows == 0            ? 0u
+        const unsigned units = a.s.lost > 0         ? kAttnLostRows
+                               : a.rows == 0        ? 0u
                                : a.rows > item_rows ? kAttnSeveralItems
-                                                        : attn_units(attn_tiles(attn_keys(p, a, a.rows)));
+                                                    : attn_units(p, a, 0);
+        sh.units[b]          = units;
+        several              = several || units >= kAttnLostRows;
     }
-    __syncthreads();
+    if (__syncthreads_or(several ? 1 : 0)) {
 #pragma unroll 1
-    for (int b = warp; b < B; b += kAttnThreads / 32) {
-        if (sh.units[b] < kAttnLostRows)
-            continue;
-        const AttnSequence a    = attn_sequence(p, b);
-        unsigned           mine = 0;
-        if (a.s.lost > 0 && b % gridDim.x == blockIdx.x) {
-            const long long row = static_cast<long long>(p.heads) * head_dim;
+        for (int b = warp; b < B; b += kAttnThreads / 32) {
+            if (sh.units[b] < kAttnLostRows)
+                continue;
+            const AttnSequence a    = attn_sequence(p, b);
+            unsigned           mine = 0;
+            if (a.s.lost > 0 && b % gridDim.x == blockIdx.x) {
+                const long long row = static_cast<long long>(p.heads) * head_dim;
 #pragma unroll 1
-            for (long long i = lane * 8; i < a.s.lost * row; i += 32 * 8)
-                *reinterpret_cast<uint4*>(p.out + a.s.first * row + i) = make_uint4(0, 0, 0, 0);
+                for (long long i = lane * 8; i < a.s.lost * row; i += 32 * 8)
+                    *reinterpret_cast<uint4*>(p.out + a.s.first * row + i) = make_uint4(0, 0, 0, 0);
+            }
+#pragma unroll 1
+            for (long long r = lane * item_rows; r < a.rows; r += 32 * item_rows)
+                mine += attn_units(p, a, static_cast<int>(r));
+            mine = __reduce_add_sync(0xffffffffu, mine);
+            __syncwarp();
+            if (lane == 0)
+                sh.units[b] = mine;
         }
-#pragma unroll 1
-        for (long long r = lane * item_rows; r < a.rows; r += 32 * item_rows)
-            mine += attn_units(attn_tiles(attn_keys(p, a, static_cast<int>(min(r + item_rows, static_cast<long long>(a.rows))))));
-        mine = __reduce_add_sync(0xffffffffu, mine);
-        __syncwarp();
-        if (lane == 0)
-            sh.units[b] = mine;
+        __syncthreads();
     }
-    __syncthreads();
     if (warp == 0) {
-        long long total = 0;
+        // All units of a call fit into 31 bits: so many tiles of 128 keys would take hours.
+        const unsigned heads = p.batch.kv_heads;
+        unsigned       total = 0;
 #pragma unroll 1
         for (int b = lane; b < B; b += 32)
             total += sh.units[b];
-#pragma unroll
-        for (int d = 16; d > 0; d >>= 1)
-            total += __shfl_xor_sync(0xffffffffu, total, d);
-        const int       heads = p.batch.kv_heads;
-        const long long units = total * heads;
-        long long       share = 0;
-        if (units < 0x7fffffffll)
-            share = (static_cast<unsigned>(units) + gridDim.x - 1) / gridDim.x;
-        else
-            share = (units + gridDim.x - 1) / gridDim.x;
-        share              = max(share, static_cast<long long>(kAttnLeastUnits));
-        const long long u0 = min(units, share * blockIdx.x), u1 = min(units, u0 + share);
-        // The sequence that holds unit u0: the first whose running sum passes it.
-        int       b = 0, row0 = 0;
-        long long before = 0;
+        const unsigned units = __reduce_add_sync(0xffffffffu, total) * heads;
+        const unsigned share = max((units + gridDim.x - 1) / gridDim.x, 9u);
+        const unsigned u0 = min(units, share * blockIdx.x), u1 = min(units, u0 + share);
         if (u1 > u0) {
+            // The sequence that holds unit u0: the first whose running sum passes it.
+            unsigned before = 0;
+            int      b      = 0;
 #pragma unroll 1
             for (int base = 0;; base += 32) {
-                long long mine = base + lane < B ? static_cast<long long>(sh.units[base + lane]) * heads : 0, upto = mine;
+                const unsigned mine = base + lane < B ? sh.units[base + lane] * heads : 0;
+                unsigned       upto = mine;
 #pragma unroll
                 for (int d = 1; d < 32; d <<= 1) {
-                    const long long other = __shfl_up_sync(0xffffffffu, upto, d);
+                    const unsigned other = __shfl_up_sync(0xffffffffu, upto, d);
                     if (lane >= d)
                         upto += other;
                 }
@@ -418,37 +424,39 @@ __device__ __forceinline__ void attn_plan(const AttentionParams& p, AttnShared& 
                 }
                 before += __shfl_sync(0xffffffffu, upto, 31);
             }
-            const AttnSequence a = attn_sequence(p, sh, b);
+            const AttnSequence a    = attn_sequence(p, sh, b);
+            int                row0 = 0;
+            unsigned           item = 1;
+            if (a.rows <= item_rows)
+                item = attn_units(p, a, 0);
+            else {
 #pragma unroll 1
-            for (long long base = 0;; base += 32 * item_rows) {  // ... and of its items the first
-                const long long r    = base + lane * item_rows;
-                long long       mine = 0;
-                if (r < a.rows)
-                    mine = static_cast<long long>(heads)
-                           * attn_units(attn_tiles(attn_keys(p, a, static_cast<int>(min(r + item_rows, static_cast<long long>(a.rows))))));
-                long long upto = mine;
+                for (long long base = 0;; base += 32 * item_rows) {  // ... and of its items the first
+                    const long long r    = base + lane * item_rows;
+                    const unsigned  size = r < a.rows ? attn_units(p, a, static_cast<int>(r)) : 0;
+                    unsigned        upto = size * heads;
 #pragma unroll
-                for (int d = 1; d < 32; d <<= 1) {
-                    const long long other = __shfl_up_sync(0xffffffffu, upto, d);
-                    if (lane >= d)
-                        upto += other;
+                    for (int d = 1; d < 32; d <<= 1) {
+                        const unsigned other = __shfl_up_sync(0xffffffffu, upto, d);
+                        if (lane >= d)
+                            upto += other;
+                    }
+                    const unsigned past = __ballot_sync(0xffffffffu, before + upto > u0);
+                    if (past || base + 32 * item_rows >= a.rows) {
+                        const int l = past ? __ffs(past) - 1 : 0;
+                        row0        = static_cast<int>(base) + l * item_rows;
+                        item        = max(1u, __shfl_sync(0xffffffffu, size, l));
+                        before += __shfl_sync(0xffffffffu, upto - size * heads, l);
+                        break;
+                    }
+                    before += __shfl_sync(0xffffffffu, upto, 31);
                 }
-                const unsigned past = __ballot_sync(0xffffffffu, before + upto > u0);
-                if (past || base + 32 * item_rows >= a.rows) {
-                    const int l = past ? __ffs(past) - 1 : 0;
-                    row0        = static_cast<int>(base) + l * item_rows;
-                    before += __shfl_sync(0xffffffffu, upto - mine, l);
-                    break;
-                }
-                before += __shfl_sync(0xffffffffu, upto, 31);
             }
             if (lane == 0) {
-                const unsigned item = attn_units(attn_tiles(attn_keys(p, a, min(row0 + item_rows, a.rows))));
                 sh.start_sequence = b;
                 sh.start_rows     = row0;
-                const unsigned in = static_cast<unsigned>(u0 - before);  // of the item's units of all heads
-                sh.start_head     = static_cast<int>(in / item);
-                sh.start_unit     = static_cast<int>(in % item);
+                sh.start_head     = static_cast<int>((u0 - before) / item);
+                sh.start_unit     = static_cast<int>((u0 - before) % item);
             }
         }
         if (lane == 0)
@@ -760,7 +768,7 @@ __device__ __forceinline__ void attn_softmax(AttnState& st, const AttnRow& row, 
             ptx::tmem_wait_st();
         attn_new_top(st, new_top, first, rescale);
         const float minus = st.top == -CUDART_INF_F ? 0.0f : -st.top * st.factor;
-#pragma unroll 1
+#pragma unroll 2
         for (int c = 0; c < kAttnKeys; c += 32) {  // weights take the place of scores already read
             float    s[32];
             uint32_t w[16];
@@ -846,7 +854,7 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
         const int       group = warp >> 2, thread = threadIdx.x & 127;
         const uint32_t  lanes = static_cast<uint32_t>(warp & 3) << 21;  // this warp's lanes of tensor memory
         const uint32_t  s_tmem = tmem + kS + group * 128 + lanes, o_tmem = tmem + kO + group * 128 + lanes;
-        uint32_t        s_parity = 0, o_count = 0;  // phases of s_full, products of weights and values so far
+        uint32_t        s_parity = 0, o_parity = 0;  // phases of s_full and o_done
         AttnPart* const parts = reinterpret_cast<AttnPart*>(p.workspace) + 2 * blockIdx.x;
         bool            ok = true, written[2] = {false, false};
         for (int number = 0;; ++number) {
@@ -889,9 +897,7 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
                     }
                 }
             }
-            auto rescale = [&](float keep) {
-                ok = attn_wait(&sh.o_done[group], (o_count - 1) & 1u, sh, status);  // the product before has ended
-                ptx::tc_fence_after_sync();
+            auto rescale = [&](float keep) {  // the product before has ended: these scores come after it
 #pragma unroll 1
                 for (int c = 0; c < HEAD_DIM; c += 32) {
                     uint32_t o[32];
@@ -927,10 +933,11 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
                     part_done(0);
                     part_done(1);
                 }
-                ++o_count;
             }
-            if (ok && tiles > 0)
-                ok = attn_wait(&sh.o_done[group], (o_count - 1) & 1u, sh, status);
+            if (tiles > 0) {
+                ok = ok && attn_wait(&sh.o_done[group], o_parity, sh, status);
+                o_parity ^= 1u;
+            }
             ptx::tc_fence_after_sync();
 
             // ---- the end of the segment: what is added up to a row lies in up to eight places, 2 groups x 4 copies
@@ -1166,7 +1173,9 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
                                           v + half_tile * (4 * 2048 >> 4), idesc_o, i > 0 || half_tile > 0);
             }
             parity ^= 1u;
-            ptx::umma_commit_elect(ptx::smem_u32(&sh.o_done[group]));
+            // Scores that are complete mean that the product before them is: o_done tells of a segment's last alone.
+            if (i + 1 == (group == 0 ? tiles0 : tiles1))
+                ptx::umma_commit_elect(ptx::smem_u32(&sh.o_done[group]));
             if (!pair || group == 1)
                 ptx::umma_commit_elect(ptx::smem_u32(&sh.v_empty[stage]));
             return true;
@@ -1356,10 +1365,16 @@ __global__ void __launch_bounds__(256) attention_join_kernel(const AttentionPara
     const bool            valid = place % kAttnRows < p.tile_rows && row < last.rows;
     if (last.kind != kPartEnds || !__any_sync(0xffffffffu, valid))
         return;
-    // The CTA whose segment began the item.
-    int begin = cta - 1;
-    while (begin >= 0 && parts[2 * begin].kind == kPartContinues)
-        --begin;
+    // The CTA whose segment began the item: the nearest before that did not continue it.
+    int begin = cta;
+#pragma unroll 1
+    do {
+        const int c = begin - 1 - lane;
+        const unsigned other = __ballot_sync(0xffffffffu, c < 0 || parts[2 * c].kind != kPartContinues);
+        begin -= other ? __ffs(other) : 32;
+        if (other)
+            break;
+    } while (true);
     if (begin < 0 || parts[2 * begin + 1].kind != kPartBegins)
         return;  // a CTA gave up
     auto  slot = [&](int c) { return static_cast<size_t>(2 * c + (c == begin ? 1 : 0)); };

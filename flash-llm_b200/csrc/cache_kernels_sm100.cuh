@@ -47,98 +47,132 @@ __device__ __forceinline__ uint4 pack_half8(const float (&x)[8])
 // the rest of the head, and values, pass unchanged.  One CTA per token; a thread moves 32 bytes of a head at a time, which hold
 // both members of eight pairs in either layout: (i, i + rotary_dim / 2), or INTERLEAVED (2 i, 2 i + 1).
 // The angle is reduced in 64 bits: at position 1e6 its 32-bit product would be off by 0.06 radians.
+// Bound by memory for prompts (@ROT@), for a few tokens by a chain of dependent loads: sequence, page, row.  The first loads
+// of the token's own row, which depend on none of them, are issued ahead of it.
+constexpr int kRotaryBatch = 2;  // moves of 32 bytes that a thread has in flight
+
 template<int HEAD_DIM, bool INTERLEAVED>
 __global__ void __launch_bounds__(kRotaryThreads) rotary_append_kernel(const RotaryParams p)
 {
+    constexpr int        kUnits = HEAD_DIM / 16;  // of 32 bytes per head
     __shared__ float     s_cos[HEAD_DIM / 2], s_sin[HEAD_DIM / 2];
-    __shared__ long long s_owner;  // sequence << 32 | first row; -1: nobody's
-    const CacheBatch&    c = p.batch;
-    const int            n = blockIdx.x;
+    __shared__ int       s_sequence, s_position;  // of the token; -1: nobody's, or it does not fit
+    const CacheBatch&    c     = p.batch;
+    const int            n     = blockIdx.x;
+    const int            pairs = p.rotary_dim / 2;
+    const int            units = (p.heads + 2 * c.kv_heads) * kUnits;
+    const half* const    row   = p.qkv + n * p.ld_qkv;
     if (threadIdx.x == 0)
-        s_owner = -1;
+        s_sequence = -1;
     __syncthreads();
     ptx::grid_dependency_wait();
     ptx::grid_launch_dependents();
+
+    uint4 first[kRotaryBatch], second[kRotaryBatch];
+    auto  turned_at = [&](int u) { return u / kUnits < p.heads + c.kv_heads && u % kUnits * 16 < p.rotary_dim; };
+    // Where a unit's two halves lie in its head.
+    auto offsets = [&](int u, int& a, int& z) {
+        const int part = u % kUnits;
+        const bool apart = turned_at(u) && !INTERLEAVED;
+        a = apart ? part * 8 : part * 16;
+        z = apart ? pairs + part * 8 : part * 16 + 8;
+    };
+    auto load = [&](int u0) {
+#pragma unroll
+        for (int k = 0; k < kRotaryBatch; ++k) {
+            const int u = u0 + k * kRotaryThreads;
+            if (u < units) {
+                int a, z;
+                offsets(u, a, z);
+                first[k]  = *reinterpret_cast<const uint4*>(row + u / kUnits * HEAD_DIM + a);
+                second[k] = *reinterpret_cast<const uint4*>(row + u / kUnits * HEAD_DIM + z);
+            }
+        }
+    };
+    load(threadIdx.x);
+    const double frequency = threadIdx.x < pairs ? p.frequencies[threadIdx.x] : 0.0;
+    const int    elsewhere = p.positions && threadIdx.x < pairs ? p.positions[n] : 0;
     for (int b = threadIdx.x; b < c.sequences; b += kRotaryThreads) {
-        const int begin = c.cu_tokens[b];
-        if (begin >= 0 && begin <= n && n < c.cu_tokens[b + 1])
-            s_owner = static_cast<long long>(b) << 32 | static_cast<unsigned>(begin);
+        const int begin = c.cu_tokens[b], end = c.cu_tokens[b + 1], context = c.context[b];
+        if (begin >= 0 && begin <= n && n < end) {
+            const long long position = static_cast<long long>(context) + (n - begin);
+            s_sequence               = b;
+            s_position               = context >= 0 && position < table_positions(c) ? static_cast<int>(position) : -1;
+        }
     }
     __syncthreads();
-    const long long owner = s_owner;
-    if (owner < 0)
+    const int b = s_sequence, position = s_position;
+    if (b < 0)
         return;
-    const int       b        = static_cast<int>(owner >> 32), first = static_cast<int>(owner);
-    const int       context  = c.context[b];
-    const long long position = static_cast<long long>(context) + (n - first);
-    const bool      fits     = context >= 0 && position < table_positions(c);
-    const int       pairs    = p.rotary_dim / 2;
+    if (position < 0 && threadIdx.x == 0)
+        atomicOr(c.status, kStatusBadCache);
+    const long long at = position >= 0 ? cache_row(c, b, position, 0) : -1;  // of key/value head 0
     if (threadIdx.x < pairs) {
-        const double turns  = static_cast<double>(p.positions ? p.positions[n] : position) * (p.frequencies[threadIdx.x] * 0.15915494309189535);
+        const double turns = static_cast<double>(p.positions ? elsewhere : position) * (frequency * 0.15915494309189535);
         float        sine, cosine;
         sincospif(2.0f * static_cast<float>(turns - rint(turns)), &sine, &cosine);
         s_cos[threadIdx.x] = cosine * p.magnitude;
         s_sin[threadIdx.x] = sine * p.magnitude;
     }
-    if (!fits && threadIdx.x == 0)
-        atomicOr(c.status, kStatusBadCache);
-    long long row = fits ? cache_row(c, b, static_cast<int>(position), 0) : -1;  // of key/value head 0
     __syncthreads();
 
-    constexpr int kUnits = HEAD_DIM / 16;  // of 32 bytes per head
-    const int     units  = (p.heads + 2 * c.kv_heads) * kUnits;
-    for (int u = threadIdx.x; u < units; u += kRotaryThreads) {
-        const int   head = u / kUnits, part = u % kUnits;
-        const half* src  = p.qkv + n * p.ld_qkv + static_cast<long long>(head) * HEAD_DIM;
-        half*       dst;
-        if (head < p.heads) {
-            dst = p.q + n * p.ld_q + static_cast<long long>(head) * HEAD_DIM;
-        }
-        else {
-            if (row < 0)
-                continue;
-            const bool key = head < p.heads + c.kv_heads;
-            const int  h   = head - p.heads - (key ? 0 : c.kv_heads);
-            dst            = (key ? p.k_cache : p.v_cache) + (row + (static_cast<long long>(h) << c.page_shift)) * HEAD_DIM;
-        }
-        const bool turned = head < p.heads + c.kv_heads && part * 16 < p.rotary_dim;
-        const int  a      = turned && !INTERLEAVED ? part * 8 : part * 16;
-        const int  z      = turned && !INTERLEAVED ? pairs + part * 8 : part * 16 + 8;
-        uint4      va     = *reinterpret_cast<const uint4*>(src + a);
-        uint4      vz     = *reinterpret_cast<const uint4*>(src + z);
-        if (turned) {
-            float x[8], y[8];
-            unpack_half8(va, x);
-            unpack_half8(vz, y);
-            float co[8], si[8];
+    for (int u0 = threadIdx.x; u0 < units; u0 += kRotaryBatch * kRotaryThreads) {
+        if (u0 != static_cast<int>(threadIdx.x))
+            load(u0);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                co[i] = s_cos[part * 8 + i];
-                si[i] = s_sin[part * 8 + i];
-            }
-            if constexpr (INTERLEAVED) {
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const float x0 = x[2 * i], x1 = x[2 * i + 1], y0 = y[2 * i], y1 = y[2 * i + 1];
-                    x[2 * i]     = x0 * co[i] - x1 * si[i];
-                    x[2 * i + 1] = x1 * co[i] + x0 * si[i];
-                    y[2 * i]     = y0 * co[i + 4] - y1 * si[i + 4];
-                    y[2 * i + 1] = y1 * co[i + 4] + y0 * si[i + 4];
-                }
+        for (int k = 0; k < kRotaryBatch; ++k) {
+            const int u = u0 + k * kRotaryThreads;
+            if (u >= units)
+                break;
+            const int head = u / kUnits, part = u % kUnits;
+            half*     dst;
+            if (head < p.heads) {
+                dst = p.q + n * p.ld_q + static_cast<long long>(head) * HEAD_DIM;
             }
             else {
+                if (at < 0)
+                    continue;
+                const bool key = head < p.heads + c.kv_heads;
+                const int  h   = head - p.heads - (key ? 0 : c.kv_heads);
+                dst            = (key ? p.k_cache : p.v_cache) + (at + (static_cast<long long>(h) << c.page_shift)) * HEAD_DIM;
+            }
+            int a, z;
+            offsets(u, a, z);
+            uint4 va = first[k], vz = second[k];
+            if (turned_at(u)) {
+                float x[8], y[8];
+                unpack_half8(va, x);
+                unpack_half8(vz, y);
+                float co[8], si[8];
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
-                    const float x0 = x[i], y0 = y[i];
-                    x[i] = x0 * co[i] - y0 * si[i];
-                    y[i] = y0 * co[i] + x0 * si[i];
+                    co[i] = s_cos[part * 8 + i];
+                    si[i] = s_sin[part * 8 + i];
                 }
+                if constexpr (INTERLEAVED) {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const float x0 = x[2 * i], x1 = x[2 * i + 1], y0 = y[2 * i], y1 = y[2 * i + 1];
+                        x[2 * i]     = x0 * co[i] - x1 * si[i];
+                        x[2 * i + 1] = x1 * co[i] + x0 * si[i];
+                        y[2 * i]     = y0 * co[i + 4] - y1 * si[i + 4];
+                        y[2 * i + 1] = y1 * co[i + 4] + y0 * si[i + 4];
+                    }
+                }
+                else {
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        const float x0 = x[i], y0 = y[i];
+                        x[i] = x0 * co[i] - y0 * si[i];
+                        y[i] = y0 * co[i] + x0 * si[i];
+                    }
+                }
+                va = pack_half8(x);
+                vz = pack_half8(y);
             }
-            va = pack_half8(x);
-            vz = pack_half8(y);
+            *reinterpret_cast<uint4*>(dst + a) = va;
+            *reinterpret_cast<uint4*>(dst + z) = vz;
         }
-        *reinterpret_cast<uint4*>(dst + a) = va;
-        *reinterpret_cast<uint4*>(dst + z) = vz;
     }
 }
 
@@ -149,59 +183,78 @@ struct AcceptParams {
     const int* accepted;          // [sequences][accepted_width]: drafted tokens in the order in which they are kept
     const int* accepted_lengths;  // [sequences]
     int        accepted_width;    // 1 .. kMaxDrafted
+    int        layers;
     long long  layer_elems;
 };
 
 constexpr int kAcceptThreads = 256;
 
-// Keys and values of drafted token accepted[b][i] move to position context[b] + i.  One CTA per sequence, head and layer, which
-// holds everything in registers before it writes, so that sources and targets may overlap in any way.
+// Keys and values of drafted token accepted[b][i] move to position context[b] + i.  A CTA takes a share of one sequence's heads
+// and layers, as many at a time as its registers hold whole: all of a head is read before any of it is written, so that sources
+// and targets may overlap in any way.  Bound by the chain of loads that leads to the rows, which the heads and layers of a CTA
+// share (24 sequences, 32 layers: a CTA for each head and layer 14.3 us, now @ACC@).
 template<int HEAD_DIM>
 __global__ void __launch_bounds__(kAcceptThreads) cache_accept_kernel(const AcceptParams p)
 {
-    __shared__ long long s_from[kMaxDrafted], s_to[kMaxDrafted];  // rows of the cache; from = to: nothing moves
+    constexpr int        kChunks    = 2 * HEAD_DIM / 8;  // of 16 bytes in a row of keys and the row of values
+    constexpr int        kPerThread = kMaxDrafted * kChunks / kAcceptThreads;
+    __shared__ long long s_from[kMaxDrafted], s_to[kMaxDrafted];  // rows of the first head; from = to: nothing moves
     const CacheBatch&    c = p.batch;
-    const int            b = blockIdx.x, head = blockIdx.y;
+    const int            b = blockIdx.x, i = threadIdx.x;
     ptx::grid_dependency_wait();
     ptx::grid_launch_dependents();
-    const Sequence s      = load_sequence(c, b);
+    const int      token  = i < p.accepted_width ? p.accepted[static_cast<long long>(b) * p.accepted_width + i] : 0;
     int            length = p.accepted_lengths[b];
+    const Sequence s      = load_sequence(c, b);
     if (length < 0 || length > p.accepted_width || (s.count == 0 && length > 0)) {
         if (threadIdx.x == 0)
             atomicOr(c.status, kStatusBadCache);
         length = 0;
     }
-    if (static_cast<int>(threadIdx.x) < length) {
-        const int token = p.accepted[static_cast<long long>(b) * p.accepted_width + threadIdx.x];
+    if (i < length) {
         long long from = -1, to = -1;
-        if (token >= 0 && token < s.count && static_cast<int>(threadIdx.x) < s.count) {
-            from = cache_row(c, b, s.context + token, head);
-            to   = cache_row(c, b, s.context + static_cast<int>(threadIdx.x), head);
+        if (token >= 0 && token < s.count && i < s.count) {
+            from = cache_row(c, b, s.context + token, 0);
+            to   = cache_row(c, b, s.context + i, 0);
         }
         else
             atomicOr(c.status, kStatusBadCache);
         if (from < 0 || to < 0)
             from = to = 0;
-        s_from[threadIdx.x] = from;
-        s_to[threadIdx.x]   = to;
+        s_from[i] = from;
+        s_to[i]   = to;
     }
     __syncthreads();
-    constexpr int kChunks = HEAD_DIM / 8;                                     // 16 bytes each
-    constexpr int kPerThread = 2 * kMaxDrafted * kChunks / kAcceptThreads;
-    half* const   caches[2] = {p.k_cache + blockIdx.z * p.layer_elems, p.v_cache + blockIdx.z * p.layer_elems};
-    uint4         v[kPerThread];
+    if (length == 0)
+        return;
+    const int heads    = c.kv_heads * p.layers;  // of all layers
+    const int at_once  = max(1, kPerThread * kAcceptThreads / (length * kChunks));
+    const int per_head = length * kChunks;
+    for (int head0 = blockIdx.y * at_once; head0 < heads; head0 += gridDim.y * at_once) {
+        uint4     v[kPerThread];
+        long long to[kPerThread];  // element of the cache, -1: nothing moves
 #pragma unroll
-    for (int k = 0; k < kPerThread; ++k) {
-        const int i = threadIdx.x + k * kAcceptThreads, row = i / (2 * kChunks), which = i / kChunks % 2;
-        if (row < length && s_from[row] != s_to[row])
-            v[k] = *reinterpret_cast<const uint4*>((which ? caches[1] : caches[0]) + s_from[row] * HEAD_DIM + i % kChunks * 8);
-    }
-    __syncthreads();
+        for (int k = 0; k < kPerThread; ++k) {
+            const int at = threadIdx.x + k * kAcceptThreads, head = head0 + at / per_head, in = at % per_head;
+            to[k] = -1;
+            if (at >= at_once * per_head || head >= heads)
+                continue;
+            const int row = in / kChunks, chunk = in % kChunks;
+            if (s_from[row] == s_to[row])
+                continue;
+            const long long base = head / c.kv_heads * p.layer_elems + (static_cast<long long>(head % c.kv_heads) << c.page_shift) * HEAD_DIM
+                                   + chunk % (kChunks / 2) * 8;
+            const half* src = (chunk < kChunks / 2 ? p.k_cache : p.v_cache) + base + s_from[row] * HEAD_DIM;
+            v[k]  = *reinterpret_cast<const uint4*>(src);
+            to[k] = base + s_to[row] * HEAD_DIM;
+        }
+        __syncthreads();
 #pragma unroll
-    for (int k = 0; k < kPerThread; ++k) {
-        const int i = threadIdx.x + k * kAcceptThreads, row = i / (2 * kChunks), which = i / kChunks % 2;
-        if (row < length && s_from[row] != s_to[row])
-            *reinterpret_cast<uint4*>((which ? caches[1] : caches[0]) + s_to[row] * HEAD_DIM + i % kChunks * 8) = v[k];
+        for (int k = 0; k < kPerThread; ++k)
+            if (to[k] >= 0) {
+                const int chunk = (threadIdx.x + k * kAcceptThreads) % per_head % kChunks;
+                *reinterpret_cast<uint4*>((chunk < kChunks / 2 ? p.k_cache : p.v_cache) + to[k]) = v[k];
+            }
     }
 }
 
