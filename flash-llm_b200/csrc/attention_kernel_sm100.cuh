@@ -118,8 +118,6 @@ struct AttnShared {
     unsigned long long s_full[2], p_full[2][2], o_done[2], q_full[2], q_empty[2], segment_full[kAttnSegments];
     uint32_t           tmem;
     volatile uint32_t  abort_flag;
-    int                start_sequence, start_rows, start_head, start_unit;
-    unsigned           start_units;
     // Written by the loader, which is ahead of everybody, by at most the stages and one: a segment's values cannot be loaded
     // before those of the one so many tiles earlier have been multiplied, and its place here is taken again only after
     // kAttnSegments more.
@@ -246,11 +244,19 @@ __device__ __forceinline__ int attn_tiles(int keys)
 
 // Beginning an item, and ending it, takes about as long as two of its tiles of keys, and as five where its groups share their rows
 // and join their sums (us a call with 2 / 3 / 4 for all: decoding of 64 sequences 128 / 124 / 122, prompts with a prefix 73 / 76 /
-// 79): an item counts as so many units more than it has tiles when the work is dealt out.  A CTA has at least four units more
-// than that: tiles for both groups cost little more than for one, and an item that is not cut needs no joining.
+// 79): an item counts as so many units more than it has tiles when the work is dealt out.
 __device__ __forceinline__ int attn_extra_units(const AttentionParams& p, int rows)
 {
     return rows > p.tile_rows ? 2 : 5;
+}
+
+// The tile of an item with `tiles` before which unit x of it cuts it.  Where a CTA's share is but a few tiles, one for each group is
+// the least that pays: a single tile is not cut off.  (Larger shares even out better with every cut where it falls: capped trees
+// of 64 tokens 76 us, 80 with cuts moved by up to an eighth of the share.)
+__device__ __forceinline__ int attn_cut(int x, int tiles, int extra, int share)
+{
+    const int t = x - extra, least = share <= 4 ? 1 : 0;
+    return t >= tiles ? tiles : t <= least ? 0 : tiles - t <= least ? tiles : t;
 }
 
 // Units of the item whose rows begin with row0 of the sequence's.
@@ -259,84 +265,6 @@ __device__ __forceinline__ unsigned attn_units(const AttentionParams& p, const A
     const int end = min(row0 + 2 * p.tile_rows, a.rows);
     return static_cast<unsigned>(attn_tiles(attn_keys(p, a, end)) + attn_extra_units(p, end - row0));
 }
-
-// Walks a CTA's share of the linear sequence of units, order (sequence, rows, key/value head, keys).
-struct AttnCursor {
-    AttnSequence a;
-    AttnSegment  seg;
-    unsigned     left;
-    int          next_unit;  // of the item
-    int          extra;      // units of the item beyond its tiles
-
-    __device__ __forceinline__ void enter_rows(const AttentionParams& p)
-    {
-        const int end  = min(seg.row0 + 2 * p.tile_rows, a.rows);
-        seg.rows       = end - seg.row0;
-        seg.pair       = seg.rows > p.tile_rows;
-        seg.fourfold   = seg.rows <= p.few_rows;
-        extra          = attn_extra_units(p, seg.rows);
-        seg.keys       = attn_keys(p, a, end);
-        seg.tiles      = attn_tiles(seg.keys);
-        seg.tiles0     = seg.pair ? attn_tiles(attn_keys(p, a, seg.row0 + p.tile_rows)) : seg.tiles;
-        seg.open[0]    = attn_open_keys(p, a, seg.row0);
-        seg.open[1]    = seg.pair ? attn_open_keys(p, a, seg.row0 + p.tile_rows) : seg.open[0];
-    }
-    __device__ __forceinline__ void enter_sequence(const AttentionParams& p, const AttnShared& sh)
-    {
-        for (;; ++seg.b) {
-            if (seg.b >= p.batch.sequences) {  // only if somebody writes the arrays during the call
-                left = 0;
-                return;
-            }
-            a = attn_sequence(p, sh, seg.b);
-            if (a.rows > 0)
-                break;
-        }
-        seg.first   = a.s.first;
-        seg.count   = a.s.count;
-        seg.context = a.s.context;
-        seg.prefix  = a.prefix;
-        enter_rows(p);
-    }
-    __device__ __forceinline__ AttnCursor(const AttentionParams& p, const AttnShared& sh)
-    {
-        left      = sh.start_units;
-        seg.b     = sh.start_sequence;
-        seg.row0  = sh.start_rows;
-        seg.head  = sh.start_head;
-        next_unit = sh.start_unit;
-        if (left > 0)
-            enter_sequence(p, sh);
-    }
-    // The next segment that has a tile; its `end` is 0 at the end of the share.
-    __device__ __forceinline__ void next(const AttentionParams& p, const AttnShared& sh)
-    {
-        do {
-            if (left > 0 && next_unit >= seg.tiles + extra) {
-                next_unit = 0;
-                if (++seg.head == p.batch.kv_heads) {
-                    seg.head = 0;
-                    seg.row0 += 2 * p.tile_rows;
-                    if (seg.row0 >= a.rows) {
-                        seg.row0 = 0;
-                        ++seg.b;
-                        enter_sequence(p, sh);
-                    }
-                    else
-                        enter_rows(p);
-                }
-            }
-            seg.begin = seg.end = 0;
-            if (left == 0)
-                return;
-            const int upto = static_cast<int>(min(static_cast<unsigned>(seg.tiles + extra), next_unit + left));
-            seg.begin      = max(next_unit - extra, 0);
-            seg.end        = max(upto - extra, 0);
-            left -= upto - next_unit;
-            next_unit = upto;
-        } while (seg.end == seg.begin);
-    }
-};
 
 // The segment of that number, once the loader has written it; nullptr at the end and when the CTA gives up.
 __device__ __forceinline__ const AttnSegment* attn_segment(AttnShared& sh, int number, unsigned int* status)
@@ -349,9 +277,9 @@ __device__ __forceinline__ const AttnSegment* attn_segment(AttnShared& sh, int n
 
 constexpr unsigned kAttnSeveralItems = 0xffffffffu, kAttnLostRows = 0xfffffffeu;  // in place of a sequence's units
 
-// Where this CTA's share begins and how long it is; all threads, ends with a barrier.  The rows of a sequence that does not fit
-// into the page table are cleared here, by one CTA.
-__device__ __forceinline__ void attn_plan(const AttentionParams& p, AttnShared& sh, int head_dim)
+// Units of every sequence; all threads, ends with a barrier.  The rows of a sequence that does not fit into the page table are
+// cleared here, by one CTA.
+__device__ __forceinline__ void attn_count_units(const AttentionParams& p, AttnShared& sh, int head_dim)
 {
     const int B = p.batch.sequences, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int item_rows = 2 * p.tile_rows;
@@ -391,24 +319,61 @@ __device__ __forceinline__ void attn_plan(const AttentionParams& p, AttnShared& 
         }
         __syncthreads();
     }
-    if (warp == 0) {
-        // All units of a call fit into 31 bits: so many tiles of 128 keys would take hours.
-        const unsigned heads = p.batch.kv_heads;
-        unsigned       total = 0;
+}
+
+// Where this CTA's share begins and how long it is, for a whole warp.
+struct AttnStart {
+    unsigned units;
+    int      share, sequence, row0, head, unit;
+};
+
+__device__ __forceinline__ AttnStart attn_start(const AttentionParams& p, const AttnShared& sh)
+{
+    const int B = p.batch.sequences, lane = threadIdx.x & 31, item_rows = 2 * p.tile_rows;
+    AttnStart start{0, 0, 0, 0, 0, 0};
+    // All units of a call fit into 31 bits: so many tiles of 128 keys would take hours.
+    const unsigned heads = p.batch.kv_heads;
+    unsigned       total = 0;
 #pragma unroll 1
-        for (int b = lane; b < B; b += 32)
-            total += sh.units[b];
-        const unsigned units = __reduce_add_sync(0xffffffffu, total) * heads;
-        const unsigned share = max((units + gridDim.x - 1) / gridDim.x, 9u);
-        const unsigned u0 = min(units, share * blockIdx.x), u1 = min(units, u0 + share);
-        if (u1 > u0) {
-            // The sequence that holds unit u0: the first whose running sum passes it.
-            unsigned before = 0;
-            int      b      = 0;
+    for (int b = lane; b < B; b += 32)
+        total += sh.units[b];
+    const unsigned units = __reduce_add_sync(0xffffffffu, total) * heads;
+    const unsigned share = max((units + gridDim.x - 1) / gridDim.x, 2u);  // a tile for each group
+    const unsigned u0 = min(units, share * blockIdx.x), u1 = min(units, u0 + share);
+    if (u1 > u0) {
+        // The sequence that holds unit u0: the first whose running sum passes it.
+        unsigned before = 0;
+        int      b      = 0;
 #pragma unroll 1
-            for (int base = 0;; base += 32) {
-                const unsigned mine = base + lane < B ? sh.units[base + lane] * heads : 0;
-                unsigned       upto = mine;
+        for (int base = 0; base < B; base += 32) {
+            const unsigned mine = base + lane < B ? sh.units[base + lane] * heads : 0;
+            unsigned       upto = mine;
+#pragma unroll
+            for (int d = 1; d < 32; d <<= 1) {
+                const unsigned other = __shfl_up_sync(0xffffffffu, upto, d);
+                if (lane >= d)
+                    upto += other;
+            }
+            const unsigned past = __ballot_sync(0xffffffffu, before + upto > u0);
+            if (past) {
+                const int l = __ffs(past) - 1;
+                b           = base + l;
+                before += __shfl_sync(0xffffffffu, upto - mine, l);
+                break;
+            }
+            before += __shfl_sync(0xffffffffu, upto, 31);
+        }
+        const AttnSequence a    = attn_sequence(p, sh, b);
+        int                row0 = 0;
+        unsigned           item = 1;
+        if (a.rows <= item_rows)
+            item = attn_units(p, a, 0);
+        else {
+#pragma unroll 1
+            for (long long base = 0;; base += 32 * item_rows) {  // ... and of its items the first
+                const long long r    = base + lane * item_rows;
+                const unsigned  size = r < a.rows ? attn_units(p, a, static_cast<int>(r)) : 0;
+                unsigned        upto = size * heads;
 #pragma unroll
                 for (int d = 1; d < 32; d <<= 1) {
                     const unsigned other = __shfl_up_sync(0xffffffffu, upto, d);
@@ -416,54 +381,105 @@ __device__ __forceinline__ void attn_plan(const AttentionParams& p, AttnShared& 
                         upto += other;
                 }
                 const unsigned past = __ballot_sync(0xffffffffu, before + upto > u0);
-                if (past) {
-                    const int l = __ffs(past) - 1;
-                    b           = base + l;
-                    before += __shfl_sync(0xffffffffu, upto - mine, l);
+                if (past || base + 32 * item_rows >= a.rows) {
+                    const int l = past ? __ffs(past) - 1 : 0;
+                    row0        = static_cast<int>(base) + l * item_rows;
+                    item        = max(1u, __shfl_sync(0xffffffffu, size, l));
+                    before += __shfl_sync(0xffffffffu, upto - size * heads, l);
                     break;
                 }
                 before += __shfl_sync(0xffffffffu, upto, 31);
             }
-            const AttnSequence a    = attn_sequence(p, sh, b);
-            int                row0 = 0;
-            unsigned           item = 1;
-            if (a.rows <= item_rows)
-                item = attn_units(p, a, 0);
-            else {
-#pragma unroll 1
-                for (long long base = 0;; base += 32 * item_rows) {  // ... and of its items the first
-                    const long long r    = base + lane * item_rows;
-                    const unsigned  size = r < a.rows ? attn_units(p, a, static_cast<int>(r)) : 0;
-                    unsigned        upto = size * heads;
-#pragma unroll
-                    for (int d = 1; d < 32; d <<= 1) {
-                        const unsigned other = __shfl_up_sync(0xffffffffu, upto, d);
-                        if (lane >= d)
-                            upto += other;
+        }
+        start.sequence = b;
+        start.row0     = row0;
+        start.head     = static_cast<int>((u0 - before) / item);
+        start.unit     = static_cast<int>((u0 - before) % item);
+    }
+    start.units = u1 - u0;
+    start.share = static_cast<int>(share);
+    return start;
+}
+
+// Walks a CTA's share of the linear sequence of units, order (sequence, rows, key/value head, keys).
+struct AttnCursor {
+    AttnSequence a;
+    AttnSegment  seg;
+    unsigned     left;
+    int          next_unit;  // of the item
+    int          extra;      // units of the item beyond its tiles
+    int          share;      // units of a CTA
+
+    __device__ __forceinline__ void enter_rows(const AttentionParams& p)
+    {
+        const int end  = min(seg.row0 + 2 * p.tile_rows, a.rows);
+        seg.rows       = end - seg.row0;
+        seg.pair       = seg.rows > p.tile_rows;
+        seg.fourfold   = seg.rows <= p.few_rows;
+        extra          = attn_extra_units(p, seg.rows);
+        seg.keys       = attn_keys(p, a, end);
+        seg.tiles      = attn_tiles(seg.keys);
+        seg.tiles0     = seg.pair ? attn_tiles(attn_keys(p, a, seg.row0 + p.tile_rows)) : seg.tiles;
+        seg.open[0]    = attn_open_keys(p, a, seg.row0);
+        seg.open[1]    = seg.pair ? attn_open_keys(p, a, seg.row0 + p.tile_rows) : seg.open[0];
+    }
+    __device__ __forceinline__ void enter_sequence(const AttentionParams& p, const AttnShared& sh)
+    {
+        for (;; ++seg.b) {
+            if (seg.b >= p.batch.sequences) {  // only if somebody writes the arrays during the call
+                left = 0;
+                return;
+            }
+            a = attn_sequence(p, sh, seg.b);
+            if (a.rows > 0)
+                break;
+        }
+        seg.first   = a.s.first;
+        seg.count   = a.s.count;
+        seg.context = a.s.context;
+        seg.prefix  = a.prefix;
+        enter_rows(p);
+    }
+    __device__ __forceinline__ AttnCursor(const AttentionParams& p, const AttnShared& sh, const AttnStart& start)
+    {
+        left      = start.units;
+        share     = start.share;
+        seg.b     = start.sequence;
+        seg.row0  = start.row0;
+        seg.head  = start.head;
+        next_unit = start.unit;
+        if (left > 0)
+            enter_sequence(p, sh);
+    }
+    // The next segment that has a tile; its `end` is 0 at the end of the share.
+    __device__ __forceinline__ void next(const AttentionParams& p, const AttnShared& sh)
+    {
+        do {
+            if (left > 0 && next_unit >= seg.tiles + extra) {
+                next_unit = 0;
+                if (++seg.head == p.batch.kv_heads) {
+                    seg.head = 0;
+                    seg.row0 += 2 * p.tile_rows;
+                    if (seg.row0 >= a.rows) {
+                        seg.row0 = 0;
+                        ++seg.b;
+                        enter_sequence(p, sh);
                     }
-                    const unsigned past = __ballot_sync(0xffffffffu, before + upto > u0);
-                    if (past || base + 32 * item_rows >= a.rows) {
-                        const int l = past ? __ffs(past) - 1 : 0;
-                        row0        = static_cast<int>(base) + l * item_rows;
-                        item        = max(1u, __shfl_sync(0xffffffffu, size, l));
-                        before += __shfl_sync(0xffffffffu, upto - size * heads, l);
-                        break;
-                    }
-                    before += __shfl_sync(0xffffffffu, upto, 31);
+                    else
+                        enter_rows(p);
                 }
             }
-            if (lane == 0) {
-                sh.start_sequence = b;
-                sh.start_rows     = row0;
-                sh.start_head     = static_cast<int>((u0 - before) / item);
-                sh.start_unit     = static_cast<int>((u0 - before) % item);
-            }
-        }
-        if (lane == 0)
-            sh.start_units = u1 - u0;
+            seg.begin = seg.end = 0;
+            if (left == 0)
+                return;
+            const int upto  = static_cast<int>(min(static_cast<unsigned>(seg.tiles + extra), next_unit + left));
+            seg.begin       = attn_cut(next_unit, seg.tiles, extra, share);
+            seg.end         = attn_cut(upto, seg.tiles, extra, share);
+            left -= upto - next_unit;
+            next_unit = upto;
+        } while (seg.end == seg.begin);
     }
-    __syncthreads();
-}
+};
 
 // ---------------------------------------------------------------- masks
 
@@ -838,7 +854,7 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
     }
     ptx::grid_dependency_wait();
     ptx::tc_fence_before_sync();
-    attn_plan(p, sh, HEAD_DIM);
+    attn_count_units(p, sh, HEAD_DIM);
     ptx::tc_fence_after_sync();
     const uint32_t tmem = sh.tmem;
     if (threadIdx.x == 0)
@@ -1223,7 +1239,7 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
         const int         piece    = lane / kBlocks, block = lane % kBlocks;
         const bool        active   = piece < pieces;
         const uint32_t    offset   = block * kBlock + piece * box * 128;
-        AttnCursor        cursor(p, sh);
+        AttnCursor        cursor(p, sh, attn_start(p, sh));
         const AttnSegment& seg     = cursor.seg;
         uint32_t          n        = 0;
         bool              ok       = true;
@@ -1353,8 +1369,8 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
 template<int HEAD_DIM>
 __global__ void __launch_bounds__(256) attention_join_kernel(const AttentionParams p, int ctas)
 {
-    ptx::grid_dependency_wait();
     ptx::grid_launch_dependents();
+    ptx::grid_dependency_wait();
     const AttnPart* const parts = reinterpret_cast<const AttnPart*>(p.workspace);
     const float2* const   stats = reinterpret_cast<const float2*>(p.workspace + attn_stats_offset(ctas));
     const float4* const   sums  = reinterpret_cast<const float4*>(p.workspace + attn_sums_offset(ctas));
