@@ -22,8 +22,6 @@
 #pragma once
 #include <math_constants.h>
 
-#include <type_traits>
-
 #include "cache_batch.cuh"
 #include "tiling.h"
 
@@ -70,7 +68,9 @@ constexpr int kAttnSegments  = 8;  // segments that shared memory holds at a tim
 // Registers of a thread: the softmax warps keep a row of 128 scores, 256 x 208 + 128 x 88 = 384 x 168.
 constexpr int kAttnSoftmaxRegisters = 208, kAttnOtherRegisters = 88;
 
-constexpr unsigned long long kAttnWaitLimitNs = 200ull * 1000 * 1000;
+// Looks at a barrier before a CTA gives up: some tenths of a second at least.  (Counted and not timed: the waits stand in many
+// places, and code that the instruction cache need not hold is time: ragged prompts 57 us with a clock in each, now 55.)
+constexpr uint32_t kAttnWaitLimit = 1u << 24;
 
 // Tiles of keys (and as many of values) in shared memory at a time.
 __host__ __device__ constexpr int attn_stages(int head_dim)
@@ -169,22 +169,17 @@ __host__ __device__ constexpr size_t attn_workspace_bytes(int ctas, int head_dim
 
 __device__ __forceinline__ bool attn_wait_longer(uint32_t bar, uint32_t parity, volatile uint32_t* abort_flag, unsigned int* status)
 {
-    uint64_t t0 = 0;
 #pragma unroll 1
     for (uint32_t it = 1;; ++it) {
         if (ptx::mbar_try_wait(bar, parity))
             return true;
-        if ((it & 63u) == 0u) {
-            if (*abort_flag)
-                return false;
-            const uint64_t now = ptx::globaltimer_ns();
-            if (t0 == 0)
-                t0 = now;
-            else if (now - t0 > kAttnWaitLimitNs) {
+        if ((it & 1023u) == 0u) {
+            if (it >= kAttnWaitLimit) {
                 *abort_flag = 1u;
                 atomicOr(status, kStatusWaitExpired);
-                return false;
             }
+            if (*abort_flag)
+                return false;
         }
     }
 }
@@ -410,64 +405,68 @@ struct AttnCursor {
     int          extra;      // units of the item beyond its tiles
     int          share;      // units of a CTA
 
-    __device__ __forceinline__ void enter_rows(const AttentionParams& p)
+    bool         new_sequence, new_rows;  // what `seg` does not describe yet
+
+    __device__ __forceinline__ explicit AttnCursor(const AttnStart& start)
     {
-        const int end  = min(seg.row0 + 2 * p.tile_rows, a.rows);
-        seg.rows       = end - seg.row0;
-        seg.pair       = seg.rows > p.tile_rows;
-        seg.fourfold   = seg.rows <= p.few_rows;
-        extra          = attn_extra_units(p, seg.rows);
-        seg.keys       = attn_keys(p, a, end);
-        seg.tiles      = attn_tiles(seg.keys);
-        seg.tiles0     = seg.pair ? attn_tiles(attn_keys(p, a, seg.row0 + p.tile_rows)) : seg.tiles;
-        seg.open[0]    = attn_open_keys(p, a, seg.row0);
-        seg.open[1]    = seg.pair ? attn_open_keys(p, a, seg.row0 + p.tile_rows) : seg.open[0];
-    }
-    __device__ __forceinline__ void enter_sequence(const AttentionParams& p, const AttnShared& sh)
-    {
-        for (;; ++seg.b) {
-            if (seg.b >= p.batch.sequences) {  // only if somebody writes the arrays during the call
-                left = 0;
-                return;
-            }
-            a = attn_sequence(p, sh, seg.b);
-            if (a.rows > 0)
-                break;
-        }
-        seg.first   = a.s.first;
-        seg.count   = a.s.count;
-        seg.context = a.s.context;
-        seg.prefix  = a.prefix;
-        enter_rows(p);
-    }
-    __device__ __forceinline__ AttnCursor(const AttentionParams& p, const AttnShared& sh, const AttnStart& start)
-    {
-        left      = start.units;
-        share     = start.share;
-        seg.b     = start.sequence;
-        seg.row0  = start.row0;
-        seg.head  = start.head;
-        next_unit = start.unit;
-        if (left > 0)
-            enter_sequence(p, sh);
+        left         = start.units;
+        share        = start.share;
+        seg.b        = start.sequence;
+        seg.row0     = start.row0;
+        seg.head     = start.head;
+        next_unit    = start.unit;
+        new_sequence = true;
+        new_rows     = false;
+        seg.tiles    = 0x7fffff00;  // until the sequence is entered
+        extra        = 0;
     }
     // The next segment that has a tile; its `end` is 0 at the end of the share.
     __device__ __forceinline__ void next(const AttentionParams& p, const AttnShared& sh)
     {
         do {
-            if (left > 0 && next_unit >= seg.tiles + extra) {
+            if (next_unit >= seg.tiles + extra) {
                 next_unit = 0;
                 if (++seg.head == p.batch.kv_heads) {
                     seg.head = 0;
                     seg.row0 += 2 * p.tile_rows;
+                    new_rows = true;
                     if (seg.row0 >= a.rows) {
                         seg.row0 = 0;
                         ++seg.b;
-                        enter_sequence(p, sh);
+                        new_sequence = true;
                     }
-                    else
-                        enter_rows(p);
                 }
+            }
+            if (left > 0 && new_sequence) {
+#pragma unroll 1
+                for (;; ++seg.b) {
+                    if (seg.b >= p.batch.sequences) {  // only if somebody writes the arrays during the call
+                        left = 0;
+                        break;
+                    }
+                    a = attn_sequence(p, sh, seg.b);
+                    if (a.rows > 0)
+                        break;
+                }
+                seg.first    = a.s.first;
+                seg.count    = a.s.count;
+                seg.context  = a.s.context;
+                seg.prefix   = a.prefix;
+                new_sequence = false;
+                new_rows     = true;
+            }
+            if (left > 0 && new_rows) {
+                const int end = min(seg.row0 + 2 * p.tile_rows, a.rows);
+                seg.rows      = end - seg.row0;
+                seg.pair      = seg.rows > p.tile_rows;
+                seg.fourfold  = seg.rows <= p.few_rows;
+                extra         = attn_extra_units(p, seg.rows);
+                seg.keys      = attn_keys(p, a, end);
+                seg.tiles     = attn_tiles(seg.keys);
+                seg.tiles0    = seg.pair ? attn_tiles(attn_keys(p, a, seg.row0 + p.tile_rows)) : seg.tiles;
+                seg.open[0]   = attn_open_keys(p, a, seg.row0);
+                seg.open[1]   = seg.pair ? attn_open_keys(p, a, seg.row0 + p.tile_rows) : seg.open[0];
+                new_rows      = false;
             }
             seg.begin = seg.end = 0;
             if (left == 0)
@@ -1144,61 +1143,17 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
         const uint64_t q_desc = ptx::umma_desc_kmajor_sw128(q_base), k_desc = ptx::umma_desc_kmajor_sw128(k_base);
         const uint64_t v_desc  = ptx::umma_desc_nmajor_sw128(v_base, kBlock);
         uint32_t       loaded  = 0;  // tiles of keys before this segment
-        uint32_t       q_parity0 = 0, q_parity1 = 0, p_parity0 = 0, p_parity1 = 0;
+        uint32_t       q_parity = 0, p_parity = 0;
         bool           ok = true;
-        // Everything but the group is known to the compiler, and all lanes come to the same answer.
+        // Both groups take the same code, parities of their barriers are the bits of a register: the instruction cache holds it more
+        // often (code for each group: ragged prompts 64 us, now 57).
         int  tiles0 = 0, tiles1 = 0;
         bool pair = false;
         auto have     = [&](const unsigned long long* barrier, uint32_t parity) {
             return __all_sync(0xffffffffu, attn_wait(barrier, parity, sh, status)) != 0;
         };
         auto stage_of = [&](int group, int i) { return loaded + static_cast<uint32_t>(pair ? i : group + 2 * i); };
-        auto scores   = [&](auto which, int i) {
-            constexpr int  group = decltype(which)::value;
-            const uint32_t n = stage_of(group, i), stage = n % kStages;
-            const uint64_t q = q_desc + (pair ? group * (kTileBytes >> 4) : 0), k = k_desc + stage * (kTileBytes >> 4);
-            const bool     last = i + 1 == (group == 0 ? tiles0 : tiles1);
-            if (!have(&sh.k_full[stage], n / kStages & 1u))
-                return false;
-            ptx::tc_fence_after_sync();
-#pragma unroll
-            for (int block = 0; block < kBlocks; ++block)
-                ptx::umma_f16_ss_x4_elect(tmem + kS + group * 128, q + block * (kBlock >> 4), k + block * (kBlock >> 4), idesc_s, block > 0);
-            ptx::umma_commit_elect(ptx::smem_u32(&sh.s_full[group]));
-            if (!pair || group == 1)  // the last to need this tile of keys
-                ptx::umma_commit_elect(ptx::smem_u32(&sh.k_empty[stage]));
-            // Q's room is free for the next segment's after the group's last scores; where the groups share it, after the last
-            // of both (the groups take turns: the second's if their numbers are even, else the first's).
-            if (last && (pair || (tiles0 == tiles1) == (group == 1)))
-                ptx::umma_commit_elect(ptx::smem_u32(&sh.q_empty[pair ? group : 0]));
-            return true;
-        };
-        auto products = [&](auto which, int i) {
-            constexpr int  group = decltype(which)::value;
-            const uint32_t n = stage_of(group, i), stage = n % kStages;
-            const uint64_t v = v_desc + stage * (kTileBytes >> 4);
-            uint32_t&      parity = group == 0 ? p_parity0 : p_parity1;
-            if (!have(&sh.v_clean[stage], n / kStages & 1u))
-                return false;
-#pragma unroll
-            for (int half_tile = 0; half_tile < 2; ++half_tile) {
-                if (!have(&sh.p_full[group][half_tile], parity))
-                    return false;
-                ptx::tc_fence_after_sync();
-                ptx::umma_f16_ts_x4_elect(tmem + kO + group * 128, tmem + kS + group * 128 + half_tile * 32,
-                                          v + half_tile * (4 * 2048 >> 4), idesc_o, i > 0 || half_tile > 0);
-            }
-            parity ^= 1u;
-            // Scores that are complete mean that the product before them is: o_done tells of a segment's last alone.
-            if (i + 1 == (group == 0 ? tiles0 : tiles1))
-                ptx::umma_commit_elect(ptx::smem_u32(&sh.o_done[group]));
-            if (!pair || group == 1)
-                ptx::umma_commit_elect(ptx::smem_u32(&sh.v_empty[stage]));
-            return true;
-        };
-        constexpr std::integral_constant<int, 0> first{};
-        constexpr std::integral_constant<int, 1> second{};
-        const AttnSegment*                       current = nullptr;
+        const AttnSegment* current = nullptr;
 #pragma unroll 1
         for (int number = 0; ok; ++number) {
             current = attn_segment(sh, number, status);
@@ -1208,24 +1163,60 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
             tiles1 = current->count_of(1);
             pair   = current->pair;
             const int length = current->end - current->begin;
-            if (tiles0 > 0) {
-                ok = have(&sh.q_full[0], q_parity0) && scores(first, 0);
-                q_parity0 ^= 1u;
-            }
-            if (ok && tiles1 > 0) {
-                if (pair) {
-                    ok = have(&sh.q_full[1], q_parity1);
-                    q_parity1 ^= 1u;
-                }
-                ok = ok && scores(second, 0);
-            }
+            // Step i of a group: the product of its i-th weights and values, and the scores of its next tile; step -1 has no product.
 #pragma unroll 1
-            for (int i = 0; ok && (i < tiles0 || i < tiles1); ++i) {
-                if (i < tiles0)
-                    ok = products(first, i) && (i + 1 >= tiles0 || scores(first, i + 1));
-                if (ok && i < tiles1)
-                    ok = products(second, i) && (i + 1 >= tiles1 || scores(second, i + 1));
-            }
+            for (int i = -1; ok && (i < tiles0 || i < tiles1); ++i)
+#pragma unroll 1
+                for (int group = 0; ok && group < 2; ++group) {
+                    const int tiles = group == 0 ? tiles0 : tiles1;
+                    if (i >= tiles)
+                        continue;
+                    const uint32_t d = tmem + group * 128;
+                    if (i >= 0) {
+                        const uint32_t n = stage_of(group, i), stage = n % kStages, parity = p_parity >> group & 1u;
+                        const uint64_t v = v_desc + stage * (kTileBytes >> 4);
+                        ok = have(&sh.v_clean[stage], n / kStages & 1u) && have(&sh.p_full[group][0], parity);
+                        if (!ok)
+                            break;
+                        ptx::tc_fence_after_sync();
+                        ptx::umma_f16_ts_x4_elect(d + kO, d + kS, v, idesc_o, i > 0);
+                        ok = have(&sh.p_full[group][1], parity);
+                        if (!ok)
+                            break;
+                        ptx::tc_fence_after_sync();
+                        ptx::umma_f16_ts_x4_elect(d + kO, d + kS + 32, v + (4 * 2048 >> 4), idesc_o, 1u);
+                        p_parity ^= 1u << group;
+                        // Scores that are complete mean that the product before them is: o_done tells of a segment's last alone.
+                        if (i + 1 == tiles)
+                            ptx::umma_commit_elect(ptx::smem_u32(&sh.o_done[group]));
+                        if (!pair || group == 1)
+                            ptx::umma_commit_elect(ptx::smem_u32(&sh.v_empty[stage]));
+                    }
+                    else if (pair || group == 0) {
+                        if (tiles == 0)
+                            continue;
+                        ok = have(&sh.q_full[group], q_parity >> group & 1u);
+                        q_parity ^= 1u << group;
+                    }
+                    if (!ok || i + 1 >= tiles)
+                        continue;
+                    const uint32_t n = stage_of(group, i + 1), stage = n % kStages;
+                    const uint64_t q = q_desc + (pair ? group * (kTileBytes >> 4) : 0), k = k_desc + stage * (kTileBytes >> 4);
+                    ok = have(&sh.k_full[stage], n / kStages & 1u);
+                    if (!ok)
+                        break;
+                    ptx::tc_fence_after_sync();
+#pragma unroll
+                    for (int block = 0; block < kBlocks; ++block)
+                        ptx::umma_f16_ss_x4_elect(d + kS, q + block * (kBlock >> 4), k + block * (kBlock >> 4), idesc_s, block > 0);
+                    ptx::umma_commit_elect(ptx::smem_u32(&sh.s_full[group]));
+                    if (!pair || group == 1)  // the last to need this tile of keys
+                        ptx::umma_commit_elect(ptx::smem_u32(&sh.k_empty[stage]));
+                    // Q's room is free for the next segment's after the group's last scores; where the groups share it, after the
+                    // last of both (the groups take turns: the second's if their numbers are even, else the first's).
+                    if (i + 2 == tiles && (pair || (tiles0 == tiles1) == (group == 1)))
+                        ptx::umma_commit_elect(ptx::smem_u32(&sh.q_empty[pair ? group : 0]));
+                }
             loaded += length;
         }
         __syncwarp();
@@ -1239,7 +1230,7 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
         const int         piece    = lane / kBlocks, block = lane % kBlocks;
         const bool        active   = piece < pieces;
         const uint32_t    offset   = block * kBlock + piece * box * 128;
-        AttnCursor        cursor(p, sh, attn_start(p, sh));
+        AttnCursor        cursor(attn_start(p, sh));
         const AttnSegment& seg     = cursor.seg;
         uint32_t          n        = 0;
         bool              ok       = true;
