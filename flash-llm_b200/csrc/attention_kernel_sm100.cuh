@@ -237,12 +237,13 @@ __device__ __forceinline__ int attn_tiles(int keys)
     return (keys + kAttnKeys - 1) / kAttnKeys;
 }
 
-// Beginning an item, and ending it, takes about as long as two of its tiles of keys, and as five where its groups share their rows
+// Beginning an item, and ending it, takes about as long as two of its tiles of keys, and as four where its groups share their rows
 // and join their sums (us a call with 2 / 3 / 4 for all: decoding of 64 sequences 128 / 124 / 122, prompts with a prefix 73 / 76 /
-// 79): an item counts as so many units more than it has tiles when the work is dealt out.
+// 79; later 116 with five for these, 114 with four): an item counts as so many units more than it has tiles when the work is dealt
+// out.
 __device__ __forceinline__ int attn_extra_units(const AttentionParams& p, int rows)
 {
-    return rows > p.tile_rows ? 2 : 5;
+    return rows > p.tile_rows ? 2 : 4;
 }
 
 // The tile of an item with `tiles` before which unit x of it cuts it.  Where a CTA's share is but a few tiles, one for each group is
@@ -558,31 +559,25 @@ __device__ __forceinline__ void attn_add_not_finite(const AttentionParams& p, co
         }
 }
 
+// tanh x on [-0.75, 0.75] to 2e-7: x times a polynomial in x^2, fitted to it for the smallest largest error.  A call has the
+// coefficients times its cap.
+constexpr float kAttnTanhRange = 0.75f;
+constexpr int   kAttnTanhTerms = 5;
+__device__ constexpr float kAttnTanh[kAttnTanhTerms] = {0.9999971985816956f, -0.33323076367378235f, 0.13226091861724854f, -0.04928046092391014f, 0.012318842113018036f};
+
 // What a softmax thread keeps of its row from tile to tile, and what the transformation of its scores takes.
 struct AttnState {
     float top, sum;      // the maximum that weights are taken against (of q.k, or of scores times log2 e), their sum
     float factor;        // what turns the scores at hand into powers of two
     float scale, cap;    // of scores in units of log 2; cap 0: none
     float cap_in;        // products times this are what the tanh takes
+    float tanh[kAttnTanhTerms];  // cap times the polynomial's coefficients
     float slope;         // in units of log 2
     bool  biased;        // by slopes
     int   place;         // the row's position
     const int* drafted;  // positions of drafted tokens in shared memory, or nullptr
     bool  valid;         // the row is somebody's
 };
-
-// tanh on [-1, 1] to 2.4e-7: x times a polynomial in x^2, fitted to it for the smallest largest error.
-__device__ __forceinline__ float2 attn_tanh_small(float2 x)
-{
-    const float2 y = ptx::mul_x2(x, x);
-    float2       t = make_float2(-0.002839469350874424f, -0.002839469350874424f);
-    t              = ptx::fma_x2(t, y, make_float2(0.016114192083477974f, 0.016114192083477974f));
-    t              = ptx::fma_x2(t, y, make_float2(-0.05097287520766258f, -0.05097287520766258f));
-    t              = ptx::fma_x2(t, y, make_float2(0.13253526389598846f, 0.13253526389598846f));
-    t              = ptx::fma_x2(t, y, make_float2(-0.3332400321960449f, -0.3332400321960449f));
-    t              = ptx::fma_x2(t, y, make_float2(0.9999968409538269f, 0.9999968409538269f));
-    return ptx::mul_x2(x, t);
-}
 
 // The largest of a row's scores, NaN if one of them is.
 template<int COLUMNS>
@@ -615,13 +610,17 @@ __device__ __forceinline__ void attn_transform(const AttnState& st, float (&s)[3
             largest.y = ptx::max3_nan(largest.y, fabsf(s[c + 2]), fabsf(s[c + 3]));
         }
         const float in = st.cap_in;
-        if (__all_sync(0xffffffffu, !st.valid || ptx::max3_nan(largest.x, largest.y, largest.y) * in <= 1.0f)) {
+        if (__all_sync(0xffffffffu, !st.valid || ptx::max3_nan(largest.x, largest.y, largest.y) * in <= kAttnTanhRange)) {
 #pragma unroll
             for (int c = 0; c < 32; c += 2) {
-                const float2 t = ptx::mul_x2(attn_tanh_small(ptx::mul_x2(make_float2(s[c], s[c + 1]), make_float2(in, in))),
-                                             make_float2(st.cap, st.cap));
-                s[c]           = t.x;
-                s[c + 1]       = t.y;
+                const float2 x = ptx::mul_x2(make_float2(s[c], s[c + 1]), make_float2(in, in)), y = ptx::mul_x2(x, x);
+                float2       t = make_float2(st.tanh[kAttnTanhTerms - 1], st.tanh[kAttnTanhTerms - 1]);
+#pragma unroll
+                for (int k = kAttnTanhTerms - 2; k >= 0; --k)
+                    t = ptx::fma_x2(t, y, make_float2(st.tanh[k], st.tanh[k]));
+                t        = ptx::mul_x2(x, t);
+                s[c]     = t.x;
+                s[c + 1] = t.y;
             }
         }
         else {
@@ -899,6 +898,9 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
                 st.scale = p.scale * CUDART_L2E_F;
                 st.cap    = p.cap * CUDART_L2E_F;
                 st.cap_in = p.cap > 0.0f ? p.scale / p.cap : 0.0f;
+#pragma unroll
+                for (int k = 0; k < kAttnTanhTerms; ++k)
+                    st.tanh[k] = kAttnTanh[k] * st.cap;
                 st.place = seg.context + token;
                 if (p.slopes) {
                     st.biased = true;
