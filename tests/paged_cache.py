@@ -70,8 +70,8 @@ def random_tree(counts, contexts, seed, device="cuda", reach=6):
 def attention(batch: Batch, tree_mask=None, positions=None, prefix=None, scale=None, cap=0.0, slopes=None):
     """(output, bound on the kernels' error) of every row of a sequence, [rows][heads * dim] in 64 bits.
 
-    The bound: a weight p is rounded to fp16 once (2^-11 of it, or 2^-25 where it is subnormal: weights are at most 2^8 above
-    the largest, at least 1, which their sum is divided by), the output once (2^-11 of it).  A score is a sum of `dim` products
+    The bound: a weight p is rounded to fp16 once (2^-11 of it, or 2^-25 where it is subnormal: the largest weight is at least 1,
+    and so is their sum, which they are divided by), the output once (2^-11 of it).  A score is a sum of `dim` products
     in 32 bits, truncated rather than rounded at each of dim / 16 additions of the tensor core: below 2^-20 of the sum of the
     products' sizes; cap and distance are a few roundings of 2^-24 of their own sizes each.  An error d of the scores is one of
     2 d of the weights, numerator and denominator together."""

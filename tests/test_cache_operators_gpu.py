@@ -150,6 +150,8 @@ PROMPTS = [
     ([0], [700], 8, 1, 64, 64, 0.0, False, [333]),
     ([5000], [3], 32, 8, 128, 512, 0.0, False, None),
     ([100 + 7 * i for i in range(70)], [1] * 70, 8, 2, 128, 64, 0.0, True, None),
+    ([(37 * i) % 300 for i in range(600)], [(i % 7) // 3 for i in range(600)], 7, 1, 64, 16, 0.0, False, None),  # some sequences empty
+    ([2, 700, 0], [3, 130, 61], 14, 2, 128, 64, 12.0, True, None),  # single tiles and pairs of them in one call
     ([31, 5], [1, 9], 128, 1, 64, 16, 0.0, False, None),  # a token fills a tile of rows
     ([0, 3], [50, 90], 21, 3, 128, 32, 0.0, False, [-5, 1 << 30]),  # prefixes out of range: none, and all
 ]
