@@ -65,11 +65,12 @@ constexpr int kAttnThreads   = 12 * 32;
 constexpr int kAttnTmemCols  = 512;
 constexpr int kAttnKnown     = 512;  // sequences whose sizes are kept in shared memory from the plan on
 constexpr int kAttnSegments  = 8;  // segments that shared memory holds at a time
-// Registers of a thread: the softmax warps keep a row of 128 scores, 256 x 208 + 128 x 88 = 384 x 168.
+// Registers of a thread, 256 x 208 + 128 x 88 = 384 x 168: a softmax thread keeps 32 scores of its row and what the scores of the
+// next piece and the ends of an item (32 outputs of its row and of the other group's) take besides.
 constexpr int kAttnSoftmaxRegisters = 208, kAttnOtherRegisters = 88;
 
 // Looks at a barrier before a CTA gives up: some tenths of a second at least.  (Counted and not timed: the waits stand in many
-// places, and code that the instruction cache need not hold is time: ragged prompts 57 us with a clock in each, now 55.)
+// places, and code that the instruction cache need not hold is time: ragged prompts 57 us with a clock in each, 55 without.)
 constexpr uint32_t kAttnWaitLimit = 1u << 24;
 
 // Tiles of keys (and as many of values) in shared memory at a time.
@@ -239,7 +240,7 @@ __device__ __forceinline__ int attn_tiles(int keys)
 
 // Beginning an item, and ending it, takes about as long as two of its tiles of keys, and as four where its groups share their rows
 // and join their sums (us a call with 2 / 3 / 4 for all: decoding of 64 sequences 128 / 124 / 122, prompts with a prefix 73 / 76 /
-// 79; later 116 with five for these, 114 with four): an item counts as so many units more than it has tiles when the work is dealt
+// 79; with 4 / 5 for the latter alone: decoding 114 / 116): an item counts as so many units more than it has tiles when the work is dealt
 // out.
 __device__ __forceinline__ int attn_extra_units(const AttentionParams& p, int rows)
 {
@@ -761,6 +762,32 @@ __device__ __forceinline__ void attn_softmax(AttnState& st, const AttnRow& row, 
         part_done(0);
         part_done(1);
     }
+    else if (PLAIN && !masked) {
+        // 64 columns at a time: half the waits for loads of the other way, which has more to do per column (prompt of 7000 tokens
+        // 444 us instead of 461, ragged prompts 55.0 instead of 55.7; all 128 in registers 467 and 60.9).
+        float new_top = st.top;
+#pragma unroll 1
+        for (int c = 0; c < kAttnKeys; c += 64) {
+            float s[64];
+            attn_load_scores(s_tmem + c, s);
+            new_top = attn_largest(s, new_top);
+        }
+        attn_new_top(st, new_top, first, rescale);
+        const float minus = st.top == -CUDART_INF_F ? 0.0f : -st.top * st.factor;
+#pragma unroll 1
+        for (int c = 0; c < kAttnKeys; c += 64) {  // weights take the place of scores already read
+            float    s[64];
+            uint32_t w[16];
+            attn_load_scores(s_tmem + c, s);
+#pragma unroll
+            for (int k = 0; k < 64; k += 32) {
+                attn_weights<PLAIN>(s + k, st.factor, minus, part, w);
+                ptx::tmem_st_x16(s_tmem + (c + k) / 2, w);
+            }
+            stored();
+            part_done(c / 64);
+        }
+    }
     else {
         // 32 columns at a time, masked or transformed scores back to tensor memory in between: with all 128 in registers the code of
         // one tile does not fit the instruction cache (capped trees of 64 tokens took 90 us instead of 77, ragged prompts 71
@@ -775,11 +802,9 @@ __device__ __forceinline__ void attn_softmax(AttnState& st, const AttnRow& row, 
             if (masked)
                 attn_mask(row, s, key0 + c);
             new_top = attn_largest(s, new_top);
-            if (!PLAIN || masked)
-                ptx::tmem_st_x32(s_tmem + c, reinterpret_cast<const uint32_t*>(s));
+            ptx::tmem_st_x32(s_tmem + c, reinterpret_cast<const uint32_t*>(s));
         }
-        if (!PLAIN || masked)
-            ptx::tmem_wait_st();
+        ptx::tmem_wait_st();
         attn_new_top(st, new_top, first, rescale);
         const float minus = st.top == -CUDART_INF_F ? 0.0f : -st.top * st.factor;
 #pragma unroll 2
@@ -1148,11 +1173,13 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
         uint32_t       q_parity = 0, p_parity = 0;
         bool           ok = true;
         // Both groups take the same code, parities of their barriers are the bits of a register: the instruction cache holds it more
-        // often (code for each group: ragged prompts 64 us, now 57).
+        // often (code for each group: ragged prompts 64 us instead of 57).
         int  tiles0 = 0, tiles1 = 0;
         bool pair = false;
         auto have     = [&](const unsigned long long* barrier, uint32_t parity) {
-            return __all_sync(0xffffffffu, attn_wait(barrier, parity, sh, status)) != 0;
+            const uint32_t bar = ptx::smem_u32(barrier);  // one look first (prompt of 7000 tokens 438 us instead of 444)
+            return __all_sync(0xffffffffu, ptx::mbar_try_wait(bar, parity)) != 0
+                   || __all_sync(0xffffffffu, attn_wait_longer(bar, parity, &sh.abort_flag, status)) != 0;
         };
         auto stage_of = [&](int group, int i) { return loaded + static_cast<uint32_t>(pair ? i : group + 2 * i); };
         const AttnSegment* current = nullptr;

@@ -178,7 +178,7 @@ constexpr int kAcceptThreads = 256;
 // Keys and values of drafted token accepted[b][i] move to position context[b] + i.  A CTA takes a share of one sequence's heads
 // and layers, as many at a time as its registers hold whole: all of a head is read before any of it is written, so that sources
 // and targets may overlap in any way.  Bound by the chain of loads that leads to the rows, which the heads and layers of a CTA
-// share (24 sequences, 32 layers: a CTA for each head and layer 14.3 us, now 8.4).
+// share (24 sequences, 32 layers: a CTA for each head and layer 14.3 us, this 8.0).
 template<int HEAD_DIM>
 __global__ void __launch_bounds__(kAcceptThreads) cache_accept_kernel(const AcceptParams p)
 {
