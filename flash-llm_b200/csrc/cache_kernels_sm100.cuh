@@ -87,11 +87,11 @@ __global__ void __launch_bounds__(kRotaryThreads) rotary_append_kernel(const Rot
     const double frequency = threadIdx.x < pairs ? p.frequencies[threadIdx.x] : 0.0;
     const int    elsewhere = p.positions && threadIdx.x < pairs ? p.positions[n] : 0;
     for (int b = threadIdx.x; b < c.sequences; b += kRotaryThreads) {
-        const int begin = c.cu_tokens[b], end = c.cu_tokens[b + 1], context = c.context[b];
-        if (begin >= 0 && begin <= n && n < end) {
-            const long long position = static_cast<long long>(context) + (n - begin);
-            s_sequence               = b;
-            s_position               = context >= 0 && position < table_positions(c) ? static_cast<int>(position) : -1;
+        const int begin = max(c.cu_tokens[b], 0), end = min(c.cu_tokens[b + 1], c.tokens), context = c.context[b];
+        if (begin <= n && n < end) {  // a sequence that does not fit is left out whole, as load_sequence has it
+            const bool fits = context >= 0 && static_cast<long long>(context) + (end - begin) <= table_positions(c);
+            s_sequence      = b;
+            s_position      = fits ? context + (n - begin) : -1;
         }
     }
     __syncthreads();

@@ -292,6 +292,32 @@ def test_bad_pages_and_lengths_are_reported(ops, lib):
         assert torch.equal(cache.view(torch.int16), old.view(torch.int16))
 
 
+def test_a_sequence_that_does_not_fit_is_not_appended(ops, lib):
+    """Not even those of its rows that would have room; its neighbours are."""
+    b = Batch([30, 40, 20], [2, 3, 1], 2, 1, 64, 16, seed=14)
+    positions = 16 * b.page_table.shape[1]
+    qkv = torch.randn((6, 4 * 64), device="cuda").to(torch.float16)
+    k_cache, v_cache = b.k_cache.clone(), b.v_cache.clone()
+    ops.rotary_append(qkv, k_cache, v_cache, b.cu_tokens, b.context, b.page_table)
+    assert lib.consume_status() == 0
+    for context in (-1, positions - 2, positions):
+        lengths = b.context.clone()
+        lengths[1] = context
+        k, v = b.k_cache.clone(), b.v_cache.clone()
+        ops.rotary_append(qkv, k, v, b.cu_tokens, lengths, b.page_table)
+        assert lib.consume_status() == BAD_CACHE
+        for got, old, new in ((k, b.k_cache, k_cache), (v, b.v_cache, v_cache)):
+            mine = b.page_table[1].long()
+            assert torch.equal(got[mine].view(torch.int16), old[mine].view(torch.int16))
+            for other in (0, 2):
+                pages = b.page_table[other].long()
+                assert torch.equal(got[pages].view(torch.int16), new[pages].view(torch.int16))
+    lengths = b.context.clone()
+    lengths[1] = positions - 3  # the last that fits
+    ops.rotary_append(qkv, b.k_cache, b.v_cache, b.cu_tokens, lengths, b.page_table)
+    assert lib.consume_status() == 0
+
+
 @pytest.mark.parametrize("page", [16, 128])
 def test_caches_longer_than_32_bits(ops, page):
     """Pages behind the 2^31st element of a cache, for every operator."""
