@@ -353,10 +353,12 @@ int FlashLLM_RotaryAppend(void*         stream,
 /* Attention of drafted tokens: Out[n][h] = sum over the keys j that row n sees of softmax_j(s_nj) V[j], with
  * s_nj = scale * Q[n][h] . K[j], then cap * tanh(s / cap) where cap > 0, then + slopes[h] * (position of j - position of n)
  * where slopes (device floats, [heads]) are given; zero for a row that sees no key.  Query head h reads key/value head
- * h / (heads / kv_heads), at most 128 query heads each.  The batch's own keys are in the cache already (FlashLLM_RotaryAppend).  A row sees the context of its
- * sequence and those of its sequence's first 64 new tokens whose bit tree_mask[n] has (its ancestors and itself, usually).
+ * h / (heads / kv_heads), at most 128 query heads each.  The batch's own keys are in the cache already (FlashLLM_RotaryAppend).
+ * A row sees the context of its sequence and those of its sequence's first 64 new tokens whose bit tree_mask[n] has (its
+ * ancestors and itself, usually).
  * `positions` (int32 [tokens]) are needed with slopes only: the distance is between them, for keys of the context to their
- * place.  Q is [tokens][ld_q], Out [tokens][heads * head_dim]; scale > 0.  `workspace`: FlashLLM_Attention_WorkspaceBytes on a
+ * place.  Q is [tokens][ld_q], Out [tokens][heads * head_dim], which must overlap none of the inputs; scale > 0, and scale / cap
+ * must stay finite.  `workspace`: FlashLLM_Attention_WorkspaceBytes on a
  * 16-byte boundary, its contents before and after the call of no use to anybody; calls that may overlap on the GPU need one
  * each. */
 int FlashLLM_TreeAttention(void*                     stream,

@@ -56,6 +56,9 @@ def test_bad_arguments_of_each_operator_are_refused(lib):
                    dict(cap=-1.0), dict(cap=math.nan), dict(cap=math.inf)):
         _refused(lib, lambda: lib.prompt_attention(0, **{**attend, **change}))
         _refused(lib, lambda: lib.tree_attention(0, tree_mask=P, **{**attend, **change}))
+    for change in (dict(scale=3e38), dict(cap=3e38), dict(scale=1.0, cap=1e-39), dict(scale=1e30, cap=1e-10)):  # what is made of them
+        _refused(lib, lambda: lib.prompt_attention(0, **{**attend, **change}))
+        _refused(lib, lambda: lib.tree_attention(0, tree_mask=P, **{**attend, **change}))
     _refused(lib, lambda: lib.tree_attention(0, tree_mask=None, **attend))
     _refused(lib, lambda: lib.tree_attention(0, tree_mask=P, slopes=P, **attend))  # distances need positions
     accept = dict(batch=b, accepted=P, accepted_lengths=P, accepted_width=4)
