@@ -184,16 +184,10 @@ static cudaError_t attend(cudaStream_t stream, AttentionParams p, const void* Q,
     p.v_cache = static_cast<const half*>(V_cache);
     p.slopes  = slopes;
     p.ld_q    = ld_q;
-    p.heads   = heads;
     p.scale   = scale;
     p.cap     = cap;
     p.workspace = static_cast<unsigned char*>(workspace);
-    p.share     = heads / kv_heads;
-    p.tile_rows = kAttnRows / p.share * p.share;
-    p.few_rows  = 32 / p.share * p.share;
-    while ((1 << p.share_shift) < p.share)
-        ++p.share_shift;
-    p.share_magic = static_cast<unsigned>(((1ull << 32) * ((1ull << p.share_shift) - p.share)) / p.share + 1);
+    attn_set_heads(&p, heads, kv_heads);
     return head_dim == 64 ? launch_attention<64>(stream, p) : launch_attention<128>(stream, p);
 }
 

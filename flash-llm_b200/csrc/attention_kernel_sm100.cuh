@@ -49,6 +49,18 @@ struct AttentionParams {
     float                     cap;  // 0: none
 };
 
+inline void attn_set_heads(AttentionParams* p, int heads, int kv_heads)
+{
+    p->heads          = heads;
+    p->batch.kv_heads = kv_heads;
+    p->share          = heads / kv_heads;
+    p->tile_rows      = 128 / p->share * p->share;
+    p->few_rows       = 32 / p->share * p->share;
+    for (p->share_shift = 0; (1 << p->share_shift) < p->share;)
+        ++p->share_shift;
+    p->share_magic = static_cast<unsigned>(((1ull << 32) * ((1ull << p->share_shift) - p->share)) / p->share + 1);
+}
+
 // Token of a row of a sequence's (tokens x share) rows.
 __device__ __forceinline__ int attn_token(const AttentionParams& p, int row)
 {
@@ -247,13 +259,19 @@ __device__ __forceinline__ int attn_extra_units(const AttentionParams& p, int ro
     return rows > p.tile_rows ? 2 : 4;
 }
 
-// The tile of an item with `tiles` before which unit x of it cuts it.  Where a CTA's share is but a few tiles, one for each group is
-// the least that pays: a single tile is not cut off.  (Larger shares even out better with every cut where it falls: capped trees
-// of 64 tokens 76 us, 80 with cuts moved by up to an eighth of the share.)
-__device__ __forceinline__ int attn_cut(int x, int tiles, int extra, int share)
+// The tile of an item with `tiles` before which unit x of it cuts it; no piece of `least` tiles or fewer is cut off.
+__device__ __forceinline__ int attn_cut(int x, int tiles, int extra, int least)
 {
-    const int t = x - extra, least = share <= 4 ? 1 : 0;
+    const int t = x - extra;
     return t >= tiles ? tiles : t <= least ? 0 : tiles - t <= least ? tiles : t;
+}
+
+// Where a CTA's share is but a few tiles, one for each group is the least that pays: a single tile is not cut off.  (Larger
+// shares even out better with every cut where it falls: capped trees of 64 tokens 76 us, 80 with cuts moved by up to an eighth of
+// the share.)
+__device__ __forceinline__ int attn_least(unsigned long long share)
+{
+    return share <= 4 ? 1 : 0;
 }
 
 // Units of the item whose rows begin with row0 of the sequence's.
@@ -272,7 +290,43 @@ __device__ __forceinline__ const AttnSegment* attn_segment(AttnShared& sh, int n
     return &sh.segment[place];
 }
 
-constexpr unsigned kAttnSeveralItems = 0xffffffffu, kAttnLostRows = 0xfffffffeu;  // in place of a sequence's units
+// In place of a sequence's units: several items, to be counted by a warp; rows to be cleared; in the end, more than 32 bits hold.
+constexpr unsigned kAttnSeveralItems = 0xffffffffu, kAttnLostRows = 0xfffffffeu, kAttnManyUnits = 0xffffffffu;
+
+// A sum over a warp's lanes that 64 bits hold.
+__device__ __forceinline__ unsigned long long attn_warp_sum(unsigned long long mine)
+{
+    const unsigned low = __reduce_add_sync(0xffffffffu, static_cast<unsigned>(mine) & 0xffffffu);
+    const unsigned mid = __reduce_add_sync(0xffffffffu, static_cast<unsigned>(mine >> 24) & 0xffffffu);
+    const unsigned top = __reduce_add_sync(0xffffffffu, static_cast<unsigned>(mine >> 48));
+    return low + (static_cast<unsigned long long>(mid) << 24) + (static_cast<unsigned long long>(top) << 48);
+}
+
+// Sums over a warp's lanes up to each lane.
+template<typename COUNT>
+__device__ __forceinline__ COUNT attn_warp_scan(COUNT mine)
+{
+    const int lane = threadIdx.x & 31;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+        const COUNT other = __shfl_up_sync(0xffffffffu, mine, d);
+        if (lane >= d)
+            mine += other;
+    }
+    return mine;
+}
+
+// Units of all items of a sequence's first key/value head, for a whole warp.  A sequence can have up to 2^49 of them, a call with
+// all heads of all sequences more: a prompt of 2 million tokens with 64 heads has 2^32, some 80 seconds' work.
+__device__ __forceinline__ unsigned long long attn_sequence_units(const AttentionParams& p, const AttnSequence& a)
+{
+    const int          item_rows = 2 * p.tile_rows;
+    unsigned long long mine      = 0;
+#pragma unroll 1
+    for (long long r = (threadIdx.x & 31) * item_rows; r < a.rows; r += 32 * item_rows)
+        mine += attn_units(p, a, static_cast<int>(r));
+    return attn_warp_sum(mine);
+}
 
 // Units of every sequence; all threads, ends with a barrier.  The rows of a sequence that does not fit into the page table are
 // cleared here, by one CTA.
@@ -298,21 +352,17 @@ __device__ __forceinline__ void attn_count_units(const AttentionParams& p, AttnS
         for (int b = warp; b < B; b += kAttnThreads / 32) {
             if (sh.units[b] < kAttnLostRows)
                 continue;
-            const AttnSequence a    = attn_sequence(p, b);
-            unsigned           mine = 0;
+            const AttnSequence a = attn_sequence(p, b);
             if (a.s.lost > 0 && b % gridDim.x == blockIdx.x) {
                 const long long row = static_cast<long long>(p.heads) * head_dim;
 #pragma unroll 1
                 for (long long i = lane * 8; i < a.s.lost * row; i += 32 * 8)
                     *reinterpret_cast<uint4*>(p.out + a.s.first * row + i) = make_uint4(0, 0, 0, 0);
             }
-#pragma unroll 1
-            for (long long r = lane * item_rows; r < a.rows; r += 32 * item_rows)
-                mine += attn_units(p, a, static_cast<int>(r));
-            mine = __reduce_add_sync(0xffffffffu, mine);
+            const unsigned long long units = attn_sequence_units(p, a);
             __syncwarp();
             if (lane == 0)
-                sh.units[b] = mine;
+                sh.units[b] = static_cast<unsigned>(min(units, static_cast<unsigned long long>(kAttnManyUnits)));
         }
         __syncthreads();
     }
@@ -320,81 +370,115 @@ __device__ __forceinline__ void attn_count_units(const AttentionParams& p, AttnS
 
 // Where this CTA's share begins and how long it is, for a whole warp.
 struct AttnStart {
-    unsigned units;
-    int      share, sequence, row0, head, unit;
+    unsigned long long units;
+    int                least, sequence, row0, head, unit;
 };
 
-__device__ __forceinline__ AttnStart attn_start(const AttentionParams& p, const AttnShared& sh)
+// Units of this lane's sequence of the 32 from `base` on, first key/value head, for a whole warp.
+__device__ __forceinline__ unsigned long long attn_units_of(const AttentionParams& p, const AttnShared& sh, int base)
 {
-    const int B = p.batch.sequences, lane = threadIdx.x & 31, item_rows = 2 * p.tile_rows;
-    AttnStart start{0, 0, 0, 0, 0, 0};
-    // All units of a call fit into 31 bits: so many tiles of 128 keys would take hours.
-    const unsigned heads = p.batch.kv_heads;
-    unsigned       total = 0;
+    const int          b    = base + (threadIdx.x & 31);
+    const unsigned     kept = b < p.batch.sequences ? sh.units[b] : 0;
+    unsigned long long mine = kept;
 #pragma unroll 1
-    for (int b = lane; b < B; b += 32)
-        total += sh.units[b];
-    const unsigned units = __reduce_add_sync(0xffffffffu, total) * heads;
-    const unsigned share = max((units + gridDim.x - 1) / gridDim.x, 2u);  // a tile for each group
-    const unsigned u0 = min(units, share * blockIdx.x), u1 = min(units, u0 + share);
-    if (u1 > u0) {
-        // The sequence that holds unit u0: the first whose running sum passes it.
-        unsigned before = 0;
-        int      b      = 0;
+    for (unsigned many = __ballot_sync(0xffffffffu, kept == kAttnManyUnits); many; many &= many - 1) {
+        const int                at    = base + __ffs(many) - 1;
+        const unsigned long long units = attn_sequence_units(p, attn_sequence(p, sh, at));
+        mine                           = b == at ? units : mine;
+    }
+    return mine;
+}
+
+// The item that holds unit u0 of the call.  COUNT holds all units: 32 bits if they do (small trees 12.2 us with 64 bits throughout,
+// 11.9 with 32; capped trees of 64 tokens 73.8 and 72.7).
+template<typename COUNT>
+__device__ __forceinline__ void attn_find(const AttentionParams& p, const AttnShared& sh, COUNT u0, AttnStart& start)
+{
+    const int   B = p.batch.sequences, lane = threadIdx.x & 31, item_rows = 2 * p.tile_rows;
+    const COUNT heads = p.batch.kv_heads;
+    // The sequence that holds it: the first whose running sum passes it.
+    COUNT before = 0;
+    int   b      = 0;
 #pragma unroll 1
-        for (int base = 0; base < B; base += 32) {
-            const unsigned mine = base + lane < B ? sh.units[base + lane] * heads : 0;
-            unsigned       upto = mine;
-#pragma unroll
-            for (int d = 1; d < 32; d <<= 1) {
-                const unsigned other = __shfl_up_sync(0xffffffffu, upto, d);
-                if (lane >= d)
-                    upto += other;
-            }
-            const unsigned past = __ballot_sync(0xffffffffu, before + upto > u0);
-            if (past) {
-                const int l = __ffs(past) - 1;
-                b           = base + l;
+    for (int base = 0; base < B; base += 32) {
+        COUNT mine;
+        if constexpr (sizeof(COUNT) == 4)
+            mine = base + lane < B ? sh.units[base + lane] * heads : 0;
+        else
+            mine = attn_units_of(p, sh, base) * heads;
+        const COUNT    upto = attn_warp_scan(mine);
+        const unsigned past = __ballot_sync(0xffffffffu, before + upto > u0);
+        if (past) {
+            const int l = __ffs(past) - 1;
+            b           = base + l;
+            before += __shfl_sync(0xffffffffu, upto - mine, l);
+            break;
+        }
+        before += __shfl_sync(0xffffffffu, upto, 31);
+    }
+    const AttnSequence a    = attn_sequence(p, sh, b);
+    int                row0 = 0;
+    unsigned           item = 1;
+    if (a.rows <= item_rows)
+        item = attn_units(p, a, 0);
+    else {
+#pragma unroll 1
+        for (long long base = 0;; base += 32 * item_rows) {  // ... and of its items the first
+            const long long r    = base + lane * item_rows;
+            const unsigned  size = r < a.rows ? attn_units(p, a, static_cast<int>(r)) : 0;
+            const COUNT     mine = size * heads, upto = attn_warp_scan(mine);
+            const unsigned  past = __ballot_sync(0xffffffffu, before + upto > u0);
+            if (past || base + 32 * item_rows >= a.rows) {
+                const int l = past ? __ffs(past) - 1 : 0;
+                row0        = static_cast<int>(base) + l * item_rows;
+                item        = max(1u, __shfl_sync(0xffffffffu, size, l));
                 before += __shfl_sync(0xffffffffu, upto - mine, l);
                 break;
             }
             before += __shfl_sync(0xffffffffu, upto, 31);
         }
-        const AttnSequence a    = attn_sequence(p, sh, b);
-        int                row0 = 0;
-        unsigned           item = 1;
-        if (a.rows <= item_rows)
-            item = attn_units(p, a, 0);
-        else {
-#pragma unroll 1
-            for (long long base = 0;; base += 32 * item_rows) {  // ... and of its items the first
-                const long long r    = base + lane * item_rows;
-                const unsigned  size = r < a.rows ? attn_units(p, a, static_cast<int>(r)) : 0;
-                unsigned        upto = size * heads;
-#pragma unroll
-                for (int d = 1; d < 32; d <<= 1) {
-                    const unsigned other = __shfl_up_sync(0xffffffffu, upto, d);
-                    if (lane >= d)
-                        upto += other;
-                }
-                const unsigned past = __ballot_sync(0xffffffffu, before + upto > u0);
-                if (past || base + 32 * item_rows >= a.rows) {
-                    const int l = past ? __ffs(past) - 1 : 0;
-                    row0        = static_cast<int>(base) + l * item_rows;
-                    item        = max(1u, __shfl_sync(0xffffffffu, size, l));
-                    before += __shfl_sync(0xffffffffu, upto - size * heads, l);
-                    break;
-                }
-                before += __shfl_sync(0xffffffffu, upto, 31);
-            }
-        }
-        start.sequence = b;
-        start.row0     = row0;
-        start.head     = static_cast<int>((u0 - before) / item);
-        start.unit     = static_cast<int>((u0 - before) % item);
     }
+    start.sequence = b;
+    start.row0     = row0;
+    start.head     = static_cast<int>((u0 - before) / item);
+    start.unit     = static_cast<int>((u0 - before) % item);
+}
+
+// ... where 32 bits do not hold them: code of its own, out of the way of the usual calls'.
+__device__ __noinline__ AttnStart attn_start_many(const AttentionParams& p, const AttnShared& sh)
+{
+    AttnStart          start{0, 0, 0, 0, 0, 0};
+    unsigned long long total = 0;
+#pragma unroll 1
+    for (int base = 0; base < p.batch.sequences; base += 32)
+        total += attn_units_of(p, sh, base) * p.batch.kv_heads;
+    const unsigned long long units = attn_warp_sum(total), share = (units + gridDim.x - 1) / gridDim.x;
+    const unsigned long long u0 = min(units, share * blockIdx.x), u1 = min(units, u0 + share);
+    if (u1 > u0)
+        attn_find<unsigned long long>(p, sh, u0, start);
     start.units = u1 - u0;
-    start.share = static_cast<int>(share);
+    start.least = attn_least(share);
+    return start;
+}
+
+__device__ __forceinline__ AttnStart attn_start(const AttentionParams& p, const AttnShared& sh)
+{
+    const int          lane = threadIdx.x & 31;
+    AttnStart          start{0, 0, 0, 0, 0, 0};
+    unsigned long long total = 0;
+#pragma unroll 1
+    for (int b = lane; b < p.batch.sequences; b += 32)  // kAttnManyUnits among them makes many, too
+        total += static_cast<unsigned long long>(sh.units[b]) * p.batch.kv_heads;
+    const unsigned long long units = attn_warp_sum(total);
+    if (units >= kAttnManyUnits)
+        return attn_start_many(p, sh);
+    const unsigned share = max(static_cast<unsigned>((units + gridDim.x - 1) / gridDim.x), 2u);  // a tile for each group
+    const unsigned u0    = static_cast<unsigned>(min(units, static_cast<unsigned long long>(share) * blockIdx.x));
+    const unsigned u1    = static_cast<unsigned>(min(units, static_cast<unsigned long long>(u0) + share));
+    if (u1 > u0)
+        attn_find<unsigned>(p, sh, u0, start);
+    start.units = u1 - u0;
+    start.least = attn_least(share);
     return start;
 }
 
@@ -402,17 +486,17 @@ __device__ __forceinline__ AttnStart attn_start(const AttentionParams& p, const 
 struct AttnCursor {
     AttnSequence a;
     AttnSegment  seg;
-    unsigned     left;
+    unsigned long long left;
     int          next_unit;  // of the item
     int          extra;      // units of the item beyond its tiles
-    int          share;      // units of a CTA
+    int          least;      // tiles that are not cut off
 
     bool         new_sequence, new_rows;  // what `seg` does not describe yet
 
     __device__ __forceinline__ explicit AttnCursor(const AttnStart& start)
     {
         left         = start.units;
-        share        = start.share;
+        least        = start.least;
         seg.b        = start.sequence;
         seg.row0     = start.row0;
         seg.head     = start.head;
@@ -473,9 +557,9 @@ struct AttnCursor {
             seg.begin = seg.end = 0;
             if (left == 0)
                 return;
-            const int upto  = static_cast<int>(min(static_cast<unsigned>(seg.tiles + extra), next_unit + left));
-            seg.begin       = attn_cut(next_unit, seg.tiles, extra, share);
-            seg.end         = attn_cut(upto, seg.tiles, extra, share);
+            const int upto  = static_cast<int>(min(static_cast<unsigned long long>(seg.tiles + extra), next_unit + left));
+            seg.begin       = attn_cut(next_unit, seg.tiles, extra, least);
+            seg.end         = attn_cut(upto, seg.tiles, extra, least);
             left -= upto - next_unit;
             next_unit = upto;
         } while (seg.end == seg.begin);
@@ -827,7 +911,8 @@ __device__ __forceinline__ void attn_softmax(AttnState& st, const AttnRow& row, 
 template<int HEAD_DIM, bool PLAIN>
 __global__ void __launch_bounds__(kAttnThreads, 1)
 attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_q_few,
-                 const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const AttentionParams p)
+                 const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
+                 const __grid_constant__ AttentionParams p)
 {
     constexpr int      kStages    = attn_stages(HEAD_DIM);
     constexpr int      kTileBytes = attn_tile_bytes(HEAD_DIM);
