@@ -620,6 +620,12 @@ __device__ __forceinline__ bool half_not_finite(uint32_t h)
     return (h & 0x7c00u) == 0x7c00u;
 }
 
+// Not zero if one of two halves is not finite.
+__device__ __forceinline__ uint32_t halves_not_finite(uint32_t u)
+{
+    return ((u & 0x7fff7fffu) + 0x04000400u) & 0x80008000u;
+}
+
 // Adds to o[c], element column + c of a row's output, the values that are not finite of keys that the row sees (the products
 // took zeros in their place: a weight of zero times infinity is not zero).
 template<int HEAD_DIM, int COLUMNS>
@@ -642,6 +648,69 @@ __device__ __forceinline__ void attn_add_not_finite(const AttentionParams& p, co
                 if (half_not_finite(__half_as_ushort(v[c])))
                     o[c] += __half2float(v[c]);
         }
+}
+
+// The same for keys of tiles that all rows of the segment see, which the products take as they are: infinity times a weight of zero,
+// another copy's key or one too small for fp16, has made NaN of the sums there.  Bits of columns `column` on that have a positive
+// infinity or NaN among these keys, and a negative infinity or NaN; for a whole warp.
+template<int HEAD_DIM, int COLUMNS>
+__device__ __forceinline__ uint2 attn_seen_not_finite(const AttentionParams& p, const AttnSegment& seg, int column)
+{
+    uint2     found = make_uint2(0u, 0u);
+    const int end   = min(seg.end, seg.open[0] / kAttnKeys) * kAttnKeys;
+#pragma unroll 4
+    for (int key = seg.begin * kAttnKeys + (threadIdx.x & 31); key < end; key += 32) {
+        const long long at = cache_row(p.batch, seg.b, key, seg.head);
+        if (at < 0)
+            continue;
+        const half* v   = p.v_cache + at * HEAD_DIM + column;
+        uint32_t    any = 0u;
+#pragma unroll
+        for (int c = 0; c < COLUMNS; c += 4) {
+            const uint2 w = *reinterpret_cast<const uint2*>(v + c);
+            any |= halves_not_finite(w.x) | halves_not_finite(w.y);
+        }
+        if (any)
+#pragma unroll 1
+            for (int c = 0; c < COLUMNS; ++c) {
+                const uint32_t h = __half_as_ushort(v[c]);
+                if (!half_not_finite(h))
+                    continue;
+                const bool nan = (h & 0x3ffu) != 0u;
+                found.x |= nan || h < 0x8000u ? 1u << c : 0u;
+                found.y |= nan || h >= 0x8000u ? 1u << c : 0u;
+            }
+    }
+    return make_uint2(__reduce_or_sync(0xffffffffu, found.x), __reduce_or_sync(0xffffffffu, found.y));
+}
+
+template<int COLUMNS>
+struct AttnSums {
+    float o[COLUMNS];
+};
+
+// A row's sums of columns `column` on, put right where values are not finite; for a whole warp.  A row whose weights have no finite
+// sum stays without a number.  Code of its own, out of the way of the usual items' (in their midst it cost ragged prompts 2 us of 55).
+template<int HEAD_DIM, int COLUMNS>
+__device__ __noinline__ AttnSums<COLUMNS> attn_restore(const AttentionParams& p, const AttnSegment& seg, const AttnRow row,
+                                                       const uint32_t (&list)[3][4], bool listed, float sum, int column,
+                                                       AttnSums<COLUMNS> sums)
+{
+    bool nan = false;
+#pragma unroll
+    for (int c = 0; c < COLUMNS; ++c)
+        nan = nan || sums.o[c] != sums.o[c];
+    if (__any_sync(0xffffffffu, nan && sum == sum)) {
+        const uint2 found = attn_seen_not_finite<HEAD_DIM, COLUMNS>(p, seg, column);
+#pragma unroll
+        for (int c = 0; c < COLUMNS; ++c) {
+            const float plus = found.x >> c & 1u ? CUDART_INF_F : 0.0f, minus = found.y >> c & 1u ? -CUDART_INF_F : 0.0f;
+            sums.o[c]        = sums.o[c] == sums.o[c] ? sums.o[c] : plus + minus;
+        }
+    }
+    if (listed)
+        attn_add_not_finite<HEAD_DIM, COLUMNS>(p, seg, row, list, column, sums.o);
+    return sums;
 }
 
 // tanh x on [-0.75, 0.75] to 2e-7: x times a polynomial in x^2, fitted to it for the smallest largest error.  A call has the
@@ -1140,8 +1209,17 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
                         const float4 v = four[32 * copy];
                         sum4[0] += v.x, sum4[1] += v.y, sum4[2] += v.z, sum4[3] += v.w;
                     }
-                    if (any)
-                        attn_add_not_finite<HEAD_DIM, 4>(p, seg, row, list, column, sum4);
+                    const float probe = (sum4[0] + sum4[1] + (sum4[2] + sum4[3])) * 0.0f;  // NaN if one of them is not finite
+                    if (any || __any_sync(0xffffffffu, valid && probe != probe)) {
+                        AttnSums<4> sums4;
+#pragma unroll
+                        for (int k = 0; k < 4; ++k)
+                            sums4.o[k] = sum4[k];
+                        sums4 = attn_restore<HEAD_DIM, 4>(p, seg, row, list, any, st.sum, column, sums4);
+#pragma unroll
+                        for (int k = 0; k < 4; ++k)
+                            sum4[k] = sums4.o[k];
+                    }
                     if (valid && ok && whole) {
                         const half2 x = __floats2half2_rn(sum4[0] * inverse, sum4[1] * inverse),
                                     y = __floats2half2_rn(sum4[2] * inverse, sum4[3] * inverse);
@@ -1153,13 +1231,15 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
                     ptx::named_barrier_sync(2 + group, 128);
                 }
             }
-            else if (ok && busy && pair && whole && !any) {
+            bool simple = pair && whole && !any;
+            if (ok && busy && simple) {
                 // 32 rows x 32 columns at a time through 2 KB of the warp's own, so that neighbouring lanes store neighbours
                 uint4* const    staged = reinterpret_cast<uint4*>(sh.staged[group]) + (warp & 3) * 128;
                 const long long mine   = valid ? to : -1;
                 const int       r      = lane / 4;
                 const long long at[4]  = {__shfl_sync(0xffffffffu, mine, r), __shfl_sync(0xffffffffu, mine, r + 8),
                                           __shfl_sync(0xffffffffu, mine, r + 16), __shfl_sync(0xffffffffu, mine, r + 24)};
+                half2           largest = __float2half2_rn(0.0f);
 #pragma unroll 1
                 for (int c = 0; c < HEAD_DIM; c += 32) {
                     uint32_t x[32];
@@ -1176,6 +1256,7 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
                             const half2 h = __floats2half2_rn(__uint_as_float(x[8 * k + 2 * e]) * inverse,
                                                               __uint_as_float(x[8 * k + 2 * e + 1]) * inverse);
                             w[e]          = *reinterpret_cast<const uint32_t*>(&h);
+                            largest       = __hmax2_nan(largest, __habs2(h));
                         }
                         staged[lane * 4 + (k ^ (lane >> 1 & 3))] = make_uint4(w[0], w[1], w[2], w[3]);
                     }
@@ -1190,8 +1271,9 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
                             *reinterpret_cast<uint4*>(p.out + at[k] + c + lane % 4 * 8) = v[k];
                     __syncwarp();
                 }
+                simple = !__any_sync(0xffffffffu, valid && halves_not_finite(*reinterpret_cast<const uint32_t*>(&largest)) != 0u);
             }
-            else if (ok && busy) {
+            if (ok && busy && !fourfold && !simple) {
                 // 32 rows x 16 columns at a time through 1 KB of the warp's own, so that neighbouring lanes store neighbours
                 uint4* const    staged = reinterpret_cast<uint4*>(sh.staged[group]) + (warp & 3) * 64;
                 const long long mine   = valid ? to : -1;
@@ -1199,8 +1281,20 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
                 for (int c = column0; c < column1; c += 16) {
                     float o[16];
                     outputs(c, o);
-                    if (any)
-                        attn_add_not_finite<HEAD_DIM, 16>(p, seg, row, list, c, o);
+                    float probe = 0.0f;  // NaN if one of them is not finite
+#pragma unroll
+                    for (int k = 0; k < 16; ++k)
+                        probe = fmaf(o[k], 0.0f, probe);
+                    if (any || __any_sync(0xffffffffu, valid && probe != probe)) {
+                        AttnSums<16> sums16;
+#pragma unroll
+                        for (int k = 0; k < 16; ++k)
+                            sums16.o[k] = o[k];
+                        sums16 = attn_restore<HEAD_DIM, 16>(p, seg, row, list, any, st.sum, c, sums16);
+#pragma unroll
+                        for (int k = 0; k < 16; ++k)
+                            o[k] = sums16.o[k];
+                    }
                     if (whole) {
 #pragma unroll
                         for (int k = 0; k < 16; k += 8) {
@@ -1436,10 +1530,9 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
                         for (int x = 0; x < HEAD_DIM / 8; ++x) {
                             uint4& at = v[(x / 8) * (kBlock / 16) + ((x + r) & 7)];  // any order of chunks: banks
                             uint4  w  = key < seg.keys ? at : make_uint4(0, 0, 0, 0);
-                            auto   spoilt = [](uint32_t u) { return ((u & 0x7fff7fffu) + 0x04000400u) & 0x80008000u; };
                             if (key >= seg.keys)
                                 at = w;
-                            else if (spoilt(w.x) | spoilt(w.y) | spoilt(w.z) | spoilt(w.w)) {
+                            else if (halves_not_finite(w.x) | halves_not_finite(w.y) | halves_not_finite(w.z) | halves_not_finite(w.w)) {
                                 bad        = true;
                                 auto clean = [&](uint32_t u) {
                                     return (half_not_finite(u) ? 0u : u & 0xffffu) | (half_not_finite(u >> 16) ? 0u : u & 0xffff0000u);
@@ -1510,7 +1603,8 @@ __global__ void __launch_bounds__(256) attention_join_kernel(const AttentionPara
         o[k] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
     for (int c = begin; c <= cta; ++c) {
         const float2 stat = stats[slot(c) * kAttnSlotRows + place];
-        const float  keep = stat.x == top ? 1.0f : ptx::exp2_approx(stat.x - top);
+        // Never zero: a part's infinity stays one.
+        const float  keep = stat.x == top ? 1.0f : fmaxf(ptx::exp2_approx(stat.x - top), 0x1p-126f);
         sum += stat.y * keep;
         const float4* src = sums + ((slot(c) * 2 + place / kAttnRows) * (HEAD_DIM / 4) + warp * kPer) * kAttnRows + place % kAttnRows;
 #pragma unroll

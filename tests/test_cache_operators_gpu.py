@@ -225,6 +225,45 @@ def test_values_that_are_not_finite_reach_those_who_see_them(ops, tree):
     near(got[~spoilt], want.view(60, 4, 128)[~spoilt], bound.view(60, 4, 128)[~spoilt])
 
 
+IN_CONTEXTS = [
+    # contexts, counts, heads, kv_heads, dim, tree
+    ([300], [1], 1, 1, 64, False),             # one row, laid four times in its tile
+    ([300, 129], [1, 1], 8, 2, 128, False),
+    ([9000], [1], 8, 2, 128, False),           # cut into parts
+    ([9000, 200], [3, 2], 16, 2, 64, True),
+    ([260], [20], 4, 2, 128, True),            # a tile of rows
+    ([6000, 300], [64, 40], 2, 1, 64, True),
+    ([200], [300], 2, 2, 128, False),          # pairs of tiles
+    ([3000, 0], [700, 200], 6, 2, 64, False),
+]
+
+
+@pytest.mark.parametrize("contexts,counts,heads,kv_heads,dim,tree", IN_CONTEXTS)
+def test_infinite_values_of_a_context_reach_all_rows(ops, contexts, counts, heads, kv_heads, dim, tree):
+    """A weight is never zero by its definition: infinity times it is infinity, for keys that weigh next to nothing too."""
+    b = Batch(contexts, counts, heads, kv_heads, dim, 32, seed=9, gain=1.5)
+    page, at = b.pages_of(0, torch.tensor([5, 37, 70, 101, 102], device="cuda"))
+    b.k_cache[page[1], :, at[1]] *= 30.0  # takes some rows' whole weight, and next to none of others'
+    inf, column = float("inf"), torch.arange(dim, device="cuda")
+    spoilt = [(0, 7, inf), (1, 11, -inf), (1, 40, inf), (2, 50, float("nan")), (3, 13, inf), (4, 13, -inf), (4, 14, inf)]
+    want_there = torch.zeros(dim, device="cuda")
+    for key, c, value in spoilt:
+        b.v_cache[page[key], 0, at[key], c] = value
+        want_there[c] += value
+    masks, _ = random_tree(counts, contexts, 10) if tree else (None, None)
+    got = ops.tree_attention(b.q, *b.arrays, masks) if tree else ops.prompt_attention(b.q, *b.arrays)
+    for key, c, value in spoilt:
+        b.v_cache[page[key], 0, at[key], c] = 0.0
+    want, bound = attention(b, masks)
+    share = heads // kv_heads
+    mine = got[:counts[0]].view(counts[0], heads, dim)[:, :share]  # of the first sequence, and the heads that read the spoilt one
+    there = want_there != 0
+    assert torch.equal(mine[..., there].float().nan_to_num(nan=7.0), want_there[there].nan_to_num(nan=7.0).expand(counts[0], share, -1))
+    clean = torch.ones((b.rows, heads, dim), dtype=torch.bool, device="cuda")
+    clean[:counts[0], :share, there] = False
+    near(got.view(b.rows, heads, dim)[clean], want.view(b.rows, heads, dim)[clean], bound.view(b.rows, heads, dim)[clean])
+
+
 def test_large_scores(ops):
     """Scores far apart, rising along the cache, so that the running maximum moves at every tile; and scores of -60000 s."""
     b = Batch([700], [3], 4, 1, 64, 32, seed=9)
