@@ -626,6 +626,15 @@ __device__ __forceinline__ uint32_t halves_not_finite(uint32_t u)
     return ((u & 0x7fff7fffu) + 0x04000400u) & 0x80008000u;
 }
 
+// Two outputs as fp16.  Weights of 11 bits and their sum of 24 can take an average past the largest value that fp16 holds, which then
+// is the average: only infinities become one.
+__device__ __forceinline__ uint32_t attn_pack_bounded(float x, float y)
+{
+    auto bounded = [](float v) { return fabsf(v) < 131072.0f ? fminf(fmaxf(v, -65504.0f), 65504.0f) : v; };
+    const half2 h = __floats2half2_rn(bounded(x), bounded(y));
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+
 // Adds to o[c], element column + c of a row's output, the values that are not finite of keys that the row sees (the products
 // took zeros in their place: a weight of zero times infinity is not zero).
 template<int HEAD_DIM, int COLUMNS>
@@ -1221,10 +1230,9 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
                             sum4[k] = sums4.o[k];
                     }
                     if (valid && ok && whole) {
-                        const half2 x = __floats2half2_rn(sum4[0] * inverse, sum4[1] * inverse),
-                                    y = __floats2half2_rn(sum4[2] * inverse, sum4[3] * inverse);
                         *reinterpret_cast<uint2*>(p.out + to + column) =
-                            make_uint2(*reinterpret_cast<const uint32_t*>(&x), *reinterpret_cast<const uint32_t*>(&y));
+                            make_uint2(attn_pack_bounded(sum4[0] * inverse, sum4[1] * inverse),
+                                       attn_pack_bounded(sum4[2] * inverse, sum4[3] * inverse));
                     }
                     else if (valid && ok)
                         sums[column / 4 * kAttnRows + lane] = make_float4(sum4[0], sum4[1], sum4[2], sum4[3]);
@@ -1300,10 +1308,8 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
                         for (int k = 0; k < 16; k += 8) {
                             uint32_t w[4];
 #pragma unroll
-                            for (int e = 0; e < 4; ++e) {  // a row that sees no key: what its sums hold are zeros
-                                const half2 h = __floats2half2_rn(o[k + 2 * e] * inverse, o[k + 2 * e + 1] * inverse);
-                                w[e]          = *reinterpret_cast<const uint32_t*>(&h);
-                            }
+                            for (int e = 0; e < 4; ++e)  // a row that sees no key: what its sums hold are zeros
+                                w[e] = attn_pack_bounded(o[k + 2 * e] * inverse, o[k + 2 * e + 1] * inverse);
                             staged[lane * 2 + (k / 8 ^ (lane >> 2 & 1))] = make_uint4(w[0], w[1], w[2], w[3]);
                         }
                         __syncwarp();
@@ -1624,8 +1630,8 @@ __global__ void __launch_bounds__(256) attention_join_kernel(const AttentionPara
                 + warp * kPer * 4;
 #pragma unroll
     for (int k = 0; k < kPer; ++k) {
-        const half2 a = __floats2half2_rn(o[k].x * inverse, o[k].y * inverse), b = __floats2half2_rn(o[k].z * inverse, o[k].w * inverse);
-        *reinterpret_cast<uint2*>(out + 4 * k) = make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b));
+        *reinterpret_cast<uint2*>(out + 4 * k) = make_uint2(attn_pack_bounded(o[k].x * inverse, o[k].y * inverse),
+                                                            attn_pack_bounded(o[k].z * inverse, o[k].w * inverse));
     }
 }
 

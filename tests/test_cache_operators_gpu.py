@@ -264,6 +264,23 @@ def test_infinite_values_of_a_context_reach_all_rows(ops, contexts, counts, head
     near(got.view(b.rows, heads, dim)[clean], want.view(b.rows, heads, dim)[clean], bound.view(b.rows, heads, dim)[clean])
 
 
+@pytest.mark.parametrize("contexts,counts,heads,dim", [([11], [1], 1, 64), ([11], [1], 4, 128), ([11], [40], 2, 64), ([3000], [2], 1, 128),
+                                                       ([11], [300], 1, 128)])
+@pytest.mark.parametrize("value", [65504.0, -65504.0])
+def test_averages_of_the_largest_value_are_that_value(ops, contexts, counts, heads, dim, value):
+    """Weights of 0.50026 all round up, by 4.6e-4 of themselves: their products' sum, divided by that of the unrounded ones, passes
+    65520, from where on fp16 rounds to infinity."""
+    b = Batch(contexts, counts, heads, 1, dim, 16, seed=9)
+    b.q.zero_(), b.k_cache.nan_to_num_(nan=0.0).zero_()
+    b.q.view(b.rows, heads, dim)[:, :, 0] = 1.0
+    b.k_cache[..., 0] = -1.0
+    page, at = b.pages_of(0, torch.tensor([0], device="cuda"))
+    b.k_cache[page, :, at, 0] = 0.0
+    b.v_cache.nan_to_num_(nan=0.0).fill_(value)
+    got = ops.prompt_attention(b.q, *b.arrays, scale=-math.log(0.5 + 1.05 * 2.0 ** -12))
+    assert bool((got == value).all())
+
+
 def test_large_scores(ops):
     """Scores far apart, rising along the cache, so that the running maximum moves at every tile; and scores of -60000 s."""
     b = Batch([700], [3], 4, 1, 64, 32, seed=9)
