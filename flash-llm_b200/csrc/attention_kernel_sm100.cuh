@@ -889,6 +889,17 @@ __device__ __forceinline__ void attn_load_scores(uint32_t s_tmem, float (&s)[COL
         asm volatile("" : "+r"(raw[c]));  // not read before the wait
 }
 
+// Weights are 2^7 times what they are against the maximum: fp16 holds the largest, 2^15 where the maximum lags by 2^8, and those down
+// to 2^-21 of it in full, down to 2^-32 at all.  Without the factor, which the sum has too, a long flat tail is lost: 40000 keys of 2^-26
+// each are 6e-4 of the sum.
+constexpr float kAttnWeightExponent = 7.0f;
+
+// What is added to a score times `factor` to make the exponent of its weight.
+__device__ __forceinline__ float attn_minus(const AttnState& st)
+{
+    return st.top == -CUDART_INF_F ? 0.0f : fmaf(-st.top, st.factor, kAttnWeightExponent);
+}
+
 // One tile of scores of one row, from tensor memory to weights there: all 128 of them, or, where the row lies in the tile four
 // times, the 32 from `column` on and zeros for the others.  The tile's first key is `key0`; keys before `open` are seen by all
 // rows.  `part_done(half)` tells that the weights of that half of the tile are in place.
@@ -911,7 +922,7 @@ __device__ __forceinline__ void attn_softmax(AttnState& st, const AttnRow& row, 
         if (masked)
             attn_mask(row, s, key0 + column);
         attn_new_top(st, attn_largest(s, st.top), first, rescale);
-        const float    minus     = st.top == -CUDART_INF_F ? 0.0f : -st.top * st.factor;
+        const float    minus     = attn_minus(st);
         const uint32_t zeros[16] = {0};
         uint32_t       w[16];
 #pragma unroll
@@ -935,7 +946,7 @@ __device__ __forceinline__ void attn_softmax(AttnState& st, const AttnRow& row, 
             new_top = attn_largest(s, new_top);
         }
         attn_new_top(st, new_top, first, rescale);
-        const float minus = st.top == -CUDART_INF_F ? 0.0f : -st.top * st.factor;
+        const float minus = attn_minus(st);
 #pragma unroll 1
         for (int c = 0; c < kAttnKeys; c += 64) {  // weights take the place of scores already read
             float    s[64];
@@ -968,7 +979,7 @@ __device__ __forceinline__ void attn_softmax(AttnState& st, const AttnRow& row, 
         }
         ptx::tmem_wait_st();
         attn_new_top(st, new_top, first, rescale);
-        const float minus = st.top == -CUDART_INF_F ? 0.0f : -st.top * st.factor;
+        const float minus = attn_minus(st);
 #pragma unroll 2
         for (int c = 0; c < kAttnKeys; c += 32) {  // weights take the place of scores already read
             float    s[32];

@@ -281,6 +281,26 @@ def test_averages_of_the_largest_value_are_that_value(ops, contexts, counts, hea
     assert bool((got == value).all())
 
 
+@pytest.mark.parametrize("count,heads,dim,cap", [(1, 1, 64, 0.0), (40, 2, 128, 0.0), (300, 1, 64, 0.0), (150, 1, 128, 300.0)])
+def test_long_flat_tails_are_not_lost(ops, count, heads, dim, cap):
+    """One key that weighs 2^25.5 times each of 40000 others, whose values alone are not zero; 300 sequences over the same pages, so
+    that most rows are one CTA's.  A weight is off by 2^-11 of itself, or by 2^-32 of the largest (half of fp16's least step, 2^-24,
+    where the largest is 2^7), the output by 2^-11 besides."""
+    one, many = Batch([40000], [count], heads, 1, dim, 64, seed=9), 300
+    one.q.zero_(), one.k_cache.nan_to_num_(nan=0.0).zero_()
+    one.q.view(count, heads, dim)[:, :, 0] = 1.0
+    one.k_cache[..., 0] = -17.671875
+    one.v_cache.nan_to_num_(nan=0.0).fill_(1.0)
+    page, at = one.pages_of(0, torch.tensor([0], device="cuda"))
+    one.k_cache[page, :, at, 0], one.v_cache[page, :, at] = 0.0, 0.0
+    got = ops.prompt_attention(one.q.repeat(many, 1), one.k_cache, one.v_cache,
+                               torch.arange(0, (many + 1) * count, count, dtype=torch.int32, device="cuda"),
+                               one.context.repeat(many), one.page_table.repeat(many, 1), scale=1.0, cap=cap)
+    want, _ = attention(one, scale=1.0, cap=cap)
+    bound = 2.0 ** -10 * want + 2.0 ** -32 * (40000 + count) + 2.0 ** -25
+    near(got, want.repeat(many, 1), bound.repeat(many, 1))
+
+
 def test_large_scores(ops):
     """Scores far apart, rising along the cache, so that the running maximum moves at every tile; and scores of -60000 s."""
     b = Batch([700], [3], 4, 1, 64, 32, seed=9)
