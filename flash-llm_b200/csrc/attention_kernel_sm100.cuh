@@ -81,9 +81,14 @@ constexpr int kAttnSegments  = 8;  // segments that shared memory holds at a tim
 // next piece and the ends of an item (32 outputs of its row and of the other group's) take besides.
 constexpr int kAttnSoftmaxRegisters = 208, kAttnOtherRegisters = 88;
 
-// Looks at a barrier before a CTA gives up: some tenths of a second at least.  (Counted and not timed: the waits stand in many
-// places, and code that the instruction cache need not hold is time: ragged prompts 57 us with a clock in each, 55 without.)
-constexpr uint32_t kAttnWaitLimit = 1u << 24;
+// Looks at a barrier before a CTA gives up: 0.35 seconds, 21 ns for each look at a barrier that does not change.  (Counted and not
+// timed: the waits stand in many places, and code that the instruction cache need not hold is time: ragged prompts 60 us with a
+// clock in each, 55 without.)  A CTA that gave up leaves rows as they were, those of items that others share with it too; all
+// other rows are right.
+#ifndef FLASHLLM_ATTENTION_LOOKS  // the tests have a build that gives up early, elsewhere in each CTA
+#define FLASHLLM_ATTENTION_LOOKS (1u << 24)
+#define FLASHLLM_ATTENTION_LOOKS_AT_ONCE 1024u
+#endif
 
 // Tiles of keys (and as many of values) in shared memory at a time.
 __host__ __device__ constexpr int attn_stages(int head_dim)
@@ -186,8 +191,8 @@ __device__ __forceinline__ bool attn_wait_longer(uint32_t bar, uint32_t parity, 
     for (uint32_t it = 1;; ++it) {
         if (ptx::mbar_try_wait(bar, parity))
             return true;
-        if ((it & 1023u) == 0u) {
-            if (it >= kAttnWaitLimit) {
+        if (it % FLASHLLM_ATTENTION_LOOKS_AT_ONCE == 0u) {
+            if (it >= FLASHLLM_ATTENTION_LOOKS) {
                 *abort_flag = 1u;
                 atomicOr(status, kStatusWaitExpired);
             }
@@ -1151,7 +1156,7 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
                 }
             }
             if (tiles > 0) {
-                ok = ok && attn_wait(&sh.o_done[group], o_parity, sh, status);
+                ok = __all_sync(0xffffffffu, ok && attn_wait(&sh.o_done[group], o_parity, sh, status));
                 o_parity ^= 1u;
             }
             ptx::tc_fence_after_sync();
@@ -1183,7 +1188,6 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
                 column0    = group * (HEAD_DIM / 2);
                 column1    = column0 + HEAD_DIM / 2;
             }
-            ok = ok && sh.abort_flag == 0u;
             const bool      whole = seg.begin == 0 && seg.end == seg.tiles;
             const unsigned  kind  = whole ? kPartNone : seg.begin == 0 ? kPartBegins : seg.end == seg.tiles ? kPartEnds : kPartContinues;
             const int       slot  = kind == kPartBegins ? 1 : 0;
@@ -1347,8 +1351,9 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
                     make_float2(st.top * st.factor, st.sum);
             if (kind != kPartNone) {
                 written[slot] = true;
+                const bool all = !ptx::named_barrier_any(1, 256, !ok);  // a part is there for all rows or for none
                 if (threadIdx.x == 0)
-                    parts[slot] = AttnPart{ok ? kind : kPartNone, seg.first, seg.row0, seg.rows, seg.head, {0, 0, 0}};
+                    parts[slot] = AttnPart{all ? kind : kPartNone, seg.first, seg.row0, seg.rows, seg.head, {0, 0, 0}};
             }
             // The barrier before the next segment: both groups are done with both outputs and with the joined sums' room.
             ptx::tc_fence_before_sync();
@@ -1534,8 +1539,8 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
             }
             for (int t = seg.begin; t < seg.end; ++t, ++n) {
                 const uint32_t stage = n % kStages;
-                ok                   = attn_wait(&sh.v_full[stage], n / kStages & 1u, sh, status);
-                if (!ok)
+                ok                   = ok && attn_wait(&sh.v_full[stage], n / kStages & 1u, sh, status);
+                if (!ok)  // nor without the rows of Q: those of the next segment would be taken for them
                     break;
                 if ((t + 1) * kAttnKeys > open) {
 #pragma unroll 1
