@@ -143,6 +143,11 @@ class CachedAttention:
     slopes: torch.Tensor | None = None
 
     def __call__(self, y_qkv: torch.Tensor) -> torch.Tensor:
+        if self.tree_mask is not None and self.frequencies is not None and self.positions is None:
+            # Turned by its row, a drafted token would go into the cache with the angle of another depth.
+            raise ValueError("a drafted tree with rotary positions needs the positions of its tokens")
+        if self.tree_mask is not None and self.prefix is not None:
+            raise ValueError("a prefix is for prompts: a tree's masks say what its tokens see")
         from . import torch_op  # noqa: F401  (registers torch.ops.flashllm)
         ops = torch.ops.flashllm
         batch = (self.k_cache, self.v_cache, self.cu_tokens, self.context, self.page_table)

@@ -139,6 +139,20 @@ def test_the_oracle_gives_what_a_softmax_of_few_keys_gives():
     assert torch.allclose(y[0, 0, :16], torch.tensor([-2.0, 2.0], dtype=torch.float64).repeat(8)) and bool((y[0, 0, 16:] == 1).all())
 
 
+def test_cached_attention_refuses_trees_without_positions_or_with_a_prefix():
+    from flash_llm_b200.tp_chain import CachedAttention
+    k = torch.zeros((4, 2, 16, 64), dtype=torch.float16)
+    ints = torch.tensor([0, 3], dtype=torch.int32), torch.zeros(1, dtype=torch.int32), torch.zeros((1, 2), dtype=torch.int32)
+    rows, masks = torch.zeros((3, 6 * 64), dtype=torch.float16), torch.ones(3, dtype=torch.int64)
+    with pytest.raises(ValueError, match="positions"):
+        CachedAttention(k, k.clone(), *ints, tree_mask=masks, frequencies=torch.ones(32, dtype=torch.float64))(rows)
+    with pytest.raises(ValueError, match="prefix"):
+        CachedAttention(k, k.clone(), *ints, tree_mask=masks, prefix=torch.zeros(1, dtype=torch.int32))(rows)
+    for more in (dict(frequencies=torch.ones(32, dtype=torch.float64), positions=torch.zeros(3, dtype=torch.int32)), {}):
+        with pytest.raises(RuntimeError, match="no CPU implementation"):  # not refused here
+            CachedAttention(k, k.clone(), *ints, tree_mask=masks, **more)(rows)
+
+
 def test_chain_with_an_attention_of_its_own():
     """Two ranks' chains, each with the attention of its heads (a causal one over the batch's rows), add up to the whole layer."""
     shape, dim = ChainShape(hidden=256, ffn=512, tokens=8, world=2), 64
