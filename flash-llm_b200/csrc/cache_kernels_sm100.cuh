@@ -127,7 +127,9 @@ __global__ void __launch_bounds__(kRotaryThreads) rotary_append_kernel(const Rot
         }
         int a, z;
         offsets(u, a, z);
-        if (turned_at(u)) {
+        if (position < 0)  // queries of a sequence that does not fit
+            va = vz = make_uint4(0, 0, 0, 0);
+        else if (turned_at(u)) {
             float x[8], y[8], co[8], si[8];
             unpack_half8(va, x);
             unpack_half8(vz, y);

@@ -315,8 +315,8 @@ int FlashLLM_SplitK_Reduction(void* stream, void* C, const void* Reduction_Works
  *
  * Results are cudaError_t values; bad sizes or pointers return cudaErrorInvalidValue.  What the host cannot see sets bit 64 of
  * the status word (FlashLLM_ConsumeStatus): a page id outside the cache (its keys and values read as zeros, writes to it are
- * left out), or a sequence that does not fit into its row of the page table (its attention output is zero, it is not written
- * to the cache).  No two sequences may share a page that a call writes to.
+ * left out), or a sequence that does not fit into its row of the page table (its turned queries and its attention output are
+ * zero, it is not written to the cache).  No two sequences may share a page that a call writes to.
  * ---------------------------------------------------------------------------------------------------------- */
 
 /* Rotary positions and the append.  QKV [tokens][ld_qkv] holds the query heads, the key heads and the value heads of each row

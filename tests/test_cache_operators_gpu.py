@@ -394,6 +394,21 @@ def test_a_sequence_that_does_not_fit_is_not_appended(ops, lib):
     assert lib.consume_status() == 0
 
 
+@pytest.mark.parametrize("turned,placed", [(False, False), (True, False), (True, True)])
+def test_queries_of_a_sequence_that_does_not_fit_are_zero(ops, lib, turned, placed):
+    b = Batch([30, 40, 20], [2, 3, 1], 2, 1, 64, 16, seed=14, extra_rows=1)
+    qkv = torch.randn((7, 4 * 64), device="cuda").to(torch.float16)
+    f = torch.from_numpy(lib.rotary_frequencies(64)[0]).cuda() if turned else None
+    positions = torch.arange(7, dtype=torch.int32, device="cuda") if placed else None
+    want = ops.rotary_append(qkv, *b.arrays, f, False, 1.0, positions)
+    for context in (-1, 16 * b.page_table.shape[1] - 2, 1 << 30):
+        lengths = b.context.clone()
+        lengths[1] = context
+        got = ops.rotary_append(qkv, b.k_cache, b.v_cache, b.cu_tokens, lengths, b.page_table, f, False, 1.0, positions)
+        assert lib.consume_status() == BAD_CACHE
+        assert bool((got[2:5] == 0).all()) and torch.equal(got[:2], want[:2]) and torch.equal(got[5], want[5])
+
+
 @pytest.mark.parametrize("page", [16, 128])
 def test_caches_longer_than_32_bits(ops, page):
     """Pages behind the 2^31st element of a cache, for every operator."""
