@@ -170,8 +170,8 @@ static cudaError_t attend(cudaStream_t stream, AttentionParams p, const void* Q,
                         kv_heads, head_dim)
         || heads < 1 || heads % kv_heads != 0 || heads / kv_heads > kAttnRows || static_cast<long long>(heads) * head_dim > (1 << 24) || !rows_fit(Q, ld_q, heads, head_dim)
         || workspace == nullptr || !aligned16(workspace) || Out == nullptr || !aligned16(Out) || !(scale > 0.0f) || !std::isfinite(scale) || !(cap >= 0.0f) || !std::isfinite(cap)
-        // What the kernels make of them is finite too.
-        || !std::isfinite(scale * 1.45f) || !std::isfinite(cap * 1.45f) || (cap > 0.0f && !std::isfinite(scale / cap * 3.0f))
+        // What the kernels make of them is finite too, scores times log2 e of 128 products of the largest fp16 values among it.
+        || !std::isfinite(scale * 8e11f) || !std::isfinite(cap * 1.45f) || (cap > 0.0f && !std::isfinite(scale / cap * 3.0f))
         || static_cast<long long>(tokens) * heads > 0x7fffffffll - 256)
         return cudaErrorInvalidValue;
     if (tokens == 0 || sequences == 0)

@@ -745,6 +745,7 @@ struct AttnState {
     int   place;         // the row's position
     const int* drafted;  // positions of drafted tokens in shared memory, or nullptr
     bool  valid;         // the row is somebody's
+    bool  far;           // a row of the warp has a maximum beyond kAttnFarExponent
 };
 
 // The largest of a row's scores, NaN if one of them is.
@@ -842,23 +843,34 @@ __device__ __forceinline__ void attn_mask(const AttnRow& row, float (&s)[COLUMNS
     }
 }
 
+// Where the maximum times `factor` is this large, its rounding takes a power of two and more off the weights, in the end all they have:
+// then scores are taken against the maximum before they are multiplied.  One operation per pair of scores more; the code stands by
+// itself.
+constexpr float kAttnFarExponent = 8388608.0f;
+
 // The maximum that weights are taken against, from the largest score of a tile.  `rescale(keep)` multiplies the row's output by
 // `keep`, and is called by whole warps.
-template<typename Rescale>
+template<bool PLAIN, typename Rescale>
 __device__ __forceinline__ void attn_new_top(AttnState& st, float new_top, bool first, Rescale&& rescale)
 {
+    auto far = [&]() {
+        return PLAIN && __any_sync(0xffffffffu, st.valid && st.top != -CUDART_INF_F && fabsf(st.top) * st.factor > kAttnFarExponent);
+    };
     if (!(new_top < CUDART_INF_F)) {  // a score that is no number, or infinity less itself: neither has the row's output a number
         st.sum  = CUDART_NAN_F;
         new_top = st.top;
     }
-    if (first)
+    if (first) {
         st.top = new_top;
+        st.far = far();
+    }
     else if (__any_sync(0xffffffffu, st.valid && (new_top - st.top) * st.factor > 8.0f)) {  // rows of nobody have no say
         // It moves only when it has grown by more than 2^8, which 32-bit sums and fp16 weights have room for: rarely after the
         // first tiles.
         const float keep = new_top == st.top ? 1.0f : ptx::exp2_approx((st.top - new_top) * st.factor);
         st.top           = new_top;
         st.sum *= keep;
+        st.far = far();
         rescale(keep);
     }
 }
@@ -899,10 +911,35 @@ __device__ __forceinline__ void attn_load_scores(uint32_t s_tmem, float (&s)[COL
 // each are 6e-4 of the sum.
 constexpr float kAttnWeightExponent = 7.0f;
 
-// What is added to a score times `factor` to make the exponent of its weight.
+// What is added to a score times `factor` to make the exponent of its weight; rounded down, so that no weight passes 2^15.
 __device__ __forceinline__ float attn_minus(const AttnState& st)
 {
-    return st.top == -CUDART_INF_F ? 0.0f : fmaf(-st.top, st.factor, kAttnWeightExponent);
+    return st.top == -CUDART_INF_F ? 0.0f : __fmaf_rd(-st.top, st.factor, kAttnWeightExponent);
+}
+
+// Plain scores of one row in tensor memory, 128 of them, to weights there; their sum.  For a whole warp.
+__device__ __noinline__ float attn_far_weights(uint32_t s_tmem, float top, float factor)
+{
+    const float minus = top == -CUDART_INF_F ? 0.0f : -top;
+    float2      part  = make_float2(0.0f, 0.0f);
+#pragma unroll 1
+    for (int c = 0; c < kAttnKeys; c += 32) {  // weights take the place of scores already read
+        float    s[32];
+        uint32_t w[16];
+        attn_load_scores(s_tmem + c, s);
+#pragma unroll
+        for (int k = 0; k < 16; ++k) {
+            float2 x = ptx::add_x2(make_float2(s[2 * k], s[2 * k + 1]), make_float2(minus, minus));
+            x        = ptx::fma_x2(x, make_float2(factor, factor), make_float2(kAttnWeightExponent, kAttnWeightExponent));
+            x        = make_float2(ptx::exp2_approx(x.x), ptx::exp2_approx(x.y));
+            part     = ptx::add_x2(part, x);
+
+            const half2 h = __floats2half2_rn(x.x, x.y);
+            w[k]          = *reinterpret_cast<const uint32_t*>(&h);
+        }
+        ptx::tmem_st_x16(s_tmem + c / 2, w);
+    }
+    return part.x + part.y;
 }
 
 // One tile of scores of one row, from tensor memory to weights there: all 128 of them, or, where the row lies in the tile four
@@ -926,8 +963,17 @@ __device__ __forceinline__ void attn_softmax(AttnState& st, const AttnRow& row, 
             attn_transform(st, s, key0 + column, open, masked && st.drafted != nullptr);
         if (masked)
             attn_mask(row, s, key0 + column);
-        attn_new_top(st, attn_largest(s, st.top), first, rescale);
-        const float    minus     = attn_minus(st);
+        attn_new_top<PLAIN>(st, attn_largest(s, st.top), first, rescale);
+        if constexpr (PLAIN) {  // (as attn_far_weights, always)
+            const float top = st.top == -CUDART_INF_F ? 0.0f : st.top;
+#pragma unroll
+            for (int c = 0; c < 32; c += 2) {
+                const float2 x = ptx::add_x2(make_float2(s[c], s[c + 1]), make_float2(-top, -top));
+                s[c]           = x.x;
+                s[c + 1]       = x.y;
+            }
+        }
+        const float    minus     = PLAIN ? kAttnWeightExponent : attn_minus(st);
         const uint32_t zeros[16] = {0};
         uint32_t       w[16];
 #pragma unroll
@@ -950,7 +996,14 @@ __device__ __forceinline__ void attn_softmax(AttnState& st, const AttnRow& row, 
             attn_load_scores(s_tmem + c, s);
             new_top = attn_largest(s, new_top);
         }
-        attn_new_top(st, new_top, first, rescale);
+        attn_new_top<PLAIN>(st, new_top, first, rescale);
+        if (PLAIN && st.far) {
+            st.sum += attn_far_weights(s_tmem, st.top, st.factor);
+            stored();
+            part_done(0);
+            part_done(1);
+            return;
+        }
         const float minus = attn_minus(st);
 #pragma unroll 1
         for (int c = 0; c < kAttnKeys; c += 64) {  // weights take the place of scores already read
@@ -983,7 +1036,14 @@ __device__ __forceinline__ void attn_softmax(AttnState& st, const AttnRow& row, 
             ptx::tmem_st_x32(s_tmem + c, reinterpret_cast<const uint32_t*>(s));
         }
         ptx::tmem_wait_st();
-        attn_new_top(st, new_top, first, rescale);
+        attn_new_top<PLAIN>(st, new_top, first, rescale);
+        if (PLAIN && st.far) {
+            st.sum += attn_far_weights(s_tmem, st.top, st.factor);
+            stored();
+            part_done(0);
+            part_done(1);
+            return;
+        }
         const float minus = attn_minus(st);
 #pragma unroll 2
         for (int c = 0; c < kAttnKeys; c += 32) {  // weights take the place of scores already read

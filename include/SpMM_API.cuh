@@ -357,7 +357,7 @@ int FlashLLM_RotaryAppend(void*         stream,
  * A row sees the context of its sequence and those of its sequence's first 64 new tokens whose bit tree_mask[n] has (its
  * ancestors and itself, usually).
  * `positions` (int32 [tokens]) are needed with slopes only: the distance is between them, for keys of the context to their
- * place.  Q is [tokens][ld_q], Out [tokens][heads * head_dim], which must overlap none of the inputs; scale > 0, and scale / cap
+ * place.  Q is [tokens][ld_q], Out [tokens][heads * head_dim], which must overlap none of the inputs; 0 < scale <= 4e26, and scale / cap
  * must stay finite.  `workspace`: FlashLLM_Attention_WorkspaceBytes on a
  * 16-byte boundary, its contents before and after the call of no use to anybody; calls that may overlap on the GPU need one
  * each. */

@@ -67,6 +67,13 @@ def test_bad_arguments_of_each_operator_are_refused(lib):
         _refused(lib, lambda: lib.cache_accept(0, **{**accept, **change}))
 
 
+def test_scales_whose_largest_scores_are_not_finite_are_refused(lib):
+    attend = dict(Q=P, ld_q=512, batch=_batch(), heads=4, Out=P, workspace=P)
+    for change in (dict(scale=1e27), dict(scale=1e27, cap=1e20)):
+        _refused(lib, lambda: lib.prompt_attention(0, **{**attend, **change}))
+        _refused(lib, lambda: lib.tree_attention(0, tree_mask=P, **{**attend, **change}))
+
+
 def test_empty_batches_are_accepted_without_a_device(lib):
     for change in (dict(tokens=0), dict(sequences=0)):
         b = _batch(**change)

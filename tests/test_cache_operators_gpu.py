@@ -301,6 +301,34 @@ def test_long_flat_tails_are_not_lost(ops, count, heads, dim, cap):
     near(got, want.repeat(many, 1), bound.repeat(many, 1))
 
 
+@pytest.mark.parametrize("contexts,counts,heads,kv_heads,dim,tree,scale,cap", [
+    ([300], [1], 1, 1, 64, False, 1.0, 0.0), ([9000, 70], [1, 1], 8, 2, 128, False, 0.1, 0.0), ([700], [40], 2, 1, 64, True, 1.0, 0.0),
+    ([2000], [64], 8, 2, 128, True, 1e16, 0.0), ([0], [700], 2, 1, 64, False, 1.0, 0.0), ([1000], [900], 1, 1, 128, False, 1e-2, 0.0),
+    ([300], [1], 1, 1, 64, False, 1.0, 1e8), ([700], [40], 2, 1, 64, True, 1e16, 1e12), ([0], [700], 2, 1, 64, False, 1e26, 1e30)])
+def test_scores_beyond_what_their_exponents_hold(ops, contexts, counts, heads, kv_heads, dim, tree, scale, cap):
+    """Scores of 1e7 to 1e30, which 32 bits hold to 1 to 1e23: rounded on its own, the largest one's multiple of log2 e must not decide
+    about its weight.  Each row points at one key, next to which all others, 1e7 below at least, weigh nothing."""
+    b = Batch(contexts, counts, heads, kv_heads, dim, 32, seed=9)
+    g = torch.Generator().manual_seed(10)
+    rows, some = counts[0], 16
+    place = torch.linspace(0, max(contexts[0] - 1, some - 1), some).long()  # of the keys that are pointed at
+    page, at = b.pages_of(0, torch.arange(contexts[0] + rows, device="cuda"))
+    b.k_cache[page, :, at] = 0.0
+    for i, j in enumerate(place.tolist()):
+        b.k_cache[page[j], :, at[j], i] = 30000.0 + 1900.0 * i
+    aim = torch.randint(0, some, (rows, heads), generator=g)
+    if contexts[0] == 0:
+        aim = torch.minimum(aim, torch.arange(rows)[:, None])  # none behind the row
+    q = torch.zeros((rows, heads, dim)).scatter_(2, aim[..., None], torch.randint(40000, 60000, (rows, heads, 1), generator=g).float())
+    b.q[:rows] = q.view(rows, -1).to(torch.float16).cuda()
+    masks, _ = random_tree(counts, contexts, 11) if tree else (None, None)
+    got = (ops.tree_attention(b.q, *b.arrays, masks, scale=scale, cap=cap) if tree
+           else ops.prompt_attention(b.q, *b.arrays, scale=scale, cap=cap))
+    values = b.rows_of(b.v_cache, 0)[place.cuda()]  # [some][kv_heads][dim]
+    want = values[aim.cuda(), torch.arange(heads, device="cuda") // (heads // kv_heads)]
+    assert torch.equal(got[:rows].view(rows, heads, dim).double(), want)
+
+
 def test_large_scores(ops):
     """Scores far apart, rising along the cache, so that the running maximum moves at every tile; and scores of -60000 s."""
     b = Batch([700], [3], 4, 1, 64, 32, seed=9)
