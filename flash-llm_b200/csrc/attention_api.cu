@@ -211,6 +211,8 @@ int FlashLLM_RotaryAppend(void* stream, const void* QKV, int ld_qkv, void* Q, in
         return static_cast<int>(cudaErrorInvalidValue);
     if (tokens == 0 || sequences == 0)
         return 0;
+    if (Q == QKV && ld_q != ld_qkv)  // a row's queries would go where another CTA still reads
+        return static_cast<int>(cudaErrorInvalidValue);
     if (const int err = device_status_pointer(&p.batch.status))
         return err;
     p.qkv         = static_cast<const half*>(QKV);

@@ -67,6 +67,11 @@ def test_bad_arguments_of_each_operator_are_refused(lib):
         _refused(lib, lambda: lib.cache_accept(0, **{**accept, **change}))
 
 
+def test_appends_in_place_with_other_row_lengths_are_refused(lib):
+    for ld_qkv, ld_q in ((1024, 512), (1024, 1032)):
+        _refused(lib, lambda: lib.rotary_append(0, P, ld_qkv, P, ld_q, _batch(), 4, P, 128))
+
+
 def test_scales_whose_largest_scores_are_not_finite_are_refused(lib):
     attend = dict(Q=P, ld_q=512, batch=_batch(), heads=4, Out=P, workspace=P)
     for change in (dict(scale=1e27), dict(scale=1e27, cap=1e20)):
