@@ -245,7 +245,8 @@ at::Tensor attention(const char* what, const at::Tensor& q, const Paged& p, cons
                 " heads of ", p.head_dim, ", but has ", q.size(1), " columns");
     const double factor = scale.has_value() ? *scale : 1.0 / std::sqrt(static_cast<double>(p.head_dim));
     TORCH_CHECK(factor > 0 && std::isfinite(static_cast<float>(factor)) && static_cast<float>(factor) > 0, "scale must be positive and finite");
-    TORCH_CHECK(cap >= 0 && std::isfinite(static_cast<float>(cap)), "cap must be positive and finite, or 0 for none");
+    TORCH_CHECK(cap >= 0 && std::isfinite(static_cast<float>(cap)) && (cap == 0 || static_cast<float>(cap) > 0),
+                "cap must be positive and finite in 32 bits, or 0 for none");
     const float* slope = nullptr;
     if (slopes.has_value() && slopes->defined()) {
         TORCH_CHECK(slopes->scalar_type() == at::kFloat && slopes->dim() == 1 && slopes->size(0) == heads && slopes->is_contiguous()

@@ -530,6 +530,14 @@ def test_refusals_of_the_operators(ops, lib):
     assert ops.prompt_attention(empty, *b.arrays).shape == (0, 256)
 
 
+def test_a_cap_that_32_bits_take_for_none_is_refused(ops):
+    b = Batch([20], [3], 4, 2, 64, 16, seed=16)
+    for call in (lambda: ops.prompt_attention(b.q, *b.arrays, cap=1e-50),
+                 lambda: ops.tree_attention(b.q, *b.arrays, torch.ones(3, dtype=torch.int64, device="cuda"), cap=1e-50)):
+        with pytest.raises(RuntimeError, match="cap"):
+            call()
+
+
 def test_captured_calls_follow_the_arrays(ops):
     """One graph of append and attention, replayed with other lengths, pages and masks; and two graphs at once."""
     contexts, counts = [60, 200, 1500], [16, 16, 16]
