@@ -286,9 +286,12 @@ int FlashLLM_CacheAccept(void* stream, void* K_cache, void* V_cache, int layers,
     p.layer_elems      = static_cast<long long>(pages) * kv_heads * page_size * head_dim;
     p.layers           = layers;
     // Some four CTAs for each multiprocessor, of a sequence's heads and layers at most as many as there are.
+    int sms = 0;
+    if (const cudaError_t err = multiprocessors(&sms))
+        return static_cast<int>(err);
     const long long heads = static_cast<long long>(kv_heads) * layers;
-    const dim3      grid(sequences, static_cast<unsigned>(std::min(heads, (4 * 148ll + sequences - 1) / sequences)));
-    auto       launch = [&](auto kernel) {
+    const dim3      grid(sequences, static_cast<unsigned>(std::min(heads, (4ll * sms + sequences - 1) / sequences)));
+    auto            launch = [&](auto kernel) {
         return launch_in_stream_order(kernel, grid, dim3(kAcceptThreads), 0, static_cast<cudaStream_t>(stream), 1, p);
     };
     return static_cast<int>(head_dim == 64 ? launch(cache_accept_kernel<64>) : launch(cache_accept_kernel<128>));
