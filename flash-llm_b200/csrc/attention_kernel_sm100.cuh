@@ -1357,8 +1357,9 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
                 simple = !__any_sync(0xffffffffu, valid && halves_not_finite(*reinterpret_cast<const uint32_t*>(&largest)) != 0u);
             }
             if (ok && busy && !fourfold && !simple) {
-                // 32 rows x 16 columns at a time through 1 KB of the warp's own, so that neighbouring lanes store neighbours
-                uint4* const    staged = reinterpret_cast<uint4*>(sh.staged[group]) + (warp & 3) * 64;
+                // 32 rows x 16 columns at a time through 1 KB of the warp's own 2 (another warp may still be in the loop above), so that
+                // neighbouring lanes store neighbours
+                uint4* const    staged = reinterpret_cast<uint4*>(sh.staged[group]) + (warp & 3) * 128;
                 const long long mine   = valid ? to : -1;
 #pragma unroll 1
                 for (int c = column0; c < column1; c += 16) {

@@ -264,6 +264,24 @@ def test_infinite_values_of_a_context_reach_all_rows(ops, contexts, counts, head
     near(got.view(b.rows, heads, dim)[clean], want.view(b.rows, heads, dim)[clean], bound.view(b.rows, heads, dim)[clean])
 
 
+@pytest.mark.parametrize("heads,kv_heads,dim,count", [(66, 2, 128, 260), (128, 1, 128, 250), (64, 1, 64, 400), (8, 8, 128, 900)])
+def test_infinite_values_in_whole_items(ops, heads, kv_heads, dim, count):
+    """Items that no other CTA shares, whose warps write their outputs by the plain way and find out about infinities at different
+    times: ten calls, every element."""
+    b = Batch([140], [count], heads, kv_heads, dim, 64, seed=9, gain=1.5)
+    page, at = b.pages_of(0, torch.tensor([5, 100], device="cuda"))
+    for key, c, value in ((0, 1, float("inf")), (0, 90 % dim, -float("inf")), (1, 50, float("nan"))):
+        b.v_cache[page[key], :, at[key], c] = value
+    got = [ops.prompt_attention(b.q, *b.arrays).view(count, heads, dim) for _ in range(10)]
+    b.v_cache[page, :, at, 1] = b.v_cache[page, :, at, 90 % dim] = b.v_cache[page, :, at, 50] = 0.0
+    want, bound = attention(b)
+    there = torch.ones(dim, dtype=torch.bool, device="cuda")
+    there[[1, 90 % dim, 50]] = False
+    for x in got:
+        assert bool((x[..., 1] == float("inf")).all()) and bool((x[..., 90 % dim] == -float("inf")).all()) and bool(x[..., 50].isnan().all())
+        near(x[..., there], want.view(count, heads, dim)[..., there], bound.view(count, heads, dim)[..., there])
+
+
 @pytest.mark.parametrize("contexts,counts,heads,dim", [([11], [1], 1, 64), ([11], [1], 4, 128), ([11], [40], 2, 64), ([3000], [2], 1, 128),
                                                        ([11], [300], 1, 128)])
 @pytest.mark.parametrize("value", [65504.0, -65504.0])
