@@ -704,11 +704,11 @@ struct AttnSums {
 };
 
 // A row's sums of columns `column` on, put right where values are not finite; for a whole warp.  A row whose weights have no finite
-// sum stays without a number.  Code of its own, out of the way of the usual items' (in their midst it cost ragged prompts 2 us of 55).
+// sum stays without a number.
 template<int HEAD_DIM, int COLUMNS>
-__device__ __noinline__ AttnSums<COLUMNS> attn_restore(const AttentionParams& p, const AttnSegment& seg, const AttnRow row,
-                                                       const uint32_t (&list)[3][4], bool listed, float sum, int column,
-                                                       AttnSums<COLUMNS> sums)
+__device__ __forceinline__ AttnSums<COLUMNS> attn_restore(const AttentionParams& p, const AttnSegment& seg, const AttnRow& row,
+                                                          const uint32_t (&list)[3][4], bool listed, float sum, int column,
+                                                          AttnSums<COLUMNS> sums)
 {
     bool nan = false;
 #pragma unroll
@@ -725,6 +725,67 @@ __device__ __noinline__ AttnSums<COLUMNS> attn_restore(const AttentionParams& p,
     if (listed)
         attn_add_not_finite<HEAD_DIM, COLUMNS>(p, seg, row, list, column, sums.o);
     return sums;
+}
+
+// What the end of a segment adds up to a lane's row: its group's output and, where the groups share the rows, the other's.
+struct AttnOutputs {
+    uint32_t mine_tmem, other_tmem;  // of this warp's lanes
+    float    mine_keep, other_keep;
+    bool     mine, other;  // there at all
+
+    // 16 columns from `c` on.
+    __device__ __forceinline__ void load(int c, bool shared, float (&o)[16]) const
+    {
+        uint32_t x[16], y[16];
+        ptx::tmem_ld_x16(mine_tmem + c, x);
+        if (shared)
+            ptx::tmem_ld_x16(other_tmem + c, y);
+        ptx::tmem_wait_ld();
+#pragma unroll
+        for (int k = 0; k < 16; ++k) {
+            asm volatile("" : "+r"(x[k]), "+r"(y[k]));
+            o[k] = mine ? __uint_as_float(x[k]) * mine_keep : 0.0f;
+            o[k] = other ? fmaf(__uint_as_float(y[k]), other_keep, o[k]) : o[k];
+        }
+    }
+};
+
+// The end of a segment for a warp with an output that is not finite, or may not be: its rows (`out` of a whole item's, or `sums` of a
+// part's; neither for a lane without a row) are written anew.  Code of its own, out of the way of the usual ends: in their midst it
+// cost ragged prompts 2 us of 55.
+template<int HEAD_DIM>
+__device__ __noinline__ void attn_end_carefully(const AttentionParams& p, const AttnSegment& seg, const AttnRow row,
+                                                const uint32_t (&list)[3][4], bool listed, AttnOutputs outputs, float sum, int column0,
+                                                int column1, half* out, float4* sums)
+{
+    const float inverse = sum == 0.0f ? 0.0f : 1.0f / sum;
+#pragma unroll 1
+    for (int c = column0; c < column1; c += 16) {
+        AttnSums<16> s;
+        outputs.load(c, !seg.pair, s.o);
+        s = attn_restore<HEAD_DIM, 16>(p, seg, row, list, listed, sum, c, s);
+#pragma unroll
+        for (int k = 0; k < 16; k += 8) {
+            if (out)
+                *reinterpret_cast<uint4*>(out + c + k) =
+                    make_uint4(attn_pack_bounded(s.o[k] * inverse, s.o[k + 1] * inverse),
+                               attn_pack_bounded(s.o[k + 2] * inverse, s.o[k + 3] * inverse),
+                               attn_pack_bounded(s.o[k + 4] * inverse, s.o[k + 5] * inverse),
+                               attn_pack_bounded(s.o[k + 6] * inverse, s.o[k + 7] * inverse));
+            else if (sums) {
+                sums[(c + k) / 4 * kAttnRows]     = make_float4(s.o[k], s.o[k + 1], s.o[k + 2], s.o[k + 3]);
+                sums[(c + k + 4) / 4 * kAttnRows] = make_float4(s.o[k + 4], s.o[k + 5], s.o[k + 6], s.o[k + 7]);
+            }
+        }
+    }
+}
+
+// ... of 4 columns of rows that lie in the tile four times, added up already.
+template<int HEAD_DIM>
+__device__ __noinline__ AttnSums<4> attn_restore_four(const AttentionParams& p, const AttnSegment& seg, const AttnRow row,
+                                                      const uint32_t (&list)[3][4], bool listed, float sum, int column, AttnSums<4> sums)
+{
+    return attn_restore<HEAD_DIM, 4>(p, seg, row, list, listed, sum, column, sums);
 }
 
 // tanh x on [-0.75, 0.75] to 2e-7: x times a polynomial in x^2, fitted to it for the smallest largest error.  A call has the
@@ -1260,27 +1321,14 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
             const bool  any             = sh.any_not_finite[number % kAttnSegments] != 0;
             // An accumulator that no product has written may hold anything: this group's without a tile of its own, where the groups
             // share the rows the second group's with a single tile.
-            const bool mine_there = pair ? tiles > 0 : group == 0 || join, other_there = !pair && (group == 1 || join);
-            // 16 columns of this lane's row, both groups' where they share it
-            auto outputs = [&](int c, float(&o)[16]) {
-                uint32_t x[16], y[16];
-                ptx::tmem_ld_x16(o_tmem + c, x);
-                if (!pair)
-                    ptx::tmem_ld_x16(tmem + kO + (group ^ 1) * 128 + lanes + c, y);
-                ptx::tmem_wait_ld();
-#pragma unroll
-                for (int k = 0; k < 16; ++k) {
-                    asm volatile("" : "+r"(x[k]), "+r"(y[k]));
-                    o[k] = mine_there ? __uint_as_float(x[k]) * keep : 0.0f;
-                    o[k] = other_there ? fmaf(__uint_as_float(y[k]), keep_other, o[k]) : o[k];
-                }
-            };
+            const AttnOutputs outputs{o_tmem, tmem + kO + (group ^ 1) * 128 + lanes, keep, keep_other,
+                                      pair ? tiles > 0 : group == 0 || join, !pair && (group == 1 || join)};
             if (fourfold) {
                 float4* const staged = sh.staged[group];  // [4 x 4 columns][lane]
 #pragma unroll 1
                 for (int c = column0; c < column1; c += 16) {
                     float o[16];
-                    outputs(c, o);
+                    outputs.load(c, true, o);
 #pragma unroll
                     for (int k = 0; k < 16; k += 4)
                         staged[k / 4 * kAttnRows + thread] = make_float4(o[k], o[k + 1], o[k + 2], o[k + 3]);
@@ -1299,7 +1347,7 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
 #pragma unroll
                         for (int k = 0; k < 4; ++k)
                             sums4.o[k] = sum4[k];
-                        sums4 = attn_restore<HEAD_DIM, 4>(p, seg, row, list, any, st.sum, column, sums4);
+                        sums4 = attn_restore_four<HEAD_DIM>(p, seg, row, list, any, st.sum, column, sums4);
 #pragma unroll
                         for (int k = 0; k < 4; ++k)
                             sum4[k] = sums4.o[k];
@@ -1314,8 +1362,11 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
                     ptx::named_barrier_sync(2 + group, 128);
                 }
             }
-            bool simple = pair && whole && !any;
-            if (ok && busy && simple) {
+            // Of the others 32 rows are written at a time, and written again if one of them is not finite.
+            bool again = any;
+            if (fourfold || !ok || !busy)
+                again = false;
+            else if (!any && pair && whole) {
                 // 32 rows x 32 columns at a time through 2 KB of the warp's own, so that neighbouring lanes store neighbours
                 uint4* const    staged = reinterpret_cast<uint4*>(sh.staged[group]) + (warp & 3) * 128;
                 const long long mine   = valid ? to : -1;
@@ -1354,38 +1405,28 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
                             *reinterpret_cast<uint4*>(p.out + at[k] + c + lane % 4 * 8) = v[k];
                     __syncwarp();
                 }
-                simple = !__any_sync(0xffffffffu, valid && halves_not_finite(*reinterpret_cast<const uint32_t*>(&largest)) != 0u);
+                again = __any_sync(0xffffffffu, valid && halves_not_finite(*reinterpret_cast<const uint32_t*>(&largest)) != 0u);
             }
-            if (ok && busy && !fourfold && !simple) {
-                // 32 rows x 16 columns at a time through 1 KB of the warp's own 2 (another warp may still be in the loop above), so that
-                // neighbouring lanes store neighbours
+            else if (!any) {
+                // 32 rows x 16 columns at a time through 1 KB of the warp's own, so that neighbouring lanes store neighbours
                 uint4* const    staged = reinterpret_cast<uint4*>(sh.staged[group]) + (warp & 3) * 128;
                 const long long mine   = valid ? to : -1;
+                float           probe  = 0.0f;  // NaN if one of the row's sums is not finite
+                half2           largest = __float2half2_rn(0.0f);
 #pragma unroll 1
                 for (int c = column0; c < column1; c += 16) {
                     float o[16];
-                    outputs(c, o);
-                    float probe = 0.0f;  // NaN if one of them is not finite
-#pragma unroll
-                    for (int k = 0; k < 16; ++k)
-                        probe = fmaf(o[k], 0.0f, probe);
-                    if (any || __any_sync(0xffffffffu, valid && probe != probe)) {
-                        AttnSums<16> sums16;
-#pragma unroll
-                        for (int k = 0; k < 16; ++k)
-                            sums16.o[k] = o[k];
-                        sums16 = attn_restore<HEAD_DIM, 16>(p, seg, row, list, any, st.sum, c, sums16);
-#pragma unroll
-                        for (int k = 0; k < 16; ++k)
-                            o[k] = sums16.o[k];
-                    }
+                    outputs.load(c, !pair, o);
                     if (whole) {
 #pragma unroll
                         for (int k = 0; k < 16; k += 8) {
                             uint32_t w[4];
 #pragma unroll
-                            for (int e = 0; e < 4; ++e)  // a row that sees no key: what its sums hold are zeros
-                                w[e] = attn_pack_bounded(o[k + 2 * e] * inverse, o[k + 2 * e + 1] * inverse);
+                            for (int e = 0; e < 4; ++e) {  // a row that sees no key: what its sums hold are zeros
+                                const half2 h = __floats2half2_rn(o[k + 2 * e] * inverse, o[k + 2 * e + 1] * inverse);
+                                w[e]          = *reinterpret_cast<const uint32_t*>(&h);
+                                largest       = __hmax2_nan(largest, __habs2(h));
+                            }
                             staged[lane * 2 + (k / 8 ^ (lane >> 2 & 1))] = make_uint4(w[0], w[1], w[2], w[3]);
                         }
                         __syncwarp();
@@ -1402,10 +1443,17 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
 #pragma unroll
                         for (int k = 0; k < 16; k += 4)
                             sums[(c + k) / 4 * kAttnRows + thread] = make_float4(o[k], o[k + 1], o[k + 2], o[k + 3]);
+#pragma unroll
+                        for (int k = 0; k < 16; ++k)
+                            probe = fmaf(o[k], 0.0f, probe);
                     }
                     __syncwarp();
                 }
+                again = __any_sync(0xffffffffu, valid && (probe != probe || halves_not_finite(*reinterpret_cast<const uint32_t*>(&largest)) != 0u));
             }
+            if (again)
+                attn_end_carefully<HEAD_DIM>(p, seg, row, list, any, outputs, st.sum, column0, column1, valid && whole ? p.out + to : nullptr,
+                                             valid && !whole ? sums + thread : nullptr);
             if (ok && !whole && valid && column0 == 0 && (!fourfold || thread < 32))
                 reinterpret_cast<float2*>(p.workspace + attn_stats_offset(gridDim.x))[static_cast<size_t>(2 * blockIdx.x + slot) * kAttnSlotRows
                                                                                       + tile_row * kAttnRows + thread] =
