@@ -1047,15 +1047,34 @@ __device__ __forceinline__ void attn_softmax(AttnState& st, const AttnRow& row, 
         part_done(0);
         part_done(1);
     }
-    else if (PLAIN && !masked) {
-        // 64 columns at a time: half the waits for loads of the other way, which has more to do per column (prompt of 7000 tokens
-        // 444 us instead of 461, ragged prompts 55.0 instead of 55.7; all 128 in registers 467 and 60.9).
+    else {
         float new_top = st.top;
+        if (PLAIN && !masked) {
+            // 64 columns at a time: half the waits for loads of the other way, which has more to do per column (prompt of 7000 tokens
+            // 444 us instead of 461, ragged prompts 55.0 instead of 55.7; all 128 in registers 467 and 60.9).
 #pragma unroll 1
-        for (int c = 0; c < kAttnKeys; c += 64) {
-            float s[64];
-            attn_load_scores(s_tmem + c, s);
-            new_top = attn_largest(s, new_top);
+            for (int c = 0; c < kAttnKeys; c += 64) {
+                float s[64];
+                attn_load_scores(s_tmem + c, s);
+                new_top = attn_largest(s, new_top);
+            }
+        }
+        else {
+            // 32 columns at a time, masked or transformed scores back to tensor memory in between: with all 128 in registers the code of
+            // one tile does not fit the instruction cache (capped trees of 64 tokens took 90 us instead of 77, ragged prompts 71
+            // instead of 60).
+#pragma unroll 1
+            for (int c = 0; c < kAttnKeys; c += 32) {
+                float s[32];
+                attn_load_scores(s_tmem + c, s);
+                if constexpr (!PLAIN)
+                    attn_transform(st, s, key0 + c, open, masked && st.drafted != nullptr);
+                if (masked)
+                    attn_mask(row, s, key0 + c);
+                new_top = attn_largest(s, new_top);
+                ptx::tmem_st_x32(s_tmem + c, reinterpret_cast<const uint32_t*>(s));
+            }
+            ptx::tmem_wait_st();
         }
         attn_new_top<PLAIN>(st, new_top, first, rescale);
         if (PLAIN && st.far) {
@@ -1065,55 +1084,20 @@ __device__ __forceinline__ void attn_softmax(AttnState& st, const AttnRow& row, 
             part_done(1);
             return;
         }
-        const float minus = attn_minus(st);
-#pragma unroll 1
-        for (int c = 0; c < kAttnKeys; c += 64) {  // weights take the place of scores already read
-            float    s[64];
-            uint32_t w[16];
+        // Weights take the place of scores already read.
+        const float   minus    = attn_minus(st);
+        constexpr int kColumns = PLAIN ? 64 : 32;
+#pragma unroll (PLAIN ? 1 : 2)
+        for (int c = 0; c < kAttnKeys; c += kColumns) {
+            float s[kColumns];
             attn_load_scores(s_tmem + c, s);
 #pragma unroll
-            for (int k = 0; k < 64; k += 32) {
+            for (int k = 0; k < kColumns; k += 32) {
+                uint32_t w[16];
                 attn_weights<PLAIN>(s + k, st.factor, minus, part, w);
                 ptx::tmem_st_x16(s_tmem + (c + k) / 2, w);
             }
-            stored();
-            part_done(c / 64);
-        }
-    }
-    else {
-        // 32 columns at a time, masked or transformed scores back to tensor memory in between: with all 128 in registers the code of
-        // one tile does not fit the instruction cache (capped trees of 64 tokens took 90 us instead of 77, ragged prompts 71
-        // instead of 60).
-        float new_top = st.top;
-#pragma unroll 1
-        for (int c = 0; c < kAttnKeys; c += 32) {
-            float s[32];
-            attn_load_scores(s_tmem + c, s);
-            if constexpr (!PLAIN)
-                attn_transform(st, s, key0 + c, open, masked && st.drafted != nullptr);
-            if (masked)
-                attn_mask(row, s, key0 + c);
-            new_top = attn_largest(s, new_top);
-            ptx::tmem_st_x32(s_tmem + c, reinterpret_cast<const uint32_t*>(s));
-        }
-        ptx::tmem_wait_st();
-        attn_new_top<PLAIN>(st, new_top, first, rescale);
-        if (PLAIN && st.far) {
-            st.sum += attn_far_weights(s_tmem, st.top, st.factor);
-            stored();
-            part_done(0);
-            part_done(1);
-            return;
-        }
-        const float minus = attn_minus(st);
-#pragma unroll 2
-        for (int c = 0; c < kAttnKeys; c += 32) {  // weights take the place of scores already read
-            float    s[32];
-            uint32_t w[16];
-            attn_load_scores(s_tmem + c, s);
-            attn_weights<PLAIN>(s, st.factor, minus, part, w);
-            ptx::tmem_st_x16(s_tmem + c / 2, w);
-            if (c % 64 == 32) {
+            if ((c + kColumns) % 64 == 0) {
                 stored();
                 part_done(c / 64);
             }
@@ -1267,10 +1251,10 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
                     break;
                 }
                 ptx::tc_fence_after_sync();
-                if (fourfold)
-                    attn_softmax<PLAIN, true>(st, row, s_tmem, thread & ~31, key0, open, i == 0, rescale, part_done);
-                else if (busy)
+                if (busy && !fourfold)
                     attn_softmax<PLAIN, false>(st, row, s_tmem, 0, key0, open, i == 0, rescale, part_done);
+                else if (fourfold)
+                    attn_softmax<PLAIN, true>(st, row, s_tmem, thread & ~31, key0, open, i == 0, rescale, part_done);
                 else {
                     part_done(0);
                     part_done(1);
