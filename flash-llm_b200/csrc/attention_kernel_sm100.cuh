@@ -81,13 +81,14 @@ constexpr int kAttnSegments  = 8;  // segments that shared memory holds at a tim
 // next piece and the ends of an item (32 outputs of its row and of the other group's) take besides.
 constexpr int kAttnSoftmaxRegisters = 208, kAttnOtherRegisters = 88;
 
-// Looks at a barrier before a CTA gives up: 0.35 seconds, 21 ns for each look at a barrier that does not change.  (Counted and not
-// timed: the waits stand in many places, and code that the instruction cache need not hold is time: ragged prompts 60 us with a
-// clock in each, 55 without.)  A CTA that gave up leaves rows as they were, those of items that others share with it too; all
-// other rows are right.
+// Looks at a barrier before a CTA gives up: a second.  A look suspends the thread until the barrier changes, for 4.0 us at most
+// (measured on B200).  (Counted and not timed: the waits stand in many places, and code that the instruction cache need not hold is
+// time: ragged prompts 60 us with a clock in each, 55 without.)  A CTA that gave up leaves rows as they were, those of items that
+// others share with it too; all other rows are right.
 #ifndef FLASHLLM_ATTENTION_LOOKS  // the tests have a build that gives up early, elsewhere in each CTA
-#define FLASHLLM_ATTENTION_LOOKS (1u << 24)
-#define FLASHLLM_ATTENTION_LOOKS_AT_ONCE 1024u
+#define FLASHLLM_ATTENTION_LOOKS (1u << 18)
+#define FLASHLLM_ATTENTION_LOOKS_AT_ONCE 32u
+#define FLASHLLM_ATTENTION_LOOK ptx::mbar_try_wait
 #endif
 
 // Tiles of keys (and as many of values) in shared memory at a time.
@@ -189,7 +190,7 @@ __device__ __forceinline__ bool attn_wait_longer(uint32_t bar, uint32_t parity, 
 {
 #pragma unroll 1
     for (uint32_t it = 1;; ++it) {
-        if (ptx::mbar_try_wait(bar, parity))
+        if (FLASHLLM_ATTENTION_LOOK(bar, parity))
             return true;
         if (it % FLASHLLM_ATTENTION_LOOKS_AT_ONCE == 0u) {
             if (it >= FLASHLLM_ATTENTION_LOOKS) {
@@ -206,7 +207,7 @@ __device__ __forceinline__ bool attn_wait_longer(uint32_t bar, uint32_t parity, 
 __device__ __forceinline__ bool attn_wait(const unsigned long long* barrier, uint32_t parity, AttnShared& sh, unsigned int* status)
 {
     const uint32_t bar = ptx::smem_u32(barrier);
-    return ptx::mbar_try_wait(bar, parity) || attn_wait_longer(bar, parity, &sh.abort_flag, status);
+    return FLASHLLM_ATTENTION_LOOK(bar, parity) || attn_wait_longer(bar, parity, &sh.abort_flag, status);
 }
 
 // ---------------------------------------------------------------- the work of a call
@@ -1472,7 +1473,7 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
         bool pair = false;
         auto have     = [&](const unsigned long long* barrier, uint32_t parity) {
             const uint32_t bar = ptx::smem_u32(barrier);  // one look first (prompt of 7000 tokens 438 us instead of 444)
-            return __all_sync(0xffffffffu, ptx::mbar_try_wait(bar, parity)) != 0
+            return __all_sync(0xffffffffu, FLASHLLM_ATTENTION_LOOK(bar, parity)) != 0
                    || __all_sync(0xffffffffu, attn_wait_longer(bar, parity, &sh.abort_flag, status)) != 0;
         };
         auto stage_of = [&](int group, int i) { return loaded + static_cast<uint32_t>(pair ? i : group + 2 * i); };
