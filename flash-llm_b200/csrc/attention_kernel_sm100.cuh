@@ -7,10 +7,10 @@
 // tokens either those up to itself and those of the prefix (prompts), or those whose bit its mask has (trees).
 //
 // One pass over the keys in tiles of 128 with the running maximum and sum of a softmax: S = Q K^T on the tensor cores, P =
-// exp(S - maximum) in registers, one thread per row, rounded to fp16 (the type of the other operand of its product; 2^-11 of a
-// weight) and back to tensor memory, O += P V from there.  The query heads that share a key/value head are rows of one tile:
-// row r of a sequence's (tokens x share) rows is token r / share, head r % share of the group.  A tile holds the rows of as many
-// whole tokens as its 128 have room for: one tensor copy brings 64 columns of them.
+// exp(S - maximum) in registers, one thread per row, rounded to fp16 (the type of the other operand of its product; kAttnWeightExponent
+// says what that takes off a weight) and back to tensor memory, O += P V from there.  The query heads that share a key/value head
+// are rows of one tile: row r of a sequence's (tokens x share) rows is token r / share, head r % share of the group.  A tile holds
+// the rows of as many whole tokens as its 128 have room for: one tensor copy brings 64 columns of them.
 //
 // An item is two such tiles of one sequence and one key/value head.  Its two tiles of rows are two groups of softmax warps that
 // take turns on the tensor core; an item of one tile (single tokens, drafted trees) is the same tile for both groups,
@@ -77,8 +77,8 @@ constexpr int kAttnThreads   = 12 * 32;
 constexpr int kAttnTmemCols  = 512;
 constexpr int kAttnKnown     = 512;  // sequences whose sizes are kept in shared memory from the plan on
 constexpr int kAttnSegments  = 8;  // segments that shared memory holds at a time
-// Registers of a thread, 256 x 208 + 128 x 88 = 384 x 168: a softmax thread keeps 32 scores of its row and what the scores of the
-// next piece and the ends of an item (32 outputs of its row and of the other group's) take besides.
+// Registers of a thread, 256 x 208 + 128 x 88 = 384 x 168: a softmax thread keeps 64 plain scores of its row, or 32 that are masked,
+// capped or biased, and what their transformation and the ends of an item (32 outputs of its row) take besides.
 constexpr int kAttnSoftmaxRegisters = 208, kAttnOtherRegisters = 88;
 
 // Looks at a barrier before a CTA gives up: a second.  A look suspends the thread until the barrier changes, for 4.0 us at most
@@ -789,8 +789,8 @@ __device__ __noinline__ AttnSums<4> attn_restore_four(const AttentionParams& p, 
     return attn_restore<HEAD_DIM, 4>(p, seg, row, list, listed, sum, column, sums);
 }
 
-// tanh x on [-0.75, 0.75] to 2e-7: x times a polynomial in x^2, fitted to it for the smallest largest error.  A call has the
-// coefficients times its cap.
+// tanh x on [-0.75, 0.75] to 2.7e-7, rounding included: x times a polynomial in x^2, fitted to it for the smallest largest error
+// (weights depend on the differences of scores; of a small score it is 2.9e-6).  A call has the coefficients times its cap.
 constexpr float kAttnTanhRange = 0.75f;
 constexpr int   kAttnTanhTerms = 5;
 __device__ constexpr float kAttnTanh[kAttnTanhTerms] = {0.9999971985816956f, -0.33323076367378235f, 0.13226091861724854f, -0.04928046092391014f, 0.012318842113018036f};
@@ -855,7 +855,7 @@ __device__ __forceinline__ void attn_transform(const AttnState& st, float (&s)[3
             }
         }
         else {
-            const float twice = 2.0f * CUDART_L2E_F * in;  // tanh x = 1 - 2 / (1 + e^2x)
+            const float twice = 2.0f * CUDART_L2E_F * in;  // tanh x = 1 - 2 / (1 + e^2x), to some 2^-21
 #pragma unroll
             for (int c = 0; c < 32; ++c)
                 s[c] = fmaf(-2.0f * st.cap, ptx::rcp_approx(1.0f + ptx::exp2_approx(s[c] * twice)), st.cap);
@@ -1434,11 +1434,12 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
                     }
                     __syncwarp();
                 }
-                again = __any_sync(0xffffffffu, valid && (probe != probe || halves_not_finite(*reinterpret_cast<const uint32_t*>(&largest)) != 0u));
+                const bool bad = probe != probe || halves_not_finite(*reinterpret_cast<const uint32_t*>(&largest)) != 0u;
+                again          = __any_sync(0xffffffffu, valid && bad);
             }
             if (again)
-                attn_end_carefully<HEAD_DIM>(p, seg, row, list, any, outputs, st.sum, column0, column1, valid && whole ? p.out + to : nullptr,
-                                             valid && !whole ? sums + thread : nullptr);
+                attn_end_carefully<HEAD_DIM>(p, seg, row, list, any, outputs, st.sum, column0, column1,
+                                             valid && whole ? p.out + to : nullptr, valid && !whole ? sums + thread : nullptr);
             if (ok && !whole && valid && column0 == 0 && (!fourfold || thread < 32))
                 reinterpret_cast<float2*>(p.workspace + attn_stats_offset(gridDim.x))[static_cast<size_t>(2 * blockIdx.x + slot) * kAttnSlotRows
                                                                                       + tile_row * kAttnRows + thread] =

@@ -310,7 +310,7 @@ int FlashLLM_SplitK_Reduction(void* stream, void* C, const void* Reduction_Works
  * page_table[b * table_width + j / page_size].  A batch is `sequences` (at most 4096) sequences whose new tokens lie one
  * behind another in `tokens` rows: sequence b owns rows cu_tokens[b] up to cu_tokens[b + 1] (cu_tokens has sequences + 1
  * entries), and its first row stands at position context[b] of its cache: so many positions are in the cache already.  Rows
- * behind the last sequence are neither read nor written.  All index arrays are int32 device arrays and are read by the
+ * behind the last sequence are not written, and what they hold is of no account.  All index arrays are int32 device arrays and are read by the
  * kernels, so a captured call may be replayed with other lengths and pages in them.
  *
  * Results are cudaError_t values; bad sizes or pointers return cudaErrorInvalidValue.  What the host cannot see sets bit 64 of
