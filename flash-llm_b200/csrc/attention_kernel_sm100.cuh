@@ -49,6 +49,7 @@ struct AttentionParams {
     float                     cap;  // 0: none
 };
 
+// What follows from the heads: how rows are tokens and heads, and how many of them tiles hold (kAttnRows at most).
 inline void attn_set_heads(AttentionParams* p, int heads, int kv_heads)
 {
     p->heads          = heads;
