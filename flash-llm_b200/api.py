@@ -110,6 +110,16 @@ def library() -> C.CDLL:
     L.FlashLLM_PromptAttention.restype = C.c_int
     L.FlashLLM_PromptAttention.argtypes = ([C.c_void_p, C.c_void_p, C.c_int] + cache + batch + [C.c_int] * 3 + [C.c_void_p]
                                            + [C.c_float] * 2 + [C.c_void_p] * 3)
+    for name in ("FlashLLM_NormRotaryAppend", "FlashLLM_FourBitAppend"):
+        f = getattr(L, name)
+        f.restype = C.c_int
+        f.argtypes = L.FlashLLM_RotaryAppend.argtypes + [C.c_void_p] * 2 + [C.c_float]
+    for name in ("FlashLLM_WindowAttention", "FlashLLM_FourBitAttention"):
+        f = getattr(L, name)
+        f.restype = C.c_int
+        f.argtypes = ([C.c_void_p, C.c_void_p, C.c_int] + cache + batch + [C.c_int] * 5 + [C.c_float] * 2 + [C.c_void_p] * 3)
+    L.FlashLLM_FourBitRead.restype = C.c_int
+    L.FlashLLM_FourBitRead.argtypes = [C.c_void_p] + cache + batch + [C.c_int] * 2 + [C.c_void_p] * 2
     L.FlashLLM_Attention_WorkspaceBytes.restype = C.c_ulonglong
     L.FlashLLM_Attention_WorkspaceBytes.argtypes = [C.c_int]
     L.FlashLLM_CacheAccept.restype = C.c_int
@@ -308,7 +318,8 @@ def spmm_splitk_no_alloc(stream: int, Compressed_A: int, TileOffsets: int, B: in
 @dataclass(frozen=True)
 class PagedBatch:
     """A cache and the batch a call works on, as integer device pointers and sizes: ``K_cache`` and ``V_cache`` are fp16
-    ``[pages][kv_heads][page_size][head_dim]`` (``layers`` of them one behind another for :func:`cache_accept`), sequence b owns
+    ``[pages][kv_heads][page_size][head_dim]`` (``layers`` of them one behind another for :func:`cache_accept`), for the ``four_bit``
+    calls bytes ``[pages][kv_heads][page_size][head_dim * 9 / 16]`` (include/SpMM_API.cuh has the layout), sequence b owns
     rows ``cu_tokens[b]`` up to ``cu_tokens[b + 1]`` of the ``tokens`` rows, and ``context[b]`` of its positions, which lie in the
     pages ``page_table[b * table_width + ...]``, are filled before the call (int32 device arrays)."""
     K_cache: int
@@ -345,7 +356,7 @@ def rotary_append(stream: int, QKV: int, ld_qkv: int, Q: int, ld_q: int, batch: 
 
 
 def attention_workspace_bytes(head_dim: int) -> int:
-    """Bytes of the workspace that :func:`tree_attention` and :func:`prompt_attention` take on the current device."""
+    """Bytes of the workspace that each of the attention calls takes on the current device."""
     return int(library().FlashLLM_Attention_WorkspaceBytes(head_dim))
 
 
@@ -370,6 +381,57 @@ def prompt_attention(stream: int, Q: int, ld_q: int, batch: PagedBatch, heads: i
                                               Out, workspace)
     if code:
         _check(code, f"PromptAttention(heads={heads}, ld_q={ld_q}, scale={scale}, cap={cap}, {batch})")
+
+
+def norm_rotary_append(stream: int, QKV: int, ld_qkv: int, Q: int, ld_q: int, batch: PagedBatch, heads: int, q_norm: int, k_norm: int,
+                       eps: float = 1e-6, frequencies: int | None = None, rotary_dim: int = 0, interleaved: bool = False,
+                       magnitude: float = 1.0, positions: int | None = None) -> None:
+    """:func:`rotary_append` of query and key heads that are normed first: ``x w / sqrt(mean(x^2) + eps)`` with the fp16 weights
+    ``q_norm`` and ``k_norm`` of ``head_dim`` entries."""
+    code = library().FlashLLM_NormRotaryAppend(stream, QKV, ld_qkv, Q, ld_q, *batch._cache(), *batch._batch(), heads, batch.kv_heads,
+                                               batch.head_dim, frequencies, rotary_dim, int(interleaved), magnitude, positions, q_norm,
+                                               k_norm, eps)
+    if code:
+        _check(code, f"NormRotaryAppend(heads={heads}, rotary_dim={rotary_dim}, ld_qkv={ld_qkv}, ld_q={ld_q}, eps={eps}, {batch})")
+
+
+def window_attention(stream: int, Q: int, ld_q: int, batch: PagedBatch, heads: int, Out: int, workspace: int, window: int,
+                     sinks: int = 0, scale: float | None = None, cap: float = 0.0, slopes: int | None = None) -> None:
+    """:func:`prompt_attention` through a window: row n sees the last ``window`` positions of its sequence up to itself and the
+    first ``sinks``."""
+    code = library().FlashLLM_WindowAttention(stream, Q, ld_q, *batch._cache(), *batch._batch(), heads, batch.kv_heads,
+                                              batch.head_dim, window, sinks, batch.head_dim ** -0.5 if scale is None else scale, cap,
+                                              slopes, Out, workspace)
+    if code:
+        _check(code, f"WindowAttention(heads={heads}, ld_q={ld_q}, window={window}, sinks={sinks}, scale={scale}, cap={cap}, {batch})")
+
+
+def four_bit_append(stream: int, QKV: int, ld_qkv: int, Q: int, ld_q: int, batch: PagedBatch, heads: int, q_norm: int | None = None,
+                    k_norm: int | None = None, eps: float = 1e-6, frequencies: int | None = None, rotary_dim: int = 0,
+                    interleaved: bool = False, magnitude: float = 1.0, positions: int | None = None) -> None:
+    """:func:`norm_rotary_append`, its norms optional, into a cache of 4 bits."""
+    code = library().FlashLLM_FourBitAppend(stream, QKV, ld_qkv, Q, ld_q, *batch._cache(), *batch._batch(), heads, batch.kv_heads,
+                                            batch.head_dim, frequencies, rotary_dim, int(interleaved), magnitude, positions, q_norm,
+                                            k_norm, eps)
+    if code:
+        _check(code, f"FourBitAppend(heads={heads}, rotary_dim={rotary_dim}, ld_qkv={ld_qkv}, ld_q={ld_q}, eps={eps}, {batch})")
+
+
+def four_bit_attention(stream: int, Q: int, ld_q: int, batch: PagedBatch, heads: int, Out: int, workspace: int, window: int = 0,
+                       sinks: int = 0, scale: float | None = None, cap: float = 0.0, slopes: int | None = None) -> None:
+    """:func:`prompt_attention` (``window`` 0) or :func:`window_attention` over a cache of 4 bits."""
+    code = library().FlashLLM_FourBitAttention(stream, Q, ld_q, *batch._cache(), *batch._batch(), heads, batch.kv_heads,
+                                               batch.head_dim, window, sinks, batch.head_dim ** -0.5 if scale is None else scale, cap,
+                                               slopes, Out, workspace)
+    if code:
+        _check(code, f"FourBitAttention(heads={heads}, ld_q={ld_q}, window={window}, sinks={sinks}, scale={scale}, cap={cap}, {batch})")
+
+
+def four_bit_read(stream: int, batch: PagedBatch, K_out: int, V_out: int) -> None:
+    """The batch's rows from a cache of 4 bits, ``K_out`` and ``V_out`` fp16 ``[tokens][kv_heads * head_dim]``."""
+    code = library().FlashLLM_FourBitRead(stream, *batch._cache(), *batch._batch(), batch.kv_heads, batch.head_dim, K_out, V_out)
+    if code:
+        _check(code, f"FourBitRead({batch})")
 
 
 def cache_accept(stream: int, batch: PagedBatch, accepted: int, accepted_lengths: int, accepted_width: int) -> None:

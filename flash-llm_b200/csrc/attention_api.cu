@@ -9,47 +9,12 @@
 
 #include "../../include/SpMM_API.cuh"
 #include "attention_kernel_sm100.cuh"
+#include "cache_api.h"
 #include "cache_kernels_sm100.cuh"
 #include "launch.h"
 #include "tiled_csl_host.h"
 
 namespace flashllm {
-
-static bool aligned16(const void* p)
-{
-    return (reinterpret_cast<uintptr_t>(p) & 15u) == 0;
-}
-
-// What every operator's cache and batch have to be.
-static bool describe_batch(CacheBatch* batch, const void* K_cache, const void* V_cache, int pages, int page_size,
-                           const int* cu_tokens, const int* context, const int* page_table, int table_width, int sequences,
-                           int tokens, int kv_heads, int head_dim)
-{
-    if (K_cache == nullptr || V_cache == nullptr || cu_tokens == nullptr || context == nullptr || page_table == nullptr
-        || !aligned16(K_cache) || !aligned16(V_cache) || pages < 1 || kv_heads < 1 || (head_dim != 64 && head_dim != 128)
-        || page_size < 16 || (page_size & (page_size - 1)) != 0 || table_width < 1 || sequences < 0
-        || sequences > kMaxSequences || tokens < 0)
-        return false;
-    // Positions, and the pages of all heads, are counted in ints; a tile may reach 127 positions behind the last.
-    if (static_cast<long long>(table_width) * page_size > 0x7fffffffll - 256
-        || static_cast<long long>(pages) * kv_heads > 0x7fffffffll - 1)
-        return false;
-    batch->cu_tokens   = cu_tokens;
-    batch->context     = context;
-    batch->page_table  = page_table;
-    batch->sequences   = sequences;
-    batch->tokens      = tokens;
-    batch->table_width = table_width;
-    batch->pages       = pages;
-    batch->page_shift  = __builtin_ctz(static_cast<unsigned>(page_size));
-    batch->kv_heads    = kv_heads;
-    return true;
-}
-
-static bool rows_fit(const void* matrix, int ld, int heads, int head_dim)
-{
-    return matrix != nullptr && aligned16(matrix) && ld % 8 == 0 && ld >= static_cast<long long>(heads) * head_dim;
-}
 
 static cudaError_t launch_rotary(cudaStream_t stream, const RotaryParams& p, int head_dim, bool interleaved)
 {
@@ -82,29 +47,23 @@ static EncodeTiledFn encode_tiled()
 // device.
 static cudaError_t multiprocessors(int* count)
 {
-    constexpr int           kMaxDevices = 64;
-    static std::atomic<int> known[kMaxDevices];
-    int                     device = 0;
-    cudaError_t             err    = cudaGetDevice(&device);
-    if (err != cudaSuccess)
+    static std::atomic<int> known[64];
+    return multiprocessors_once(known, count, []() {
+        cudaError_t err   = cudaSuccess;
+        auto        raise = [&](auto kernel, int bytes) {
+            if (err == cudaSuccess)
+                err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+        };
+        raise(attention_kernel<64, true>, attn_smem_bytes(64));
+        raise(attention_kernel<64, false>, attn_smem_bytes(64));
+        raise(attention_kernel<128, true>, attn_smem_bytes(128));
+        raise(attention_kernel<128, false>, attn_smem_bytes(128));
+        raise(attention_kernel<64, true, true>, attn_smem_bytes<true>(64));
+        raise(attention_kernel<64, false, true>, attn_smem_bytes<true>(64));
+        raise(attention_kernel<128, true, true>, attn_smem_bytes<true>(128));
+        raise(attention_kernel<128, false, true>, attn_smem_bytes<true>(128));
         return err;
-    if (device < 0 || device >= kMaxDevices)
-        return cudaErrorInvalidDevice;
-    *count = known[device].load(std::memory_order_acquire);
-    if (*count > 0)
-        return cudaSuccess;
-    err = cudaDeviceGetAttribute(count, cudaDevAttrMultiProcessorCount, device);
-    auto raise = [&](auto kernel, int bytes) {
-        if (err == cudaSuccess)
-            err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
-    };
-    raise(attention_kernel<64, true>, attn_smem_bytes(64));
-    raise(attention_kernel<64, false>, attn_smem_bytes(64));
-    raise(attention_kernel<128, true>, attn_smem_bytes(128));
-    raise(attention_kernel<128, false>, attn_smem_bytes(128));
-    if (err == cudaSuccess)
-        known[device].store(*count, std::memory_order_release);
-    return err;
+    });
 }
 
 // A cache tensor as (head_dim, page_size, pages * kv_heads), copied in boxes of 64 columns and the rows of a page, 128 at most.
@@ -153,14 +112,18 @@ static cudaError_t launch_attention(cudaStream_t stream, const AttentionParams& 
         || !encode_cache(&map_k, p.k_cache, p.batch, HEAD_DIM) || !encode_cache(&map_v, p.v_cache, p.batch, HEAD_DIM))
         return cudaErrorInvalidValue;
     const bool plain = p.cap == 0.0f && p.slopes == nullptr;
-    err = launch_in_stream_order(plain ? attention_kernel<HEAD_DIM, true> : attention_kernel<HEAD_DIM, false>, dim3(sms), dim3(kAttnThreads), attn_smem_bytes(HEAD_DIM), stream, 1, map_q,
-                                 map_q_few, map_k, map_v, p);
+    if (p.window > 0)
+        err = launch_in_stream_order(plain ? attention_kernel<HEAD_DIM, true, true> : attention_kernel<HEAD_DIM, false, true>, dim3(sms),
+                                     dim3(kAttnThreads), attn_smem_bytes<true>(HEAD_DIM), stream, 1, map_q, map_q_few, map_k, map_v, p);
+    else
+        err = launch_in_stream_order(plain ? attention_kernel<HEAD_DIM, true> : attention_kernel<HEAD_DIM, false>, dim3(sms),
+                                     dim3(kAttnThreads), attn_smem_bytes(HEAD_DIM), stream, 1, map_q, map_q_few, map_k, map_v, p);
     if (err != cudaSuccess)
         return err;
     return launch_in_stream_order(attention_join_kernel<HEAD_DIM>, dim3(sms, kAttnSlotRows / 32), dim3(256), 0, stream, 1, p, sms);
 }
 
-// The checks that tree and prompt attention share, and the launch.
+// The checks that the attention operators share, and the launch.
 static cudaError_t attend(cudaStream_t stream, AttentionParams p, const void* Q, int ld_q, const void* K_cache,
                           const void* V_cache, int pages, int page_size, const int* cu_tokens, const int* context,
                           const int* page_table, int table_width, int sequences, int tokens, int heads, int kv_heads,
@@ -169,9 +132,7 @@ static cudaError_t attend(cudaStream_t stream, AttentionParams p, const void* Q,
     if (!describe_batch(&p.batch, K_cache, V_cache, pages, page_size, cu_tokens, context, page_table, table_width, sequences, tokens,
                         kv_heads, head_dim)
         || heads < 1 || heads % kv_heads != 0 || heads / kv_heads > kAttnRows || static_cast<long long>(heads) * head_dim > (1 << 24) || !rows_fit(Q, ld_q, heads, head_dim)
-        || workspace == nullptr || !aligned16(workspace) || Out == nullptr || !aligned16(Out) || !(scale > 0.0f) || !std::isfinite(scale) || !(cap >= 0.0f) || !std::isfinite(cap)
-        // What the kernels make of them is finite too, scores times log2 e of 128 products of the largest fp16 values among it.
-        || !std::isfinite(scale * 8e11f) || !std::isfinite(cap * 1.45f) || (cap > 0.0f && !std::isfinite(scale / cap * 3.0f))
+        || workspace == nullptr || !aligned16(workspace) || Out == nullptr || !aligned16(Out) || !scores_fit(scale, cap)
         || static_cast<long long>(tokens) * heads > 0x7fffffffll - 256)
         return cudaErrorInvalidValue;
     if (tokens == 0 || sequences == 0)
@@ -259,6 +220,24 @@ int FlashLLM_PromptAttention(void* stream, const void* Q, int ld_q, const void* 
 {
     AttentionParams p{};
     p.prefix = prefix;
+    return static_cast<int>(attend(static_cast<cudaStream_t>(stream), p, Q, ld_q, K_cache, V_cache, pages, page_size, cu_tokens,
+                                   context, page_table, table_width, sequences, tokens, heads, kv_heads, head_dim, scale, cap,
+                                   slopes, Out, workspace));
+}
+
+int FlashLLM_WindowAttention(void* stream, const void* Q, int ld_q, const void* K_cache, const void* V_cache, int pages,
+                             int page_size, const int* cu_tokens, const int* context, const int* page_table, int table_width,
+                             int sequences, int tokens, int heads, int kv_heads, int head_dim, int window, int sinks, float scale,
+                             float cap, const float* slopes, void* Out, void* workspace)
+{
+    if (window < 1 || sinks < 0)
+        return static_cast<int>(cudaErrorInvalidValue);
+    AttentionParams p{};
+    // A window over all that a sequence can hold hides nothing: the kernels without one.
+    if (static_cast<long long>(table_width) * page_size > window) {
+        p.window = window;
+        p.sinks  = sinks;
+    }
     return static_cast<int>(attend(static_cast<cudaStream_t>(stream), p, Q, ld_q, K_cache, V_cache, pages, page_size, cu_tokens,
                                    context, page_table, table_width, sequences, tokens, heads, kv_heads, head_dim, scale, cap,
                                    slopes, Out, workspace));

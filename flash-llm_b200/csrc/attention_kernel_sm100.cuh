@@ -4,7 +4,8 @@
 //   o_i  = sum over the keys j that i sees of softmax_j(s_ij) v_j;  zero for a row that sees none
 //
 // What token i of a sequence (rows first + i, place context + i in the cache) sees: the whole context, and of the batch's own
-// tokens either those up to itself and those of the prefix (prompts), or those whose bit its mask has (trees).
+// tokens either those up to itself and those of the prefix (prompts), or those whose bit its mask has (trees).  With a window
+// it sees, of those up to itself, the last `window` and the first `sinks` of the sequence.
 //
 // One pass over the keys in tiles of 128 with the running maximum and sum of a softmax: S = Q K^T on the tensor cores, P =
 // exp(S - maximum) in registers, one thread per row, rounded to fp16 (the type of the other operand of its product; kAttnWeightExponent
@@ -47,6 +48,8 @@ struct AttentionParams {
     int                       few_rows;   // ... at most 32; 0 where not one fits
     float                     scale;
     float                     cap;  // 0: none
+    int                       window;  // keys up to itself that a row sees, kernels with a window alone
+    int                       sinks;   // ... and of its sequence's first
 };
 
 // What follows from the heads: how rows are tokens and heads, and how many of them tiles hold (kAttnRows at most).
@@ -103,8 +106,22 @@ __host__ __device__ constexpr int attn_tile_bytes(int head_dim)
     return kAttnKeys * head_dim * 2;
 }
 
+// What an item sees through a window.  Tiles of keys between the sinks and the window of its first row are left out: its tiles are
+// numbered without them.
+template<bool WINDOW>
+struct AttnSight {};
+
+template<>
+struct AttnSight<true> {
+    int sinks;
+    int sink_tiles;  // tiles before those that are left out
+    int skip;        // tiles that are left out
+    int low[2];      // first key, sinks aside, that every row of a group sees: the last row's
+};
+
 // The part of an item that one CTA takes in one go.
-struct AttnSegment {
+template<bool WINDOW>
+struct AttnSegmentOf : AttnSight<WINDOW> {
     int  b;
     int  first, count, context, prefix;  // of the sequence: first row, rows, position of the first row, keys that all see
     int  head;     // key/value head
@@ -130,10 +147,56 @@ struct AttnSegment {
     {
         return pair ? begin + i : begin + group + 2 * i;
     }
+    // First key of a tile.
+    __device__ __forceinline__ int key_of(int tile) const
+    {
+        if constexpr (WINDOW)
+            tile += tile < this->sink_tiles ? 0 : this->skip;
+        return tile * kAttnKeys;
+    }
+    // Whether some row of the group does not see all of the tile that begins with that key (of the item: see `mixed`).
+    __device__ __forceinline__ bool masked(int key0, int group) const
+    {
+        if constexpr (WINDOW)
+            if (key0 < this->low[group] && key0 + kAttnKeys > this->sinks)
+                return true;
+        return key0 + kAttnKeys > open[group];
+    }
+    __device__ __forceinline__ bool mixed(int tile) const
+    {
+        const int key0 = key_of(tile);
+        if constexpr (WINDOW)
+            if (key0 < this->low[1] && key0 + kAttnKeys > this->sinks)
+                return true;
+        return key0 + kAttnKeys > open[0];
+    }
+    // Such tiles are few: the last three, and with a window the one that the sinks end in and the three that begin it (an item's
+    // rows are at most 256 tokens).  Which of them a tile is, and back.
+    static constexpr int kMixed = WINDOW ? 7 : 3;
+    __device__ __forceinline__ int mixed_of(int tile) const
+    {
+        const int last = tiles - 1 - tile;
+        if constexpr (WINDOW) {
+            if (last < 3)
+                return last;
+            const int behind = tile - this->sink_tiles;
+            return behind < 0 ? 3 : behind < 3 ? 4 + behind : kMixed;
+        }
+        return last < 3 ? last : kMixed;
+    }
+    __device__ __forceinline__ int tile_of(int mixed) const
+    {
+        if constexpr (WINDOW)
+            if (mixed >= 3)
+                return this->sink_tiles + mixed - 4;
+        return tiles - 1 - mixed;
+    }
 };
+using AttnSegment = AttnSegmentOf<false>;
 
 // Dynamic shared memory: two tiles of Q, the stages, and what AttnShared holds.
-struct AttnShared {
+template<bool WINDOW>
+struct AttnSharedOf {
     unsigned long long k_full[4], k_empty[4], v_full[4], v_clean[4], v_empty[4];
     unsigned long long s_full[2], p_full[2][2], o_done[2], q_full[2], q_empty[2], segment_full[kAttnSegments];
     uint32_t           tmem;
@@ -141,10 +204,10 @@ struct AttnShared {
     // Written by the loader, which is ahead of everybody, by at most the stages and one: a segment's values cannot be loaded
     // before those of the one so many tiles earlier have been multiplied, and its place here is taken again only after
     // kAttnSegments more.
-    AttnSegment        segment[kAttnSegments];
+    AttnSegmentOf<WINDOW> segment[kAttnSegments];
     float              top[2][kAttnRows], sum[2][kAttnRows];
     uint32_t           any_not_finite[kAttnSegments];
-    uint32_t           not_finite[kAttnSegments][3][4];  // keys of an item's last three tiles whose values are not finite
+    uint32_t           not_finite[kAttnSegments][AttnSegmentOf<WINDOW>::kMixed][4];  // keys of such tiles whose values are not finite
     int                drafted[2][kMaxDrafted];          // positions of drafted tokens, by group
     union {
         unsigned int units[kMaxSequences];  // of all items of a sequence's first key/value head; the plan's alone
@@ -152,10 +215,12 @@ struct AttnShared {
     };
     int4               known[kAttnKnown];                // first row, rows, context and prefix of the first sequences
 };
+using AttnShared = AttnSharedOf<false>;
 
+template<bool WINDOW = false>
 __host__ __device__ constexpr int attn_smem_bytes(int head_dim)
 {
-    return (2 + 2 * attn_stages(head_dim)) * attn_tile_bytes(head_dim) + static_cast<int>(sizeof(AttnShared)) + 1024;
+    return (2 + 2 * attn_stages(head_dim)) * attn_tile_bytes(head_dim) + static_cast<int>(sizeof(AttnSharedOf<WINDOW>)) + 1024;
 }
 
 // The workspace: for each CTA two slots, the segment that continues an item that another CTA began, and the one that begins an
@@ -205,7 +270,8 @@ __device__ __forceinline__ bool attn_wait_longer(uint32_t bar, uint32_t parity, 
 }
 
 // A bounded wait; false once the CTA gives up.
-__device__ __forceinline__ bool attn_wait(const unsigned long long* barrier, uint32_t parity, AttnShared& sh, unsigned int* status)
+template<bool WINDOW>
+__device__ __forceinline__ bool attn_wait(const unsigned long long* barrier, uint32_t parity, AttnSharedOf<WINDOW>& sh, unsigned int* status)
 {
     const uint32_t bar = ptx::smem_u32(barrier);
     return FLASHLLM_ATTENTION_LOOK(bar, parity) || attn_wait_longer(bar, parity, &sh.abort_flag, status);
@@ -230,7 +296,8 @@ __device__ __forceinline__ AttnSequence attn_sequence(const AttentionParams& p, 
 }
 
 // ... what the plan has kept of it.
-__device__ __forceinline__ AttnSequence attn_sequence(const AttentionParams& p, const AttnShared& sh, int b)
+template<bool WINDOW>
+__device__ __forceinline__ AttnSequence attn_sequence(const AttentionParams& p, const AttnSharedOf<WINDOW>& sh, int b)
 {
     if (b >= kAttnKnown)
         return attn_sequence(p, b);
@@ -255,6 +322,28 @@ __device__ __forceinline__ int attn_open_keys(const AttentionParams& p, const At
 __device__ __forceinline__ int attn_tiles(int keys)
 {
     return (keys + kAttnKeys - 1) / kAttnKeys;
+}
+
+// What an item whose first row is `row` and whose rows see `keys` keys at most leaves out between sinks and window.
+__device__ __forceinline__ void attn_set_sight(const AttentionParams& p, const AttnSequence& a, int row, int keys, AttnSight<true>& sight)
+{
+    const int first  = max(0, a.s.context + attn_token(p, row) - p.window + 1);
+    sight.sinks      = p.sinks;
+    sight.sink_tiles = attn_tiles(min(p.sinks, keys));
+    sight.skip       = max(0, first / kAttnKeys - sight.sink_tiles);
+}
+
+// Tiles of keys of the item with rows `row` up to `row_end`.
+template<bool WINDOW>
+__device__ __forceinline__ int attn_item_tiles(const AttentionParams& p, const AttnSequence& a, int row, int row_end)
+{
+    const int keys = attn_keys(p, a, row_end);
+    if constexpr (WINDOW) {
+        AttnSight<true> sight;
+        attn_set_sight(p, a, row, keys, sight);
+        return attn_tiles(keys) - sight.skip;
+    }
+    return attn_tiles(keys);
 }
 
 // Beginning an item, and ending it, takes about as long as two of its tiles of keys, and as four where its groups share their rows
@@ -282,14 +371,16 @@ __device__ __forceinline__ int attn_least(unsigned long long share)
 }
 
 // Units of the item whose rows begin with row0 of the sequence's.
+template<bool WINDOW>
 __device__ __forceinline__ unsigned attn_units(const AttentionParams& p, const AttnSequence& a, int row0)
 {
     const int end = min(row0 + 2 * p.tile_rows, a.rows);
-    return static_cast<unsigned>(attn_tiles(attn_keys(p, a, end)) + attn_extra_units(p, end - row0));
+    return static_cast<unsigned>(attn_item_tiles<WINDOW>(p, a, row0, end) + attn_extra_units(p, end - row0));
 }
 
 // The segment of that number, once the loader has written it; nullptr at the end and when the CTA gives up.
-__device__ __forceinline__ const AttnSegment* attn_segment(AttnShared& sh, int number, unsigned int* status)
+template<bool WINDOW>
+__device__ __forceinline__ const AttnSegmentOf<WINDOW>* attn_segment(AttnSharedOf<WINDOW>& sh, int number, unsigned int* status)
 {
     const int place = number % kAttnSegments;
     if (!attn_wait(&sh.segment_full[place], number / kAttnSegments & 1, sh, status) || sh.segment[place].end == 0)
@@ -325,19 +416,21 @@ __device__ __forceinline__ COUNT attn_warp_scan(COUNT mine)
 
 // Units of all items of a sequence's first key/value head, for a whole warp.  A sequence can have up to 2^49 of them, a call with
 // all heads of all sequences more: a prompt of 2 million tokens with 64 heads has 2^32, some 80 seconds' work.
+template<bool WINDOW>
 __device__ __forceinline__ unsigned long long attn_sequence_units(const AttentionParams& p, const AttnSequence& a)
 {
     const int          item_rows = 2 * p.tile_rows;
     unsigned long long mine      = 0;
 #pragma unroll 1
     for (long long r = (threadIdx.x & 31) * item_rows; r < a.rows; r += 32 * item_rows)
-        mine += attn_units(p, a, static_cast<int>(r));
+        mine += attn_units<WINDOW>(p, a, static_cast<int>(r));
     return attn_warp_sum(mine);
 }
 
 // Units of every sequence; all threads, ends with a barrier.  The rows of a sequence that does not fit into the page table are
 // cleared here, by one CTA.
-__device__ __forceinline__ void attn_count_units(const AttentionParams& p, AttnShared& sh, int head_dim)
+template<bool WINDOW>
+__device__ __forceinline__ void attn_count_units(const AttentionParams& p, AttnSharedOf<WINDOW>& sh, int head_dim)
 {
     const int B = p.batch.sequences, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int item_rows = 2 * p.tile_rows;
@@ -350,7 +443,7 @@ __device__ __forceinline__ void attn_count_units(const AttentionParams& p, AttnS
         const unsigned units = a.s.lost > 0         ? kAttnLostRows
                                : a.rows == 0        ? 0u
                                : a.rows > item_rows ? kAttnSeveralItems
-                                                    : attn_units(p, a, 0);
+                                                    : attn_units<WINDOW>(p, a, 0);
         sh.units[b]          = units;
         several              = several || units >= kAttnLostRows;
     }
@@ -366,7 +459,7 @@ __device__ __forceinline__ void attn_count_units(const AttentionParams& p, AttnS
                 for (long long i = lane * 8; i < a.s.lost * row; i += 32 * 8)
                     *reinterpret_cast<uint4*>(p.out + a.s.first * row + i) = make_uint4(0, 0, 0, 0);
             }
-            const unsigned long long units = attn_sequence_units(p, a);
+            const unsigned long long units = attn_sequence_units<WINDOW>(p, a);
             __syncwarp();
             if (lane == 0)
                 sh.units[b] = static_cast<unsigned>(min(units, static_cast<unsigned long long>(kAttnManyUnits)));
@@ -382,7 +475,8 @@ struct AttnStart {
 };
 
 // Units of this lane's sequence of the 32 from `base` on, first key/value head, for a whole warp.
-__device__ __forceinline__ unsigned long long attn_units_of(const AttentionParams& p, const AttnShared& sh, int base)
+template<bool WINDOW>
+__device__ __forceinline__ unsigned long long attn_units_of(const AttentionParams& p, const AttnSharedOf<WINDOW>& sh, int base)
 {
     const int          b    = base + (threadIdx.x & 31);
     const unsigned     kept = b < p.batch.sequences ? sh.units[b] : 0;
@@ -390,7 +484,7 @@ __device__ __forceinline__ unsigned long long attn_units_of(const AttentionParam
 #pragma unroll 1
     for (unsigned many = __ballot_sync(0xffffffffu, kept == kAttnManyUnits); many; many &= many - 1) {
         const int                at    = base + __ffs(many) - 1;
-        const unsigned long long units = attn_sequence_units(p, attn_sequence(p, sh, at));
+        const unsigned long long units = attn_sequence_units<WINDOW>(p, attn_sequence(p, sh, at));
         mine                           = b == at ? units : mine;
     }
     return mine;
@@ -398,8 +492,8 @@ __device__ __forceinline__ unsigned long long attn_units_of(const AttentionParam
 
 // The item that holds unit u0 of the call.  COUNT holds all units: 32 bits if they do (small trees 12.2 us with 64 bits throughout,
 // 11.9 with 32; capped trees of 64 tokens 73.8 and 72.7).
-template<typename COUNT>
-__device__ __forceinline__ void attn_find(const AttentionParams& p, const AttnShared& sh, COUNT u0, AttnStart& start)
+template<typename COUNT, bool WINDOW>
+__device__ __forceinline__ void attn_find(const AttentionParams& p, const AttnSharedOf<WINDOW>& sh, COUNT u0, AttnStart& start)
 {
     const int   B = p.batch.sequences, lane = threadIdx.x & 31, item_rows = 2 * p.tile_rows;
     const COUNT heads = p.batch.kv_heads;
@@ -427,12 +521,12 @@ __device__ __forceinline__ void attn_find(const AttentionParams& p, const AttnSh
     int                row0 = 0;
     unsigned           item = 1;
     if (a.rows <= item_rows)
-        item = attn_units(p, a, 0);
+        item = attn_units<WINDOW>(p, a, 0);
     else {
 #pragma unroll 1
         for (long long base = 0;; base += 32 * item_rows) {  // ... and of its items the first
             const long long r    = base + lane * item_rows;
-            const unsigned  size = r < a.rows ? attn_units(p, a, static_cast<int>(r)) : 0;
+            const unsigned  size = r < a.rows ? attn_units<WINDOW>(p, a, static_cast<int>(r)) : 0;
             const COUNT     mine = size * heads, upto = attn_warp_scan(mine);
             const unsigned  past = __ballot_sync(0xffffffffu, before + upto > u0);
             if (past || base + 32 * item_rows >= a.rows) {
@@ -452,7 +546,8 @@ __device__ __forceinline__ void attn_find(const AttentionParams& p, const AttnSh
 }
 
 // ... where 32 bits do not hold them: code of its own, out of the way of the usual calls'.
-__device__ __noinline__ AttnStart attn_start_many(const AttentionParams& p, const AttnShared& sh)
+template<bool WINDOW>
+__device__ __noinline__ AttnStart attn_start_many(const AttentionParams& p, const AttnSharedOf<WINDOW>& sh)
 {
     AttnStart          start{0, 0, 0, 0, 0, 0};
     unsigned long long total = 0;
@@ -468,7 +563,8 @@ __device__ __noinline__ AttnStart attn_start_many(const AttentionParams& p, cons
     return start;
 }
 
-__device__ __forceinline__ AttnStart attn_start(const AttentionParams& p, const AttnShared& sh)
+template<bool WINDOW>
+__device__ __forceinline__ AttnStart attn_start(const AttentionParams& p, const AttnSharedOf<WINDOW>& sh)
 {
     const int          lane = threadIdx.x & 31;
     AttnStart          start{0, 0, 0, 0, 0, 0};
@@ -490,9 +586,10 @@ __device__ __forceinline__ AttnStart attn_start(const AttentionParams& p, const 
 }
 
 // Walks a CTA's share of the linear sequence of units, order (sequence, rows, key/value head, keys).
-struct AttnCursor {
+template<bool WINDOW>
+struct AttnCursorOf {
     AttnSequence a;
-    AttnSegment  seg;
+    AttnSegmentOf<WINDOW> seg;
     unsigned long long left;
     int          next_unit;  // of the item
     int          extra;      // units of the item beyond its tiles
@@ -500,7 +597,7 @@ struct AttnCursor {
 
     bool         new_sequence, new_rows;  // what `seg` does not describe yet
 
-    __device__ __forceinline__ explicit AttnCursor(const AttnStart& start)
+    __device__ __forceinline__ explicit AttnCursorOf(const AttnStart& start)
     {
         left         = start.units;
         least        = start.least;
@@ -514,7 +611,7 @@ struct AttnCursor {
         extra        = 0;
     }
     // The next segment that has a tile; its `end` is 0 at the end of the share.
-    __device__ __forceinline__ void next(const AttentionParams& p, const AttnShared& sh)
+    __device__ __forceinline__ void next(const AttentionParams& p, const AttnSharedOf<WINDOW>& sh)
     {
         do {
             if (next_unit >= seg.tiles + extra) {
@@ -557,6 +654,14 @@ struct AttnCursor {
                 seg.keys      = attn_keys(p, a, end);
                 seg.tiles     = attn_tiles(seg.keys);
                 seg.tiles0    = seg.pair ? attn_tiles(attn_keys(p, a, seg.row0 + p.tile_rows)) : seg.tiles;
+                if constexpr (WINDOW) {
+                    attn_set_sight(p, a, seg.row0, seg.keys, seg);
+                    const int low = seg.context - p.window + 1;  // of the sequence's first row
+                    seg.tiles -= seg.skip;
+                    seg.tiles0 -= seg.skip;
+                    seg.low[1] = low + attn_token(p, end - 1);
+                    seg.low[0] = seg.pair ? low + attn_token(p, seg.row0 + p.tile_rows - 1) : seg.low[1];
+                }
                 seg.open[0]   = attn_open_keys(p, a, seg.row0);
                 seg.open[1]   = seg.pair ? attn_open_keys(p, a, seg.row0 + p.tile_rows) : seg.open[0];
                 new_rows      = false;
@@ -572,11 +677,35 @@ struct AttnCursor {
         } while (seg.end == seg.begin);
     }
 };
+using AttnCursor = AttnCursorOf<false>;
 
 // ---------------------------------------------------------------- masks
 
+// The bits of 32 keys that lie before the n-th of them.
+__device__ __forceinline__ uint32_t attn_bits_before(int n)
+{
+    return n >= 32 ? 0xffffffffu : n > 0 ? (1u << n) - 1u : 0u;
+}
+
 // What a row sees.
-struct AttnRow {
+template<bool WINDOW>
+struct AttnRowOf;
+
+template<>
+struct AttnRowOf<true> {
+    int limit;  // keys before this one that are
+    int low;    // at or behind this one
+    int sinks;  // or before this one
+
+    __device__ __forceinline__ bool sees(int key) const { return key < limit && (key >= low || key < sinks); }
+    __device__ __forceinline__ uint32_t word(int key0) const
+    {
+        return attn_bits_before(limit - key0) & (~attn_bits_before(low - key0) | attn_bits_before(sinks - key0));
+    }
+};
+
+template<>
+struct AttnRowOf<false> {
     int                limit;   // all keys before this one
     int                drafts;  // ... and, for trees, key drafts + i where bit i is set
     unsigned long long bits;
@@ -589,8 +718,7 @@ struct AttnRow {
     // Bit c: the row sees key `key0` + c.
     __device__ __forceinline__ uint32_t word(int key0) const
     {
-        const int n = limit - key0;
-        uint32_t  w = n >= 32 ? 0xffffffffu : n > 0 ? (1u << n) - 1u : 0u;
+        uint32_t  w = attn_bits_before(limit - key0);
         const int d = drafts - key0;
         if (d >= 0 && d < 32)
             w |= static_cast<uint32_t>(bits << d);
@@ -600,9 +728,15 @@ struct AttnRow {
     }
 };
 
-__device__ __forceinline__ AttnRow attn_row(const AttentionParams& p, const AttnSegment& seg, int row, bool valid)
+__device__ __forceinline__ AttnRowOf<true> attn_row(const AttentionParams& p, const AttnSegmentOf<true>& seg, int row, bool valid)
 {
-    AttnRow r;
+    const int place = seg.context + (valid ? attn_token(p, row) : 0);
+    return AttnRowOf<true>{valid ? place + 1 : 0, place - p.window + 1, p.sinks};
+}
+
+__device__ __forceinline__ AttnRowOf<false> attn_row(const AttentionParams& p, const AttnSegmentOf<false>& seg, int row, bool valid)
+{
+    AttnRowOf<false> r;
     r.limit  = 0;
     r.drafts = seg.context;
     r.bits   = 0;
@@ -642,17 +776,21 @@ __device__ __forceinline__ uint32_t attn_pack_bounded(float x, float y)
     return *reinterpret_cast<const uint32_t*>(&h);
 }
 
+template<bool WINDOW>
+using AttnList = uint32_t[AttnSegmentOf<WINDOW>::kMixed][4];
+
 // Adds to o[c], element column + c of a row's output, the values that are not finite of keys that the row sees (the products
 // took zeros in their place: a weight of zero times infinity is not zero).
-template<int HEAD_DIM, int COLUMNS>
-__device__ __forceinline__ void attn_add_not_finite(const AttentionParams& p, const AttnSegment& seg, const AttnRow& row,
-                                                    const uint32_t (&list)[3][4], int column, float (&o)[COLUMNS])
+template<int HEAD_DIM, int COLUMNS, bool WINDOW>
+__device__ __forceinline__ void attn_add_not_finite(const AttentionParams& p, const AttnSegmentOf<WINDOW>& seg,
+                                                    const AttnRowOf<WINDOW>& row, const AttnList<WINDOW>& list, int column,
+                                                    float (&o)[COLUMNS])
 {
 #pragma unroll 1
-    for (int i = 0; i < 12; ++i)
+    for (int i = 0; i < 4 * AttnSegmentOf<WINDOW>::kMixed; ++i)
 #pragma unroll 1
         for (uint32_t w = list[i / 4][i % 4]; w != 0; w &= w - 1) {
-            const int key = (seg.tiles - 1 - i / 4) * kAttnKeys + 32 * (i % 4) + __ffs(w) - 1;
+            const int key = seg.key_of(seg.tile_of(i / 4)) + 32 * (i % 4) + __ffs(w) - 1;
             if (!row.sees(key))
                 continue;
             const long long at = cache_row(p.batch, seg.b, key, seg.head);
@@ -669,14 +807,17 @@ __device__ __forceinline__ void attn_add_not_finite(const AttentionParams& p, co
 // The same for keys of tiles that all rows of the segment see, which the products take as they are: infinity times a weight of zero,
 // another copy's key or one too small for fp16, has made NaN of the sums there.  Bits of columns `column` on that have a positive
 // infinity or NaN among these keys, and a negative infinity or NaN; for a whole warp.
-template<int HEAD_DIM, int COLUMNS>
-__device__ __forceinline__ uint2 attn_seen_not_finite(const AttentionParams& p, const AttnSegment& seg, int column)
+template<int HEAD_DIM, int COLUMNS, bool WINDOW>
+__device__ __forceinline__ uint2 attn_seen_not_finite(const AttentionParams& p, const AttnSegmentOf<WINDOW>& seg, int column)
 {
     uint2     found = make_uint2(0u, 0u);
-    const int end   = min(seg.end, seg.open[0] / kAttnKeys) * kAttnKeys;
+    const int end   = (WINDOW ? seg.end : min(seg.end, seg.open[0] / kAttnKeys)) * kAttnKeys;
 #pragma unroll 4
-    for (int key = seg.begin * kAttnKeys + (threadIdx.x & 31); key < end; key += 32) {
-        const long long at = cache_row(p.batch, seg.b, key, seg.head);
+    for (int place = seg.begin * kAttnKeys + (threadIdx.x & 31); place < end; place += 32) {
+        if (WINDOW && seg.mixed(place / kAttnKeys))
+            continue;
+        const int       key = seg.key_of(place / kAttnKeys) + place % kAttnKeys;
+        const long long at  = cache_row(p.batch, seg.b, key, seg.head);
         if (at < 0)
             continue;
         const half* v   = p.v_cache + at * HEAD_DIM + column;
@@ -707,9 +848,10 @@ struct AttnSums {
 
 // A row's sums of columns `column` on, put right where values are not finite; for a whole warp.  A row whose weights have no finite
 // sum stays without a number.
-template<int HEAD_DIM, int COLUMNS>
-__device__ __forceinline__ AttnSums<COLUMNS> attn_restore(const AttentionParams& p, const AttnSegment& seg, const AttnRow& row,
-                                                          const uint32_t (&list)[3][4], bool listed, float sum, int column,
+template<int HEAD_DIM, int COLUMNS, bool WINDOW>
+__device__ __forceinline__ AttnSums<COLUMNS> attn_restore(const AttentionParams& p, const AttnSegmentOf<WINDOW>& seg,
+                                                          const AttnRowOf<WINDOW>& row, const AttnList<WINDOW>& list, bool listed,
+                                                          float sum, int column,
                                                           AttnSums<COLUMNS> sums)
 {
     bool nan = false;
@@ -755,9 +897,9 @@ struct AttnOutputs {
 // The end of a segment for a warp with an output that is not finite, or may not be: its rows (`out` of a whole item's, or `sums` of a
 // part's; neither for a lane without a row) are written anew.  Code of its own, out of the way of the usual ends: in their midst it
 // cost ragged prompts 2 us of 55.
-template<int HEAD_DIM>
-__device__ __noinline__ void attn_end_carefully(const AttentionParams& p, const AttnSegment& seg, const AttnRow row,
-                                                const uint32_t (&list)[3][4], bool listed, AttnOutputs outputs, float sum, int column0,
+template<int HEAD_DIM, bool WINDOW>
+__device__ __noinline__ void attn_end_carefully(const AttentionParams& p, const AttnSegmentOf<WINDOW>& seg, const AttnRowOf<WINDOW> row,
+                                                const AttnList<WINDOW>& list, bool listed, AttnOutputs outputs, float sum, int column0,
                                                 int column1, half* out, float4* sums)
 {
     const float inverse = sum == 0.0f ? 0.0f : 1.0f / sum;
@@ -783,9 +925,10 @@ __device__ __noinline__ void attn_end_carefully(const AttentionParams& p, const 
 }
 
 // ... of 4 columns of rows that lie in the tile four times, added up already.
-template<int HEAD_DIM>
-__device__ __noinline__ AttnSums<4> attn_restore_four(const AttentionParams& p, const AttnSegment& seg, const AttnRow row,
-                                                      const uint32_t (&list)[3][4], bool listed, float sum, int column, AttnSums<4> sums)
+template<int HEAD_DIM, bool WINDOW>
+__device__ __noinline__ AttnSums<4> attn_restore_four(const AttentionParams& p, const AttnSegmentOf<WINDOW>& seg,
+                                                      const AttnRowOf<WINDOW> row, const AttnList<WINDOW>& list, bool listed, float sum,
+                                                      int column, AttnSums<4> sums)
 {
     return attn_restore<HEAD_DIM, 4>(p, seg, row, list, listed, sum, column, sums);
 }
@@ -894,8 +1037,8 @@ __device__ __forceinline__ void attn_transform(const AttnState& st, float (&s)[3
 }
 
 // Minus infinity for the keys, from `key0` on, that the row does not see.
-template<int COLUMNS>
-__device__ __forceinline__ void attn_mask(const AttnRow& row, float (&s)[COLUMNS], int key0)
+template<int COLUMNS, bool WINDOW>
+__device__ __forceinline__ void attn_mask(const AttnRowOf<WINDOW>& row, float (&s)[COLUMNS], int key0)
 {
 #pragma unroll
     for (int k = 0; k < COLUMNS / 32; ++k) {
@@ -981,7 +1124,7 @@ __device__ __forceinline__ float attn_minus(const AttnState& st)
 }
 
 // Plain scores of one row in tensor memory, 128 of them, to weights there; their sum.  For a whole warp.
-__device__ __noinline__ float attn_far_weights(uint32_t s_tmem, float top, float factor)
+inline __device__ __noinline__ float attn_far_weights(uint32_t s_tmem, float top, float factor)
 {
     const float minus = top == -CUDART_INF_F ? 0.0f : -top;
     float2      part  = make_float2(0.0f, 0.0f);
@@ -1006,13 +1149,12 @@ __device__ __noinline__ float attn_far_weights(uint32_t s_tmem, float top, float
 }
 
 // One tile of scores of one row, from tensor memory to weights there: all 128 of them, or, where the row lies in the tile four
-// times, the 32 from `column` on and zeros for the others.  The tile's first key is `key0`; keys before `open` are seen by all
-// rows.  `part_done(half)` tells that the weights of that half of the tile are in place.
-template<bool PLAIN, bool FOURFOLD, typename Rescale, typename PartDone>
-__device__ __forceinline__ void attn_softmax(AttnState& st, const AttnRow& row, uint32_t s_tmem, int column, int key0, int open,
-                                             bool first, Rescale&& rescale, PartDone&& part_done)
+// times, the 32 from `column` on and zeros for the others.  The tile's first key is `key0`; `masked` unless all rows see all of
+// it, as keys before `open` are seen.  `part_done(half)` tells that the weights of that half of the tile are in place.
+template<bool PLAIN, bool FOURFOLD, bool WINDOW, typename Rescale, typename PartDone>
+__device__ __forceinline__ void attn_softmax(AttnState& st, const AttnRowOf<WINDOW>& row, uint32_t s_tmem, int column, int key0, int open,
+                                             bool masked, bool first, Rescale&& rescale, PartDone&& part_done)
 {
-    const bool masked  = key0 + kAttnKeys > open;
     float2     part[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
     auto       stored  = [&]() {
         ptx::tmem_wait_st();
@@ -1109,7 +1251,7 @@ __device__ __forceinline__ void attn_softmax(AttnState& st, const AttnRow& row, 
 }
 
 // PLAIN: neither cap nor slopes.
-template<int HEAD_DIM, bool PLAIN>
+template<int HEAD_DIM, bool PLAIN, bool WINDOW = false>
 __global__ void __launch_bounds__(kAttnThreads, 1)
 attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_q_few,
                  const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
@@ -1125,7 +1267,7 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
     const uint32_t base = (raw + 1023u) & ~1023u;
     unsigned char* const smem = smem_raw + (base - raw);
     const uint32_t       q_base = base, k_base = base + 2 * kTileBytes, v_base = k_base + kStages * kTileBytes;
-    AttnShared&          sh     = *reinterpret_cast<AttnShared*>(smem + (2 + 2 * kStages) * kTileBytes);
+    AttnSharedOf<WINDOW>& sh    = *reinterpret_cast<AttnSharedOf<WINDOW>*>(smem + (2 + 2 * kStages) * kTileBytes);
     unsigned int* const  status = p.batch.status;
     const int            warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
@@ -1183,12 +1325,12 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
         AttnPart* const parts = reinterpret_cast<AttnPart*>(p.workspace) + 2 * blockIdx.x;
         bool            ok = true, written[2] = {false, false};
         for (int number = 0;; ++number) {
-            const AttnSegment* const current = attn_segment(sh, number, status);
+            const AttnSegmentOf<WINDOW>* const current = attn_segment(sh, number, status);
             // All or none: the barriers below count every thread of the two groups.
             if (ptx::named_barrier_any(1, 256, current == nullptr || !ok))
                 break;
             ptx::tc_fence_after_sync();
-            const AttnSegment& seg     = *current;
+            const AttnSegmentOf<WINDOW>& seg = *current;
             const bool         pair = seg.pair, fourfold = seg.fourfold;
             const int          in_tile = fourfold ? lane : thread, tile0 = pair ? group * p.tile_rows : 0;
             const int          row_id  = seg.row0 + tile0 + in_tile;  // of the sequence
@@ -1198,7 +1340,7 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
             const int          token   = valid ? attn_token(p, row_id) : 0;
             const int          head    = seg.head * p.share + (valid ? row_id - token * p.share : 0);
             const long long    in_row  = static_cast<long long>(head) * HEAD_DIM;
-            const AttnRow      row     = attn_row(p, seg, row_id, valid);
+            const AttnRowOf<WINDOW> row = attn_row(p, seg, row_id, valid);
             const int open  = seg.open[group];
             const int tiles = seg.count_of(group);
             AttnState st{};
@@ -1245,7 +1387,8 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
             };
             const int key_begin = seg.tile(group, 0) * kAttnKeys, key_step = (pair ? 1 : 2) * kAttnKeys;
             for (int i = 0; i < tiles; ++i) {
-                const int key0 = key_begin + i * key_step;
+                const int  key0   = WINDOW ? seg.key_of(seg.tile(group, i)) : key_begin + i * key_step;
+                const bool masked = WINDOW ? seg.masked(key0, group) : key0 + kAttnKeys > open;
                 ok             = attn_wait(&sh.s_full[group], s_parity, sh, status) && ok;
                 s_parity ^= 1u;
                 if (!__all_sync(0xffffffffu, ok)) {
@@ -1254,9 +1397,9 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
                 }
                 ptx::tc_fence_after_sync();
                 if (busy && !fourfold)
-                    attn_softmax<PLAIN, false>(st, row, s_tmem, 0, key0, open, i == 0, rescale, part_done);
+                    attn_softmax<PLAIN, false>(st, row, s_tmem, 0, key0, open, masked, i == 0, rescale, part_done);
                 else if (fourfold)
-                    attn_softmax<PLAIN, true>(st, row, s_tmem, thread & ~31, key0, open, i == 0, rescale, part_done);
+                    attn_softmax<PLAIN, true>(st, row, s_tmem, thread & ~31, key0, open, masked, i == 0, rescale, part_done);
                 else {
                     part_done(0);
                     part_done(1);
@@ -1302,7 +1445,7 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
             const long long to       = static_cast<long long>(seg.first + token) * p.heads * HEAD_DIM + in_row;
             float4* const   sums     = reinterpret_cast<float4*>(p.workspace + attn_sums_offset(gridDim.x))
                                  + (static_cast<size_t>(2 * blockIdx.x + slot) * 2 + tile_row) * (HEAD_DIM / 4) * kAttnRows;
-            const uint32_t(&list)[3][4] = sh.not_finite[number % kAttnSegments];
+            const AttnList<WINDOW>& list = sh.not_finite[number % kAttnSegments];
             const float inverse         = st.sum == 0.0f ? 0.0f : 1.0f / st.sum;
             const bool  any             = sh.any_not_finite[number % kAttnSegments] != 0;
             // An accumulator that no product has written may hold anything: this group's without a tile of its own, where the groups
@@ -1479,7 +1622,7 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
                    || __all_sync(0xffffffffu, attn_wait_longer(bar, parity, &sh.abort_flag, status)) != 0;
         };
         auto stage_of = [&](int group, int i) { return loaded + static_cast<uint32_t>(pair ? i : group + 2 * i); };
-        const AttnSegment* current = nullptr;
+        const AttnSegmentOf<WINDOW>* current = nullptr;
 #pragma unroll 1
         for (int number = 0; ok; ++number) {
             current = attn_segment(sh, number, status);
@@ -1556,8 +1699,8 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
         const int         piece    = lane / kBlocks, block = lane % kBlocks;
         const bool        active   = piece < pieces;
         const uint32_t    offset   = block * kBlock + piece * box * 128;
-        AttnCursor        cursor(attn_start(p, sh));
-        const AttnSegment& seg     = cursor.seg;
+        AttnCursorOf<WINDOW> cursor(attn_start(p, sh));
+        const AttnSegmentOf<WINDOW>& seg = cursor.seg;
         uint32_t          n        = 0;
         bool              ok       = true;
         for (int number = 0; ok; ++number) {
@@ -1570,7 +1713,7 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
                 break;
             const int* table = c.page_table + static_cast<long long>(seg.b) * c.table_width;
             for (int t = seg.begin; ok && t < seg.end; ++t, ++n) {
-                const int key   = t * kAttnKeys + piece * box;
+                const int key   = seg.key_of(t) + piece * box;
                 int       z     = c.pages * c.kv_heads;  // behind the cache: reads as zeros
                 if (active && key < seg.keys) {
                     const int id = table[key >> c.page_shift];
@@ -1603,16 +1746,15 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
         uint32_t  n           = 0, q_parity[2] = {1, 1};
         bool      ok          = true;
         for (int number = 0;; ++number) {
-            const AttnSegment* const current = attn_segment(sh, number, status);
-            uint32_t(&list)[3][4] = sh.not_finite[number % kAttnSegments];
-            if (t64 < 12)
+            const AttnSegmentOf<WINDOW>* const current = attn_segment(sh, number, status);
+            AttnList<WINDOW>& list = sh.not_finite[number % kAttnSegments];
+            if (t64 < 4 * AttnSegmentOf<WINDOW>::kMixed)
                 (&list[0][0])[t64] = 0u;
             if (t64 == 0)
                 sh.any_not_finite[number % kAttnSegments] = 0u;
             if (ptx::named_barrier_any(4, 64, current == nullptr || !ok))  // all or none
                 break;
-            const AttnSegment& seg  = *current;
-            const int          open = seg.open[0];
+            const AttnSegmentOf<WINDOW>& seg = *current;
             if (t64 == 0) {
                 const CUtensorMap* map   = seg.fourfold ? &map_q_few : &map_q;
                 const int          bytes = (seg.fourfold ? 4 * p.few_rows : p.tile_rows) * HEAD_DIM * 2;
@@ -1638,10 +1780,11 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
                 ok                   = ok && attn_wait(&sh.v_full[stage], n / kStages & 1u, sh, status);
                 if (!ok)  // nor without the rows of Q: those of the next segment would be taken for them
                     break;
-                if ((t + 1) * kAttnKeys > open) {
+                if (seg.mixed(t)) {
+                    const int key0 = seg.key_of(t), mixed = seg.mixed_of(t);
 #pragma unroll 1
                     for (int r = t64; r < kAttnKeys; r += 64) {
-                        const int key = t * kAttnKeys + r;
+                        const int key = key0 + r;
                         uint4*    v   = reinterpret_cast<uint4*>(smem + (2 + kStages) * kTileBytes + stage * kTileBytes + r * 128);
                         bool      bad = false;
 #pragma unroll 2
@@ -1658,8 +1801,8 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
                                 at = make_uint4(clean(w.x), clean(w.y), clean(w.z), clean(w.w));
                             }
                         }
-                        if (bad && seg.tiles - 1 - t < 3) {
-                            atomicOr(&list[seg.tiles - 1 - t][r / 32], 1u << r % 32);
+                        if (bad && mixed < AttnSegmentOf<WINDOW>::kMixed) {
+                            atomicOr(&list[mixed][r / 32], 1u << r % 32);
                             sh.any_not_finite[number % kAttnSegments] = 1u;
                         }
                     }

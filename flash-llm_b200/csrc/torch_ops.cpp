@@ -1,5 +1,5 @@
-// CUDA implementations of torch.ops.flashllm.{spmm, spmm_epilogue, encode, rotary_append, tree_attention, prompt_attention,
-// cache_accept} (schemas, shape inference and the refusals for other devices are registered by torch_op.py).  Checks, result allocation and the call into libSpMM_API.so run here
+// CUDA implementations of torch.ops.flashllm.{spmm, spmm_epilogue, encode, rotary_append, norm_rotary_append, tree_attention,
+// prompt_attention, window_attention, cache_accept, four_bit_append, four_bit_attention, four_bit_read} (schemas, shape inference and the refusals for other devices are registered by torch_op.py).  Checks, result allocation and the call into libSpMM_API.so run here
 // because a decode step is launch-bound: from Python the same work took 18-22 us per call, four times the kernel.
 //
 // The library's entry points are handed over as addresses (flashllm_torch_bind), so that the operators call whichever
@@ -31,6 +31,11 @@ decltype(&FlashLLM_TreeAttention)             g_tree            = nullptr;
 decltype(&FlashLLM_PromptAttention)           g_prompt          = nullptr;
 decltype(&FlashLLM_CacheAccept)               g_accept          = nullptr;
 decltype(&FlashLLM_Attention_WorkspaceBytes)  g_workspace_bytes = nullptr;
+decltype(&FlashLLM_NormRotaryAppend)          g_norm_rotary     = nullptr;
+decltype(&FlashLLM_WindowAttention)           g_window          = nullptr;
+decltype(&FlashLLM_FourBitAppend)             g_four_append     = nullptr;
+decltype(&FlashLLM_FourBitAttention)          g_four_attention  = nullptr;
+decltype(&FlashLLM_FourBitRead)               g_four_read       = nullptr;
 
 SpmmFn        g_spmm         = nullptr;
 TileOffsetsFn g_tile_offsets = nullptr;
@@ -148,14 +153,15 @@ int as_int(int64_t value)
 }
 
 Paged paged(const at::Tensor& k_cache, const at::Tensor& v_cache, const at::Tensor& cu_tokens, const at::Tensor& context,
-            const at::Tensor& page_table, bool may_have_layers = false)
+            const at::Tensor& page_table, bool may_have_layers = false, bool four_bit = false)
 {
     TORCH_CHECK(k_cache.is_cuda(), "the flashllm cache operators run on CUDA tensors only");
     const bool layers = may_have_layers && k_cache.dim() == 5;
-    TORCH_CHECK(k_cache.scalar_type() == at::kHalf && k_cache.is_contiguous() && (k_cache.dim() == 4 || layers),
-                "k_cache must be a contiguous fp16 tensor [pages][kv_heads][page_size][head_dim]",
+    TORCH_CHECK(k_cache.scalar_type() == (four_bit ? at::kByte : at::kHalf) && k_cache.is_contiguous() && (k_cache.dim() == 4 || layers),
+                "k_cache must be a contiguous ",
+                four_bit ? "uint8 tensor [pages][kv_heads][page_size][head_dim * 9 / 16]" : "fp16 tensor [pages][kv_heads][page_size][head_dim]",
                 may_have_layers ? ", with or without a leading [layers]" : "");
-    TORCH_CHECK(v_cache.scalar_type() == at::kHalf && v_cache.is_contiguous() && v_cache.sizes() == k_cache.sizes()
+    TORCH_CHECK(v_cache.scalar_type() == k_cache.scalar_type() && v_cache.is_contiguous() && v_cache.sizes() == k_cache.sizes()
                     && v_cache.device() == k_cache.device(),
                 "v_cache must be laid out like k_cache");
     Paged     p{};
@@ -165,6 +171,11 @@ Paged paged(const at::Tensor& k_cache, const at::Tensor& v_cache, const at::Tens
     p.kv_heads  = as_int(k_cache.size(d + 1));
     p.page_size = as_int(k_cache.size(d + 2));
     p.head_dim  = as_int(k_cache.size(d + 3));
+    if (four_bit) {
+        TORCH_CHECK(p.head_dim == 36 || p.head_dim == 72, "the last dimension of a cache of 4 bits (", p.head_dim,
+                    ") must be 36 or 72: 9 / 16 of a head_dim of 64 or 128");
+        p.head_dim = p.head_dim / 9 * 16;
+    }
     TORCH_CHECK(p.head_dim == 64 || p.head_dim == 128, "head_dim (", p.head_dim, ") must be 64 or 128");
     TORCH_CHECK(p.page_size >= 16 && (p.page_size & (p.page_size - 1)) == 0, "page_size (", p.page_size,
                 ") must be a power of two of at least 16");
@@ -201,14 +212,13 @@ int row_length(const at::Tensor& t, const at::Device& device, const char* name)
                         code);
 }
 
-at::Tensor rotary_append(const at::Tensor& qkv, const at::Tensor& k_cache, const at::Tensor& v_cache, const at::Tensor& cu_tokens,
-                         const at::Tensor& context, const at::Tensor& page_table, const std::optional<at::Tensor>& frequencies,
-                         bool interleaved, double magnitude, const std::optional<at::Tensor>& positions)
+// What the appends share; `call` is handed (stream, ld_qkv, q, ld_q, tokens, heads, frequencies, rotary_dim, positions).
+template<typename Call>
+at::Tensor append(const char* what, const at::Tensor& qkv, const Paged& p, const at::Device& device,
+                  const std::optional<at::Tensor>& frequencies, const std::optional<at::Tensor>& positions, Call&& call)
 {
-    const Paged      p      = paged(k_cache, v_cache, cu_tokens, context, page_table);
-    const at::Device device = k_cache.device();
-    const int        ld     = row_length(qkv, device, "qkv");
-    const int64_t    tokens = qkv.size(0), heads = qkv.size(1) / p.head_dim - 2 * static_cast<int64_t>(p.kv_heads);
+    const int     ld     = row_length(qkv, device, "qkv");
+    const int64_t tokens = qkv.size(0), heads = qkv.size(1) / p.head_dim - 2 * static_cast<int64_t>(p.kv_heads);
     TORCH_CHECK(qkv.size(1) % p.head_dim == 0 && heads >= 1, "qkv must hold query heads and ", p.kv_heads,
                 " key and value heads of ", p.head_dim, " each, but has ", qkv.size(1), " columns");
     const bool turned = frequencies.has_value() && frequencies->defined() && frequencies->numel() > 0;
@@ -223,18 +233,94 @@ at::Tensor rotary_append(const at::Tensor& qkv, const at::Tensor& k_cache, const
     const at::Tensor           q    = at::empty({tokens, heads * p.head_dim}, qkv.options());
     if (tokens == 0 || p.sequences == 0)
         return q;
-    const int code = g_rotary(c10::cuda::getCurrentCUDAStream().stream(), qkv.const_data_ptr(), ld, q.mutable_data_ptr(),
-                              as_int(q.size(1)), k_cache.mutable_data_ptr(), v_cache.mutable_data_ptr(), p.pages, p.page_size,
-                              p.cu_tokens, p.context, p.page_table, p.table_width, p.sequences, as_int(tokens), as_int(heads),
-                              p.kv_heads, p.head_dim, turned ? static_cast<const double*>(frequencies->const_data_ptr()) : nullptr,
-                              turned ? as_int(2 * frequencies->size(0)) : 0, interleaved, static_cast<float>(magnitude),
-                              has_positions ? int_array(*positions, 1, device, "positions") : nullptr);
+    const int code = call(c10::cuda::getCurrentCUDAStream().stream(), ld, q.mutable_data_ptr(), as_int(q.size(1)), as_int(tokens),
+                          as_int(heads), turned ? static_cast<const double*>(frequencies->const_data_ptr()) : nullptr,
+                          turned ? as_int(2 * frequencies->size(0)) : 0,
+                          has_positions ? int_array(*positions, 1, device, "positions") : nullptr);
     if (code != 0)
-        raise_paged("RotaryAppend", p, tokens, heads, code);
+        raise_paged(what, p, tokens, heads, code);
     return q;
 }
 
-// What the two attention operators share; `call` is handed (workspace, out, ld_q, tokens, heads, scale, slopes).
+at::Tensor rotary_append(const at::Tensor& qkv, const at::Tensor& k_cache, const at::Tensor& v_cache, const at::Tensor& cu_tokens,
+                         const at::Tensor& context, const at::Tensor& page_table, const std::optional<at::Tensor>& frequencies,
+                         bool interleaved, double magnitude, const std::optional<at::Tensor>& positions)
+{
+    const Paged p = paged(k_cache, v_cache, cu_tokens, context, page_table);
+    return append("RotaryAppend", qkv, p, k_cache.device(), frequencies, positions,
+                  [&](void* stream, int ld, void* q, int ld_q, int tokens, int heads, const double* angles, int rotary_dim, const int* place) {
+                      return g_rotary(stream, qkv.const_data_ptr(), ld, q, ld_q, k_cache.mutable_data_ptr(), v_cache.mutable_data_ptr(),
+                                      p.pages, p.page_size, p.cu_tokens, p.context, p.page_table, p.table_width, p.sequences, tokens,
+                                      heads, p.kv_heads, p.head_dim, angles, rotary_dim, interleaved, static_cast<float>(magnitude), place);
+                  });
+}
+
+// A norm's weights, or nullptr for none.
+const void* norm_weights(const std::optional<at::Tensor>& t, const Paged& p, const at::Device& device, const char* name)
+{
+    if (!t.has_value() || !t->defined())
+        return nullptr;
+    TORCH_CHECK(t->scalar_type() == at::kHalf && t->dim() == 1 && t->size(0) == p.head_dim && t->is_contiguous() && t->device() == device,
+                name, " must be a contiguous fp16 tensor of ", p.head_dim, " weights on the cache's device");
+    return t->const_data_ptr();
+}
+
+at::Tensor norm_rotary_append(const at::Tensor& qkv, const at::Tensor& k_cache, const at::Tensor& v_cache, const at::Tensor& cu_tokens,
+                              const at::Tensor& context, const at::Tensor& page_table, const at::Tensor& q_norm,
+                              const at::Tensor& k_norm, double eps, const std::optional<at::Tensor>& frequencies, bool interleaved,
+                              double magnitude, const std::optional<at::Tensor>& positions)
+{
+    const Paged       p  = paged(k_cache, v_cache, cu_tokens, context, page_table);
+    const void* const wq = norm_weights(q_norm, p, k_cache.device(), "q_norm");
+    const void* const wk = norm_weights(k_norm, p, k_cache.device(), "k_norm");
+    TORCH_CHECK(eps >= 0 && std::isfinite(static_cast<float>(eps)), "eps must not be negative, and finite");
+    return append("NormRotaryAppend", qkv, p, k_cache.device(), frequencies, positions,
+                  [&](void* stream, int ld, void* q, int ld_q, int tokens, int heads, const double* angles, int rotary_dim, const int* place) {
+                      return g_norm_rotary(stream, qkv.const_data_ptr(), ld, q, ld_q, k_cache.mutable_data_ptr(),
+                                           v_cache.mutable_data_ptr(), p.pages, p.page_size, p.cu_tokens, p.context, p.page_table,
+                                           p.table_width, p.sequences, tokens, heads, p.kv_heads, p.head_dim, angles, rotary_dim,
+                                           interleaved, static_cast<float>(magnitude), place, wq, wk, static_cast<float>(eps));
+                  });
+}
+
+at::Tensor four_bit_append(const at::Tensor& qkv, const at::Tensor& k_cache, const at::Tensor& v_cache, const at::Tensor& cu_tokens,
+                           const at::Tensor& context, const at::Tensor& page_table, const std::optional<at::Tensor>& q_norm,
+                           const std::optional<at::Tensor>& k_norm, double eps, const std::optional<at::Tensor>& frequencies,
+                           bool interleaved, double magnitude, const std::optional<at::Tensor>& positions)
+{
+    const Paged       p  = paged(k_cache, v_cache, cu_tokens, context, page_table, false, true);
+    const void* const wq = norm_weights(q_norm, p, k_cache.device(), "q_norm");
+    const void* const wk = norm_weights(k_norm, p, k_cache.device(), "k_norm");
+    TORCH_CHECK(eps >= 0 && std::isfinite(static_cast<float>(eps)), "eps must not be negative, and finite");
+    return append("FourBitAppend", qkv, p, k_cache.device(), frequencies, positions,
+                  [&](void* stream, int ld, void* q, int ld_q, int tokens, int heads, const double* angles, int rotary_dim, const int* place) {
+                      return g_four_append(stream, qkv.const_data_ptr(), ld, q, ld_q, k_cache.mutable_data_ptr(),
+                                           v_cache.mutable_data_ptr(), p.pages, p.page_size, p.cu_tokens, p.context, p.page_table,
+                                           p.table_width, p.sequences, tokens, heads, p.kv_heads, p.head_dim, angles, rotary_dim,
+                                           interleaved, static_cast<float>(magnitude), place, wq, wk, static_cast<float>(eps));
+                  });
+}
+
+std::tuple<at::Tensor, at::Tensor> four_bit_read(const at::Tensor& k_cache, const at::Tensor& v_cache, const at::Tensor& cu_tokens,
+                                                 const at::Tensor& context, const at::Tensor& page_table, int64_t tokens)
+{
+    const Paged p = paged(k_cache, v_cache, cu_tokens, context, page_table, false, true);
+    TORCH_CHECK(tokens >= 0, "tokens (", tokens, ") must not be negative");
+    const c10::cuda::CUDAGuard guard(k_cache.device());
+    const auto                 options = k_cache.options().dtype(at::kHalf);
+    const int64_t              width   = static_cast<int64_t>(p.kv_heads) * p.head_dim;
+    const at::Tensor           k = at::empty({tokens, width}, options), v = at::empty({tokens, width}, options);
+    if (tokens == 0 || p.sequences == 0)
+        return {k, v};
+    const int code = g_four_read(c10::cuda::getCurrentCUDAStream().stream(), k_cache.const_data_ptr(), v_cache.const_data_ptr(), p.pages,
+                                 p.page_size, p.cu_tokens, p.context, p.page_table, p.table_width, p.sequences, as_int(tokens), p.kv_heads,
+                                 p.head_dim, k.mutable_data_ptr(), v.mutable_data_ptr());
+    if (code != 0)
+        raise_paged("FourBitRead", p, tokens, p.kv_heads, code);
+    return {k, v};
+}
+
+// What the attention operators share; `call` is handed (workspace, out, ld_q, tokens, heads, scale, slopes).
 template<typename Call>
 at::Tensor attention(const char* what, const at::Tensor& q, const Paged& p, const at::Device& device, std::optional<double> scale,
                      double cap, const std::optional<at::Tensor>& slopes, Call&& call)
@@ -308,6 +394,37 @@ at::Tensor prompt_attention(const at::Tensor& q, const at::Tensor& k_cache, cons
                      });
 }
 
+at::Tensor window_attention(const at::Tensor& q, const at::Tensor& k_cache, const at::Tensor& v_cache, const at::Tensor& cu_tokens,
+                            const at::Tensor& context, const at::Tensor& page_table, int64_t window, int64_t sinks,
+                            std::optional<double> scale, double cap, const std::optional<at::Tensor>& slopes)
+{
+    const Paged p = paged(k_cache, v_cache, cu_tokens, context, page_table);
+    TORCH_CHECK(window >= 1 && sinks >= 0, "window (", window, ") must be at least 1 and sinks (", sinks, ") not negative");
+    const int near = as_int(window), first = as_int(sinks);
+    return attention("WindowAttention", q, p, k_cache.device(), scale, cap, slopes,
+                     [&](void* stream, int ld, int tokens, int heads, float factor, const float* slope, void* out, void* workspace) {
+                         return g_window(stream, q.const_data_ptr(), ld, k_cache.const_data_ptr(), v_cache.const_data_ptr(), p.pages,
+                                         p.page_size, p.cu_tokens, p.context, p.page_table, p.table_width, p.sequences, tokens, heads,
+                                         p.kv_heads, p.head_dim, near, first, factor, static_cast<float>(cap), slope, out, workspace);
+                     });
+}
+
+at::Tensor four_bit_attention(const at::Tensor& q, const at::Tensor& k_cache, const at::Tensor& v_cache, const at::Tensor& cu_tokens,
+                              const at::Tensor& context, const at::Tensor& page_table, int64_t window, int64_t sinks,
+                              std::optional<double> scale, double cap, const std::optional<at::Tensor>& slopes)
+{
+    const Paged p = paged(k_cache, v_cache, cu_tokens, context, page_table, false, true);
+    TORCH_CHECK(window >= 0 && sinks >= 0, "window (", window, ") and sinks (", sinks, ") must not be negative");
+    const int near = as_int(window), first = as_int(sinks);
+    return attention("FourBitAttention", q, p, k_cache.device(), scale, cap, slopes,
+                     [&](void* stream, int ld, int tokens, int heads, float factor, const float* slope, void* out, void* workspace) {
+                         return g_four_attention(stream, q.const_data_ptr(), ld, k_cache.const_data_ptr(), v_cache.const_data_ptr(),
+                                                 p.pages, p.page_size, p.cu_tokens, p.context, p.page_table, p.table_width, p.sequences,
+                                                 tokens, heads, p.kv_heads, p.head_dim, near, first, factor, static_cast<float>(cap),
+                                                 slope, out, workspace);
+                     });
+}
+
 void cache_accept(const at::Tensor& k_cache, const at::Tensor& v_cache, const at::Tensor& cu_tokens, const at::Tensor& context,
                   const at::Tensor& page_table, const at::Tensor& accepted, const at::Tensor& accepted_lengths)
 {
@@ -331,8 +448,14 @@ void cache_accept(const at::Tensor& k_cache, const at::Tensor& v_cache, const at
 }  // namespace
 
 extern "C" void flashllm_torch_bind(void* spmm_fn, void* tile_offsets_fn, void* pack_fn, void* rotary_fn, void* tree_fn,
-                                    void* prompt_fn, void* accept_fn, void* workspace_bytes_fn, PyObject* error_class)
+                                    void* prompt_fn, void* accept_fn, void* workspace_bytes_fn, void* norm_rotary_fn, void* window_fn,
+                                    void* four_append_fn, void* four_attention_fn, void* four_read_fn, PyObject* error_class)
 {
+    g_norm_rotary     = reinterpret_cast<decltype(g_norm_rotary)>(norm_rotary_fn);
+    g_window          = reinterpret_cast<decltype(g_window)>(window_fn);
+    g_four_append     = reinterpret_cast<decltype(g_four_append)>(four_append_fn);
+    g_four_attention  = reinterpret_cast<decltype(g_four_attention)>(four_attention_fn);
+    g_four_read       = reinterpret_cast<decltype(g_four_read)>(four_read_fn);
     g_rotary          = reinterpret_cast<decltype(g_rotary)>(rotary_fn);
     g_tree            = reinterpret_cast<decltype(g_tree)>(tree_fn);
     g_prompt          = reinterpret_cast<decltype(g_prompt)>(prompt_fn);
@@ -353,4 +476,9 @@ TORCH_LIBRARY_IMPL(flashllm, CUDA, m)
     m.impl("tree_attention", &tree_attention);
     m.impl("prompt_attention", &prompt_attention);
     m.impl("cache_accept", &cache_accept);
+    m.impl("norm_rotary_append", &norm_rotary_append);
+    m.impl("window_attention", &window_attention);
+    m.impl("four_bit_append", &four_bit_append);
+    m.impl("four_bit_attention", &four_bit_attention);
+    m.impl("four_bit_read", &four_bit_read);
 }

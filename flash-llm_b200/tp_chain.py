@@ -126,7 +126,9 @@ class CachedAttention:
     rotary positions and the append of the batch's rows, then attention of drafted trees (`tree_mask`, with `positions` = depth +
     context for the angles and distances) or, without masks, of prompts and single tokens.  cu_tokens, context and page_table
     describe the batch (int32; see torch_op); the caller advances `context` between steps, and accepts a drafted path with
-    torch.ops.flashllm.cache_accept first.  `frequencies` None: no rotary positions."""
+    torch.ops.flashllm.cache_accept first.  `frequencies` None: no rotary positions.  `q_norm` and `k_norm`: queries and keys are
+    normed first.  `window`: prompts and single tokens see so many positions, and the first `sinks` (0: all).  A cache of uint8
+    `[pages][heads][page_size][head_dim * 9 / 16]` holds 4 bits an element; trees, which are accepted by moving rows, need 16."""
 
     k_cache: torch.Tensor
     v_cache: torch.Tensor
@@ -141,6 +143,11 @@ class CachedAttention:
     magnitude: float = 1.0
     cap: float = 0.0
     slopes: torch.Tensor | None = None
+    q_norm: torch.Tensor | None = None
+    k_norm: torch.Tensor | None = None
+    eps: float = 1e-6
+    window: int = 0
+    sinks: int = 0
 
     def __call__(self, y_qkv: torch.Tensor) -> torch.Tensor:
         if self.tree_mask is not None and self.frequencies is not None and self.positions is None:
@@ -148,12 +155,28 @@ class CachedAttention:
             raise ValueError("a drafted tree with rotary positions needs the positions of its tokens")
         if self.tree_mask is not None and self.prefix is not None:
             raise ValueError("a prefix is for prompts: a tree's masks say what its tokens see")
+        four_bit = self.k_cache.dtype == torch.uint8
+        if four_bit and (self.tree_mask is not None or self.prefix is not None):
+            raise ValueError("a cache of 4 bits is for prompts and single tokens, without a prefix")
+        if self.window and (self.tree_mask is not None or self.prefix is not None):
+            raise ValueError("a window is for prompts and single tokens, without a prefix")
+        if not four_bit and (self.q_norm is None) != (self.k_norm is None):
+            raise ValueError("a cache of 16 bits takes both norms or none")
         from . import torch_op  # noqa: F401  (registers torch.ops.flashllm)
         ops = torch.ops.flashllm
         batch = (self.k_cache, self.v_cache, self.cu_tokens, self.context, self.page_table)
-        q = ops.rotary_append(y_qkv, *batch, self.frequencies, self.interleaved, self.magnitude, self.positions)
+        rotary = (self.frequencies, self.interleaved, self.magnitude, self.positions)
+        if four_bit:
+            q = ops.four_bit_append(y_qkv, *batch, self.q_norm, self.k_norm, self.eps, *rotary)
+            return ops.four_bit_attention(q, *batch, self.window, self.sinks, None, self.cap, self.slopes)
+        if self.q_norm is not None:
+            q = ops.norm_rotary_append(y_qkv, *batch, self.q_norm, self.k_norm, self.eps, *rotary)
+        else:
+            q = ops.rotary_append(y_qkv, *batch, *rotary)
         if self.tree_mask is not None:
             return ops.tree_attention(q, *batch, self.tree_mask, None, self.cap, self.slopes, self.positions)
+        if self.window:
+            return ops.window_attention(q, *batch, self.window, self.sinks, None, self.cap, self.slopes)
         return ops.prompt_attention(q, *batch, self.prefix, None, self.cap, self.slopes)
 
 

@@ -412,8 +412,143 @@ int FlashLLM_PromptAttention(void*        stream,
                              void*        Out,
                              void*        workspace);
 
-/* Bytes of `workspace` for the two calls above on the current device; 0 for an unsupported head_dim. */
+/* Attention through a sliding window with sinks: as FlashLLM_PromptAttention without a prefix, but of the keys up to itself a row
+ * sees the last `window` (itself among them, at least 1) and the first `sinks` (0 or more) of its sequence.  Keys that no row
+ * sees are not read.  The same workspace. */
+int FlashLLM_WindowAttention(void*        stream,
+                             const void*  Q,
+                             int          ld_q,
+                             const void*  K_cache,
+                             const void*  V_cache,
+                             int          pages,
+                             int          page_size,
+                             const int*   cu_tokens,
+                             const int*   context,
+                             const int*   page_table,
+                             int          table_width,
+                             int          sequences,
+                             int          tokens,
+                             int          heads,
+                             int          kv_heads,
+                             int          head_dim,
+                             int          window,
+                             int          sinks,
+                             float        scale,
+                             float        cap,
+                             const float* slopes,
+                             void*        Out,
+                             void*        workspace);
+
+/* Bytes of `workspace` for each of the attention calls on the current device; 0 for an unsupported head_dim. */
 unsigned long long FlashLLM_Attention_WorkspaceBytes(int head_dim);
+
+/* FlashLLM_RotaryAppend with norms: each query and key head is y = x w / sqrt(mean(x^2) + eps) before it is turned (w: q_norm or
+ * k_norm, fp16 [head_dim] on 16-byte boundaries; eps >= 0), all in 32 bits, one rounding. */
+int FlashLLM_NormRotaryAppend(void*         stream,
+                              const void*   QKV,
+                              int           ld_qkv,
+                              void*         Q,
+                              int           ld_q,
+                              void*         K_cache,
+                              void*         V_cache,
+                              int           pages,
+                              int           page_size,
+                              const int*    cu_tokens,
+                              const int*    context,
+                              const int*    page_table,
+                              int           table_width,
+                              int           sequences,
+                              int           tokens,
+                              int           heads,
+                              int           kv_heads,
+                              int           head_dim,
+                              const double* frequencies,
+                              int           rotary_dim,
+                              int           interleaved,
+                              float         magnitude,
+                              const int*    positions,
+                              const void*   q_norm,
+                              const void*   k_norm,
+                              float         eps);
+
+/* A cache of 4 bits: K_cache and V_cache are bytes [pages][kv_heads][page_size * head_dim * 9 / 16] on 16-byte boundaries; pages,
+ * tables and batches are the same.  What a head keeps of a page begins with its codes [page_size][head_dim / 2], two to a byte, the
+ * even element in the low bits; behind them lie the scales [page_size][head_dim / 64][2] fp16, step and lowest value of 64 elements
+ * each.  An element is lowest + step * code: lowest = fp16(min), step = fp16((max - lowest) / 15), code = (x - lowest) / step to
+ * the nearest (0 where step is 0), from 32 bits; read as fp16 an element is at most 65504.  64 elements among which one is not finite, or beyond 65504, are all NaN.
+ * page_size is at most 2^24.
+ *
+ * FlashLLM_FourBitAppend is FlashLLM_NormRotaryAppend into such a cache; q_norm, k_norm or both may be nullptr (no norm). */
+int FlashLLM_FourBitAppend(void*         stream,
+                           const void*   QKV,
+                           int           ld_qkv,
+                           void*         Q,
+                           int           ld_q,
+                           void*         K_cache,
+                           void*         V_cache,
+                           int           pages,
+                           int           page_size,
+                           const int*    cu_tokens,
+                           const int*    context,
+                           const int*    page_table,
+                           int           table_width,
+                           int           sequences,
+                           int           tokens,
+                           int           heads,
+                           int           kv_heads,
+                           int           head_dim,
+                           const double* frequencies,
+                           int           rotary_dim,
+                           int           interleaved,
+                           float         magnitude,
+                           const int*    positions,
+                           const void*   q_norm,
+                           const void*   k_norm,
+                           float         eps);
+
+/* FlashLLM_WindowAttention over such a cache; window 0: none (and sinks do not matter). */
+int FlashLLM_FourBitAttention(void*        stream,
+                              const void*  Q,
+                              int          ld_q,
+                              const void*  K_cache,
+                              const void*  V_cache,
+                              int          pages,
+                              int          page_size,
+                              const int*   cu_tokens,
+                              const int*   context,
+                              const int*   page_table,
+                              int          table_width,
+                              int          sequences,
+                              int          tokens,
+                              int          heads,
+                              int          kv_heads,
+                              int          head_dim,
+                              int          window,
+                              int          sinks,
+                              float        scale,
+                              float        cap,
+                              const float* slopes,
+                              void*        Out,
+                              void*        workspace);
+
+/* The batch's rows (positions context[b] up to context[b] plus its rows of sequence b) from such a cache as fp16 [tokens][kv_heads *
+ * head_dim], one rounding: a sequence moves to a cache of 16 bits, or to another worker.  Rows of a sequence that does not fit, and
+ * of bad pages, are zero. */
+int FlashLLM_FourBitRead(void*       stream,
+                         const void* K_cache,
+                         const void* V_cache,
+                         int         pages,
+                         int         page_size,
+                         const int*  cu_tokens,
+                         const int*  context,
+                         const int*  page_table,
+                         int         table_width,
+                         int         sequences,
+                         int         tokens,
+                         int         kv_heads,
+                         int         head_dim,
+                         void*       K_out,
+                         void*       V_out);
 
 /* Accepts a path of a drafted tree: keys and values of sequence b's new token accepted[b * accepted_width + i] (its row in the
  * sequence) move to position context[b] + i, for i < accepted_lengths[b] (0 .. accepted_width, at most 64).  `layers` caches lie
