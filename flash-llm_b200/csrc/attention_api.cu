@@ -62,6 +62,10 @@ static cudaError_t multiprocessors(int* count)
         raise(attention_kernel<64, false, true>, attn_smem_bytes<true>(64));
         raise(attention_kernel<128, true, true>, attn_smem_bytes<true>(128));
         raise(attention_kernel<128, false, true>, attn_smem_bytes<true>(128));
+        raise(attention_kernel<64, true, true, true>, attn_smem_bytes<true>(64));
+        raise(attention_kernel<64, false, true, true>, attn_smem_bytes<true>(64));
+        raise(attention_kernel<128, true, true, true>, attn_smem_bytes<true>(128));
+        raise(attention_kernel<128, false, true, true>, attn_smem_bytes<true>(128));
         return err;
     });
 }
@@ -101,7 +105,7 @@ static bool encode_rows(CUtensorMap* map, const AttentionParams& p, int head_dim
 }
 
 template<int HEAD_DIM>
-static cudaError_t launch_attention(cudaStream_t stream, const AttentionParams& p)
+static cudaError_t launch_attention(cudaStream_t stream, const AttentionParams& p, bool four_bit = false)
 {
     int         sms = 0;
     cudaError_t err = multiprocessors(&sms);
@@ -109,10 +113,14 @@ static cudaError_t launch_attention(cudaStream_t stream, const AttentionParams& 
         return err;
     CUtensorMap map_q, map_q_few, map_k, map_v;
     if (!encode_rows(&map_q, p, HEAD_DIM, p.tile_rows) || !encode_rows(&map_q_few, p, HEAD_DIM, p.few_rows > 0 ? p.few_rows : p.tile_rows)
-        || !encode_cache(&map_k, p.k_cache, p.batch, HEAD_DIM) || !encode_cache(&map_v, p.v_cache, p.batch, HEAD_DIM))
+        || (!four_bit && (!encode_cache(&map_k, p.k_cache, p.batch, HEAD_DIM) || !encode_cache(&map_v, p.v_cache, p.batch, HEAD_DIM))))
         return cudaErrorInvalidValue;
     const bool plain = p.cap == 0.0f && p.slopes == nullptr;
-    if (p.window > 0)
+    if (four_bit)  // (its codes are read without tensor copies)
+        err = launch_in_stream_order(plain ? attention_kernel<HEAD_DIM, true, true, true> : attention_kernel<HEAD_DIM, false, true, true>,
+                                     dim3(sms), dim3(kAttnFourThreads), attn_smem_bytes<true>(HEAD_DIM), stream, 1, map_q, map_q_few,
+                                     map_q, map_q, p);
+    else if (p.window > 0)
         err = launch_in_stream_order(plain ? attention_kernel<HEAD_DIM, true, true> : attention_kernel<HEAD_DIM, false, true>, dim3(sms),
                                      dim3(kAttnThreads), attn_smem_bytes<true>(HEAD_DIM), stream, 1, map_q, map_q_few, map_k, map_v, p);
     else
@@ -121,6 +129,11 @@ static cudaError_t launch_attention(cudaStream_t stream, const AttentionParams& 
     if (err != cudaSuccess)
         return err;
     return launch_in_stream_order(attention_join_kernel<HEAD_DIM>, dim3(sms, kAttnSlotRows / 32), dim3(256), 0, stream, 1, p, sms);
+}
+
+cudaError_t launch_rows_over_four_bits(cudaStream_t stream, const AttentionParams& p, int head_dim)
+{
+    return head_dim == 64 ? launch_attention<64>(stream, p, true) : launch_attention<128>(stream, p, true);
 }
 
 // The checks that the attention operators share, and the launch.

@@ -24,6 +24,7 @@
 #include <math_constants.h>
 
 #include "cache_batch.cuh"
+#include "four_bit_cache.cuh"
 #include "tiling.h"
 
 namespace flashllm {
@@ -50,6 +51,7 @@ struct AttentionParams {
     float                     cap;  // 0: none
     int                       window;  // keys up to itself that a row sees, kernels with a window alone
     int                       sinks;   // ... and of its sequence's first
+    int                       least_rows;  // sequences with fewer rows (tokens x share) are somebody else's
 };
 
 // What follows from the heads: how rows are tokens and heads, and how many of them tiles hold (kAttnRows at most).
@@ -84,6 +86,12 @@ constexpr int kAttnSegments  = 8;  // segments that shared memory holds at a tim
 // Registers of a thread, 256 x 208 + 128 x 88 = 384 x 168: a softmax thread keeps 64 plain scores of its row, or 32 that are masked,
 // capped or biased, and what their transformation and the ends of an item (32 outputs of its row) take besides.
 constexpr int kAttnSoftmaxRegisters = 208, kAttnOtherRegisters = 88;
+
+// Over a cache of 4 bits four more warps turn codes into the elements that the products take.  256 x 184 + 128 x 64 + 128 x 80 = 512 x
+// 128.
+constexpr int kAttnTurnWarp     = 12;
+constexpr int kAttnFourThreads  = 16 * 32;
+constexpr int kAttnFourSoftmaxRegisters = 184, kAttnFourOtherRegisters = 64, kAttnFourTurnRegisters = 80;
 
 // Looks at a barrier before a CTA gives up: a second.  A look suspends the thread until the barrier changes, for 4.0 us at most
 // (measured on B200).  (Counted and not timed: the waits stand in many places, and code that the instruction cache need not hold is
@@ -286,10 +294,13 @@ struct AttnSequence {
     int      rows;    // count * share
 };
 
+template<bool WINDOW>
 __device__ __forceinline__ AttnSequence attn_sequence(const AttentionParams& p, int b)
 {
     AttnSequence a;
     a.s      = load_sequence(p.batch, b);
+    if (WINDOW && a.s.count * p.share < p.least_rows)
+        a.s.count = 0;
     a.prefix = p.prefix ? min(p.prefix[b], a.s.context + a.s.count) : 0;
     a.rows   = a.s.count * p.share;
     return a;
@@ -300,7 +311,7 @@ template<bool WINDOW>
 __device__ __forceinline__ AttnSequence attn_sequence(const AttentionParams& p, const AttnSharedOf<WINDOW>& sh, int b)
 {
     if (b >= kAttnKnown)
-        return attn_sequence(p, b);
+        return attn_sequence<WINDOW>(p, b);
     const int4 known = sh.known[b];
     return AttnSequence{{known.x, known.y, known.z, 0}, known.w, known.y * p.share};
 }
@@ -437,7 +448,7 @@ __device__ __forceinline__ void attn_count_units(const AttentionParams& p, AttnS
     bool      several   = false;
 #pragma unroll 1
     for (int b = threadIdx.x; b < B; b += kAttnThreads) {
-        const AttnSequence a = attn_sequence(p, b);
+        const AttnSequence a = attn_sequence<WINDOW>(p, b);
         if (b < kAttnKnown)
             sh.known[b] = make_int4(a.s.first, a.s.count, a.s.context, a.prefix);
         const unsigned units = a.s.lost > 0         ? kAttnLostRows
@@ -452,7 +463,7 @@ __device__ __forceinline__ void attn_count_units(const AttentionParams& p, AttnS
         for (int b = warp; b < B; b += kAttnThreads / 32) {
             if (sh.units[b] < kAttnLostRows)
                 continue;
-            const AttnSequence a = attn_sequence(p, b);
+            const AttnSequence a = attn_sequence<WINDOW>(p, b);
             if (a.s.lost > 0 && b % gridDim.x == blockIdx.x) {
                 const long long row = static_cast<long long>(p.heads) * head_dim;
 #pragma unroll 1
@@ -776,12 +787,26 @@ __device__ __forceinline__ uint32_t attn_pack_bounded(float x, float y)
     return *reinterpret_cast<const uint32_t*>(&h);
 }
 
+// Elements `column` up to `column` + 4 of a row of values.
+template<int HEAD_DIM, bool FOUR_BIT>
+__device__ __forceinline__ uint2 attn_values(const AttentionParams& p, long long row, int column)
+{
+    if constexpr (FOUR_BIT) {
+        const unsigned char* const cache = reinterpret_cast<const unsigned char*>(p.v_cache);
+        const uint32_t codes = *reinterpret_cast<const uint32_t*>(cache + four_bit_codes<HEAD_DIM>(p.batch, row) + column / 8 * 4);
+        const half2    scale = *reinterpret_cast<const half2*>(cache + four_bit_scales<HEAD_DIM>(p.batch, row) + column / kFourBitGroup * 4);
+        const uint4    v     = four_bit_values(codes, scale);
+        return column % 8 == 0 ? make_uint2(v.x, v.y) : make_uint2(v.z, v.w);
+    }
+    return *reinterpret_cast<const uint2*>(p.v_cache + row * HEAD_DIM + column);
+}
+
 template<bool WINDOW>
 using AttnList = uint32_t[AttnSegmentOf<WINDOW>::kMixed][4];
 
 // Adds to o[c], element column + c of a row's output, the values that are not finite of keys that the row sees (the products
 // took zeros in their place: a weight of zero times infinity is not zero).
-template<int HEAD_DIM, int COLUMNS, bool WINDOW>
+template<int HEAD_DIM, bool FOUR_BIT, int COLUMNS, bool WINDOW>
 __device__ __forceinline__ void attn_add_not_finite(const AttentionParams& p, const AttnSegmentOf<WINDOW>& seg,
                                                     const AttnRowOf<WINDOW>& row, const AttnList<WINDOW>& list, int column,
                                                     float (&o)[COLUMNS])
@@ -796,18 +821,23 @@ __device__ __forceinline__ void attn_add_not_finite(const AttentionParams& p, co
             const long long at = cache_row(p.batch, seg.b, key, seg.head);
             if (at < 0)
                 continue;
-            const half* v = p.v_cache + at * HEAD_DIM + column;
 #pragma unroll
-            for (int c = 0; c < COLUMNS; ++c)
-                if (half_not_finite(__half_as_ushort(v[c])))
-                    o[c] += __half2float(v[c]);
+            for (int c = 0; c < COLUMNS; c += 4) {
+                const uint2 v = attn_values<HEAD_DIM, FOUR_BIT>(p, at, column + c);
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    const uint32_t h = (k < 2 ? v.x : v.y) >> (16 * (k & 1)) & 0xffffu;
+                    if (half_not_finite(h))
+                        o[c + k] += __half2float(__ushort_as_half(static_cast<unsigned short>(h)));
+                }
+            }
         }
 }
 
 // The same for keys of tiles that all rows of the segment see, which the products take as they are: infinity times a weight of zero,
 // another copy's key or one too small for fp16, has made NaN of the sums there.  Bits of columns `column` on that have a positive
 // infinity or NaN among these keys, and a negative infinity or NaN; for a whole warp.
-template<int HEAD_DIM, int COLUMNS, bool WINDOW>
+template<int HEAD_DIM, bool FOUR_BIT, int COLUMNS, bool WINDOW>
 __device__ __forceinline__ uint2 attn_seen_not_finite(const AttentionParams& p, const AttnSegmentOf<WINDOW>& seg, int column)
 {
     uint2     found = make_uint2(0u, 0u);
@@ -820,23 +850,20 @@ __device__ __forceinline__ uint2 attn_seen_not_finite(const AttentionParams& p, 
         const long long at  = cache_row(p.batch, seg.b, key, seg.head);
         if (at < 0)
             continue;
-        const half* v   = p.v_cache + at * HEAD_DIM + column;
-        uint32_t    any = 0u;
 #pragma unroll
         for (int c = 0; c < COLUMNS; c += 4) {
-            const uint2 w = *reinterpret_cast<const uint2*>(v + c);
-            any |= halves_not_finite(w.x) | halves_not_finite(w.y);
-        }
-        if (any)
+            const uint2 v = attn_values<HEAD_DIM, FOUR_BIT>(p, at, column + c);
+            if (halves_not_finite(v.x) | halves_not_finite(v.y))
 #pragma unroll 1
-            for (int c = 0; c < COLUMNS; ++c) {
-                const uint32_t h = __half_as_ushort(v[c]);
-                if (!half_not_finite(h))
-                    continue;
-                const bool nan = (h & 0x3ffu) != 0u;
-                found.x |= nan || h < 0x8000u ? 1u << c : 0u;
-                found.y |= nan || h >= 0x8000u ? 1u << c : 0u;
-            }
+                for (int k = 0; k < 4; ++k) {
+                    const uint32_t h = (k < 2 ? v.x : v.y) >> (16 * (k & 1)) & 0xffffu;
+                    if (!half_not_finite(h))
+                        continue;
+                    const bool nan = (h & 0x3ffu) != 0u;
+                    found.x |= nan || h < 0x8000u ? 1u << (c + k) : 0u;
+                    found.y |= nan || h >= 0x8000u ? 1u << (c + k) : 0u;
+                }
+        }
     }
     return make_uint2(__reduce_or_sync(0xffffffffu, found.x), __reduce_or_sync(0xffffffffu, found.y));
 }
@@ -848,7 +875,7 @@ struct AttnSums {
 
 // A row's sums of columns `column` on, put right where values are not finite; for a whole warp.  A row whose weights have no finite
 // sum stays without a number.
-template<int HEAD_DIM, int COLUMNS, bool WINDOW>
+template<int HEAD_DIM, bool FOUR_BIT, int COLUMNS, bool WINDOW>
 __device__ __forceinline__ AttnSums<COLUMNS> attn_restore(const AttentionParams& p, const AttnSegmentOf<WINDOW>& seg,
                                                           const AttnRowOf<WINDOW>& row, const AttnList<WINDOW>& list, bool listed,
                                                           float sum, int column,
@@ -859,7 +886,7 @@ __device__ __forceinline__ AttnSums<COLUMNS> attn_restore(const AttentionParams&
     for (int c = 0; c < COLUMNS; ++c)
         nan = nan || sums.o[c] != sums.o[c];
     if (__any_sync(0xffffffffu, nan && sum == sum)) {
-        const uint2 found = attn_seen_not_finite<HEAD_DIM, COLUMNS>(p, seg, column);
+        const uint2 found = attn_seen_not_finite<HEAD_DIM, FOUR_BIT, COLUMNS>(p, seg, column);
 #pragma unroll
         for (int c = 0; c < COLUMNS; ++c) {
             const float plus = found.x >> c & 1u ? CUDART_INF_F : 0.0f, minus = found.y >> c & 1u ? -CUDART_INF_F : 0.0f;
@@ -867,7 +894,7 @@ __device__ __forceinline__ AttnSums<COLUMNS> attn_restore(const AttentionParams&
         }
     }
     if (listed)
-        attn_add_not_finite<HEAD_DIM, COLUMNS>(p, seg, row, list, column, sums.o);
+        attn_add_not_finite<HEAD_DIM, FOUR_BIT, COLUMNS>(p, seg, row, list, column, sums.o);
     return sums;
 }
 
@@ -897,7 +924,7 @@ struct AttnOutputs {
 // The end of a segment for a warp with an output that is not finite, or may not be: its rows (`out` of a whole item's, or `sums` of a
 // part's; neither for a lane without a row) are written anew.  Code of its own, out of the way of the usual ends: in their midst it
 // cost ragged prompts 2 us of 55.
-template<int HEAD_DIM, bool WINDOW>
+template<int HEAD_DIM, bool FOUR_BIT, bool WINDOW>
 __device__ __noinline__ void attn_end_carefully(const AttentionParams& p, const AttnSegmentOf<WINDOW>& seg, const AttnRowOf<WINDOW> row,
                                                 const AttnList<WINDOW>& list, bool listed, AttnOutputs outputs, float sum, int column0,
                                                 int column1, half* out, float4* sums)
@@ -907,7 +934,7 @@ __device__ __noinline__ void attn_end_carefully(const AttentionParams& p, const 
     for (int c = column0; c < column1; c += 16) {
         AttnSums<16> s;
         outputs.load(c, !seg.pair, s.o);
-        s = attn_restore<HEAD_DIM, 16>(p, seg, row, list, listed, sum, c, s);
+        s = attn_restore<HEAD_DIM, FOUR_BIT, 16>(p, seg, row, list, listed, sum, c, s);
 #pragma unroll
         for (int k = 0; k < 16; k += 8) {
             if (out)
@@ -925,12 +952,12 @@ __device__ __noinline__ void attn_end_carefully(const AttentionParams& p, const 
 }
 
 // ... of 4 columns of rows that lie in the tile four times, added up already.
-template<int HEAD_DIM, bool WINDOW>
+template<int HEAD_DIM, bool FOUR_BIT, bool WINDOW>
 __device__ __noinline__ AttnSums<4> attn_restore_four(const AttentionParams& p, const AttnSegmentOf<WINDOW>& seg,
                                                       const AttnRowOf<WINDOW> row, const AttnList<WINDOW>& list, bool listed, float sum,
                                                       int column, AttnSums<4> sums)
 {
-    return attn_restore<HEAD_DIM, 4>(p, seg, row, list, listed, sum, column, sums);
+    return attn_restore<HEAD_DIM, FOUR_BIT, 4>(p, seg, row, list, listed, sum, column, sums);
 }
 
 // tanh x on [-0.75, 0.75] to 2.7e-7, rounding included: x times a polynomial in x^2, fitted to it for the smallest largest error
@@ -1250,9 +1277,139 @@ __device__ __forceinline__ void attn_softmax(AttnState& st, const AttnRowOf<WIND
     st.sum += (part[0].x + part[1].x) + (part[0].y + part[1].y);
 }
 
+// Warps 12 to 15 over a cache of 4 bits: a tile's codes to elements of fp16 in the stages of K and V, as the tensor copies would lay
+// them.  Codes are read straight into registers, those of the next tile while this one's wait for its room: a thread has 32 elements
+// of a key, neighbours have the rest of it and the keys behind.  Elements are rounded to fp16 once, as four_bit_read gives them.
+template<int HEAD_DIM, bool WINDOW>
+__device__ __forceinline__ void attn_turn_codes(const AttentionParams& p, AttnSharedOf<WINDOW>& sh, unsigned char* k_stages, unsigned char* v_stages)
+{
+    constexpr int kStages = attn_stages(HEAD_DIM), kTileBytes = attn_tile_bytes(HEAD_DIM), kBlock = kAttnKeys * 128;
+    constexpr int kChunks = HEAD_DIM / 32, kRows = 32 / kChunks, kJobs = 32 / kRows;  // of 16 bytes of a key; keys of a job; jobs of a warp
+    const CacheBatch& c = p.batch;
+    const int warp = (threadIdx.x >> 5) - kAttnTurnWarp, lane = threadIdx.x & 31, q = lane % kChunks, r0 = 32 * warp + lane / kChunks;
+    const uint32_t page_bytes = static_cast<uint32_t>(four_bit_row_bytes(HEAD_DIM)) << c.page_shift;
+    const uint32_t scales_at  = static_cast<uint32_t>(HEAD_DIM / 2) << c.page_shift;
+    uint32_t n  = 0;
+    bool     ok = true;
+#pragma unroll 1
+    for (int number = 0;; ++number) {
+        const AttnSegmentOf<WINDOW>* const current = attn_segment(sh, number, c.status);
+        AttnList<WINDOW>& list = sh.not_finite[number % kAttnSegments];
+        const int         t128 = threadIdx.x - kAttnTurnWarp * 32;
+        if (t128 < 4 * AttnSegmentOf<WINDOW>::kMixed)
+            (&list[0][0])[t128] = 0u;
+        if (t128 == 0)
+            sh.any_not_finite[number % kAttnSegments] = 0u;
+        if (ptx::named_barrier_any(5, 128, current == nullptr || !ok))  // all or none
+            break;
+        const AttnSegmentOf<WINDOW>& seg = *current;
+        const int* const table = c.page_table + static_cast<long long>(seg.b) * c.table_width;
+        // Pages of the warp's two sixteens of keys; -1: zeros.
+        auto pages = [&](int t, int (&ids)[2]) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const int key = seg.key_of(t) + 32 * warp + 16 * h;
+                ids[h]        = -1;
+                if (t < seg.end && key < seg.keys) {
+                    const int id = table[key >> c.page_shift];
+                    if (static_cast<unsigned>(id) < static_cast<unsigned>(c.pages))
+                        ids[h] = id;
+                    else
+                        atomicOr(c.status, kStatusBadCache);
+                }
+            }
+        };
+        auto load = [&](const half* cache, int t, const int (&ids)[2], uint4 (&codes)[kJobs], half2 (&scale)[kJobs]) {
+#pragma unroll
+            for (int j = 0; j < kJobs; ++j) {
+                const int      id = ids[j * kRows / 16];
+                const uint32_t in = (seg.key_of(t) + r0 + kRows * j) & ((1 << c.page_shift) - 1);
+                const unsigned char* const page = reinterpret_cast<const unsigned char*>(cache) + static_cast<unsigned long long>(static_cast<uint32_t>(max(id, 0) * c.kv_heads + seg.head)) * page_bytes;
+                codes[j] = make_uint4(0, 0, 0, 0);
+                scale[j] = __float2half2_rn(0.0f);
+                if (id >= 0) {
+                    codes[j] = *reinterpret_cast<const uint4*>(page + in * (HEAD_DIM / 2) + 16 * q);
+                    scale[j] = *reinterpret_cast<const half2*>(page + scales_at + in * (4 * four_bit_groups(HEAD_DIM)) + q / 2 * 4);
+                }
+            }
+        };
+        auto at = [&](unsigned char* stage, int j, int i) -> uint4& {
+            // Chunks of threads with the second 64 elements change places: banks.
+            const int r = r0 + kRows * j, chunk = (q & 1) * 4 + (i ^ (q >> 1) * 2);
+            return *reinterpret_cast<uint4*>(stage + (q >> 1) * kBlock + r * 128 + (chunk ^ (r & 7)) * 16);
+        };
+        auto word = [&](const uint4& w, int i) {  // the i-th of the words, in the order of `at`
+            const int k = i ^ (q >> 1) * 2;
+            return k == 0 ? w.x : k == 1 ? w.y : k == 2 ? w.z : w.w;
+        };
+        int   ids[2], ids_next[2];
+        uint4 k_codes[kJobs], v_codes[kJobs];
+        half2 k_scale[kJobs], v_scale[kJobs];
+        pages(seg.begin, ids);
+        load(p.k_cache, seg.begin, ids, k_codes, k_scale);
+        load(p.v_cache, seg.begin, ids, v_codes, v_scale);
+        pages(seg.begin + 1, ids_next);
+#pragma unroll 1
+        for (int t = seg.begin; t < seg.end; ++t, ++n) {
+            const uint32_t stage = n % kStages, parity = (n / kStages & 1u) ^ 1u;
+            ok = __all_sync(0xffffffffu, attn_wait(&sh.k_empty[stage], parity, sh, c.status));
+            if (!ok)
+                break;
+#pragma unroll
+            for (int j = 0; j < kJobs; ++j)
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    at(k_stages + stage * kTileBytes, j, i) = four_bit_values(word(k_codes[j], i), k_scale[j]);
+            ptx::fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0)
+                ptx::mbar_arrive(ptx::smem_u32(&sh.k_full[stage]));
+            load(p.k_cache, t + 1, ids_next, k_codes, k_scale);
+            ok = __all_sync(0xffffffffu, attn_wait(&sh.v_empty[stage], parity, sh, c.status));
+            if (!ok)
+                break;
+            if (!seg.mixed(t)) {
+#pragma unroll
+                for (int j = 0; j < kJobs; ++j)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        at(v_stages + stage * kTileBytes, j, i) = four_bit_values(word(v_codes[j], i), v_scale[j]);
+            }
+            else {  // values that not all rows see: zeros in the place of what is not finite, and behind the last
+                const int key0 = seg.key_of(t), mixed = seg.mixed_of(t);
+#pragma unroll
+                for (int j = 0; j < kJobs; ++j) {
+                    const int  r   = r0 + kRows * j;
+                    bool       bad = false;
+#pragma unroll 1
+                    for (int i = 0; i < 4; ++i) {
+                        uint4 w     = four_bit_values(word(v_codes[j], i), v_scale[j]);
+                        auto  clean = [&](uint32_t u) {
+                            bad = bad || halves_not_finite(u) != 0u;
+                            return (half_not_finite(u) ? 0u : u & 0xffffu) | (half_not_finite(u >> 16) ? 0u : u & 0xffff0000u);
+                        };
+                        w = make_uint4(clean(w.x), clean(w.y), clean(w.z), clean(w.w));
+                        at(v_stages + stage * kTileBytes, j, i) = key0 + r < seg.keys ? w : make_uint4(0, 0, 0, 0);
+                    }
+                    if (bad && key0 + r < seg.keys && mixed < AttnSegmentOf<WINDOW>::kMixed) {
+                        atomicOr(&list[mixed][r / 32], 1u << r % 32);
+                        sh.any_not_finite[number % kAttnSegments] = 1u;
+                    }
+                }
+            }
+            ptx::fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0)
+                ptx::mbar_arrive(ptx::smem_u32(&sh.v_clean[stage]));
+            load(p.v_cache, t + 1, ids_next, v_codes, v_scale);
+            pages(t + 2, ids_next);
+        }
+    }
+}
+
 // PLAIN: neither cap nor slopes.
-template<int HEAD_DIM, bool PLAIN, bool WINDOW = false>
-__global__ void __launch_bounds__(kAttnThreads, 1)
+template<int HEAD_DIM, bool PLAIN, bool WINDOW = false, bool FOUR_BIT = false>
+__global__ void __launch_bounds__(FOUR_BIT ? kAttnFourThreads : kAttnThreads, 1)
 attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_q_few,
                  const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
                  const __grid_constant__ AttentionParams p)
@@ -1274,10 +1431,10 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
     if (threadIdx.x == 0) {
 #pragma unroll 1
         for (int i = 0; i < 4; ++i) {
-            ptx::mbar_init(ptx::smem_u32(&sh.k_full[i]), 1);
+            ptx::mbar_init(ptx::smem_u32(&sh.k_full[i]), FOUR_BIT ? 4 : 1);
             ptx::mbar_init(ptx::smem_u32(&sh.k_empty[i]), 1);
             ptx::mbar_init(ptx::smem_u32(&sh.v_full[i]), 1);
-            ptx::mbar_init(ptx::smem_u32(&sh.v_clean[i]), 64);
+            ptx::mbar_init(ptx::smem_u32(&sh.v_clean[i]), FOUR_BIT ? 4 : 64);
             ptx::mbar_init(ptx::smem_u32(&sh.v_empty[i]), 1);
         }
 #pragma unroll 1
@@ -1296,8 +1453,10 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
         ptx::fence_mbar_init();
         ptx::prefetch_tensormap(&map_q);
         ptx::prefetch_tensormap(&map_q_few);
-        ptx::prefetch_tensormap(&map_k);
-        ptx::prefetch_tensormap(&map_v);
+        if constexpr (!FOUR_BIT) {
+            ptx::prefetch_tensormap(&map_k);
+            ptx::prefetch_tensormap(&map_v);
+        }
     }
     if (warp == kAttnMmaWarp) {
         ptx::tmem_alloc(ptx::smem_u32(&sh.tmem), kAttnTmemCols);
@@ -1312,9 +1471,11 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
         ptx::grid_launch_dependents();
 
     if (warp < kAttnMmaWarp)
-        ptx::take_registers<kAttnSoftmaxRegisters>();
+        ptx::take_registers<FOUR_BIT ? kAttnFourSoftmaxRegisters : kAttnSoftmaxRegisters>();
+    else if (FOUR_BIT && warp >= kAttnTurnWarp)
+        ptx::give_registers<kAttnFourTurnRegisters>();
     else
-        ptx::give_registers<kAttnOtherRegisters>();
+        ptx::give_registers<FOUR_BIT ? kAttnFourOtherRegisters : kAttnOtherRegisters>();
 
     if (warp < kAttnMmaWarp) {
         // ================================================================ softmax: one thread per row
@@ -1476,7 +1637,7 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
 #pragma unroll
                         for (int k = 0; k < 4; ++k)
                             sums4.o[k] = sum4[k];
-                        sums4 = attn_restore_four<HEAD_DIM>(p, seg, row, list, any, st.sum, column, sums4);
+                        sums4 = attn_restore_four<HEAD_DIM, FOUR_BIT>(p, seg, row, list, any, st.sum, column, sums4);
 #pragma unroll
                         for (int k = 0; k < 4; ++k)
                             sum4[k] = sums4.o[k];
@@ -1582,7 +1743,7 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
                 again          = __any_sync(0xffffffffu, valid && bad);
             }
             if (again)
-                attn_end_carefully<HEAD_DIM>(p, seg, row, list, any, outputs, st.sum, column0, column1,
+                attn_end_carefully<HEAD_DIM, FOUR_BIT>(p, seg, row, list, any, outputs, st.sum, column0, column1,
                                              valid && whole ? p.out + to : nullptr, valid && !whole ? sums + thread : nullptr);
             if (ok && !whole && valid && column0 == 0 && (!fourfold || thread < 32))
                 reinterpret_cast<float2*>(p.workspace + attn_stats_offset(gridDim.x))[static_cast<size_t>(2 * blockIdx.x + slot) * kAttnSlotRows
@@ -1713,6 +1874,10 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
                 break;
             const int* table = c.page_table + static_cast<long long>(seg.b) * c.table_width;
             for (int t = seg.begin; ok && t < seg.end; ++t, ++n) {
+                if constexpr (FOUR_BIT) {  // only as far ahead as the copies would be: the segments' places
+                    ok = __all_sync(0xffffffffu, attn_wait(&sh.v_empty[n % kStages], (n / kStages & 1u) ^ 1u, sh, status));
+                    continue;
+                }
                 const int key   = seg.key_of(t) + piece * box;
                 int       z     = c.pages * c.kv_heads;  // behind the cache: reads as zeros
                 if (active && key < seg.keys) {
@@ -1740,6 +1905,11 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
             }
         }
     }
+    else if (FOUR_BIT && warp >= kAttnTurnWarp) {
+        // ================================================================ codes to elements
+        if constexpr (FOUR_BIT)
+            attn_turn_codes<HEAD_DIM>(p, sh, smem + 2 * kTileBytes, smem + (2 + kStages) * kTileBytes);
+    }
     else {
         // ================================================================ rows of Q, and values that no product may see
         const int t64         = threadIdx.x - kAttnHelpWarp * 32;
@@ -1748,9 +1918,9 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
         for (int number = 0;; ++number) {
             const AttnSegmentOf<WINDOW>* const current = attn_segment(sh, number, status);
             AttnList<WINDOW>& list = sh.not_finite[number % kAttnSegments];
-            if (t64 < 4 * AttnSegmentOf<WINDOW>::kMixed)
+            if (!FOUR_BIT && t64 < 4 * AttnSegmentOf<WINDOW>::kMixed)
                 (&list[0][0])[t64] = 0u;
-            if (t64 == 0)
+            if (!FOUR_BIT && t64 == 0)
                 sh.any_not_finite[number % kAttnSegments] = 0u;
             if (ptx::named_barrier_any(4, 64, current == nullptr || !ok))  // all or none
                 break;
@@ -1775,7 +1945,7 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
                             ptx::tma_load_3d(dst + block * kBlock + copy * 32 * 128, map, block * 64, seg.head * p.share, token, bar);
                 }
             }
-            for (int t = seg.begin; t < seg.end; ++t, ++n) {
+            for (int t = seg.begin; !FOUR_BIT && t < seg.end; ++t, ++n) {
                 const uint32_t stage = n % kStages;
                 ok                   = ok && attn_wait(&sh.v_full[stage], n / kStages & 1u, sh, status);
                 if (!ok)  // nor without the rows of Q: those of the next segment would be taken for them

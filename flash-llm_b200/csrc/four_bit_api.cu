@@ -3,6 +3,7 @@
 #include <cuda_runtime.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "append_kernels_sm100.cuh"
 #include "attention_four_bit_sm100.cuh"
@@ -11,6 +12,9 @@
 #include "tiled_csl_host.h"
 
 namespace flashllm {
+
+// The attention kernel of many rows over a cache of 4 bits (attention_api.cu).
+cudaError_t launch_rows_over_four_bits(cudaStream_t stream, const AttentionParams& p, int head_dim);
 
 static cudaError_t four_multiprocessors(int* count)
 {
@@ -85,6 +89,9 @@ static cudaError_t append(cudaStream_t stream, bool four_bit, const void* QKV, i
     return interleaved ? of_cache(norm_append_kernel<128, true, false>, norm_append_kernel<128, true, true>)
                        : of_cache(norm_append_kernel<128, false, false>, norm_append_kernel<128, false, true>);
 }
+
+// Rows of a sequence (tokens x query heads of a key/value head) up to which it goes through the warps' kernel.
+constexpr int kFourMostRows = 16;
 
 template<int HEAD_DIM, int TILES>
 static cudaError_t launch_four_bit(cudaStream_t stream, const FourBitParams& p, int ctas)
@@ -186,14 +193,39 @@ int FlashLLM_FourBitAttention(void* stream, const void* Q, int ld_q, const void*
     p.share     = heads / kv_heads;
     p.window    = window > 0 ? window : 0x7fffffff;
     p.sinks     = window > 0 ? sinks : 0;
-    p.most_rows = 0x7fffffff;
+    // Sequences of many rows are the other kernel's, which the host cannot tell: where there is a token for each sequence, or fewer
+    // rows in all, it takes them for single tokens (and rows that are more are right, if slower).
+    const bool many = tokens > sequences && static_cast<long long>(tokens) * p.share > kFourMostRows;
+    p.most_rows     = many ? kFourMostRows : 0x7fffffff;
     p.scale     = scale;
     p.cap       = cap;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
+    auto few = [&](auto dim, auto tiles) { return launch_four_bit<decltype(dim)::value, decltype(tiles)::value>(s, p, sms); };
+    using Dim64 = std::integral_constant<int, 64>;
+    using Dim128 = std::integral_constant<int, 128>;
+    using One = std::integral_constant<int, 1>;
+    using Two = std::integral_constant<int, 2>;
     // Sixteen rows at a time where a sequence has more than eight.
-    if (p.share > 8 || tokens > sequences)
-        return static_cast<int>(head_dim == 64 ? launch_four_bit<64, 2>(s, p, sms) : launch_four_bit<128, 2>(s, p, sms));
-    return static_cast<int>(head_dim == 64 ? launch_four_bit<64, 1>(s, p, sms) : launch_four_bit<128, 1>(s, p, sms));
+    const bool      two = p.share > 8 || tokens > sequences;
+    const cudaError_t err = head_dim == 64 ? (two ? few(Dim64{}, Two{}) : few(Dim64{}, One{})) : (two ? few(Dim128{}, Two{}) : few(Dim128{}, One{}));
+    if (err != cudaSuccess || !many)
+        return static_cast<int>(err);
+    AttentionParams a{};
+    a.batch      = p.batch;
+    a.q          = p.q;
+    a.out        = p.out;
+    a.k_cache    = reinterpret_cast<const half*>(p.k_cache);
+    a.v_cache    = reinterpret_cast<const half*>(p.v_cache);
+    a.slopes     = slopes;
+    a.workspace  = p.workspace;
+    a.ld_q       = ld_q;
+    a.scale      = scale;
+    a.cap        = cap;
+    a.window     = p.window;
+    a.sinks      = p.sinks;
+    a.least_rows = kFourMostRows + 1;
+    attn_set_heads(&a, heads, kv_heads);
+    return static_cast<int>(launch_rows_over_four_bits(s, a, head_dim));
 }
 
 }  // extern "C"

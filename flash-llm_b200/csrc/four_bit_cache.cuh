@@ -11,6 +11,8 @@
 // large, for 0.25 bits an element.  A group that holds a value which is not finite, or beyond fp16's range, has a step of NaN, and so
 // have its elements.
 #pragma once
+#include <math_constants.h>
+
 #include "cache_batch.cuh"
 
 namespace flashllm {
@@ -44,10 +46,11 @@ __device__ __forceinline__ long long four_bit_scales(const CacheBatch& c, long l
 }
 
 // Eight elements, one rounding to fp16 each: product and sum are one operation, a code is exact.  (Lowest value and step, rounded, can
-// take the last past the largest number of fp16, which then is the element.)
+// take the last past the largest number of fp16, which then is the element.  A lowest value that is infinite, which no append
+// writes, makes infinite elements.)
 __device__ __forceinline__ uint4 four_bit_values(uint32_t codes, half2 scale)
 {
-    const half2 step = __low2half2(scale), low = __high2half2(scale), offset = __float2half2_rn(1024.0f), largest = __float2half2_rn(65504.0f);
+    const half2 step = __low2half2(scale), low = __high2half2(scale), offset = __float2half2_rn(1024.0f), largest = __float2half2_rn(__hisinf(__high2half(scale)) ? CUDART_INF_F : 65504.0f);
     uint32_t    v[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
