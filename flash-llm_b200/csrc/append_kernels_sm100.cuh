@@ -269,7 +269,7 @@ __global__ void __launch_bounds__(kReadThreads) four_bit_read_kernel(const __gri
             const long long row   = at + (static_cast<long long>(h) << c.page_shift);
             const uint32_t  codes = *reinterpret_cast<const uint32_t*>(p.cache[kind] + four_bit_codes<HEAD_DIM>(c, row) + 4 * word);
             const half2     scale = *reinterpret_cast<const half2*>(p.cache[kind] + four_bit_scales<HEAD_DIM>(c, row) + word / 8 * 4);
-            v                     = four_bit_values(codes, scale);
+            v                     = four_bit_values<true>(codes, scale);
         }
         *reinterpret_cast<uint4*>(p.out[kind] + (static_cast<long long>(n0 + i) * c.kv_heads + h) * HEAD_DIM + 8 * word) = v;
     }

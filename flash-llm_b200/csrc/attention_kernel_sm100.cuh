@@ -87,11 +87,11 @@ constexpr int kAttnSegments  = 8;  // segments that shared memory holds at a tim
 // capped or biased, and what their transformation and the ends of an item (32 outputs of its row) take besides.
 constexpr int kAttnSoftmaxRegisters = 208, kAttnOtherRegisters = 88;
 
-// Over a cache of 4 bits four more warps turn codes into the elements that the products take.  256 x 184 + 128 x 64 + 128 x 80 = 512 x
+// Over a cache of 4 bits four more warps turn codes into the elements that the products take.  256 x 152 + 128 x 96 + 128 x 112 = 512 x
 // 128.
 constexpr int kAttnTurnWarp     = 12;
 constexpr int kAttnFourThreads  = 16 * 32;
-constexpr int kAttnFourSoftmaxRegisters = 184, kAttnFourOtherRegisters = 64, kAttnFourTurnRegisters = 80;
+constexpr int kAttnFourSoftmaxRegisters = 152, kAttnFourOtherRegisters = 96, kAttnFourTurnRegisters = 112;
 
 // Looks at a barrier before a CTA gives up: a second.  A look suspends the thread until the barrier changes, for 4.0 us at most
 // (measured on B200).  (Counted and not timed: the waits stand in many places, and code that the instruction cache need not hold is
@@ -795,7 +795,7 @@ __device__ __forceinline__ uint2 attn_values(const AttentionParams& p, long long
         const unsigned char* const cache = reinterpret_cast<const unsigned char*>(p.v_cache);
         const uint32_t codes = *reinterpret_cast<const uint32_t*>(cache + four_bit_codes<HEAD_DIM>(p.batch, row) + column / 8 * 4);
         const half2    scale = *reinterpret_cast<const half2*>(cache + four_bit_scales<HEAD_DIM>(p.batch, row) + column / kFourBitGroup * 4);
-        const uint4    v     = four_bit_values(codes, scale);
+        const uint4    v     = four_bit_values<true>(codes, scale);
         return column % 8 == 0 ? make_uint2(v.x, v.y) : make_uint2(v.z, v.w);
     }
     return *reinterpret_cast<const uint2*>(p.v_cache + row * HEAD_DIM + column);
@@ -1304,33 +1304,31 @@ __device__ __forceinline__ void attn_turn_codes(const AttentionParams& p, AttnSh
             break;
         const AttnSegmentOf<WINDOW>& seg = *current;
         const int* const table = c.page_table + static_cast<long long>(seg.b) * c.table_width;
-        // Pages of the warp's two sixteens of keys; -1: zeros.
+        // Pages of the warp's two sixteens of keys, looked up a tile ahead of the loads that need them.
         auto pages = [&](int t, int (&ids)[2]) {
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
                 const int key = seg.key_of(t) + 32 * warp + 16 * h;
-                ids[h]        = -1;
-                if (t < seg.end && key < seg.keys) {
-                    const int id = table[key >> c.page_shift];
-                    if (static_cast<unsigned>(id) < static_cast<unsigned>(c.pages))
-                        ids[h] = id;
-                    else
-                        atomicOr(c.status, kStatusBadCache);
-                }
+                ids[h]        = t < seg.end && key < seg.keys ? table[key >> c.page_shift] : 0;
             }
         };
+        // Codes and scales of the thread's keys; zeros, which stand for zeros, where there are none.
         auto load = [&](const half* cache, int t, const int (&ids)[2], uint4 (&codes)[kJobs], half2 (&scale)[kJobs]) {
+            const int key0 = seg.key_of(t);
 #pragma unroll
             for (int j = 0; j < kJobs; ++j) {
-                const int      id = ids[j * kRows / 16];
-                const uint32_t in = (seg.key_of(t) + r0 + kRows * j) & ((1 << c.page_shift) - 1);
-                const unsigned char* const page = reinterpret_cast<const unsigned char*>(cache) + static_cast<unsigned long long>(static_cast<uint32_t>(max(id, 0) * c.kv_heads + seg.head)) * page_bytes;
+                const int      id = ids[j * kRows / 16], key = key0 + r0 + kRows * j;
+                const uint32_t in = key & ((1 << c.page_shift) - 1);
+                const unsigned char* const page = reinterpret_cast<const unsigned char*>(cache) + static_cast<unsigned long long>(static_cast<uint32_t>(id * c.kv_heads + seg.head)) * page_bytes;
+                const bool there = static_cast<unsigned>(id) < static_cast<unsigned>(c.pages), wanted = t < seg.end && key < seg.keys;
                 codes[j] = make_uint4(0, 0, 0, 0);
                 scale[j] = __float2half2_rn(0.0f);
-                if (id >= 0) {
+                if (there && wanted) {
                     codes[j] = *reinterpret_cast<const uint4*>(page + in * (HEAD_DIM / 2) + 16 * q);
                     scale[j] = *reinterpret_cast<const half2*>(page + scales_at + in * (4 * four_bit_groups(HEAD_DIM)) + q / 2 * 4);
                 }
+                if (!there && wanted)
+                    atomicOr(c.status, kStatusBadCache);
             }
         };
         auto at = [&](unsigned char* stage, int j, int i) -> uint4& {
@@ -1341,6 +1339,25 @@ __device__ __forceinline__ void attn_turn_codes(const AttentionParams& p, AttnSh
         auto word = [&](const uint4& w, int i) {  // the i-th of the words, in the order of `at`
             const int k = i ^ (q >> 1) * 2;
             return k == 0 ? w.x : k == 1 ? w.y : k == 2 ? w.z : w.w;
+        };
+        auto turn = [&](unsigned char* stage, const uint4 (&codes)[kJobs], const half2 (&scale)[kJobs]) {
+            bool beyond = false;
+#pragma unroll
+            for (int j = 0; j < kJobs; ++j)
+                beyond = beyond || four_bit_beyond(scale[j]);
+            if (__any_sync(0xffffffffu, beyond)) {
+#pragma unroll 1
+                for (int i = 0; i < 4; ++i)
+#pragma unroll
+                    for (int j = 0; j < kJobs; ++j)
+                        at(stage, j, i) = four_bit_values<true>(word(codes[j], i), scale[j]);
+                return;
+            }
+#pragma unroll
+            for (int j = 0; j < kJobs; ++j)
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    at(stage, j, i) = four_bit_values<false>(word(codes[j], i), scale[j]);
         };
         int   ids[2], ids_next[2];
         uint4 k_codes[kJobs], v_codes[kJobs];
@@ -1355,11 +1372,7 @@ __device__ __forceinline__ void attn_turn_codes(const AttentionParams& p, AttnSh
             ok = __all_sync(0xffffffffu, attn_wait(&sh.k_empty[stage], parity, sh, c.status));
             if (!ok)
                 break;
-#pragma unroll
-            for (int j = 0; j < kJobs; ++j)
-#pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    at(k_stages + stage * kTileBytes, j, i) = four_bit_values(word(k_codes[j], i), k_scale[j]);
+            turn(k_stages + stage * kTileBytes, k_codes, k_scale);
             ptx::fence_proxy_async_smem();
             __syncwarp();
             if (lane == 0)
@@ -1368,30 +1381,25 @@ __device__ __forceinline__ void attn_turn_codes(const AttentionParams& p, AttnSh
             ok = __all_sync(0xffffffffu, attn_wait(&sh.v_empty[stage], parity, sh, c.status));
             if (!ok)
                 break;
-            if (!seg.mixed(t)) {
+            bool odd = false;
+            if (seg.mixed(t)) {
 #pragma unroll
                 for (int j = 0; j < kJobs; ++j)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i)
-                        at(v_stages + stage * kTileBytes, j, i) = four_bit_values(word(v_codes[j], i), v_scale[j]);
+                    odd = odd || halves_not_finite(*reinterpret_cast<const uint32_t*>(&v_scale[j])) != 0u;
+                odd = __any_sync(0xffffffffu, odd);
             }
-            else {  // values that not all rows see: zeros in the place of what is not finite, and behind the last
-                const int key0 = seg.key_of(t), mixed = seg.mixed_of(t);
+            if (!odd)
+                turn(v_stages + stage * kTileBytes, v_codes, v_scale);
+            else {  // values that not all rows see, and that are not finite: zeros in their place
+                const int mixed = seg.mixed_of(t);
 #pragma unroll
                 for (int j = 0; j < kJobs; ++j) {
                     const int  r   = r0 + kRows * j;
-                    bool       bad = false;
+                    const bool bad = halves_not_finite(*reinterpret_cast<const uint32_t*>(&v_scale[j])) != 0u;
 #pragma unroll 1
-                    for (int i = 0; i < 4; ++i) {
-                        uint4 w     = four_bit_values(word(v_codes[j], i), v_scale[j]);
-                        auto  clean = [&](uint32_t u) {
-                            bad = bad || halves_not_finite(u) != 0u;
-                            return (half_not_finite(u) ? 0u : u & 0xffffu) | (half_not_finite(u >> 16) ? 0u : u & 0xffff0000u);
-                        };
-                        w = make_uint4(clean(w.x), clean(w.y), clean(w.z), clean(w.w));
-                        at(v_stages + stage * kTileBytes, j, i) = key0 + r < seg.keys ? w : make_uint4(0, 0, 0, 0);
-                    }
-                    if (bad && key0 + r < seg.keys && mixed < AttnSegmentOf<WINDOW>::kMixed) {
+                    for (int i = 0; i < 4; ++i)
+                        at(v_stages + stage * kTileBytes, j, i) = bad ? make_uint4(0, 0, 0, 0) : four_bit_values<true>(word(v_codes[j], i), v_scale[j]);
+                    if (bad && mixed < AttnSegmentOf<WINDOW>::kMixed) {
                         atomicOr(&list[mixed][r / 32], 1u << r % 32);
                         sh.any_not_finite[number % kAttnSegments] = 1u;
                     }

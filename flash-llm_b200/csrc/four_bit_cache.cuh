@@ -45,18 +45,31 @@ __device__ __forceinline__ long long four_bit_scales(const CacheBatch& c, long l
            + in * (4 * four_bit_groups(HEAD_DIM));
 }
 
-// Eight elements, one rounding to fp16 each: product and sum are one operation, a code is exact.  (Lowest value and step, rounded, can
-// take the last past the largest number of fp16, which then is the element.  A lowest value that is infinite, which no append
-// writes, makes infinite elements.)
+// Whether the last of the codes stands for more than fp16 holds (lowest value and step, rounded, can take it there), or the lowest
+// value is infinite, which no append writes.
+__device__ __forceinline__ bool four_bit_beyond(half2 scale)
+{
+    return __hisinf(__hfma(__float2half_rn(15.0f), __low2half(scale), __high2half(scale))) != 0;
+}
+
+// Eight elements, one rounding to fp16 each: product and sum are one operation, a code is exact (four bits put into the mantissa of 1024
+// or, where they lie, of 64 are so much more).  BOUNDED: elements past the largest number of fp16 are that number, unless the lowest
+// value is infinite.
+template<bool BOUNDED>
 __device__ __forceinline__ uint4 four_bit_values(uint32_t codes, half2 scale)
 {
-    const half2 step = __low2half2(scale), low = __high2half2(scale), offset = __float2half2_rn(1024.0f), largest = __float2half2_rn(__hisinf(__high2half(scale)) ? CUDART_INF_F : 65504.0f);
-    uint32_t    v[4];
+    const half2    step = __low2half2(scale), low = __high2half2(scale);
+    const half2    largest = __float2half2_rn(__hisinf(__high2half(scale)) ? CUDART_INF_F : 65504.0f);
+    const uint32_t codes8 = codes >> 8;
+    uint32_t       v[4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const uint32_t two = (codes >> (4 * i) & 0x000f000fu) | 0x64006400u;  // 1024 + code of elements i and i + 4
-        const half2    h   = __hmin2_nan(__hfma2(__hsub2(*reinterpret_cast<const half2*>(&two), offset), step, low), largest);
-        v[i]               = *reinterpret_cast<const uint32_t*>(&h);
+    for (int i = 0; i < 4; ++i) {  // elements i and i + 4
+        const uint32_t w   = i < 2 ? codes : codes8;
+        const uint32_t two = i % 2 == 0 ? (w & 0x000f000fu) | 0x64006400u : (w & 0x00f000f0u) | 0x54005400u;
+        half2          h   = __hfma2(__hsub2(*reinterpret_cast<const half2*>(&two), __float2half2_rn(i % 2 == 0 ? 1024.0f : 64.0f)), step, low);
+        if constexpr (BOUNDED)
+            h = __hmin2_nan(h, largest);
+        v[i] = *reinterpret_cast<const uint32_t*>(&h);
     }
     return make_uint4(__byte_perm(v[0], v[1], 0x5410), __byte_perm(v[2], v[3], 0x5410), __byte_perm(v[0], v[1], 0x7632),
                       __byte_perm(v[2], v[3], 0x7632));
