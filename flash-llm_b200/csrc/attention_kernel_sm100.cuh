@@ -87,11 +87,12 @@ constexpr int kAttnSegments  = 8;  // segments that shared memory holds at a tim
 // capped or biased, and what their transformation and the ends of an item (32 outputs of its row) take besides.
 constexpr int kAttnSoftmaxRegisters = 208, kAttnOtherRegisters = 88;
 
-// Over a cache of 4 bits four more warps turn codes into the elements that the products take.  256 x 152 + 128 x 96 + 128 x 112 = 512 x
-// 128.
+// Over a cache of 4 bits four more warps turn codes into the elements that the products take.  256 x 152 + 128 x 104 + 128 x 104 = 512 x
+// 128: what the softmax gives up costs it little, registers that the warps of products and work lack spill in their loops (a prompt of
+// 7000 tokens, before other steps: 184, 64 and 80 registers 738 us, 168, 72 and 104 691, 160, 88 and 104 653, 152, 96 and 112 624).
 constexpr int kAttnTurnWarp     = 12;
 constexpr int kAttnFourThreads  = 16 * 32;
-constexpr int kAttnFourSoftmaxRegisters = 152, kAttnFourOtherRegisters = 96, kAttnFourTurnRegisters = 112;
+constexpr int kAttnFourSoftmaxRegisters = 152, kAttnFourOtherRegisters = 104, kAttnFourTurnRegisters = 104;
 
 // Looks at a barrier before a CTA gives up: a second.  A look suspends the thread until the barrier changes, for 4.0 us at most
 // (measured on B200).  (Counted and not timed: the waits stand in many places, and code that the instruction cache need not hold is
@@ -1289,6 +1290,7 @@ __device__ __forceinline__ void attn_turn_codes(const AttentionParams& p, AttnSh
     const int warp = (threadIdx.x >> 5) - kAttnTurnWarp, lane = threadIdx.x & 31, q = lane % kChunks, r0 = 32 * warp + lane / kChunks;
     const uint32_t page_bytes = static_cast<uint32_t>(four_bit_row_bytes(HEAD_DIM)) << c.page_shift;
     const uint32_t scales_at  = static_cast<uint32_t>(HEAD_DIM / 2) << c.page_shift;
+    const uint32_t offset     = (q >> 1) * kBlock + r0 * 128 + (((q & 1) * 4 + (q >> 1) * 2) ^ (r0 & 7)) * 16;
     uint32_t n  = 0;
     bool     ok = true;
 #pragma unroll 1
@@ -1314,38 +1316,44 @@ __device__ __forceinline__ void attn_turn_codes(const AttentionParams& p, AttnSh
         };
         // Codes and scales of the thread's keys; zeros, which stand for zeros, where there are none.
         auto load = [&](const half* cache, int t, const int (&ids)[2], uint4 (&codes)[kJobs], half2 (&scale)[kJobs]) {
-            const int key0 = seg.key_of(t);
+            const int key0 = seg.key_of(t) + 32 * warp;
 #pragma unroll
-            for (int j = 0; j < kJobs; ++j) {
-                const int      id = ids[j * kRows / 16], key = key0 + r0 + kRows * j;
-                const uint32_t in = key & ((1 << c.page_shift) - 1);
+            for (int h = 0; h < 2; ++h) {
+                const int      id = ids[h], left = t < seg.end ? seg.keys - key0 - 16 * h : 0;  // keys of the sixteen that there are
+                const bool     there = static_cast<unsigned>(id) < static_cast<unsigned>(c.pages);
+                const uint32_t in = ((key0 + 16 * h) & ((1 << c.page_shift) - 1)) + lane / kChunks;
                 const unsigned char* const page = reinterpret_cast<const unsigned char*>(cache) + static_cast<unsigned long long>(static_cast<uint32_t>(id * c.kv_heads + seg.head)) * page_bytes;
-                const bool there = static_cast<unsigned>(id) < static_cast<unsigned>(c.pages), wanted = t < seg.end && key < seg.keys;
-                codes[j] = make_uint4(0, 0, 0, 0);
-                scale[j] = __float2half2_rn(0.0f);
-                if (there && wanted) {
-                    codes[j] = *reinterpret_cast<const uint4*>(page + in * (HEAD_DIM / 2) + 16 * q);
-                    scale[j] = *reinterpret_cast<const half2*>(page + scales_at + in * (4 * four_bit_groups(HEAD_DIM)) + q / 2 * 4);
+                const unsigned char* const from = page + in * (HEAD_DIM / 2) + 16 * q;
+                const unsigned char* const from_scales = page + scales_at + in * (4 * four_bit_groups(HEAD_DIM)) + q / 2 * 4;
+#pragma unroll
+                for (int k = 0; k < kJobs / 2; ++k) {
+                    const int j = h * (kJobs / 2) + k;
+                    codes[j]    = make_uint4(0, 0, 0, 0);
+                    scale[j]    = __float2half2_rn(0.0f);
+                    if (there && lane / kChunks + kRows * k < left) {
+                        codes[j] = *reinterpret_cast<const uint4*>(from + kRows * k * (HEAD_DIM / 2));
+                        scale[j] = *reinterpret_cast<const half2*>(from_scales + kRows * k * (4 * four_bit_groups(HEAD_DIM)));
+                    }
                 }
-                if (!there && wanted)
+                if (!there && left > 0)
                     atomicOr(c.status, kStatusBadCache);
             }
         };
+        // Where the i-th eight elements of a job's keys go, and the word that has them: threads with a head's second 64 elements begin
+        // with their third, for the banks.
         auto at = [&](unsigned char* stage, int j, int i) -> uint4& {
-            // Chunks of threads with the second 64 elements change places: banks.
-            const int r = r0 + kRows * j, chunk = (q & 1) * 4 + (i ^ (q >> 1) * 2);
-            return *reinterpret_cast<uint4*>(stage + (q >> 1) * kBlock + r * 128 + (chunk ^ (r & 7)) * 16);
+            return *reinterpret_cast<uint4*>(stage + (offset ^ 16 * i) + j * kRows * 128);
         };
-        auto word = [&](const uint4& w, int i) {  // the i-th of the words, in the order of `at`
-            const int k = i ^ (q >> 1) * 2;
-            return k == 0 ? w.x : k == 1 ? w.y : k == 2 ? w.z : w.w;
+        auto word = [&](const uint4& w, int i) {
+            const uint32_t x = q < 2 ? (i == 0 ? w.x : i == 1 ? w.y : i == 2 ? w.z : w.w) : (i == 0 ? w.z : i == 1 ? w.w : i == 2 ? w.x : w.y);
+            return x;
         };
         auto turn = [&](unsigned char* stage, const uint4 (&codes)[kJobs], const half2 (&scale)[kJobs]) {
-            bool beyond = false;
+            half last = __ushort_as_half(0);  // the largest last element: see four_bit_values
 #pragma unroll
             for (int j = 0; j < kJobs; ++j)
-                beyond = beyond || four_bit_beyond(scale[j]);
-            if (__any_sync(0xffffffffu, beyond)) {
+                last = __hmax(last, __hfma(__float2half_rn(15.0f), __low2half(scale[j]), __high2half(scale[j])));
+            if (__any_sync(0xffffffffu, __half_as_ushort(last) == 0x7c00u)) {
 #pragma unroll 1
                 for (int i = 0; i < 4; ++i)
 #pragma unroll
@@ -1353,52 +1361,52 @@ __device__ __forceinline__ void attn_turn_codes(const AttentionParams& p, AttnSh
                         at(stage, j, i) = four_bit_values<true>(word(codes[j], i), scale[j]);
                 return;
             }
+#pragma unroll 1  // (whole 557 us, half of the words at a time 535, a word at a time 666)
+            for (int half = 0; half < 4; half += 2)
 #pragma unroll
-            for (int j = 0; j < kJobs; ++j)
-#pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    at(stage, j, i) = four_bit_values<false>(word(codes[j], i), scale[j]);
+                for (int j = 0; j < kJobs; ++j) {
+                    const bool     second = (half == 0) != (q < 2);  // of the words' two halves
+                    const uint32_t w0 = second ? codes[j].z : codes[j].x, w1 = second ? codes[j].w : codes[j].y;
+                    at(stage, j, half)     = four_bit_values<false>(w0, scale[j]);
+                    at(stage, j, half + 1) = four_bit_values<false>(w1, scale[j]);
+                }
         };
+        // A tile's keys, its values, the next tile's keys and so on through the same code: twice of it do not fit the instruction cache
+        // beside the softmax's (a prompt of 7000 tokens 626 us, so 557).
         int   ids[2], ids_next[2];
-        uint4 k_codes[kJobs], v_codes[kJobs];
-        half2 k_scale[kJobs], v_scale[kJobs];
+        uint4 codes[kJobs], codes_next[kJobs];
+        half2 scale[kJobs], scale_next[kJobs];
         pages(seg.begin, ids);
-        load(p.k_cache, seg.begin, ids, k_codes, k_scale);
-        load(p.v_cache, seg.begin, ids, v_codes, v_scale);
+        load(p.k_cache, seg.begin, ids, codes, scale);
+        load(p.v_cache, seg.begin, ids, codes_next, scale_next);
         pages(seg.begin + 1, ids_next);
+        const int steps = 2 * (seg.end - seg.begin);
 #pragma unroll 1
-        for (int t = seg.begin; t < seg.end; ++t, ++n) {
-            const uint32_t stage = n % kStages, parity = (n / kStages & 1u) ^ 1u;
-            ok = __all_sync(0xffffffffu, attn_wait(&sh.k_empty[stage], parity, sh, c.status));
-            if (!ok)
-                break;
-            turn(k_stages + stage * kTileBytes, k_codes, k_scale);
-            ptx::fence_proxy_async_smem();
-            __syncwarp();
-            if (lane == 0)
-                ptx::mbar_arrive(ptx::smem_u32(&sh.k_full[stage]));
-            load(p.k_cache, t + 1, ids_next, k_codes, k_scale);
-            ok = __all_sync(0xffffffffu, attn_wait(&sh.v_empty[stage], parity, sh, c.status));
+        for (int step = 0; step < steps; ++step) {
+            const int            which = step & 1, t = seg.begin + step / 2;
+            const uint32_t       in = n + step / 2, stage = in % kStages, parity = (in / kStages & 1u) ^ 1u;
+            unsigned char* const to = (which ? v_stages : k_stages) + stage * kTileBytes;
+            ok = __all_sync(0xffffffffu, attn_wait(which ? &sh.v_empty[stage] : &sh.k_empty[stage], parity, sh, c.status));
             if (!ok)
                 break;
             bool odd = false;
-            if (seg.mixed(t)) {
+            if (which && seg.mixed(t)) {
 #pragma unroll
                 for (int j = 0; j < kJobs; ++j)
-                    odd = odd || halves_not_finite(*reinterpret_cast<const uint32_t*>(&v_scale[j])) != 0u;
+                    odd = odd || halves_not_finite(*reinterpret_cast<const uint32_t*>(&scale[j])) != 0u;
                 odd = __any_sync(0xffffffffu, odd);
             }
             if (!odd)
-                turn(v_stages + stage * kTileBytes, v_codes, v_scale);
+                turn(to, codes, scale);
             else {  // values that not all rows see, and that are not finite: zeros in their place
                 const int mixed = seg.mixed_of(t);
 #pragma unroll
                 for (int j = 0; j < kJobs; ++j) {
                     const int  r   = r0 + kRows * j;
-                    const bool bad = halves_not_finite(*reinterpret_cast<const uint32_t*>(&v_scale[j])) != 0u;
+                    const bool bad = halves_not_finite(*reinterpret_cast<const uint32_t*>(&scale[j])) != 0u;
 #pragma unroll 1
                     for (int i = 0; i < 4; ++i)
-                        at(v_stages + stage * kTileBytes, j, i) = bad ? make_uint4(0, 0, 0, 0) : four_bit_values<true>(word(v_codes[j], i), v_scale[j]);
+                        at(to, j, i) = bad ? make_uint4(0, 0, 0, 0) : four_bit_values<true>(word(codes[j], i), scale[j]);
                     if (bad && mixed < AttnSegmentOf<WINDOW>::kMixed) {
                         atomicOr(&list[mixed][r / 32], 1u << r % 32);
                         sh.any_not_finite[number % kAttnSegments] = 1u;
@@ -1408,10 +1416,21 @@ __device__ __forceinline__ void attn_turn_codes(const AttentionParams& p, AttnSh
             ptx::fence_proxy_async_smem();
             __syncwarp();
             if (lane == 0)
-                ptx::mbar_arrive(ptx::smem_u32(&sh.v_clean[stage]));
-            load(p.v_cache, t + 1, ids_next, v_codes, v_scale);
-            pages(t + 2, ids_next);
+                ptx::mbar_arrive(ptx::smem_u32(which ? &sh.v_clean[stage] : &sh.k_full[stage]));
+#pragma unroll
+            for (int j = 0; j < kJobs; ++j) {
+                codes[j] = codes_next[j];
+                scale[j] = scale_next[j];
+            }
+            if (which == 0) {
+                ids[0] = ids_next[0];
+                ids[1] = ids_next[1];
+            }
+            load(which ? p.v_cache : p.k_cache, t + 1, ids, codes_next, scale_next);
+            if (which)
+                pages(t + 2, ids_next);
         }
+        n += steps / 2;
     }
 }
 

@@ -79,8 +79,13 @@ static cudaError_t append(cudaStream_t stream, bool four_bit, const void* QKV, i
     p.q_norm      = static_cast<const half*>(q_norm);
     p.k_norm      = static_cast<const half*>(k_norm);
     p.eps         = eps;
-    auto launch   = [&](auto kernel) {
-        return launch_in_stream_order(kernel, dim3(tokens), dim3(kRotaryThreads), 0, stream, 1, p);
+    int sms       = 0;
+    if (const cudaError_t err = four_multiprocessors(&sms))
+        return err;
+    // As many tokens for a CTA as leave a CTA for each place on the multiprocessors (some four).
+    p.rows      = std::max(1, std::min(kAppendRows, tokens / (4 * sms)));
+    auto launch = [&](auto kernel) {
+        return launch_in_stream_order(kernel, dim3((tokens + p.rows - 1) / p.rows), dim3(kRotaryThreads), 0, stream, 1, p);
     };
     auto of_cache = [&](auto sixteen, auto four) { return four_bit ? launch(four) : launch(sixteen); };
     if (head_dim == 64)
@@ -156,9 +161,11 @@ int FlashLLM_FourBitRead(void* stream, const void* K_cache, const void* V_cache,
     p.out[0]   = static_cast<half*>(K_out);
     p.out[1]   = static_cast<half*>(V_out);
     // As many rows for a CTA as leave several CTAs for each multiprocessor.
-    p.rows      = std::max(1, std::min(kReadRows, tokens / (8 * sms)));
-    auto launch = [&](auto kernel) {
-        return launch_in_stream_order(kernel, dim3((tokens + p.rows - 1) / p.rows), dim3(kReadThreads), 0, static_cast<cudaStream_t>(stream), 1, p);
+    for (p.row_shift = 0; p.row_shift < 4 && tokens >> (p.row_shift + 1) >= 8 * sms;)
+        ++p.row_shift;
+    const int rows   = 1 << p.row_shift;
+    auto      launch = [&](auto kernel) {
+        return launch_in_stream_order(kernel, dim3((tokens + rows - 1) / rows), dim3(kReadThreads), 0, static_cast<cudaStream_t>(stream), 1, p);
     };
     return static_cast<int>(head_dim == 64 ? launch(four_bit_read_kernel<64>) : launch(four_bit_read_kernel<128>));
 }

@@ -45,16 +45,9 @@ __device__ __forceinline__ long long four_bit_scales(const CacheBatch& c, long l
            + in * (4 * four_bit_groups(HEAD_DIM));
 }
 
-// Whether the last of the codes stands for more than fp16 holds (lowest value and step, rounded, can take it there), or the lowest
-// value is infinite, which no append writes.
-__device__ __forceinline__ bool four_bit_beyond(half2 scale)
-{
-    return __hisinf(__hfma(__float2half_rn(15.0f), __low2half(scale), __high2half(scale))) != 0;
-}
-
 // Eight elements, one rounding to fp16 each: product and sum are one operation, a code is exact (four bits put into the mantissa of 1024
-// or, where they lie, of 64 are so much more).  BOUNDED: elements past the largest number of fp16 are that number, unless the lowest
-// value is infinite.
+// or, where they lie, of 64 are so much more).  BOUNDED: lowest value and step, rounded, can take the last codes past the largest
+// number of fp16, which then is the element (unless the lowest value is infinite, which no append writes).
 template<bool BOUNDED>
 __device__ __forceinline__ uint4 four_bit_values(uint32_t codes, half2 scale)
 {
