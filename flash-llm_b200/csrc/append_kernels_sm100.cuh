@@ -17,16 +17,16 @@ struct AppendParams {
 };
 
 // What eight elements add to the smallest and the largest of their 64; minus infinity if one of them fp16 does not hold.
-__device__ __forceinline__ float2 four_bit_range(const float (&x)[8])
+__device__ __forceinline__ float2 four_bit_range(const float2 (&x)[4])
 {
-    float low = x[0], high = x[0], size = fabsf(x[0]);
-    bool  bad = !(size <= 65504.0f);
+    float low = fminf(x[0].x, x[0].y), high = fmaxf(x[0].x, x[0].y), probe = fmaf(x[0].x, 0.0f, x[0].y * 0.0f);
 #pragma unroll
-    for (int i = 1; i < 8; ++i) {
-        low  = fminf(low, x[i]);
-        high = fmaxf(high, x[i]);
-        bad  = bad || !(fabsf(x[i]) <= 65504.0f);
+    for (int k = 1; k < 4; ++k) {
+        low   = fminf(low, fminf(x[k].x, x[k].y));
+        high  = fmaxf(high, fmaxf(x[k].x, x[k].y));
+        probe = fmaf(x[k].x, 0.0f, fmaf(x[k].y, 0.0f, probe));  // no number if one is none or infinite (which min and max may pass over)
     }
+    const bool bad = probe != 0.0f || low < -65504.0f || high > 65504.0f;
     return make_float2(bad ? -CUDART_INF_F : low, high);
 }
 
@@ -40,14 +40,14 @@ __device__ __forceinline__ half2 four_bit_scale(float2 range)
     return __halves2half2(step, low);
 }
 
-__device__ __forceinline__ uint32_t four_bit_pack(const float (&x)[8], half2 scale)
+__device__ __forceinline__ uint32_t four_bit_pack(const float2 (&x)[4], half2 scale)
 {
     const float step = __low2float(scale), low = __high2float(scale);
     uint32_t    codes = 0;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        const float code = fminf(fmaxf(rintf(__fdiv_rn(x[i] - low, step)), 0.0f), 15.0f);
-        codes |= (step > 0.0f ? static_cast<uint32_t>(code) : 0u) << (4 * i);
+    for (int k = 0; k < 8; ++k) {
+        const float code = fminf(fmaxf(rintf(__fdiv_rn((k % 2 ? x[k / 2].y : x[k / 2].x) - low, step)), 0.0f), 15.0f);
+        codes |= (step > 0.0f ? static_cast<uint32_t>(code) : 0u) << (4 * k);
     }
     return codes;
 }
@@ -98,7 +98,9 @@ __global__ void __launch_bounds__(kRotaryThreads) norm_append_kernel(const __gri
 {
     constexpr int        kUnits  = HEAD_DIM / 16;  // of 32 bytes per head
     constexpr int        kGroups = four_bit_groups(HEAD_DIM);
-    __shared__ float2    s_turn[kAppendRows][HEAD_DIM / 2];  // cosine and sine
+    // Cosines and sines, of four pairs at a time: first those of the units' first (in the interleaved layout, first half's), so that
+    // neighbouring units' are neighbours (banks).
+    __shared__ float4    s_cos[kAppendRows][2][kUnits], s_sin[kAppendRows][2][kUnits];
     __shared__ long long s_at[kAppendRows];
     __shared__ int       s_position[kAppendRows];
     const RotaryParams&  r     = p.rotary;
@@ -110,9 +112,13 @@ __global__ void __launch_bounds__(kRotaryThreads) norm_append_kernel(const __gri
     ptx::grid_dependency_wait();
     ptx::grid_launch_dependents();
 
-    // Where a unit's two halves lie in its head: of query and key heads, and of value heads.
-    const bool turned   = part * 16 < r.rotary_dim;
-    const int  a_turned = turned && !INTERLEAVED ? part * 8 : part * 16, z_turned = turned && !INTERLEAVED ? pairs + part * 8 : part * 16 + 8;
+    // Where the unit's two eights of elements lie in its head, such that neighbouring threads' are neighbours: of query and key heads, and
+    // of value heads.  Interleaved pairs lie within an eight; others are one of each, and what is not turned is split in two as well.
+    const int  a_value = part * 8, z_value = HEAD_DIM / 2 + part * 8;
+    const bool paired = part * 16 < r.rotary_dim;
+    const int  a_turned = INTERLEAVED || paired ? a_value : r.rotary_dim + part * 8 - pairs;
+    const int  z_turned = INTERLEAVED ? z_value : paired ? pairs + part * 8 : (HEAD_DIM + r.rotary_dim) / 2 + part * 8 - pairs;
+    const bool turn_a = INTERLEAVED ? a_value < r.rotary_dim : paired, turn_z = INTERLEAVED ? z_value < r.rotary_dim : paired;
     // The thread's next unit: row of the CTA, unit of the row.
     int   i_next = 0, u_next = threadIdx.x;
     uint4 va_next{}, vz_next{};
@@ -124,8 +130,8 @@ __global__ void __launch_bounds__(kRotaryThreads) norm_append_kernel(const __gri
         if (i_next < rows) {
             const bool        value = u_next / kUnits >= r.heads + c.kv_heads;
             const half* const head  = r.qkv + (n0 + i_next) * r.ld_qkv + u_next / kUnits * HEAD_DIM;
-            va_next                 = *reinterpret_cast<const uint4*>(head + (value ? part * 16 : a_turned));
-            vz_next                 = *reinterpret_cast<const uint4*>(head + (value ? part * 16 + 8 : z_turned));
+            va_next                 = *reinterpret_cast<const uint4*>(head + (value ? a_value : a_turned));
+            vz_next                 = *reinterpret_cast<const uint4*>(head + (value ? z_value : z_turned));
         }
     };
     load_next();
@@ -135,7 +141,9 @@ __global__ void __launch_bounds__(kRotaryThreads) norm_append_kernel(const __gri
         const double turns = static_cast<double>(position) * (r.frequencies[pair] * 0.15915494309189535);
         float        sine, cosine;
         sincospif(2.0f * static_cast<float>(turns - rint(turns)), &sine, &cosine);
-        s_turn[i][pair] = make_float2(cosine * r.magnitude, sine * r.magnitude);
+        const int half = INTERLEAVED ? pair / 4 / kUnits : pair / 4 % 2, unit = INTERLEAVED ? pair / 4 % kUnits : pair / 8;
+        reinterpret_cast<float*>(&s_cos[i][half][unit])[pair % 4] = cosine * r.magnitude;
+        reinterpret_cast<float*>(&s_sin[i][half][unit])[pair % 4] = sine * r.magnitude;
     }
     __syncthreads();
 
@@ -145,67 +153,81 @@ __global__ void __launch_bounds__(kRotaryThreads) norm_append_kernel(const __gri
             v = with(v, __shfl_xor_sync(0xffffffffu, v, d));
         return v;
     };
-    const int lane = threadIdx.x & 31;
+    auto unpack = [](const uint4& v, float2 (&x)[4]) {
+        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+            x[k] = __half22float2(*reinterpret_cast<const half2*>(&w[k]));
+    };
+    auto pack = [](const float2 (&x)[4]) {
+        uint32_t w[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const half2 h = __floats2half2_rn(x[k].x, x[k].y);
+            w[k]          = *reinterpret_cast<const uint32_t*>(&h);
+        }
+        return make_uint4(w[0], w[1], w[2], w[3]);
+    };
+    auto      minus = [](float2 v) { return make_float2(-v.x, -v.y); };
+    const int lane  = threadIdx.x & 31;
     for (int done = threadIdx.x - lane; done < all; done += kRotaryThreads) {  // whole warps, for the shuffles
         const bool  there = i_next < rows;
         const int   i = min(i_next, rows - 1), u = u_next;
         const uint4 va = va_next, vz = vz_next;
         u_next += kRotaryThreads;
         load_next();
-        const long long at = s_at[i];
-        const int       head = u / kUnits;
-        const bool      query = head < r.heads, key = !query && head < r.heads + c.kv_heads, value = !query && !key;
-        const int       a = value ? part * 16 : a_turned, z = value ? part * 16 + 8 : z_turned;
-        float           x[8], y[8];
-        unpack_half8(va, x);
-        unpack_half8(vz, y);
+        const int  head = u / kUnits;
+        const bool query = head < r.heads, key = !query && head < r.heads + c.kv_heads, value = !query && !key;
+        const int  a = value ? a_value : a_turned, z = value ? z_value : z_turned;
+        float2     x[4], y[4];
+        unpack(va, x);
+        unpack(vz, y);
         const half* const weights = query ? p.q_norm : key ? p.k_norm : nullptr;
         if (p.q_norm || p.k_norm) {
-            float squares = 0.0f;
+            float2 squares = make_float2(0.0f, 0.0f);
 #pragma unroll
-            for (int k = 0; k < 8; ++k)
-                squares = fmaf(x[k], x[k], fmaf(y[k], y[k], squares));
-            squares = reduce(squares, [](float s, float t) { return s + t; });
+            for (int k = 0; k < 4; ++k)
+                squares = ptx::fma_x2(x[k], x[k], ptx::fma_x2(y[k], y[k], squares));
+            const float all_squares = reduce(squares.x + squares.y, [](float s, float t) { return s + t; });
             if (weights) {
-                const float factor = 1.0f / sqrtf(fmaf(squares, 1.0f / HEAD_DIM, p.eps));
-                float       wa[8], wz[8];
-                unpack_half8(*reinterpret_cast<const uint4*>(weights + a), wa);
-                unpack_half8(*reinterpret_cast<const uint4*>(weights + z), wz);
+                const float  factor = rsqrtf(fmaf(all_squares, 1.0f / HEAD_DIM, p.eps));
+                const float2 both   = make_float2(factor, factor);
+                float2       wa[4], wz[4];
+                unpack(*reinterpret_cast<const uint4*>(weights + a), wa);
+                unpack(*reinterpret_cast<const uint4*>(weights + z), wz);
 #pragma unroll
-                for (int k = 0; k < 8; ++k) {
-                    x[k] = x[k] * factor * wa[k];
-                    y[k] = y[k] * factor * wz[k];
+                for (int k = 0; k < 4; ++k) {
+                    x[k] = ptx::mul_x2(ptx::mul_x2(x[k], both), wa[k]);
+                    y[k] = ptx::mul_x2(ptx::mul_x2(y[k], both), wz[k]);
                 }
             }
         }
-        if (turned && !value) {
-            const float4* const turn = reinterpret_cast<const float4*>(&s_turn[i][part * 8]);  // of two pairs
-            float               co[8], si[8];
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                const float4 two = turn[k];
-                co[2 * k] = two.x, si[2 * k] = two.y, co[2 * k + 1] = two.z, si[2 * k + 1] = two.w;
-            }
+        if (turn_a && !value) {
+            const float4 c0 = s_cos[i][0][part], c1 = s_cos[i][1][part], s0 = s_sin[i][0][part], s1 = s_sin[i][1][part];
+            const float2 co[4] = {make_float2(c0.x, c0.y), make_float2(c0.z, c0.w), make_float2(c1.x, c1.y), make_float2(c1.z, c1.w)};
+            const float2 si[4] = {make_float2(s0.x, s0.y), make_float2(s0.z, s0.w), make_float2(s1.x, s1.y), make_float2(s1.z, s1.w)};
             if constexpr (INTERLEAVED) {
+                auto turn = [](float2 v, float cosine, float sine) {
+                    return ptx::fma_x2(v, make_float2(cosine, cosine), ptx::mul_x2(make_float2(v.y, v.x), make_float2(-sine, sine)));
+                };
 #pragma unroll
                 for (int k = 0; k < 4; ++k) {
-                    const float x0 = x[2 * k], x1 = x[2 * k + 1], y0 = y[2 * k], y1 = y[2 * k + 1];
-                    x[2 * k]     = x0 * co[k] - x1 * si[k];
-                    x[2 * k + 1] = x1 * co[k] + x0 * si[k];
-                    y[2 * k]     = y0 * co[k + 4] - y1 * si[k + 4];
-                    y[2 * k + 1] = y1 * co[k + 4] + y0 * si[k + 4];
+                    x[k] = turn(x[k], k % 2 ? co[k / 2].y : co[k / 2].x, k % 2 ? si[k / 2].y : si[k / 2].x);
+                    if (turn_z)
+                        y[k] = turn(y[k], k % 2 ? co[2 + k / 2].y : co[2 + k / 2].x, k % 2 ? si[2 + k / 2].y : si[2 + k / 2].x);
                 }
             }
             else {
 #pragma unroll
-                for (int k = 0; k < 8; ++k) {
-                    const float x0 = x[k], y0 = y[k];
-                    x[k] = x0 * co[k] - y0 * si[k];
-                    y[k] = y0 * co[k] + x0 * si[k];
+                for (int k = 0; k < 4; ++k) {
+                    const float2 x0 = x[k], y0 = y[k];
+                    x[k] = ptx::fma_x2(x0, co[k], ptx::mul_x2(y0, minus(si[k])));
+                    y[k] = ptx::fma_x2(y0, co[k], ptx::mul_x2(x0, si[k]));
                 }
             }
         }
-        const int h = head - r.heads - (key ? 0 : c.kv_heads);  // key/value head
+        const int       h  = head - r.heads - (key ? 0 : c.kv_heads);  // key/value head
+        const long long at = s_at[i];
         if constexpr (FOUR_BIT) {
             if (__any_sync(0xffffffffu, !query)) {
                 const float2 ra = four_bit_range(x), rz = four_bit_range(y);
@@ -236,8 +258,8 @@ __global__ void __launch_bounds__(kRotaryThreads) norm_append_kernel(const __gri
                                 : (key ? r.k_cache : r.v_cache) + (at + (static_cast<long long>(h) << c.page_shift)) * HEAD_DIM;
         const bool  lost = s_position[i] < 0;  // queries of a sequence that does not fit
         const uint4 zero = make_uint4(0, 0, 0, 0);
-        *reinterpret_cast<uint4*>(dst + a) = lost ? zero : pack_half8(x);
-        *reinterpret_cast<uint4*>(dst + z) = lost ? zero : pack_half8(y);
+        *reinterpret_cast<uint4*>(dst + a) = lost ? zero : pack(x);
+        *reinterpret_cast<uint4*>(dst + z) = lost ? zero : pack(y);
     }
 }
 
@@ -264,26 +286,33 @@ __global__ void __launch_bounds__(kReadThreads) four_bit_read_kernel(const __gri
     ptx::grid_dependency_wait();
     ptx::grid_launch_dependents();
     find_rows<kReadThreads>(c, n0, rows, s_at, s_position);
-    const int units = 2 * c.kv_heads << (p.row_shift + kWordShift), word = threadIdx.x % kWords;
-    const long long width = static_cast<long long>(c.kv_heads) * HEAD_DIM;
+    // A thread has one row's eight elements of every head, or, where rows are few, of every so many heads.
+    const int       word = threadIdx.x % kWords, i = (threadIdx.x >> kWordShift) & ((1 << p.row_shift) - 1);
+    const long long at = i < rows ? s_at[i] : kNobodysRow;
+    if (at == kNobodysRow)
+        return;
+    const int            h0 = threadIdx.x >> (kWordShift + p.row_shift), step = kReadThreads >> (kWordShift + p.row_shift);
+    const long long      page_bytes = static_cast<long long>(four_bit_row_bytes(HEAD_DIM)) << c.page_shift;  // of a head
+    const long long      codes_at = at >= 0 ? four_bit_codes<HEAD_DIM>(c, at) + h0 * page_bytes + 4 * word : 0;
+    const long long      scales_at = at >= 0 ? four_bit_scales<HEAD_DIM>(c, at) + h0 * page_bytes + word / 8 * 4 : 0;
+    const unsigned char *k_codes = p.cache[0] + codes_at, *v_codes = p.cache[1] + codes_at;
+    const unsigned char *k_scale = p.cache[0] + scales_at, *v_scale = p.cache[1] + scales_at;
+    const long long      to = (static_cast<long long>(n0 + i) * c.kv_heads + h0) * HEAD_DIM + 8 * word;
+    half *               k_out = p.out[0] + to, *v_out = p.out[1] + to;
 #pragma unroll 4
-    for (int u = threadIdx.x; u < units; u += kReadThreads) {
-        const int i = (u >> kWordShift) & ((1 << p.row_shift) - 1), which = u >> (p.row_shift + kWordShift), h = which >> 1;
-        if (i >= rows)
-            continue;
-        const long long at = s_at[i];
-        if (at == kNobodysRow)
-            continue;
-        const unsigned char* const cache = which & 1 ? p.cache[1] : p.cache[0];
-        half* const                out   = which & 1 ? p.out[1] : p.out[0];
-        uint4                      v     = make_uint4(0, 0, 0, 0);
+    for (int h = h0; h < c.kv_heads; h += step) {
+        uint32_t k = 0, v = 0;
+        half2    ks = __float2half2_rn(0.0f), vs = ks;
         if (at >= 0) {
-            const long long row   = at + (static_cast<long long>(h) << c.page_shift);
-            const uint32_t  codes = *reinterpret_cast<const uint32_t*>(cache + four_bit_codes<HEAD_DIM>(c, row) + 4 * word);
-            const half2     scale = *reinterpret_cast<const half2*>(cache + four_bit_scales<HEAD_DIM>(c, row) + word / 8 * 4);
-            v                     = four_bit_values<true>(codes, scale);
+            k  = *reinterpret_cast<const uint32_t*>(k_codes);
+            v  = *reinterpret_cast<const uint32_t*>(v_codes);
+            ks = *reinterpret_cast<const half2*>(k_scale);
+            vs = *reinterpret_cast<const half2*>(v_scale);
         }
-        *reinterpret_cast<uint4*>(out + (n0 + i) * width + h * HEAD_DIM + 8 * word) = v;
+        *reinterpret_cast<uint4*>(k_out) = four_bit_values<true>(k, ks);
+        *reinterpret_cast<uint4*>(v_out) = four_bit_values<true>(v, vs);
+        k_codes += step * page_bytes, v_codes += step * page_bytes, k_scale += step * page_bytes, v_scale += step * page_bytes;
+        k_out += step * HEAD_DIM, v_out += step * HEAD_DIM;
     }
 }
 

@@ -82,8 +82,10 @@ static cudaError_t append(cudaStream_t stream, bool four_bit, const void* QKV, i
     int sms       = 0;
     if (const cudaError_t err = four_multiprocessors(&sms))
         return err;
-    // As many tokens for a CTA as leave a CTA for each place on the multiprocessors (some four).
-    p.rows      = std::max(1, std::min(kAppendRows, tokens / (4 * sms)));
+    // As few rounds of CTAs over the multiprocessors, which hold four at a time, as kAppendRows allow, and tokens dealt out evenly over
+    // them (6612 tokens, 9.3 times the places: 39 us with 8 each, 1.4 rounds, ROUNDS with 6).
+    const int places = 4 * sms, rounds = (tokens + kAppendRows * places - 1) / (kAppendRows * places);
+    p.rows           = (tokens + rounds * places - 1) / (rounds * places);
     auto launch = [&](auto kernel) {
         return launch_in_stream_order(kernel, dim3((tokens + p.rows - 1) / p.rows), dim3(kRotaryThreads), 0, stream, 1, p);
     };
