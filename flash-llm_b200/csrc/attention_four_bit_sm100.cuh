@@ -38,7 +38,9 @@ struct FourBitParams {
     unsigned char*       workspace;
     long long            ld_q;
     int                  heads;
-    int                  share;  // query heads per key/value head
+    int                  share;  // query heads per key/value head, and what divides by it (see AttentionParams)
+    unsigned             share_magic;
+    int                  share_shift;
     int                  window;  // keys up to itself that a row sees
     int                  sinks;   // ... and of its sequence's first
     int                  most_rows;  // sequences with more rows (tokens x share) are somebody else's
@@ -81,8 +83,11 @@ struct FourPart {
     int      pad[3];
 };
 
+constexpr int kFourKnown = 384;  // sequences whose sizes are kept in shared memory
+
 struct FourShared {
     unsigned long long before[512];  // units before a thread's sequences
+    int4               known[kFourKnown];  // first row, rows, context, units of the first sequences
     unsigned long long total;
     unsigned long long warp_sums[16];
     FourPart           part[16][2];       // of each warp: a piece of an item begun before it, and one that others end
@@ -139,33 +144,55 @@ __device__ __forceinline__ FourTile four_tile(const FourBitParams& p, int contex
     return t;
 }
 
-// Tiles of a sequence's rows, and the units that each of them counts: at least its blocks and what beginning it takes, the same for
+// Token of a row of a sequence's (tokens x share) rows.
+__device__ __forceinline__ int four_token(const FourBitParams& p, int row)
+{
+    return static_cast<int>((__umulhi(static_cast<unsigned>(row), p.share_magic) + static_cast<unsigned>(row)) >> p.share_shift);
+}
+
+// A sequence's tiles of rows, and the units that each of them counts: at least its blocks and what beginning it takes, the same for
 // all (exact for a single tile; the tiles of longer prompts share a bound).
 struct FourSequence {
-    Sequence s;
-    int      rows, tiles, units;
+    int first, count, context;  // first row, rows of the batch, position of the first
+    int rows, tiles, units;
 };
 
 template<int ROWS, int KEYS>
-__device__ __forceinline__ FourSequence four_sequence(const FourBitParams& p, int b)
+__device__ __forceinline__ FourSequence four_sequence(const FourBitParams& p, int b, int* lost = nullptr)
 {
-    FourSequence q;
-    q.s     = load_sequence(p.batch, b);
-    q.rows  = q.s.count * p.share;
+    const Sequence s = load_sequence(p.batch, b);
+    FourSequence   q{s.first, s.count, s.context, s.count * p.share, 0, 0};
+    if (lost)
+        *lost = s.lost;
     if (q.rows > p.most_rows)
-        q.rows = 0;
+        q.rows = q.count = 0;
     q.tiles = (q.rows + ROWS - 1) / ROWS;
-    q.units = 0;
     if (q.tiles == 1)
-        q.units = four_tile<KEYS>(p, q.s.context, 0, q.s.count - 1).blocks + kFourExtra;
+        q.units = four_tile<KEYS>(p, q.context, 0, q.count - 1).blocks + kFourExtra;
     else if (q.tiles > 1) {
-        const long long all = (static_cast<long long>(q.s.context) + q.s.count + KEYS - 1) / KEYS;
+        const long long all = (static_cast<long long>(q.context) + q.count + KEYS - 1) / KEYS;
         // Behind the sinks: a window's keys and those of the tile's tokens, wherever blocks begin.
-        const long long seen = (static_cast<long long>(min(p.sinks, q.s.context + q.s.count)) + KEYS - 1) / KEYS
+        const long long seen = (static_cast<long long>(min(p.sinks, q.context + q.count)) + KEYS - 1) / KEYS
                                + (static_cast<long long>(p.window) + ROWS + 2 * KEYS) / KEYS;
         q.units = static_cast<int>(min(all, seen)) + kFourExtra;
     }
     return q;
+}
+
+// ... what the plan has kept of it.
+template<int ROWS, int KEYS>
+__device__ __forceinline__ FourSequence four_sequence(const FourBitParams& p, const FourShared& sh, int b)
+{
+    if (b >= kFourKnown)
+        return four_sequence<ROWS, KEYS>(p, b);
+    const int4 known = sh.known[b];
+    return FourSequence{known.x, known.y, known.z, known.y * p.share, (known.y * p.share + ROWS - 1) / ROWS, known.w};
+}
+
+// a / b, of 32 bits where they are that.
+__device__ __forceinline__ unsigned long long four_divide(unsigned long long a, unsigned long long b)
+{
+    return ((a | b) >> 32) == 0 ? static_cast<unsigned>(a) / static_cast<unsigned>(b) : a / b;
 }
 
 // ---------------------------------------------------------------- pieces of the kernel
@@ -219,28 +246,36 @@ __device__ __forceinline__ int four_value_place(int key)
     return (key & 8) | (key & 1) << 2 | (key >> 1 & 3);
 }
 
-// Adds up one item's parts, in key order, for all threads of the CTA: `part(i)` is the i-th of `count`: its maxima and sums of rows
-// and its outputs.  Rows go to `out_row(row)`, or, where the item has more parts elsewhere, to the workspace.
+// Adds up one item's parts, in key order, for all threads of the CTA: `stats(i, row)` is the i-th part's maximum and sum of a row,
+// `sums(i)` its outputs.  Four columns of a row for a thread; four parts' loads are under way at a time.
 template<int HEAD_DIM, typename Stats, typename Sums, typename Store>
 __device__ __forceinline__ void four_add_up(int count, int rows, Stats&& stats, Sums&& sums, Store&& store)
 {
-    for (int u = threadIdx.x; u < rows * (HEAD_DIM / 8); u += blockDim.x) {
-        const int row = u / (HEAD_DIM / 8), column = u % (HEAD_DIM / 8) * 8;
+    for (int u = threadIdx.x; u < rows * (HEAD_DIM / 4); u += blockDim.x) {
+        const int row = u / (HEAD_DIM / 4), column = u % (HEAD_DIM / 4) * 4;
         float     top = -CUDART_INF_F;
+#pragma unroll 4
         for (int i = 0; i < count; ++i)
             top = fmaxf(top, stats(i, row).x);
-        float o[8] = {}, sum = 0.0f;
+        float4 o   = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        float  sum = 0.0f;
+#pragma unroll 4
         for (int i = 0; i < count; ++i) {
-            const float2  s    = stats(i, row);
-            const float   keep = four_weight(s.x, top);
-            const float4* from = reinterpret_cast<const float4*>(sums(i) + row * HEAD_DIM + column);
-            const float4  x = from[0], y = from[1];
-            sum             = fmaf(s.y, keep, sum);
-            o[0] = fmaf(x.x, keep, o[0]), o[1] = fmaf(x.y, keep, o[1]), o[2] = fmaf(x.z, keep, o[2]), o[3] = fmaf(x.w, keep, o[3]);
-            o[4] = fmaf(y.x, keep, o[4]), o[5] = fmaf(y.y, keep, o[5]), o[6] = fmaf(y.z, keep, o[6]), o[7] = fmaf(y.w, keep, o[7]);
+            const float2 s    = stats(i, row);
+            const float4 x    = *reinterpret_cast<const float4*>(sums(i) + row * HEAD_DIM + column);
+            const float  keep = four_weight(s.x, top);
+            sum               = fmaf(s.y, keep, sum);
+            o                 = make_float4(fmaf(x.x, keep, o.x), fmaf(x.y, keep, o.y), fmaf(x.z, keep, o.z), fmaf(x.w, keep, o.w));
         }
         store(row, column, top, sum, o);
     }
+}
+
+// Four outputs of a row, divided by its sum.
+__device__ __forceinline__ uint2 four_outputs(float4 o, float sum)
+{
+    const float inverse = sum == 0.0f ? 0.0f : 1.0f / sum;
+    return make_uint2(attn_pack_bounded(o.x * inverse, o.y * inverse), attn_pack_bounded(o.z * inverse, o.w * inverse));
 }
 
 // Eight outputs of a row, divided by its sum.
@@ -254,7 +289,7 @@ __device__ __forceinline__ uint4 four_outputs(const float (&o)[8], float sum)
 template<int HEAD_DIM>
 __device__ __forceinline__ half* four_out(const FourBitParams& p, int first, int head, int row)
 {
-    const int token = row / p.share;
+    const int token = four_token(p, row);
     return p.out + (static_cast<long long>(first + token) * p.heads + head * p.share + (row - token * p.share)) * HEAD_DIM;
 }
 
@@ -297,7 +332,7 @@ __global__ void __launch_bounds__(four_warps(TILES) * 32, 1) four_bit_attention_
     ptx::grid_launch_dependents();
 
     // ---- where each warp's share begins: a thread counts the units of a few sequences in a row
-    const int per_thread = (c.sequences + kThreads - 1) / kThreads;
+    const int per_thread = c.sequences <= kThreads ? 1 : (c.sequences + kThreads - 1) / kThreads;
     {
         unsigned long long mine = 0;
         bool               lost = false;
@@ -305,9 +340,12 @@ __global__ void __launch_bounds__(four_warps(TILES) * 32, 1) four_bit_attention_
             const int b = threadIdx.x * per_thread + k;
             if (b >= c.sequences)
                 break;
-            const FourSequence q = four_sequence<kRows, kKeys>(p, b);
-            mine += static_cast<unsigned long long>(q.tiles) * q.units * c.kv_heads;
-            lost = lost || q.s.lost > 0;
+            int                rows_lost;
+            const FourSequence q = four_sequence<kRows, kKeys>(p, b, &rows_lost);
+            mine += static_cast<unsigned long long>(q.tiles) * (static_cast<unsigned long long>(q.units) * c.kv_heads);
+            lost = lost || rows_lost > 0;
+            if (b < kFourKnown)
+                sh.known[b] = make_int4(q.first, q.count, q.context, q.units);
         }
         const unsigned long long upto = attn_warp_scan(mine);
         if (lane == 31)
@@ -323,8 +361,9 @@ __global__ void __launch_bounds__(four_warps(TILES) * 32, 1) four_bit_attention_
             }
         }
         unsigned long long before = upto - mine;
-        for (int w = 0; w < warp; ++w)
-            before += sh.warp_sums[w];
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w)
+            before += w < warp ? sh.warp_sums[w] : 0;
         sh.before[threadIdx.x] = before;
         if (threadIdx.x == kThreads - 1)
             sh.total = before + mine;
@@ -337,10 +376,10 @@ __global__ void __launch_bounds__(four_warps(TILES) * 32, 1) four_bit_attention_
         return;
     }
     // Small calls take as few warps of each CTA as leave them a few blocks each.
-    const unsigned long long least = kFourExtra + 2, all = static_cast<unsigned long long>(gridDim.x) * kWarps;
-    const int                busy  = static_cast<int>(min(static_cast<unsigned long long>(kWarps), (total / least + gridDim.x) / gridDim.x));
-    const unsigned long long workers = busy == kWarps ? all : static_cast<unsigned long long>(gridDim.x) * busy;
-    const unsigned long long share   = (total + workers - 1) / workers;
+    constexpr unsigned       kLeast = kFourExtra + 2;
+    const int                busy   = total >= static_cast<unsigned long long>(kLeast) * kWarps * gridDim.x ? kWarps : static_cast<int>(total) / static_cast<int>(kLeast * gridDim.x) + 1;
+    const unsigned           workers = gridDim.x * busy;
+    const unsigned long long share   = four_divide(total + workers - 1, workers);
     const unsigned long long worker  = static_cast<unsigned long long>(blockIdx.x) * busy + warp;
     unsigned long long       u0 = min(total, share * worker), u1 = warp < busy ? min(total, u0 + share) : u0;
 
@@ -371,23 +410,24 @@ __global__ void __launch_bounds__(four_warps(TILES) * 32, 1) four_bit_attention_
         // (several threads may have the same count: the last of them has units)
         unsigned long long at = sh.before[lo];
         int                b  = lo * per_thread;
-        FourSequence       q  = four_sequence<kRows, kKeys>(p, b);
-        auto               whole = [&]() { return static_cast<unsigned long long>(q.tiles) * q.units * c.kv_heads; };
+        FourSequence       q  = four_sequence<kRows, kKeys>(p, sh, b);
+        auto               whole = [&]() { return static_cast<unsigned long long>(q.tiles) * (static_cast<unsigned long long>(q.units) * c.kv_heads); };
         while (at + whole() <= u0 && b + 1 < c.sequences) {
             at += whole();
-            q = four_sequence<kRows, kKeys>(p, ++b);
+            q = four_sequence<kRows, kKeys>(p, sh, ++b);
         }
-        unsigned long long in   = u0 - at;  // unit of the sequence
+        const unsigned long long in       = u0 - at;  // unit of the sequence
         const unsigned long long per_tile = static_cast<unsigned long long>(max(q.units, 1)) * c.kv_heads;
-        int                tile = static_cast<int>(in / per_tile);
-        int                head = static_cast<int>(in % per_tile / max(q.units, 1));
-        int                unit = static_cast<int>(in % per_tile % max(q.units, 1));
+        int                      tile     = q.tiles > 1 ? static_cast<int>(four_divide(in, per_tile)) : 0;
+        const unsigned long long in_tile  = in - tile * per_tile;
+        int                      head     = static_cast<int>(four_divide(in_tile, max(q.units, 1)));
+        int                      unit     = static_cast<int>(in_tile - static_cast<unsigned long long>(head) * max(q.units, 1));
         unsigned long long left = u1 - u0;
 
         while (left > 0) {
             // ---- a piece of an item
-            const int row0 = tile * kRows, rows = min(kRows, q.rows - row0);
-            const FourTile sight = four_tile<kKeys>(p, q.s.context, row0 / p.share, (row0 + rows - 1) / p.share);
+            const int row0 = tile * kRows, rows = min(kRows, q.rows - row0), token0 = four_token(p, row0), token1 = four_token(p, row0 + rows - 1);
+            const FourTile sight = four_tile<kKeys>(p, q.context, token0, token1);
             const int      upto  = static_cast<int>(min(static_cast<unsigned long long>(q.units), unit + left));
             // Units of the tile to its blocks: exact where the tile's blocks are what it counts, in proportion where they are fewer.
             auto cut = [&](int x) {
@@ -397,9 +437,21 @@ __global__ void __launch_bounds__(four_warps(TILES) * 32, 1) four_bit_attention_
             const int begin = cut(unit), end = cut(upto);
             left -= upto - unit;
             if (begin < end) {
+                // The rows of Q, on their way while pages are looked up.
+                uint4 q_raw[TILES][kGroups][2];
+#pragma unroll
+                for (int n = 0; n < TILES; ++n) {
+                    const int         row = 8 * n + g, token = four_token(p, row0 + row);
+                    const half* const from = p.q + (q.first + token) * p.ld_q + static_cast<long long>(head * p.share + row0 + row - token * p.share) * HEAD_DIM;
+#pragma unroll
+                    for (int gr = 0; gr < kGroups; ++gr)
+#pragma unroll
+                        for (int w = 0; w < 2; ++w)
+                            q_raw[n][gr][w] = row < rows ? *reinterpret_cast<const uint4*>(from + gr * kFourBitGroup + 16 * t + 8 * w) : make_uint4(0, 0, 0, 0);
+                }
                 const int* const table = c.page_table + static_cast<long long>(b) * c.table_width;
                 auto key_of = [&](int block) { return (block + (block < sight.skip_from ? 0 : sight.skip)) * kKeys; };
-                const int keys = q.s.context + (row0 + rows - 1) / p.share + 1;  // none at or behind this is seen
+                const int keys = q.context + token1 + 1;  // none at or behind this is seen
                 // Page ids of 32 sixteens at a time, a lane each, the next 32 ahead of their use; -1: reads as zeros.
                 auto ids_from = [&](int block) {
                     block += lane / kSixteens;
@@ -462,17 +514,15 @@ __global__ void __launch_bounds__(four_warps(TILES) * 32, 1) four_bit_attention_
                 int      limit[TILES][2], low[TILES][2];
                 float    slope[TILES][2];
                 // Keys from the one on (or sinks) and before the other are seen by all rows.
-                const int seen_from = q.s.context + (row0 + rows - 1) / p.share - p.window + 1, seen_upto = q.s.context + row0 / p.share + 1;
+                const int seen_from = q.context + token1 - p.window + 1, seen_upto = q.context + token0 + 1;
 #pragma unroll
                 for (int n = 0; n < TILES; ++n) {
-                    const int  row = 8 * n + g, token = (row0 + row) / p.share;
-                    const half* from = p.q + (q.s.first + token) * p.ld_q + static_cast<long long>(head * p.share + row0 + row - token * p.share) * HEAD_DIM;
 #pragma unroll
                     for (int gr = 0; gr < kGroups; ++gr) {
                         float sum = 0.0f;
 #pragma unroll
                         for (int w = 0; w < 2; ++w) {
-                            const uint4 x = row < rows ? *reinterpret_cast<const uint4*>(from + gr * kFourBitGroup + 16 * t + 8 * w) : make_uint4(0, 0, 0, 0);
+                            const uint4 x = q_raw[n][gr][w];
                             // Elements i and i + 4 of a word's eight are neighbours in the products: even ones, odd ones.
                             qf[n][4 * gr + 2 * w][0]     = __byte_perm(x.x, x.z, 0x5410);
                             qf[n][4 * gr + 2 * w][1]     = __byte_perm(x.y, x.w, 0x5410);
@@ -491,7 +541,7 @@ __global__ void __launch_bounds__(four_warps(TILES) * 32, 1) four_bit_attention_
                     }
 #pragma unroll
                     for (int e = 0; e < 2; ++e) {
-                        const int r = 8 * n + 2 * t + e, tok = (row0 + min(r, rows - 1)) / p.share, at_key = q.s.context + tok;
+                        const int r = 8 * n + 2 * t + e, tok = four_token(p, row0 + min(r, rows - 1)), at_key = q.context + tok;
                         limit[n][e] = r < rows ? at_key + 1 : 0;
                         low[n][e]   = at_key - p.window + 1;
                         if constexpr (!PLAIN)
@@ -807,8 +857,10 @@ __global__ void __launch_bounds__(four_warps(TILES) * 32, 1) four_bit_attention_
                             if (row >= rows)
                                 continue;
                             const int column = gr * kFourBitGroup + 8 * g;
-                            if (item)
-                                *reinterpret_cast<uint4*>(four_out<HEAD_DIM>(p, q.s.first, head, row0 + row) + column) = four_outputs(o, all_sum);
+                            if (item) {
+                                const uint2 x = four_outputs(make_float4(o[0], o[1], o[2], o[3]), all_sum), y = four_outputs(make_float4(o[4], o[5], o[6], o[7]), all_sum);
+                                *reinterpret_cast<uint4*>(four_out<HEAD_DIM>(p, q.first, head, row0 + row) + column) = make_uint4(x.x, x.y, y.x, y.y);
+                            }
                             else {
                                 float4* const at4 = reinterpret_cast<float4*>(to + row * HEAD_DIM + column);
                                 at4[0]            = make_float4(o[0], o[1], o[2], o[3]);
@@ -819,7 +871,7 @@ __global__ void __launch_bounds__(four_warps(TILES) * 32, 1) four_bit_attention_
                             sh.stats[warp][slot][row] = make_float2(top[n][e], all_sum);
                     }
                 if (!item && lane == 0)
-                    sh.part[warp][slot] = FourPart{kind, q.s.first, row0, rows, head, {0, 0, 0}};
+                    sh.part[warp][slot] = FourPart{kind, q.first, row0, rows, head, {0, 0, 0}};
                 __syncwarp();
             }
             else if (begin > 0) {
@@ -830,7 +882,7 @@ __global__ void __launch_bounds__(four_warps(TILES) * 32, 1) four_bit_attention_
                 if (lane < rows)
                     sh.stats[warp][0][lane] = make_float2(-CUDART_INF_F, 0.0f);
                 if (lane == 0)
-                    sh.part[warp][0] = FourPart{kPartContinues, q.s.first, row0, rows, head, {0, 0, 0}};
+                    sh.part[warp][0] = FourPart{kPartContinues, q.first, row0, rows, head, {0, 0, 0}};
             }
             // ---- the next item
             if (left == 0)
@@ -847,7 +899,7 @@ __global__ void __launch_bounds__(four_warps(TILES) * 32, 1) four_bit_attention_
                                 left = 0;
                                 break;
                             }
-                            q = four_sequence<kRows, kKeys>(p, b);
+                            q = four_sequence<kRows, kKeys>(p, sh, b);
                         } while (q.tiles == 0);
                     }
                 }
@@ -859,46 +911,38 @@ __global__ void __launch_bounds__(four_warps(TILES) * 32, 1) four_bit_attention_
     // ---- items that several warps have worked on, in key order; what began before this CTA, or ends behind it, to the workspace
     FourPart* const parts = reinterpret_cast<FourPart*>(p.workspace) + 2 * blockIdx.x;
     bool            written[2] = {false, false};
-    auto            part_of = [&](int i) -> const FourPart& { return sh.part[i >> 1][i & 1]; };  // i = 2 warp + slot
-    for (int i = 0; i < 2 * kWarps;) {
-        const FourPart from = part_of(i);
-        if (from.kind == kPartNone) {
-            ++i;
-            continue;
-        }
-        int      list[kWarps + 1], count = 0;
-        unsigned last = from.kind;
-        for (; i < 2 * kWarps; ++i) {
-            const unsigned kind = part_of(i).kind;
-            if (kind == kPartNone)
-                continue;
-            if (count > 0 && kind == kPartBegins)
-                break;  // (the one before has ended)
-            list[count++] = i;
-            last          = kind;
-            if (kind == kPartEnds) {
-                ++i;
-                break;
-            }
-        }
-        const bool item = from.kind == kPartBegins && last == kPartEnds;
-        const unsigned kind = from.kind == kPartBegins ? kPartBegins : last == kPartEnds ? kPartEnds : kPartContinues;
-        const int  slot = kind == kPartBegins ? 1 : 0;
-        float2* const stats = reinterpret_cast<float2*>(p.workspace + four_stats_offset(gridDim.x)) + (2 * blockIdx.x + slot) * 16;
-        float* const  sums  = reinterpret_cast<float*>(p.workspace + four_sums_offset(gridDim.x)) + static_cast<size_t>(2 * blockIdx.x + slot) * 16 * HEAD_DIM;
+    // Parts in key order, of warp i / 2: that is their kinds, and which of them belong to the item at hand.
+    const unsigned kind_here = lane < 2 * kWarps ? sh.part[lane >> 1][lane & 1].kind : kPartNone;
+    const unsigned begins = __ballot_sync(0xffffffffu, kind_here == kPartBegins), ends = __ballot_sync(0xffffffffu, kind_here == kPartEnds);
+    unsigned       present = __ballot_sync(0xffffffffu, kind_here != kPartNone);
+    while (present) {
+        const unsigned first_bit = present & -present;
+        // Up to the part that ends the item, or before the next that begins one.
+        const unsigned stop  = (ends & present) ? (ends & present) & -(ends & present) : 0x80000000u;
+        const unsigned other = begins & present & ~first_bit;
+        unsigned       mine  = present & (stop | (stop - 1));
+        if (other)
+            mine &= (other & -other) - 1;
+        present &= ~mine;
+        const FourPart  from  = sh.part[(__ffs(mine) - 1) >> 1][(__ffs(mine) - 1) & 1];
+        const bool      ended = (mine & ends) != 0, item = from.kind == kPartBegins && ended;
+        const unsigned  kind  = from.kind == kPartBegins ? kPartBegins : ended ? kPartEnds : kPartContinues;
+        const int       slot  = kind == kPartBegins ? 1 : 0;
+        float2* const   stats = reinterpret_cast<float2*>(p.workspace + four_stats_offset(gridDim.x)) + (2 * blockIdx.x + slot) * 16;
+        float* const    sums  = reinterpret_cast<float*>(p.workspace + four_sums_offset(gridDim.x)) + static_cast<size_t>(2 * blockIdx.x + slot) * 16 * HEAD_DIM;
+        // The parts are those of neighbouring warps, the first of which may be the last piece of its warp; the others are first pieces.
+        const int begin = (__ffs(mine) - 1) >> 1, tail = (__ffs(mine) - 1) & 1, count = (31 - __clz(mine)) / 2 - begin + 1;
         four_add_up<HEAD_DIM>(
-            count, from.rows, [&](int k, int row) { return sh.stats[list[k] >> 1][list[k] & 1][row]; },
+            count, from.rows, [&](int k, int row) { return (mine >> (2 * (begin + k) + (k == 0 ? tail : 0)) & 1u) ? sh.stats[begin + k][k == 0 ? tail : 0][row] : make_float2(-CUDART_INF_F, 0.0f); },
             [&](int k) {
-                const int w = list[k] >> 1;
-                return reinterpret_cast<const float*>(list[k] & 1 ? smem + w * (kStages * kStageBytes) : first_sums + w * four_rows_bytes(HEAD_DIM, TILES));
+                const int w = begin + k;
+                return reinterpret_cast<const float*>(k == 0 && tail ? smem + w * (kStages * kStageBytes) : first_sums + w * four_rows_bytes(HEAD_DIM, TILES));
             },
-            [&](int row, int column, float top, float sum, const float (&o)[8]) {
+            [&](int row, int column, float top, float sum, float4 o) {
                 if (item)
-                    *reinterpret_cast<uint4*>(four_out<HEAD_DIM>(p, from.first, from.head, from.row0 + row) + column) = four_outputs(o, sum);
+                    *reinterpret_cast<uint2*>(four_out<HEAD_DIM>(p, from.first, from.head, from.row0 + row) + column) = four_outputs(o, sum);
                 else {
-                    float4* const to = reinterpret_cast<float4*>(sums + row * HEAD_DIM + column);
-                    to[0]            = make_float4(o[0], o[1], o[2], o[3]);
-                    to[1]            = make_float4(o[4], o[5], o[6], o[7]);
+                    *reinterpret_cast<float4*>(sums + row * HEAD_DIM + column) = o;
                     if (column == 0)
                         stats[row] = make_float2(top, sum);
                 }
@@ -941,8 +985,8 @@ __global__ void __launch_bounds__(256) four_bit_join_kernel(const __grid_constan
     four_add_up<HEAD_DIM>(
         cta - begin + 1, last.rows, [&](int i, int row) { return stats[slot(i) * 16 + row]; },
         [&](int i) { return sums + slot(i) * 16 * HEAD_DIM; },
-        [&](int row, int column, float, float sum, const float (&o)[8]) {
-            *reinterpret_cast<uint4*>(four_out<HEAD_DIM>(p, last.first, last.head, last.row0 + row) + column) = four_outputs(o, sum);
+        [&](int row, int column, float, float sum, float4 o) {
+            *reinterpret_cast<uint2*>(four_out<HEAD_DIM>(p, last.first, last.head, last.row0 + row) + column) = four_outputs(o, sum);
         });
 }
 

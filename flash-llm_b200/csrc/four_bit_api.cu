@@ -199,7 +199,11 @@ int FlashLLM_FourBitAttention(void* stream, const void* Q, int ld_q, const void*
     p.workspace = static_cast<unsigned char*>(workspace);
     p.ld_q      = ld_q;
     p.heads     = heads;
-    p.share     = heads / kv_heads;
+    AttentionParams a{};
+    attn_set_heads(&a, heads, kv_heads);
+    p.share       = a.share;
+    p.share_magic = a.share_magic;
+    p.share_shift = a.share_shift;
     p.window    = window > 0 ? window : 0x7fffffff;
     p.sinks     = window > 0 ? sinks : 0;
     // Sequences of many rows are the other kernel's, which the host cannot tell: where there is a token for each sequence, or fewer
@@ -219,7 +223,6 @@ int FlashLLM_FourBitAttention(void* stream, const void* Q, int ld_q, const void*
     const cudaError_t err = head_dim == 64 ? (two ? few(Dim64{}, Two{}) : few(Dim64{}, One{})) : (two ? few(Dim128{}, Two{}) : few(Dim128{}, One{}));
     if (err != cudaSuccess || !many)
         return static_cast<int>(err);
-    AttentionParams a{};
     a.batch      = p.batch;
     a.q          = p.q;
     a.out        = p.out;
@@ -233,7 +236,6 @@ int FlashLLM_FourBitAttention(void* stream, const void* Q, int ld_q, const void*
     a.window     = p.window;
     a.sinks      = p.sinks;
     a.least_rows = kFourMostRows + 1;
-    attn_set_heads(&a, heads, kv_heads);
     return static_cast<int>(launch_rows_over_four_bits(s, a, head_dim));
 }
 
