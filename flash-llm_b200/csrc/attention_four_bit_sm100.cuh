@@ -179,12 +179,18 @@ __device__ __forceinline__ FourSequence four_sequence(const FourBitParams& p, in
     return q;
 }
 
+template<int ROWS, int KEYS>
+__device__ __noinline__ FourSequence four_sequence_again(const FourBitParams& p, int b)
+{
+    return four_sequence<ROWS, KEYS>(p, b);
+}
+
 // ... what the plan has kept of it.
 template<int ROWS, int KEYS>
 __device__ __forceinline__ FourSequence four_sequence(const FourBitParams& p, const FourShared& sh, int b)
 {
     if (b >= kFourKnown)
-        return four_sequence<ROWS, KEYS>(p, b);
+        return four_sequence_again<ROWS, KEYS>(p, b);
     const int4 known = sh.known[b];
     return FourSequence{known.x, known.y, known.z, known.y * p.share, (known.y * p.share + ROWS - 1) / ROWS, known.w};
 }
@@ -246,29 +252,27 @@ __device__ __forceinline__ int four_value_place(int key)
     return (key & 8) | (key & 1) << 2 | (key >> 1 & 3);
 }
 
-// Adds up one item's parts, in key order, for all threads of the CTA: `stats(i, row)` is the i-th part's maximum and sum of a row,
-// `sums(i)` its outputs.  Four columns of a row for a thread; four parts' loads are under way at a time.
-template<int HEAD_DIM, typename Stats, typename Sums, typename Store>
-__device__ __forceinline__ void four_add_up(int count, int rows, Stats&& stats, Sums&& sums, Store&& store)
+// Adds up four columns of a row of one item's parts, in key order: `stats(i)` is the i-th part's maximum and sum of the row, `sums(i)`
+// its outputs of these columns.  UNROLL parts' loads are under way at a time.
+template<int UNROLL, typename Stats, typename Sums>
+__device__ __forceinline__ float4 four_add_up(int count, Stats&& stats, Sums&& sums, float2& all)
 {
-    for (int u = threadIdx.x; u < rows * (HEAD_DIM / 4); u += blockDim.x) {
-        const int row = u / (HEAD_DIM / 4), column = u % (HEAD_DIM / 4) * 4;
-        float     top = -CUDART_INF_F;
-#pragma unroll 4
-        for (int i = 0; i < count; ++i)
-            top = fmaxf(top, stats(i, row).x);
-        float4 o   = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        float  sum = 0.0f;
-#pragma unroll 4
-        for (int i = 0; i < count; ++i) {
-            const float2 s    = stats(i, row);
-            const float4 x    = *reinterpret_cast<const float4*>(sums(i) + row * HEAD_DIM + column);
-            const float  keep = four_weight(s.x, top);
-            sum               = fmaf(s.y, keep, sum);
-            o                 = make_float4(fmaf(x.x, keep, o.x), fmaf(x.y, keep, o.y), fmaf(x.z, keep, o.z), fmaf(x.w, keep, o.w));
-        }
-        store(row, column, top, sum, o);
+    float top = -CUDART_INF_F;
+#pragma unroll UNROLL
+    for (int i = 0; i < count; ++i)
+        top = fmaxf(top, stats(i).x);
+    float4 o   = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    float  sum = 0.0f;
+#pragma unroll UNROLL
+    for (int i = 0; i < count; ++i) {
+        const float2 s    = stats(i);
+        const float4 x    = *sums(i);
+        const float  keep = four_weight(s.x, top);
+        sum               = fmaf(s.y, keep, sum);
+        o                 = make_float4(fmaf(x.x, keep, o.x), fmaf(x.y, keep, o.y), fmaf(x.z, keep, o.z), fmaf(x.w, keep, o.w));
     }
+    all = make_float2(top, sum);
+    return o;
 }
 
 // Four outputs of a row, divided by its sum.
@@ -504,9 +508,6 @@ __global__ void __launch_bounds__(four_warps(TILES) * 32, 1) four_bit_attention_
                     four_copies_done();
                 };
                 copied = 0;
-#pragma unroll
-                for (int i = 0; i < kStages - 1; ++i)
-                    copy(i);
 
                 // ---- the rows: queries as the products' columns, and what they see
                 uint32_t qf[TILES][4 * kGroups][2];
@@ -587,11 +588,16 @@ __global__ void __launch_bounds__(four_warps(TILES) * 32, 1) four_bit_attention_
                 float    against[TILES][2] = {};  // the maximum, 0 where there is none
                 uint32_t at_hand = 0;             // the block's place in the ring
 
+                // The first steps only copy: code that is executed once costs its fetch, and this is not there twice.
 #pragma unroll 1
-                for (int i = 0; i < end - begin; ++i) {
-                    four_copies_wait<kStages - 2>();
-                    __syncwarp();  // the block is there, and the one before it no longer read
+                for (int i = 1 - kStages; i < end - begin; ++i) {
+                    if (i >= 0) {
+                        four_copies_wait<kStages - 2>();
+                        __syncwarp();  // the block is there, and the one before it no longer read
+                    }
                     copy(i + kStages - 1);
+                    if (i < 0)
+                        continue;
                     const unsigned char* const stage = ring_ptr + at_hand;
                     const int                  key0  = key_of(begin + i);
                     at_hand = at_hand == (kStages - 1) * kStageBytes ? 0 : at_hand + kStageBytes;
@@ -909,52 +915,69 @@ __global__ void __launch_bounds__(four_warps(TILES) * 32, 1) four_bit_attention_
     __syncthreads();
 
     // ---- items that several warps have worked on, in key order; what began before this CTA, or ends behind it, to the workspace
-    FourPart* const parts = reinterpret_cast<FourPart*>(p.workspace) + 2 * blockIdx.x;
-    bool            written[2] = {false, false};
-    // Parts in key order, of warp i / 2: that is their kinds, and which of them belong to the item at hand.
+    // Parts in key order, of warp i / 2: that is their kinds, and which of them belong to an item.  All items side by side.
     const unsigned kind_here = lane < 2 * kWarps ? sh.part[lane >> 1][lane & 1].kind : kPartNone;
     const unsigned begins = __ballot_sync(0xffffffffu, kind_here == kPartBegins), ends = __ballot_sync(0xffffffffu, kind_here == kPartEnds);
-    unsigned       present = __ballot_sync(0xffffffffu, kind_here != kPartNone);
-    while (present) {
-        const unsigned first_bit = present & -present;
-        // Up to the part that ends the item, or before the next that begins one.
-        const unsigned stop  = (ends & present) ? (ends & present) & -(ends & present) : 0x80000000u;
-        const unsigned other = begins & present & ~first_bit;
-        unsigned       mine  = present & (stop | (stop - 1));
-        if (other)
-            mine &= (other & -other) - 1;
-        present &= ~mine;
-        const FourPart  from  = sh.part[(__ffs(mine) - 1) >> 1][(__ffs(mine) - 1) & 1];
+    const unsigned all_present = __ballot_sync(0xffffffffu, kind_here != kPartNone);
+    constexpr int  kPerItem = kRows * (HEAD_DIM / 4);
+    unsigned       present = all_present;
+    int            number  = 0;  // of the item that `present` begins with
+#pragma unroll 1
+    for (int u = threadIdx.x;; u += kThreads) {
+        unsigned mine = 0;
+#pragma unroll 1
+        for (;;) {
+            // Up to the part that ends the item, or before the next that begins one.
+            const unsigned ending = ends & present, other = begins & present & (present - 1);
+            mine = present;
+            if (ending)
+                mine &= ending ^ (ending - 1);
+            if (other)
+                mine &= (other & -other) - 1;
+            if (number == u / kPerItem || present == 0)
+                break;
+            present &= ~mine;
+            ++number;
+        }
+        if (mine == 0)
+            break;
+        const int       row = u / (HEAD_DIM / 4) % kRows, column = u % (HEAD_DIM / 4) * 4;
+        // The parts are those of neighbouring warps, the first of which may be the last piece of its warp; the others are first pieces.
+        const int       begin = (__ffs(mine) - 1) >> 1, tail = (__ffs(mine) - 1) & 1, count = (31 - __clz(mine)) / 2 - begin + 1;
+        const FourPart& from  = sh.part[begin][tail];
         const bool      ended = (mine & ends) != 0, item = from.kind == kPartBegins && ended;
         const unsigned  kind  = from.kind == kPartBegins ? kPartBegins : ended ? kPartEnds : kPartContinues;
         const int       slot  = kind == kPartBegins ? 1 : 0;
-        float2* const   stats = reinterpret_cast<float2*>(p.workspace + four_stats_offset(gridDim.x)) + (2 * blockIdx.x + slot) * 16;
-        float* const    sums  = reinterpret_cast<float*>(p.workspace + four_sums_offset(gridDim.x)) + static_cast<size_t>(2 * blockIdx.x + slot) * 16 * HEAD_DIM;
-        // The parts are those of neighbouring warps, the first of which may be the last piece of its warp; the others are first pieces.
-        const int begin = (__ffs(mine) - 1) >> 1, tail = (__ffs(mine) - 1) & 1, count = (31 - __clz(mine)) / 2 - begin + 1;
-        four_add_up<HEAD_DIM>(
-            count, from.rows, [&](int k, int row) { return (mine >> (2 * (begin + k) + (k == 0 ? tail : 0)) & 1u) ? sh.stats[begin + k][k == 0 ? tail : 0][row] : make_float2(-CUDART_INF_F, 0.0f); },
-            [&](int k) {
-                const int w = begin + k;
-                return reinterpret_cast<const float*>(k == 0 && tail ? smem + w * (kStages * kStageBytes) : first_sums + w * four_rows_bytes(HEAD_DIM, TILES));
-            },
-            [&](int row, int column, float top, float sum, float4 o) {
-                if (item)
-                    *reinterpret_cast<uint2*>(four_out<HEAD_DIM>(p, from.first, from.head, from.row0 + row) + column) = four_outputs(o, sum);
-                else {
-                    *reinterpret_cast<float4*>(sums + row * HEAD_DIM + column) = o;
-                    if (column == 0)
-                        stats[row] = make_float2(top, sum);
-                }
-            });
-        if (!item) {
-            written[slot] = true;
-            if (threadIdx.x == 0)
-                parts[slot] = FourPart{kind, from.first, from.row0, from.rows, from.head, {0, 0, 0}};
+        if (row < from.rows) {
+            float2       all;
+            const float4 o = four_add_up<1>(
+                count, [&](int k) { return sh.stats[begin + k][k == 0 ? tail : 0][row]; },
+                [&](int k) {
+                    const int            w  = begin + k;
+                    const unsigned char* at = k == 0 && tail ? smem + w * (kStages * kStageBytes) : first_sums + w * four_rows_bytes(HEAD_DIM, TILES);
+                    return reinterpret_cast<const float4*>(at) + row * (HEAD_DIM / 4) + column / 4;
+                },
+                all);
+            if (item)
+                *reinterpret_cast<uint2*>(four_out<HEAD_DIM>(p, from.first, from.head, from.row0 + row) + column) = four_outputs(o, all.y);
+            else {
+                const size_t at = static_cast<size_t>(2 * blockIdx.x + slot) * 16 + row;
+                *reinterpret_cast<float4*>(reinterpret_cast<float*>(p.workspace + four_sums_offset(gridDim.x)) + at * HEAD_DIM + column) = o;
+                if (column == 0)
+                    reinterpret_cast<float2*>(p.workspace + four_stats_offset(gridDim.x))[at] = all;
+            }
         }
+        if (!item && u % kPerItem == 0)
+            reinterpret_cast<FourPart*>(p.workspace)[2 * blockIdx.x + slot] = FourPart{kind, from.first, from.row0, from.rows, from.head, {0, 0, 0}};
     }
-    if (threadIdx.x < 2 && !written[threadIdx.x])
-        parts[threadIdx.x].kind = kPartNone;
+    if (threadIdx.x < 2) {
+        // What this CTA leaves for others: a first piece where the first part began elsewhere, a last one where the last part has not
+        // ended and its item began here.
+        const unsigned first = all_present & -all_present, last_begins = begins ? 31 - __clz(begins) : -1;
+        const bool     has   = threadIdx.x == 0 ? (first & ~begins) != 0 : begins != 0 && (ends >> last_begins) == 0;
+        if (!has)
+            reinterpret_cast<FourPart*>(p.workspace)[2 * blockIdx.x + threadIdx.x].kind = kPartNone;
+    }
 }
 
 // Adds up the parts of the item that CTA blockIdx.x ended but did not begin, in key order.
@@ -982,12 +1005,14 @@ __global__ void __launch_bounds__(256) four_bit_join_kernel(const __grid_constan
     auto                slot  = [&](int i) { return static_cast<size_t>(2 * (begin + i) + (i == 0 ? 1 : 0)); };
     const float2* const stats = reinterpret_cast<const float2*>(p.workspace + four_stats_offset(gridDim.x));
     const float* const  sums  = reinterpret_cast<const float*>(p.workspace + four_sums_offset(gridDim.x));
-    four_add_up<HEAD_DIM>(
-        cta - begin + 1, last.rows, [&](int i, int row) { return stats[slot(i) * 16 + row]; },
-        [&](int i) { return sums + slot(i) * 16 * HEAD_DIM; },
-        [&](int row, int column, float, float sum, float4 o) {
-            *reinterpret_cast<uint2*>(four_out<HEAD_DIM>(p, last.first, last.head, last.row0 + row) + column) = four_outputs(o, sum);
-        });
+    for (int u = threadIdx.x; u < last.rows * (HEAD_DIM / 4); u += blockDim.x) {
+        const int    row = u / (HEAD_DIM / 4), column = u % (HEAD_DIM / 4) * 4;
+        float2       all;
+        const float4 o = four_add_up<4>(
+            cta - begin + 1, [&](int i) { return stats[slot(i) * 16 + row]; },
+            [&](int i) { return reinterpret_cast<const float4*>(sums + (slot(i) * 16 + row) * HEAD_DIM + column); }, all);
+        *reinterpret_cast<uint2*>(four_out<HEAD_DIM>(p, last.first, last.head, last.row0 + row) + column) = four_outputs(o, all.y);
+    }
 }
 
 }  // namespace flashllm
