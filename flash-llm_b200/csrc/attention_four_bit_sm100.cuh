@@ -253,23 +253,39 @@ __device__ __forceinline__ int four_value_place(int key)
 }
 
 // Adds up four columns of a row of one item's parts, in key order: `stats(i)` is the i-th part's maximum and sum of the row, `sums(i)`
-// its outputs of these columns.  UNROLL parts' loads are under way at a time.
-template<int UNROLL, typename Stats, typename Sums>
+// its outputs of these columns.  AT_ONCE parts' loads are under way at a time.
+template<int AT_ONCE, typename Stats, typename Sums>
 __device__ __forceinline__ float4 four_add_up(int count, Stats&& stats, Sums&& sums, float2& all)
 {
-    float top = -CUDART_INF_F;
-#pragma unroll UNROLL
-    for (int i = 0; i < count; ++i)
-        top = fmaxf(top, stats(i).x);
+    float  top = -CUDART_INF_F, sum = 0.0f;
     float4 o   = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    float  sum = 0.0f;
-#pragma unroll UNROLL
-    for (int i = 0; i < count; ++i) {
-        const float2 s    = stats(i);
-        const float4 x    = *sums(i);
-        const float  keep = four_weight(s.x, top);
-        sum               = fmaf(s.y, keep, sum);
-        o                 = make_float4(fmaf(x.x, keep, o.x), fmaf(x.y, keep, o.y), fmaf(x.z, keep, o.z), fmaf(x.w, keep, o.w));
+#pragma unroll 1
+    for (int i0 = 0; i0 < count; i0 += AT_ONCE) {
+        float2 s[AT_ONCE];
+        float4 x[AT_ONCE];
+        float  newtop = top;
+#pragma unroll
+        for (int i = 0; i < AT_ONCE; ++i) {
+            s[i] = make_float2(-CUDART_INF_F, 0.0f);
+            x[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            if (i0 + i < count) {
+                s[i] = stats(i0 + i);
+                x[i] = *sums(i0 + i);
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < AT_ONCE; ++i)
+            newtop = fmaxf(newtop, s[i].x);
+        const float before = four_weight(top, newtop);
+        sum *= before;
+        o   = make_float4(o.x * before, o.y * before, o.z * before, o.w * before);
+        top = newtop;
+#pragma unroll
+        for (int i = 0; i < AT_ONCE; ++i) {
+            const float keep = four_weight(s[i].x, top);
+            sum              = fmaf(s[i].y, keep, sum);
+            o                = make_float4(fmaf(x[i].x, keep, o.x), fmaf(x[i].y, keep, o.y), fmaf(x[i].z, keep, o.z), fmaf(x[i].w, keep, o.w));
+        }
     }
     all = make_float2(top, sum);
     return o;
@@ -988,19 +1004,25 @@ __global__ void __launch_bounds__(256) four_bit_join_kernel(const __grid_constan
     ptx::grid_dependency_wait();
     const FourPart* const parts = reinterpret_cast<const FourPart*>(p.workspace);
     const int             cta = blockIdx.x, lane = threadIdx.x & 31;
-    const FourPart        last = parts[2 * cta];
-    if (last.kind != kPartEnds)
-        return;
-    // The CTA that began the item: the nearest before that did not only continue it.
-    int begin = cta;
+    // The CTA that began the item: the nearest before that did not only continue it.  (What tells is loaded at once: a call of few
+    // sequences is a chain of such loads.)
+    const FourPart last  = parts[2 * cta];
+    int            begin = cta;
+    unsigned       begun = 0;
     do {
         const int      c     = begin - 1 - lane;
-        const unsigned other = __ballot_sync(0xffffffffu, c < 0 || parts[2 * c].kind != kPartContinues);
+        const unsigned kind  = c < 0 ? kPartNone : parts[2 * c].kind, next = c < 0 ? kPartNone : parts[2 * c + 1].kind;
+        const unsigned other = __ballot_sync(0xffffffffu, kind != kPartContinues);
+        begun                = __ballot_sync(0xffffffffu, next == kPartBegins);
+        if (last.kind != kPartEnds)
+            return;
         begin -= other ? __ffs(other) : 32;
-        if (other)
+        if (other) {
+            begun = begun >> (__ffs(other) - 1) & 1u;
             break;
+        }
     } while (true);
-    if (begin < 0 || parts[2 * begin + 1].kind != kPartBegins)
+    if (begin < 0 || !begun)
         return;
     auto                slot  = [&](int i) { return static_cast<size_t>(2 * (begin + i) + (i == 0 ? 1 : 0)); };
     const float2* const stats = reinterpret_cast<const float2*>(p.workspace + four_stats_offset(gridDim.x));
@@ -1008,7 +1030,7 @@ __global__ void __launch_bounds__(256) four_bit_join_kernel(const __grid_constan
     for (int u = threadIdx.x; u < last.rows * (HEAD_DIM / 4); u += blockDim.x) {
         const int    row = u / (HEAD_DIM / 4), column = u % (HEAD_DIM / 4) * 4;
         float2       all;
-        const float4 o = four_add_up<4>(
+        const float4 o = four_add_up<8>(
             cta - begin + 1, [&](int i) { return stats[slot(i) * 16 + row]; },
             [&](int i) { return reinterpret_cast<const float4*>(sums + (slot(i) * 16 + row) * HEAD_DIM + column); }, all);
         *reinterpret_cast<uint2*>(four_out<HEAD_DIM>(p, last.first, last.head, last.row0 + row) + column) = four_outputs(o, all.y);
