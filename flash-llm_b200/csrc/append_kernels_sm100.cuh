@@ -91,8 +91,10 @@ constexpr int kAppendRows = 8;  // of a CTA, at most
 // rounding to what the cache holds.  A thread takes 32 bytes of a head (both members of its pairs), the threads of a head (8 or 4
 // neighbours) add up its squares and find the smallest and the largest of its 64s by shuffles.
 // Bound by memory for prompts, by a chain of dependent loads for a few tokens (sequence, page, row).  A CTA of many calls takes several
-// tokens: their places and angles are found side by side, and the loads of the next 32 bytes are under way while these are worked on
-// (APPENDNOTE).
+// tokens: their places and angles are found side by side, and the loads of the next 32 bytes are under way while these are worked on.
+// 6612 tokens of 56 heads of 128: 47.4 us with a CTA for each, 43.6 so, 41.5 with eights of neighbouring threads side by side in
+// memory (wavefronts of the L1 74 to 49 % of what it can), 37.5 in even rounds: 5.1 TB/s, 0.77 of the measured copy bandwidth.  What
+// is left is the work on registers, 260 operations for a thread's 16 elements.
 template<int HEAD_DIM, bool INTERLEAVED, bool FOUR_BIT>
 __global__ void __launch_bounds__(kRotaryThreads) norm_append_kernel(const __grid_constant__ AppendParams p)
 {
@@ -274,7 +276,8 @@ constexpr int kReadThreads = 256, kReadRows = 16;
 
 // Rows of the batch from a cache of 4 bits.  A CTA takes a few rows: for each its place is looked up once, then threads take eight
 // elements at a time, the rows of one head, which lie one behind another in a page, before the next head's.  Bound by memory (most
-// of it what is written): READNOTE.
+// of it what is written): 130000 rows of 8 heads of 128 122 us, 5.6 TB/s, 0.85 of the measured copy bandwidth (157 with addresses
+// worked out for every eight elements).
 template<int HEAD_DIM>
 __global__ void __launch_bounds__(kReadThreads) four_bit_read_kernel(const __grid_constant__ ReadParams p)
 {

@@ -136,6 +136,9 @@ cudaError_t launch_rows_over_four_bits(cudaStream_t stream, const AttentionParam
     return head_dim == 64 ? launch_attention<64>(stream, p, true) : launch_attention<128>(stream, p, true);
 }
 
+// Single tokens through a window (four_bit_api.cu).
+cudaError_t launch_single_tokens(cudaStream_t stream, const AttentionParams& p, int head_dim);
+
 // The checks that the attention operators share, and the launch.
 static cudaError_t attend(cudaStream_t stream, AttentionParams p, const void* Q, int ld_q, const void* K_cache,
                           const void* V_cache, int pages, int page_size, const int* cu_tokens, const int* context,
@@ -162,6 +165,9 @@ static cudaError_t attend(cudaStream_t stream, AttentionParams p, const void* Q,
     p.cap     = cap;
     p.workspace = static_cast<unsigned char*>(workspace);
     attn_set_heads(&p, heads, kv_heads);
+    // With a window and no more tokens than sequences these are single tokens (or few; the kernel takes any).
+    if (p.window > 0 && tokens <= sequences)
+        return launch_single_tokens(stream, p, head_dim);
     return head_dim == 64 ? launch_attention<64>(stream, p) : launch_attention<128>(stream, p);
 }
 

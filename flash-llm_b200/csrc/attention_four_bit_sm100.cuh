@@ -41,6 +41,7 @@ struct FourBitParams {
     int                  share;  // query heads per key/value head, and what divides by it (see AttentionParams)
     unsigned             share_magic;
     int                  share_shift;
+    int                  token_tiles;  // tiles of eight rows of a token: kernels whose tiles are of one token each
     int                  window;  // keys up to itself that a row sees
     int                  sinks;   // ... and of its sequence's first
     int                  most_rows;  // sequences with more rows (tokens x share) are somebody else's
@@ -157,7 +158,8 @@ struct FourSequence {
     int rows, tiles, units;
 };
 
-template<int ROWS, int KEYS>
+// BY_TOKEN: no tile has rows of two tokens.
+template<int ROWS, int KEYS, bool BY_TOKEN>
 __device__ __forceinline__ FourSequence four_sequence(const FourBitParams& p, int b, int* lost = nullptr)
 {
     const Sequence s = load_sequence(p.batch, b);
@@ -166,8 +168,8 @@ __device__ __forceinline__ FourSequence four_sequence(const FourBitParams& p, in
         *lost = s.lost;
     if (q.rows > p.most_rows)
         q.rows = q.count = 0;
-    q.tiles = (q.rows + ROWS - 1) / ROWS;
-    if (q.tiles == 1)
+    q.tiles = BY_TOKEN ? q.count * p.token_tiles : (q.rows + ROWS - 1) / ROWS;
+    if (q.tiles == 1 || q.count == 1)
         q.units = four_tile<KEYS>(p, q.context, 0, q.count - 1).blocks + kFourExtra;
     else if (q.tiles > 1) {
         const long long all = (static_cast<long long>(q.context) + q.count + KEYS - 1) / KEYS;
@@ -179,20 +181,21 @@ __device__ __forceinline__ FourSequence four_sequence(const FourBitParams& p, in
     return q;
 }
 
-template<int ROWS, int KEYS>
+template<int ROWS, int KEYS, bool BY_TOKEN>
 __device__ __noinline__ FourSequence four_sequence_again(const FourBitParams& p, int b)
 {
-    return four_sequence<ROWS, KEYS>(p, b);
+    return four_sequence<ROWS, KEYS, BY_TOKEN>(p, b);
 }
 
 // ... what the plan has kept of it.
-template<int ROWS, int KEYS>
+template<int ROWS, int KEYS, bool BY_TOKEN>
 __device__ __forceinline__ FourSequence four_sequence(const FourBitParams& p, const FourShared& sh, int b)
 {
     if (b >= kFourKnown)
-        return four_sequence_again<ROWS, KEYS>(p, b);
+        return four_sequence_again<ROWS, KEYS, BY_TOKEN>(p, b);
     const int4 known = sh.known[b];
-    return FourSequence{known.x, known.y, known.z, known.y * p.share, (known.y * p.share + ROWS - 1) / ROWS, known.w};
+    const int  rows  = known.y * p.share;
+    return FourSequence{known.x, known.y, known.z, rows, BY_TOKEN ? known.y * p.token_tiles : (rows + ROWS - 1) / ROWS, known.w};
 }
 
 // a / b, of 32 bits where they are that.
@@ -276,13 +279,14 @@ __device__ __forceinline__ float4 four_add_up(int count, Stats&& stats, Sums&& s
 #pragma unroll
         for (int i = 0; i < AT_ONCE; ++i)
             newtop = fmaxf(newtop, s[i].x);
-        const float before = four_weight(top, newtop);
+        // (Never zero: a part's infinity stays one.)
+        const float before = fmaxf(four_weight(top, newtop), 0x1p-126f);
         sum *= before;
         o   = make_float4(o.x * before, o.y * before, o.z * before, o.w * before);
         top = newtop;
 #pragma unroll
         for (int i = 0; i < AT_ONCE; ++i) {
-            const float keep = four_weight(s[i].x, top);
+            const float keep = fmaxf(four_weight(s[i].x, top), 0x1p-126f);
             sum              = fmaf(s[i].y, keep, sum);
             o                = make_float4(fmaf(x[i].x, keep, o.x), fmaf(x[i].y, keep, o.y), fmaf(x[i].z, keep, o.z), fmaf(x[i].w, keep, o.w));
         }
@@ -327,6 +331,224 @@ __device__ __forceinline__ float four_capped(float x, float in, float cap)
     return fmaf(-2.0f * cap, ptx::rcp_approx(1.0f + ptx::exp2_approx(2.0f * CUDART_L2E_F * y)), cap);
 }
 
+// Where each warp's share of the work begins and ends; false if there is none at all.  For all threads: each counts the units of a few
+// sequences in a row.
+template<int HEAD_DIM, int ROWS, int KEYS, int WARPS, bool BY_TOKEN>
+__device__ __forceinline__ bool four_plan(const FourBitParams& p, FourShared& sh, unsigned long long& u0, unsigned long long& u1)
+{
+    const CacheBatch& c    = p.batch;
+    const int         warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int per_thread = c.sequences <= (WARPS * 32) ? 1 : (c.sequences + (WARPS * 32) - 1) / (WARPS * 32);
+    {
+        unsigned long long mine = 0;
+        bool               lost = false;
+        for (int k = 0; k < per_thread; ++k) {
+            const int b = threadIdx.x * per_thread + k;
+            if (b >= c.sequences)
+                break;
+            int                rows_lost;
+            const FourSequence q = four_sequence<ROWS, KEYS, BY_TOKEN>(p, b, &rows_lost);
+            mine += static_cast<unsigned long long>(q.tiles) * (static_cast<unsigned long long>(q.units) * c.kv_heads);
+            lost = lost || rows_lost > 0;
+            if (b < kFourKnown)
+                sh.known[b] = make_int4(q.first, q.count, q.context, q.units);
+        }
+        const unsigned long long upto = attn_warp_scan(mine);
+        if (lane == 31)
+            sh.warp_sums[warp] = upto;
+        if (lane == 0)
+            sh.part[warp][0].kind = sh.part[warp][1].kind = kPartNone;
+        if (__syncthreads_or(lost ? 1 : 0)) {  // rows of sequences that do not fit
+            for (int b = blockIdx.x; b < c.sequences; b += gridDim.x) {
+                const Sequence  q   = load_sequence(c, b);
+                const long long row = static_cast<long long>(p.heads) * HEAD_DIM;
+                for (long long i = threadIdx.x * 8; i < q.lost * row; i += (WARPS * 32) * 8)
+                    *reinterpret_cast<uint4*>(p.out + q.first * row + i) = make_uint4(0, 0, 0, 0);
+            }
+        }
+        unsigned long long before = upto - mine;
+#pragma unroll
+        for (int w = 0; w < WARPS; ++w)
+            before += w < warp ? sh.warp_sums[w] : 0;
+        sh.before[threadIdx.x] = before;
+        if (threadIdx.x == (WARPS * 32) - 1)
+            sh.total = before + mine;
+        __syncthreads();
+    }
+    const unsigned long long total = sh.total;
+    if (total == 0) {
+        if (threadIdx.x < 2)
+            reinterpret_cast<FourPart*>(p.workspace)[2 * blockIdx.x + threadIdx.x].kind = kPartNone;
+        return false;
+    }
+    // Small calls take as few warps of each CTA as leave them a few blocks each.
+    constexpr unsigned       kLeast = kFourExtra + 2;
+    const int                busy   = total >= static_cast<unsigned long long>(kLeast) * WARPS * gridDim.x ? WARPS : static_cast<int>(total) / static_cast<int>(kLeast * gridDim.x) + 1;
+    const unsigned           workers = gridDim.x * busy;
+    const unsigned long long share   = four_divide(total + workers - 1, workers);
+    const unsigned long long worker  = static_cast<unsigned long long>(blockIdx.x) * busy + warp;
+    u0 = min(total, share * worker);
+    u1 = warp < busy ? min(total, u0 + share) : u0;
+    return true;
+
+}
+
+// Walks a warp's share: pieces of items, order (sequence, tile of rows, key/value head, blocks of keys).
+template<int ROWS, int KEYS, int WARPS, bool BY_TOKEN>
+struct FourWalk {
+    FourSequence       q;
+    FourTile           sight;
+    int                b, tile, head, unit, upto;
+    int                row0, rows, token0, token1;  // of the tile
+    int                begin, end;                  // blocks of the piece
+    unsigned long long left;
+
+    __device__ __forceinline__ void start(const FourBitParams& p, const FourShared& sh, unsigned long long u0, unsigned long long u1)
+    {
+        const int per_thread = p.batch.sequences <= WARPS * 32 ? 1 : (p.batch.sequences + WARPS * 32 - 1) / (WARPS * 32);
+        // The thread that counted the sequence of unit u0, and that sequence.
+        int lo = 0;
+#pragma unroll 1
+        for (int step = 256; step > 0; step >>= 1)
+            if (lo + step < WARPS * 32 && sh.before[lo + step] <= u0)
+                lo += step;
+        // (several threads may have the same count: the last of them has units)
+        unsigned long long at = sh.before[lo];
+        b = lo * per_thread;
+        q = four_sequence<ROWS, KEYS, BY_TOKEN>(p, sh, b);
+        auto               whole = [&]() { return static_cast<unsigned long long>(q.tiles) * (static_cast<unsigned long long>(q.units) * p.batch.kv_heads); };
+        while (at + whole() <= u0 && b + 1 < p.batch.sequences) {
+            at += whole();
+            q = four_sequence<ROWS, KEYS, BY_TOKEN>(p, sh, ++b);
+        }
+        const unsigned long long in       = u0 - at;  // unit of the sequence
+        const unsigned long long per_tile = static_cast<unsigned long long>(max(q.units, 1)) * p.batch.kv_heads;
+        tile = q.tiles > 1 ? static_cast<int>(four_divide(in, per_tile)) : 0;
+        const unsigned long long in_tile  = in - tile * per_tile;
+        head = static_cast<int>(four_divide(in_tile, max(q.units, 1)));
+        unit = static_cast<int>(in_tile - static_cast<unsigned long long>(head) * max(q.units, 1));
+        left = u1 - u0;
+
+    }
+    __device__ __forceinline__ void piece(const FourBitParams& p)
+    {
+        if constexpr (BY_TOKEN) {
+            token0 = token1 = p.token_tiles == 1 ? tile : tile / p.token_tiles;
+            row0            = token0 * p.share + (tile - token0 * p.token_tiles) * ROWS;
+            rows            = min(ROWS, (token0 + 1) * p.share - row0);
+        }
+        else {
+            row0   = tile * ROWS;
+            rows   = min(ROWS, q.rows - row0);
+            token0 = four_token(p, row0);
+            token1 = four_token(p, row0 + rows - 1);
+        }
+        sight = four_tile<KEYS>(p, q.context, token0, token1);
+        upto  = static_cast<int>(min(static_cast<unsigned long long>(q.units), unit + left));
+        // Units of the tile to its blocks: exact where the tile's blocks are what it counts, in proportion where they are fewer.
+        auto cut = [&](int x) {
+            const int counted = q.units - kFourExtra, behind = max(0, x - kFourExtra);
+            return counted == sight.blocks ? behind : static_cast<int>(static_cast<long long>(behind) * sight.blocks / counted);
+        };
+        begin = cut(unit);
+        end   = cut(upto);
+        left -= upto - unit;
+    }
+    // On to the next item; false at the end.
+    __device__ __forceinline__ bool next(const FourBitParams& p, const FourShared& sh)
+    {
+        if (left == 0)
+            return false;
+        unit = upto;
+        if (unit == q.units) {
+            unit = 0;
+            if (++head == p.batch.kv_heads) {
+                head = 0;
+                if (++tile == q.tiles) {
+                    tile = 0;
+                    do {
+                        if (++b >= p.batch.sequences)
+                            return false;
+                        q = four_sequence<ROWS, KEYS, BY_TOKEN>(p, sh, b);
+                    } while (q.tiles == 0);
+                }
+            }
+        }
+        return true;
+    }
+};
+
+// Items that several warps of a CTA have worked on, in key order; what began before this CTA, or ends behind it, to the workspace.  For all
+// threads; sums of a warp's first part lie in `first_sums`, those of its last in its ring (`ring_bytes` each).
+template<int HEAD_DIM, int ROWS, int WARPS>
+__device__ __forceinline__ void four_finish(const FourBitParams& p, const FourShared& sh, const unsigned char* smem, int ring_bytes, const unsigned char* first_sums)
+{
+    const int lane = threadIdx.x & 31;
+    // Parts in key order, of warp i / 2: that is their kinds, and which of them belong to an item.  All items side by side.
+    const unsigned kind_here = lane < 2 * WARPS ? sh.part[lane >> 1][lane & 1].kind : kPartNone;
+    const unsigned begins = __ballot_sync(0xffffffffu, kind_here == kPartBegins), ends = __ballot_sync(0xffffffffu, kind_here == kPartEnds);
+    const unsigned all_present = __ballot_sync(0xffffffffu, kind_here != kPartNone);
+    constexpr int  kPerItem = ROWS * (HEAD_DIM / 4);
+    unsigned       present = all_present;
+    int            number  = 0;  // of the item that `present` begins with
+#pragma unroll 1
+    for (int u = threadIdx.x;; u += (WARPS * 32)) {
+        unsigned mine = 0;
+#pragma unroll 1
+        for (;;) {
+            // Up to the part that ends the item, or before the next that begins one.
+            const unsigned ending = ends & present, other = begins & present & (present - 1);
+            mine = present;
+            if (ending)
+                mine &= ending ^ (ending - 1);
+            if (other)
+                mine &= (other & -other) - 1;
+            if (number == u / kPerItem || present == 0)
+                break;
+            present &= ~mine;
+            ++number;
+        }
+        if (mine == 0)
+            break;
+        const int       row = u / (HEAD_DIM / 4) % ROWS, column = u % (HEAD_DIM / 4) * 4;
+        // The parts are those of neighbouring warps, the first of which may be the last piece of its warp; the others are first pieces.
+        const int       begin = (__ffs(mine) - 1) >> 1, tail = (__ffs(mine) - 1) & 1, count = (31 - __clz(mine)) / 2 - begin + 1;
+        const FourPart& from  = sh.part[begin][tail];
+        const bool      ended = (mine & ends) != 0, item = from.kind == kPartBegins && ended;
+        const unsigned  kind  = from.kind == kPartBegins ? kPartBegins : ended ? kPartEnds : kPartContinues;
+        const int       slot  = kind == kPartBegins ? 1 : 0;
+        if (row < from.rows) {
+            float2       all;
+            const float4 o = four_add_up<1>(
+                count, [&](int k) { return sh.stats[begin + k][k == 0 ? tail : 0][row]; },
+                [&](int k) {
+                    const int            w  = begin + k;
+                    const unsigned char* at = k == 0 && tail ? smem + w * ring_bytes : first_sums + w * four_rows_bytes(HEAD_DIM, ROWS / 8);
+                    return reinterpret_cast<const float4*>(at) + row * (HEAD_DIM / 4) + column / 4;
+                },
+                all);
+            if (item)
+                *reinterpret_cast<uint2*>(four_out<HEAD_DIM>(p, from.first, from.head, from.row0 + row) + column) = four_outputs(o, all.y);
+            else {
+                const size_t at = static_cast<size_t>(2 * blockIdx.x + slot) * 16 + row;
+                *reinterpret_cast<float4*>(reinterpret_cast<float*>(p.workspace + four_sums_offset(gridDim.x)) + at * HEAD_DIM + column) = o;
+                if (column == 0)
+                    reinterpret_cast<float2*>(p.workspace + four_stats_offset(gridDim.x))[at] = all;
+            }
+        }
+        if (!item && u % kPerItem == 0)
+            reinterpret_cast<FourPart*>(p.workspace)[2 * blockIdx.x + slot] = FourPart{kind, from.first, from.row0, from.rows, from.head, {0, 0, 0}};
+    }
+    if (threadIdx.x < 2) {
+        // What this CTA leaves for others: a first piece where the first part began elsewhere, a last one where the last part has not
+        // ended and its item began here.
+        const unsigned first = all_present & -all_present, last_begins = begins ? 31 - __clz(begins) : -1;
+        const bool     has   = threadIdx.x == 0 ? (first & ~begins) != 0 : begins != 0 && (ends >> last_begins) == 0;
+        if (!has)
+            reinterpret_cast<FourPart*>(p.workspace)[2 * blockIdx.x + threadIdx.x].kind = kPartNone;
+    }
+}
+
 // PLAIN: neither cap nor slopes.  TILES of eight rows at a time.
 template<int HEAD_DIM, int TILES, bool PLAIN>
 __global__ void __launch_bounds__(four_warps(TILES) * 32, 1) four_bit_attention_kernel(const __grid_constant__ FourBitParams p)
@@ -351,57 +573,9 @@ __global__ void __launch_bounds__(four_warps(TILES) * 32, 1) four_bit_attention_
     ptx::grid_dependency_wait();
     ptx::grid_launch_dependents();
 
-    // ---- where each warp's share begins: a thread counts the units of a few sequences in a row
-    const int per_thread = c.sequences <= kThreads ? 1 : (c.sequences + kThreads - 1) / kThreads;
-    {
-        unsigned long long mine = 0;
-        bool               lost = false;
-        for (int k = 0; k < per_thread; ++k) {
-            const int b = threadIdx.x * per_thread + k;
-            if (b >= c.sequences)
-                break;
-            int                rows_lost;
-            const FourSequence q = four_sequence<kRows, kKeys>(p, b, &rows_lost);
-            mine += static_cast<unsigned long long>(q.tiles) * (static_cast<unsigned long long>(q.units) * c.kv_heads);
-            lost = lost || rows_lost > 0;
-            if (b < kFourKnown)
-                sh.known[b] = make_int4(q.first, q.count, q.context, q.units);
-        }
-        const unsigned long long upto = attn_warp_scan(mine);
-        if (lane == 31)
-            sh.warp_sums[warp] = upto;
-        if (lane == 0)
-            sh.part[warp][0].kind = sh.part[warp][1].kind = kPartNone;
-        if (__syncthreads_or(lost ? 1 : 0)) {  // rows of sequences that do not fit
-            for (int b = blockIdx.x; b < c.sequences; b += gridDim.x) {
-                const Sequence  q   = load_sequence(c, b);
-                const long long row = static_cast<long long>(p.heads) * HEAD_DIM;
-                for (long long i = threadIdx.x * 8; i < q.lost * row; i += kThreads * 8)
-                    *reinterpret_cast<uint4*>(p.out + q.first * row + i) = make_uint4(0, 0, 0, 0);
-            }
-        }
-        unsigned long long before = upto - mine;
-#pragma unroll
-        for (int w = 0; w < kWarps; ++w)
-            before += w < warp ? sh.warp_sums[w] : 0;
-        sh.before[threadIdx.x] = before;
-        if (threadIdx.x == kThreads - 1)
-            sh.total = before + mine;
-        __syncthreads();
-    }
-    const unsigned long long total = sh.total;
-    if (total == 0) {
-        if (threadIdx.x < 2)
-            reinterpret_cast<FourPart*>(p.workspace)[2 * blockIdx.x + threadIdx.x].kind = kPartNone;
+    unsigned long long u0, u1;
+    if (!four_plan<HEAD_DIM, kRows, kKeys, kWarps, false>(p, sh, u0, u1))
         return;
-    }
-    // Small calls take as few warps of each CTA as leave them a few blocks each.
-    constexpr unsigned       kLeast = kFourExtra + 2;
-    const int                busy   = total >= static_cast<unsigned long long>(kLeast) * kWarps * gridDim.x ? kWarps : static_cast<int>(total) / static_cast<int>(kLeast * gridDim.x) + 1;
-    const unsigned           workers = gridDim.x * busy;
-    const unsigned long long share   = four_divide(total + workers - 1, workers);
-    const unsigned long long worker  = static_cast<unsigned long long>(blockIdx.x) * busy + warp;
-    unsigned long long       u0 = min(total, share * worker), u1 = warp < busy ? min(total, u0 + share) : u0;
 
     // What the copies of a lane have in common: 16 bytes of the codes of a key (and of the one eight further on), and of the scales.
     // Rows of 64 bytes have their chunks 2 and 3 first in every other pair of rows, for the banks.
@@ -421,41 +595,14 @@ __global__ void __launch_bounds__(four_warps(TILES) * 32, 1) four_bit_attention_
     uint32_t       copied = 0;
 
     if (u0 < u1) {
-        // The thread that counted the sequence of unit u0, and that sequence.
-        int lo = 0;
-#pragma unroll 1
-        for (int step = 256; step > 0; step >>= 1)
-            if (lo + step < kThreads && sh.before[lo + step] <= u0)
-                lo += step;
-        // (several threads may have the same count: the last of them has units)
-        unsigned long long at = sh.before[lo];
-        int                b  = lo * per_thread;
-        FourSequence       q  = four_sequence<kRows, kKeys>(p, sh, b);
-        auto               whole = [&]() { return static_cast<unsigned long long>(q.tiles) * (static_cast<unsigned long long>(q.units) * c.kv_heads); };
-        while (at + whole() <= u0 && b + 1 < c.sequences) {
-            at += whole();
-            q = four_sequence<kRows, kKeys>(p, sh, ++b);
-        }
-        const unsigned long long in       = u0 - at;  // unit of the sequence
-        const unsigned long long per_tile = static_cast<unsigned long long>(max(q.units, 1)) * c.kv_heads;
-        int                      tile     = q.tiles > 1 ? static_cast<int>(four_divide(in, per_tile)) : 0;
-        const unsigned long long in_tile  = in - tile * per_tile;
-        int                      head     = static_cast<int>(four_divide(in_tile, max(q.units, 1)));
-        int                      unit     = static_cast<int>(in_tile - static_cast<unsigned long long>(head) * max(q.units, 1));
-        unsigned long long left = u1 - u0;
-
-        while (left > 0) {
+        FourWalk<kRows, kKeys, kWarps, false> walk;
+        walk.start(p, sh, u0, u1);
+        do {
             // ---- a piece of an item
-            const int row0 = tile * kRows, rows = min(kRows, q.rows - row0), token0 = four_token(p, row0), token1 = four_token(p, row0 + rows - 1);
-            const FourTile sight = four_tile<kKeys>(p, q.context, token0, token1);
-            const int      upto  = static_cast<int>(min(static_cast<unsigned long long>(q.units), unit + left));
-            // Units of the tile to its blocks: exact where the tile's blocks are what it counts, in proportion where they are fewer.
-            auto cut = [&](int x) {
-                const int counted = q.units - kFourExtra, behind = max(0, x - kFourExtra);
-                return counted == sight.blocks ? behind : static_cast<int>(static_cast<long long>(behind) * sight.blocks / counted);
-            };
-            const int begin = cut(unit), end = cut(upto);
-            left -= upto - unit;
+            walk.piece(p);
+            const FourSequence& q    = walk.q;
+            const FourTile      sight = walk.sight;
+            const int b = walk.b, head = walk.head, row0 = walk.row0, rows = walk.rows, token0 = walk.token0, token1 = walk.token1, begin = walk.begin, end = walk.end;
             if (begin < end) {
                 // The rows of Q, on their way while pages are looked up.
                 uint4 q_raw[TILES][kGroups][2];
@@ -906,94 +1053,11 @@ __global__ void __launch_bounds__(four_warps(TILES) * 32, 1) four_bit_attention_
                 if (lane == 0)
                     sh.part[warp][0] = FourPart{kPartContinues, q.first, row0, rows, head, {0, 0, 0}};
             }
-            // ---- the next item
-            if (left == 0)
-                break;
-            unit = upto;
-            if (unit == q.units) {
-                unit = 0;
-                if (++head == c.kv_heads) {
-                    head = 0;
-                    if (++tile == q.tiles) {
-                        tile = 0;
-                        do {
-                            if (++b >= c.sequences) {
-                                left = 0;
-                                break;
-                            }
-                            q = four_sequence<kRows, kKeys>(p, sh, b);
-                        } while (q.tiles == 0);
-                    }
-                }
-            }
-        }
+        } while (walk.next(p, sh));
     }
     __syncthreads();
 
-    // ---- items that several warps have worked on, in key order; what began before this CTA, or ends behind it, to the workspace
-    // Parts in key order, of warp i / 2: that is their kinds, and which of them belong to an item.  All items side by side.
-    const unsigned kind_here = lane < 2 * kWarps ? sh.part[lane >> 1][lane & 1].kind : kPartNone;
-    const unsigned begins = __ballot_sync(0xffffffffu, kind_here == kPartBegins), ends = __ballot_sync(0xffffffffu, kind_here == kPartEnds);
-    const unsigned all_present = __ballot_sync(0xffffffffu, kind_here != kPartNone);
-    constexpr int  kPerItem = kRows * (HEAD_DIM / 4);
-    unsigned       present = all_present;
-    int            number  = 0;  // of the item that `present` begins with
-#pragma unroll 1
-    for (int u = threadIdx.x;; u += kThreads) {
-        unsigned mine = 0;
-#pragma unroll 1
-        for (;;) {
-            // Up to the part that ends the item, or before the next that begins one.
-            const unsigned ending = ends & present, other = begins & present & (present - 1);
-            mine = present;
-            if (ending)
-                mine &= ending ^ (ending - 1);
-            if (other)
-                mine &= (other & -other) - 1;
-            if (number == u / kPerItem || present == 0)
-                break;
-            present &= ~mine;
-            ++number;
-        }
-        if (mine == 0)
-            break;
-        const int       row = u / (HEAD_DIM / 4) % kRows, column = u % (HEAD_DIM / 4) * 4;
-        // The parts are those of neighbouring warps, the first of which may be the last piece of its warp; the others are first pieces.
-        const int       begin = (__ffs(mine) - 1) >> 1, tail = (__ffs(mine) - 1) & 1, count = (31 - __clz(mine)) / 2 - begin + 1;
-        const FourPart& from  = sh.part[begin][tail];
-        const bool      ended = (mine & ends) != 0, item = from.kind == kPartBegins && ended;
-        const unsigned  kind  = from.kind == kPartBegins ? kPartBegins : ended ? kPartEnds : kPartContinues;
-        const int       slot  = kind == kPartBegins ? 1 : 0;
-        if (row < from.rows) {
-            float2       all;
-            const float4 o = four_add_up<1>(
-                count, [&](int k) { return sh.stats[begin + k][k == 0 ? tail : 0][row]; },
-                [&](int k) {
-                    const int            w  = begin + k;
-                    const unsigned char* at = k == 0 && tail ? smem + w * (kStages * kStageBytes) : first_sums + w * four_rows_bytes(HEAD_DIM, TILES);
-                    return reinterpret_cast<const float4*>(at) + row * (HEAD_DIM / 4) + column / 4;
-                },
-                all);
-            if (item)
-                *reinterpret_cast<uint2*>(four_out<HEAD_DIM>(p, from.first, from.head, from.row0 + row) + column) = four_outputs(o, all.y);
-            else {
-                const size_t at = static_cast<size_t>(2 * blockIdx.x + slot) * 16 + row;
-                *reinterpret_cast<float4*>(reinterpret_cast<float*>(p.workspace + four_sums_offset(gridDim.x)) + at * HEAD_DIM + column) = o;
-                if (column == 0)
-                    reinterpret_cast<float2*>(p.workspace + four_stats_offset(gridDim.x))[at] = all;
-            }
-        }
-        if (!item && u % kPerItem == 0)
-            reinterpret_cast<FourPart*>(p.workspace)[2 * blockIdx.x + slot] = FourPart{kind, from.first, from.row0, from.rows, from.head, {0, 0, 0}};
-    }
-    if (threadIdx.x < 2) {
-        // What this CTA leaves for others: a first piece where the first part began elsewhere, a last one where the last part has not
-        // ended and its item began here.
-        const unsigned first = all_present & -all_present, last_begins = begins ? 31 - __clz(begins) : -1;
-        const bool     has   = threadIdx.x == 0 ? (first & ~begins) != 0 : begins != 0 && (ends >> last_begins) == 0;
-        if (!has)
-            reinterpret_cast<FourPart*>(p.workspace)[2 * blockIdx.x + threadIdx.x].kind = kPartNone;
-    }
+    four_finish<HEAD_DIM, kRows, kWarps>(p, sh, smem, kStages * kStageBytes, first_sums);
 }
 
 // Adds up the parts of the item that CTA blockIdx.x ended but did not begin, in key order.

@@ -7,6 +7,7 @@
 
 #include "append_kernels_sm100.cuh"
 #include "attention_four_bit_sm100.cuh"
+#include "attention_single_sm100.cuh"
 #include "cache_api.h"
 #include "launch.h"
 #include "tiled_csl_host.h"
@@ -33,6 +34,10 @@ static cudaError_t four_multiprocessors(int* count)
         raise(four_bit_attention_kernel<128, 1, false>, four_smem_bytes(128, 1));
         raise(four_bit_attention_kernel<128, 2, true>, four_smem_bytes(128, 2));
         raise(four_bit_attention_kernel<128, 2, false>, four_smem_bytes(128, 2));
+        raise(window_single_kernel<64, true>, single_smem_bytes(64));
+        raise(window_single_kernel<64, false>, single_smem_bytes(64));
+        raise(window_single_kernel<128, true>, single_smem_bytes(128));
+        raise(window_single_kernel<128, false>, single_smem_bytes(128));
         return err;
     });
 }
@@ -83,7 +88,7 @@ static cudaError_t append(cudaStream_t stream, bool four_bit, const void* QKV, i
     if (const cudaError_t err = four_multiprocessors(&sms))
         return err;
     // As few rounds of CTAs over the multiprocessors, which hold four at a time, as kAppendRows allow, and tokens dealt out evenly over
-    // them (6612 tokens, 9.3 times the places: 39 us with 8 each, 1.4 rounds, ROUNDS with 6).
+    // them (6612 tokens, 9.3 times the places: 39 us with 8 each, 1.4 rounds, 36 with 6).
     const int places = 4 * sms, rounds = (tokens + kAppendRows * places - 1) / (kAppendRows * places);
     p.rows           = (tokens + rounds * places - 1) / (rounds * places);
     auto launch = [&](auto kernel) {
@@ -98,7 +103,7 @@ static cudaError_t append(cudaStream_t stream, bool four_bit, const void* QKV, i
 }
 
 // Rows of a sequence (tokens x query heads of a key/value head) up to which it goes through the warps' kernel, sixteen at a time (16
-// sequences of 2000 to 4000 positions, 32 rows each: 42 us, the other kernel 47; 64 rows: MORE and 50).
+// sequences of 2000 to 4000 positions, 32 rows each: 42 us, the other kernel 47; 64 rows: 63 and 51).
 constexpr int kFourMostRows = 32;
 
 template<int HEAD_DIM, int TILES>
@@ -110,6 +115,46 @@ static cudaError_t launch_four_bit(cudaStream_t stream, const FourBitParams& p, 
     if (err != cudaSuccess)
         return err;
     return launch_in_stream_order(four_bit_join_kernel<HEAD_DIM>, dim3(ctas), dim3(256), 0, stream, 1, p);
+}
+
+template<int HEAD_DIM>
+static cudaError_t launch_single(cudaStream_t stream, const FourBitParams& p, int ctas)
+{
+    const bool  plain = p.cap == 0.0f && p.slopes == nullptr;
+    cudaError_t err   = launch_in_stream_order(plain ? window_single_kernel<HEAD_DIM, true> : window_single_kernel<HEAD_DIM, false>, dim3(ctas),
+                                               dim3(kSingleWarps * 32), single_smem_bytes(HEAD_DIM), stream, 1, p);
+    if (err != cudaSuccess)
+        return err;
+    return launch_in_stream_order(four_bit_join_kernel<HEAD_DIM>, dim3(ctas), dim3(256), 0, stream, 1, p);
+}
+
+// Single tokens through a window over a cache of fp16; `a` has been checked.
+cudaError_t launch_single_tokens(cudaStream_t stream, const AttentionParams& a, int head_dim)
+{
+    int         sms = 0;
+    cudaError_t err = four_multiprocessors(&sms);
+    if (err != cudaSuccess)
+        return err;
+    FourBitParams p{};
+    p.batch       = a.batch;
+    p.q           = a.q;
+    p.out         = a.out;
+    p.k_cache     = reinterpret_cast<const unsigned char*>(a.k_cache);
+    p.v_cache     = reinterpret_cast<const unsigned char*>(a.v_cache);
+    p.slopes      = a.slopes;
+    p.workspace   = a.workspace;
+    p.ld_q        = a.ld_q;
+    p.heads       = a.heads;
+    p.share       = a.share;
+    p.share_magic = a.share_magic;
+    p.share_shift = a.share_shift;
+    p.token_tiles = (a.share + 7) / 8;
+    p.window      = a.window;
+    p.sinks       = a.sinks;
+    p.most_rows   = 0x7fffffff;
+    p.scale       = a.scale;
+    p.cap         = a.cap;
+    return head_dim == 64 ? launch_single<64>(stream, p, sms) : launch_single<128>(stream, p, sms);
 }
 
 }  // namespace flashllm

@@ -611,3 +611,79 @@ def test_refusals_of_the_operators(ops):
     with pytest.raises(RuntimeError, match="tokens"):
         ops.four_bit_read(*c.arrays, -1)
     assert ops.four_bit_read(*c.arrays, 0)[0].shape == (0, 128)
+
+
+# --------------------------------------------------------------------------------------------------- where single tokens go another way
+
+@pytest.mark.parametrize("contexts,counts,heads,kv_heads,dim,page,window,sinks,cap,distance", [
+    ([300, 5, 9, 0], [3, 0, 0, 1], 8, 2, 128, 16, 100, 3, 0.0, False),      # no more tokens than sequences, but several of one
+    ([300] + [0] * 9, [9] + [0] * 9, 12, 1, 64, 32, 40, 0, 0.0, True),
+    ([1000] * 3, [1] * 3, 40, 2, 128, 64, 333, 17, 25.0, False),            # more heads of a group than a tile's eight rows
+    ([5000], [1], 128, 1, 64, 128, 4000, 128, 0.0, False),
+    ([31, 32, 33, 47, 48, 49], [1] * 6, 3, 3, 128, 16, 16, 16, 0.0, False),
+    ([700] * 450, [1] * 450, 2, 1, 64, 16, 30, 2, 0.0, False),
+])
+@pytest.mark.parametrize("kind", [Batch, FourBitBatch])
+def test_no_more_tokens_than_sequences(ops, kind, contexts, counts, heads, kv_heads, dim, page, window, sinks, cap, distance):
+    b = kind(contexts, counts, heads, kv_heads, dim, page, gain=2.0)
+    slopes = slopes_of(heads) if distance else None
+    want, bound = four.attention(b, window, sinks, cap=cap, slopes=slopes)
+    call = ops.four_bit_attention if kind is FourBitBatch else ops.window_attention
+    near(call(b.q, *b.arrays, window, sinks, cap=cap, slopes=slopes), want, bound)
+
+
+@pytest.mark.parametrize("count", [1, 40])
+def test_long_flat_tails_through_a_window(ops, count):
+    """One key far above 15000 others whose weights together are of some size: 2^-18 of the largest each."""
+    b = Batch([20000], [count], 2, 1, 64, 64)
+    b.k_cache[:] = 0
+    where, place = b.pages_of(0, torch.tensor([19000], device="cuda"))
+    b.k_cache[where, :, place, 0] = 1.0
+    b.q[:] = 0
+    b.q.view(count, 2, 64)[:, :, 0] = 12.5
+    want, bound = four.attention(b, 15000, 5, scale=1.0)
+    near(ops.window_attention(b.q, *b.arrays, 15000, 5, scale=1.0), want, bound)
+
+
+@pytest.mark.parametrize("count", [1, 3, 40])
+@pytest.mark.parametrize("value", [65504.0, -65504.0])
+def test_averages_of_the_largest_value_through_a_window(ops, count, value):
+    b = Batch([300], [count], 4, 1, 128, 16)
+    b.v_cache[:] = value
+    assert bool((ops.window_attention(b.q, *b.arrays, 100, 3) == value).all())
+
+
+@pytest.mark.parametrize("count", [1, 60])
+def test_scores_beyond_what_their_exponents_hold_through_a_window(ops, count):
+    """Scores of 2^26 and more that differ by a few: what is left of the weights is theirs alone."""
+    b = Batch([200], [count], 2, 2, 64, 16)
+    b.k_cache[:] = 0
+    b.q[:] = 0
+    b.q.view(count, 2, 64)[:, :, 0] = 1024.0
+    b.q.view(count, 2, 64)[:, :, 1] = 1.0
+    rows = torch.arange(200 + count, device="cuda")
+    where, place = b.pages_of(0, rows)
+    b.k_cache[where, :, place, 0] = 32768.0
+    b.k_cache[where, :, place, 1] = ((rows % 3) * 4.0).half()[:, None].expand(-1, 2)
+    # products: 2^25 exactly and 0, 4 or 8, sums of 32 bits in steps of 4; times 2^2
+    want, _ = four.attention(b, 90, 2, scale=4.0)
+    got = ops.window_attention(b.q, *b.arrays, 90, 2, scale=4.0)
+    assert bool(((got.double() - want).abs() <= 2.0 ** -10 * (want.abs() + 4)).all())
+
+
+@pytest.mark.parametrize("what", [float("inf"), float("-inf"), float("nan")])
+def test_infinite_values_with_weights_too_small_through_a_window(ops, what):
+    for count, heads in ((1, 4), (1, 20), (30, 4)):
+        b = Batch([900], [count], heads, 1, 128, 16)
+        b.k_cache[:] = 0
+        b.q[:] = 0
+        b.q.view(count, heads, 128)[:, :, 0] = 60.0
+        where, place = b.pages_of(0, torch.tensor([880], device="cuda"))
+        b.k_cache[where, :, place, 0] = 1.0  # all others' weights: e^-60
+        finite = ops.window_attention(b.q, *b.arrays, 400, 2, scale=1.0)
+        where, place = b.pages_of(0, torch.tensor([700], device="cuda"))
+        b.v_cache[where, :, place, 9] = what
+        got = ops.window_attention(b.q, *b.arrays, 400, 2, scale=1.0).view(count, heads, 128)
+        assert bool((torch.isnan(got[..., 9]) if what != what else got[..., 9] == what).all())
+        rest = [c for c in range(128) if c != 9]
+        assert torch.equal(got[..., rest], finite.view(count, heads, 128)[..., rest])
