@@ -1322,7 +1322,7 @@ __device__ __forceinline__ void attn_turn_codes(const AttentionParams& p, AttnSh
                 const int      id = ids[h], left = t < seg.end ? seg.keys - key0 - 16 * h : 0;  // keys of the sixteen that there are
                 const bool     there = static_cast<unsigned>(id) < static_cast<unsigned>(c.pages);
                 const uint32_t in = ((key0 + 16 * h) & ((1 << c.page_shift) - 1)) + lane / kChunks;
-                const unsigned char* const page = reinterpret_cast<const unsigned char*>(cache) + static_cast<unsigned long long>(static_cast<uint32_t>(id * c.kv_heads + seg.head)) * page_bytes;
+                const unsigned char* const page = reinterpret_cast<const unsigned char*>(cache) + static_cast<unsigned long long>(static_cast<uint32_t>(id) * c.kv_heads + seg.head) * page_bytes;
                 const unsigned char* const from = page + in * (HEAD_DIM / 2) + 16 * q;
                 const unsigned char* const from_scales = page + scales_at + in * (4 * four_bit_groups(HEAD_DIM)) + q / 2 * 4;
 #pragma unroll

@@ -89,10 +89,10 @@ static cudaError_t append(cudaStream_t stream, bool four_bit, const void* QKV, i
         return err;
     // As few rounds of CTAs over the multiprocessors, which hold four at a time, as kAppendRows allow, and tokens dealt out evenly over
     // them (6612 tokens, 9.3 times the places: 39 us with 8 each, 1.4 rounds, 36 with 6).
-    const int places = 4 * sms, rounds = (tokens + kAppendRows * places - 1) / (kAppendRows * places);
-    p.rows           = (tokens + rounds * places - 1) / (rounds * places);
-    auto launch = [&](auto kernel) {
-        return launch_in_stream_order(kernel, dim3((tokens + p.rows - 1) / p.rows), dim3(kRotaryThreads), 0, stream, 1, p);
+    const long long places = 4ll * sms, rounds = (tokens + kAppendRows * places - 1) / (kAppendRows * places);
+    p.rows                 = static_cast<int>((tokens + rounds * places - 1) / (rounds * places));
+    auto launch            = [&](auto kernel) {
+        return launch_in_stream_order(kernel, dim3((tokens - 1) / p.rows + 1), dim3(kRotaryThreads), 0, stream, 1, p);
     };
     auto of_cache = [&](auto sixteen, auto four) { return four_bit ? launch(four) : launch(sixteen); };
     if (head_dim == 64)
@@ -213,7 +213,7 @@ int FlashLLM_FourBitRead(void* stream, const void* K_cache, const void* V_cache,
         ++p.row_shift;
     const int rows   = 1 << p.row_shift;
     auto      launch = [&](auto kernel) {
-        return launch_in_stream_order(kernel, dim3((tokens + rows - 1) / rows), dim3(kReadThreads), 0, static_cast<cudaStream_t>(stream), 1, p);
+        return launch_in_stream_order(kernel, dim3((tokens - 1) / rows + 1), dim3(kReadThreads), 0, static_cast<cudaStream_t>(stream), 1, p);
     };
     return static_cast<int>(head_dim == 64 ? launch(four_bit_read_kernel<64>) : launch(four_bit_read_kernel<128>));
 }

@@ -61,8 +61,8 @@ def turned(lib, b, qkv, rotary, interleaved, q_norm, k_norm, eps):
 
     The bound's second part: the squares' sum of `dim` terms, root, quotient and two products in 32 bits are off by less than 2^-20 of
     the result, and so is what turning makes of it, by its pair's sizes; the first is rotate()'s, the rounding to fp16 in it."""
-    frequencies, magnitude = lib.rotary_frequencies(max(rotary, 16), scaling="by parts", factor=4.0, original_length=64)
-    f = torch.from_numpy(frequencies).cuda()[:rotary // 2] if rotary else None
+    frequencies, magnitude = lib.rotary_frequencies(rotary, scaling="by parts", factor=4.0, original_length=64) if rotary else (None, 1.0)
+    f = torch.from_numpy(frequencies).cuda() if rotary else None
     owned = b.cut[-1]
     x = qkv[:owned].double().reshape(owned, b.heads + 2 * b.kv_heads, b.dim)
     place = torch.cat([torch.arange(c, c + t) for c, t in zip(b.contexts, b.counts)]).cuda()
@@ -687,3 +687,26 @@ def test_infinite_values_with_weights_too_small_through_a_window(ops, what):
         assert bool((torch.isnan(got[..., 9]) if what != what else got[..., 9] == what).all())
         rest = [c for c in range(128) if c != 9]
         assert torch.equal(got[..., rest], finite.view(count, heads, 128)[..., rest])
+
+
+@pytest.mark.parametrize("kind", [Batch, FourBitBatch])
+def test_as_many_sequences_as_a_call_can_have(ops, kind):
+    """4096 of them, every third without a token, every thousandth with many."""
+    contexts = [(7 * i) % 50 for i in range(4096)]
+    for many in (0, 20):
+        counts = [0 if i % 3 == 1 else many + 1 if i % 1000 == 5 else 1 for i in range(4096)]
+        b = kind(contexts, counts, 2, 1, 64, 16)
+        want, bound = four.attention(b, 11, 3)
+        qkv = torch.randn((b.rows, 4 * 64), device="cuda").to(torch.float16)
+        call = ops.four_bit_attention if kind is FourBitBatch else ops.window_attention
+        near(call(b.q, *b.arrays, 11, 3), want, bound)
+        w = norms(64)
+        y, off, v, _ = turned(None, b, qkv, 0, False, *w, 1e-6)
+        q = (ops.four_bit_append if kind is FourBitBatch else ops.norm_rotary_append)(qkv, *b.arrays, *w)
+        near(q.view(b.rows, 2, 64), y[:, :2], off[:, :2])
+        kept = torch.cat([b.rows_of(b.v_cache, s)[c:] for s, c in enumerate(contexts) if counts[s]])
+        if kind is FourBitBatch:
+            keys, vals = ops.four_bit_read(*b.arrays, b.rows)
+            near(vals.view(b.rows, 1, 64), kept, 2.0 ** -11 * kept.abs() + 2.0 ** -25)
+        else:
+            assert torch.equal(kept, v)
