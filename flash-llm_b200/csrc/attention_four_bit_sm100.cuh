@@ -8,18 +8,20 @@
 //   q . k       = sum_g step_g (q_g . n_g) + low_g sum(q_g)
 //   sum_j p_j v = sum_j (p_j step_j) n_j + sum_j p_j low_j
 //
-// so that an element costs one operation and a quarter of a shift: four bits masked out of a word are the mantissa of a subnormal
-// fp16 number, n x 2^-24, which the tensor core multiplies exactly.  Products are transposed, S^T = K Q^T and O^T = V^T P^T
+// so that an element costs 0.6 to 0.75 operations: four bits masked out of a word are the mantissa of a subnormal fp16 number, n x 2^-24
+// (or, where they lie four bits up, sixteen times that), which the tensor core multiplies exactly.  Products are transposed, S^T = K Q^T and O^T = V^T P^T
 // (m16n8k16): 16 keys, then 16 elements of a head, are the rows, the queries the 8 columns, so that eight queries waste nothing
-// (16 x 8 products of single queries are a quarter of the tensor core's time).  tcgen05 would want dense tiles in shared memory:
+// (the tensor core is busy a quarter of the time).  tcgen05 would want dense tiles in shared memory:
 // 64 KB written and read for each 18 KB of codes, half of the memory's time by itself.
 //
-// Every warp works by itself: it copies 16 keys and values at a time into its own ring in shared memory (cp.async, no barriers) and
-// keeps maximum, sum and outputs of its rows in registers.  The work of a call, blocks of 16 keys of all sequences, tiles of rows and
-// heads, is one linear sequence dealt out evenly over all warps; warps that share an item leave sums, which their CTA adds up in key
+// Every warp works by itself: it copies 32 keys and values at a time (16 where it has sixteen rows) into its own ring in shared memory
+// (cp.async, no barriers) and keeps maximum, sum and outputs of its rows in registers.  The work of a call, blocks of so many keys of
+// all sequences, tiles of rows and heads, is one linear sequence dealt out evenly over all warps; warps that share an item leave sums, which their CTA adds up in key
 // order, and CTAs that do leave theirs in the workspace for four_bit_join_kernel.
 //
-// Bound by memory where sequences are long (9/16 of a byte per element), by the issue of instructions next to it.
+// Bound by the issue of operations, 320 for 16 keys, next to memory (9/16 of a byte per element): 16 sequences of 4000 to 40000 positions
+// in 8 heads of 128, 274 MB, 67 us of which 50 are the loop over the keys (42 at the measured copy bandwidth); 64 sequences of 100 to
+// 9000 positions, 138 MB, 41 us.
 #pragma once
 #include <math_constants.h>
 
@@ -52,6 +54,7 @@ struct FourBitParams {
 constexpr int kFourKeys = 16;  // keys of a product: a page holds whole sixteens
 
 // TILES of eight rows each.
+// (Three or two for each scheduler.  Four, with registers spilled: 16 long sequences 70.4 us instead of 67.3; 13, unevenly: 82.)
 __host__ __device__ constexpr int four_warps(int tiles)
 {
     return tiles == 1 ? 12 : 8;
@@ -69,10 +72,11 @@ __host__ __device__ constexpr int four_stage_bytes(int head_dim, int tiles)
     return 2 * kFourKeys * four_sixteens(tiles) * four_bit_row_bytes(head_dim);
 }
 
-// Blocks in flight or at hand per warp: 110 to 150 KB of an SM.
+// Blocks in flight or at hand per warp: 110 to 150 KB of an SM.  (One on its way while another is worked on is enough: 16 long sequences
+// 67.3 us, 67.9 with two.)
 __host__ __device__ constexpr int four_stages(int head_dim, int tiles)
 {
-    return (tiles == 1 ? 3 : 8) * 128 / head_dim;
+    return (tiles == 1 ? 2 : 8) * 128 / head_dim;
 }
 
 struct FourPart {

@@ -271,7 +271,7 @@ __global__ void __launch_bounds__(kSingleWarps * 32, 1) window_single_kernel(con
                         for (int m = 0; m < HEAD_DIM / 16; ++m) {
                             to[row * HEAD_DIM + 16 * m + g]     = acc[m][e];
                             to[row * HEAD_DIM + 16 * m + 8 + g] = acc[m][e + 2];
-                            nan = nan || acc[m][e] != acc[m][e] || acc[m][e + 2] != acc[m][e + 2];
+                            nan = nan || (sum[e] == sum[e] && (acc[m][e] != acc[m][e] || acc[m][e + 2] != acc[m][e + 2]));
                         }
                         if (g == 0)
                             sh.stats[warp][slot][row] = make_float2(top[e] * factor, sum[e]);

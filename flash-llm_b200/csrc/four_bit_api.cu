@@ -102,6 +102,11 @@ static cudaError_t append(cudaStream_t stream, bool four_bit, const void* QKV, i
                        : of_cache(norm_append_kernel<128, false, false>, norm_append_kernel<128, false, true>);
 }
 
+// The warps' kernels make do with the workspace of the others.
+static_assert(four_workspace_bytes(1, 64) <= attn_workspace_bytes(1, 64) && four_workspace_bytes(1, 128) <= attn_workspace_bytes(1, 128)
+                  && four_workspace_bytes(256, 128) <= attn_workspace_bytes(256, 128),
+              "workspace");
+
 // Rows of a sequence (tokens x query heads of a key/value head) up to which it goes through the warps' kernel, sixteen at a time (16
 // sequences of 2000 to 4000 positions, 32 rows each: 42 us, the other kernel 47; 64 rows: 63 and 51).
 constexpr int kFourMostRows = 32;

@@ -414,7 +414,8 @@ int FlashLLM_PromptAttention(void*        stream,
 
 /* Attention through a sliding window with sinks: as FlashLLM_PromptAttention without a prefix, but of the keys up to itself a row
  * sees the last `window` (itself among them, at least 1) and the first `sinks` (0 or more) of its sequence.  Keys that no row
- * sees are not read.  The same workspace. */
+ * sees are not read.  The same workspace.  A call with no more tokens than sequences is taken for one of single tokens: a sequence
+ * that has many all the same is right, but takes as long as if each were a sequence. */
 int FlashLLM_WindowAttention(void*        stream,
                              const void*  Q,
                              int          ld_q,
@@ -506,7 +507,8 @@ int FlashLLM_FourBitAppend(void*         stream,
                            const void*   k_norm,
                            float         eps);
 
-/* FlashLLM_WindowAttention over such a cache; window 0: none (and sinks do not matter). */
+/* FlashLLM_WindowAttention over such a cache; window 0: none (and sinks do not matter).  What is said there of calls with no more
+ * tokens than sequences holds here too. */
 int FlashLLM_FourBitAttention(void*        stream,
                               const void*  Q,
                               int          ld_q,
