@@ -165,8 +165,11 @@ static cudaError_t attend(cudaStream_t stream, AttentionParams p, const void* Q,
     p.cap     = cap;
     p.workspace = static_cast<unsigned char*>(workspace);
     attn_set_heads(&p, heads, kv_heads);
-    // With a window and no more tokens than sequences these are single tokens (or few; the kernel takes any).
-    if (p.window > 0 && tokens <= sequences)
+    // With a window and no more tokens than sequences these are single tokens (or few; the kernel takes any).  Of many query heads to a
+    // key/value head it reads keys once for every eight (64 sequences of two key/value heads, 1000 to 4000 positions, window 1024: 16
+    // query heads each 52 us, the kernel of many rows 55; 32 41 and 35; 128 121 and 46; 8 sequences: 32 15 and 20, 64 17 and 20).
+    const bool warps = p.share <= 16 || (p.share <= 64 && static_cast<long long>(sequences) * kv_heads <= 32);
+    if (p.window > 0 && tokens <= sequences && warps)
         return launch_single_tokens(stream, p, head_dim);
     return head_dim == 64 ? launch_attention<64>(stream, p) : launch_attention<128>(stream, p);
 }

@@ -626,8 +626,10 @@ __global__ void __launch_bounds__(four_warps(TILES) * 32, 1) four_bit_attention_
                 // Page ids of 32 sixteens at a time, a lane each, the next 32 ahead of their use; -1: reads as zeros.
                 auto ids_from = [&](int block) {
                     block += lane / kSixteens;
+                    if (block >= end)
+                        return -1;
                     const int key = key_of(block) + lane % kSixteens * kFourKeys;
-                    if (block >= end || key >= keys)
+                    if (key >= keys)
                         return -1;
                     const int id = table[key >> c.page_shift];
                     if (static_cast<unsigned>(id) < static_cast<unsigned>(c.pages))

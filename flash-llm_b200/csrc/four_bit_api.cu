@@ -257,9 +257,13 @@ int FlashLLM_FourBitAttention(void* stream, const void* Q, int ld_q, const void*
     p.share_shift = a.share_shift;
     p.window    = window > 0 ? window : 0x7fffffff;
     p.sinks     = window > 0 ? sinks : 0;
-    // Sequences of many rows are the other kernel's, which the host cannot tell: where there is a token for each sequence, or fewer
-    // rows in all, it takes them for single tokens (and rows that are more are right, if slower).
-    const bool many = tokens > sequences && static_cast<long long>(tokens) * p.share > kFourMostRows;
+    // Sequences of more than kFourMostRows rows are the other kernel's.  The host does not know the rows of each: where one token has
+    // more, all are (64 sequences of 1000 to 4000 positions, two key/value heads of 64 query heads each: 67 us, by warps 81); where
+    // there is no more than a token for each sequence, or so many rows in all, none are (and rows that are more are right, if slower),
+    // since the other kernel's launch and its join's are some 8 us though they find nothing to do.  Two tokens to a sequence are not
+    // told from a long piece of one prompt among single tokens, which by warps would take as long as a sequence for every 16 rows.
+    const bool all  = p.share > kFourMostRows;
+    const bool many = all || (tokens > sequences && static_cast<long long>(tokens) * p.share > kFourMostRows);
     p.most_rows     = many ? kFourMostRows : 0x7fffffff;
     p.scale     = scale;
     p.cap       = cap;
@@ -270,8 +274,10 @@ int FlashLLM_FourBitAttention(void* stream, const void* Q, int ld_q, const void*
     using One = std::integral_constant<int, 1>;
     using Two = std::integral_constant<int, 2>;
     // Sixteen rows at a time where a sequence has more than eight.
-    const bool      two = p.share > 8 || tokens > sequences;
-    const cudaError_t err = head_dim == 64 ? (two ? few(Dim64{}, Two{}) : few(Dim64{}, One{})) : (two ? few(Dim128{}, Two{}) : few(Dim128{}, One{}));
+    const bool  two = p.share > 8 || tokens > sequences;
+    cudaError_t err = cudaSuccess;
+    if (!all)
+        err = head_dim == 64 ? (two ? few(Dim64{}, Two{}) : few(Dim64{}, One{})) : (two ? few(Dim128{}, Two{}) : few(Dim128{}, One{}));
     if (err != cudaSuccess || !many)
         return static_cast<int>(err);
     a.batch      = p.batch;
@@ -286,7 +292,7 @@ int FlashLLM_FourBitAttention(void* stream, const void* Q, int ld_q, const void*
     a.cap        = cap;
     a.window     = p.window;
     a.sinks      = p.sinks;
-    a.least_rows = kFourMostRows + 1;
+    a.least_rows = all ? 0 : kFourMostRows + 1;
     return static_cast<int>(launch_rows_over_four_bits(s, a, head_dim));
 }
 

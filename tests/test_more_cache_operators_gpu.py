@@ -621,6 +621,11 @@ def test_refusals_of_the_operators(ops):
     ([1000] * 3, [1] * 3, 40, 2, 128, 64, 333, 17, 25.0, False),            # more heads of a group than a tile's eight rows
     ([5000], [1], 128, 1, 64, 128, 4000, 128, 0.0, False),
     ([31, 32, 33, 47, 48, 49], [1] * 6, 3, 3, 128, 16, 16, 16, 0.0, False),
+    ([400] * 20, [1] * 20, 64, 2, 128, 64, 150, 4, 0.0, False),             # more than a tile takes of one token, many and few
+    ([400, 90], [1, 1], 96, 2, 64, 32, 150, 4, 0.0, True),
+    ([300, 20, 77], [2, 1, 2], 8, 2, 128, 16, 64, 0, 0.0, False),           # two tokens of some
+    ([300, 20, 77, 5], [40, 1, 2, 1], 2, 2, 64, 16, 64, 0, 0.0, False),     # few rows on average, many of one
+    ([300, 20], [17, 33], 4, 4, 64, 16, 0, 0, 0.0, False),
     ([700] * 450, [1] * 450, 2, 1, 64, 16, 30, 2, 0.0, False),
 ])
 @pytest.mark.parametrize("kind", [Batch, FourBitBatch])
@@ -629,7 +634,7 @@ def test_no_more_tokens_than_sequences(ops, kind, contexts, counts, heads, kv_he
     slopes = slopes_of(heads) if distance else None
     want, bound = four.attention(b, window, sinks, cap=cap, slopes=slopes)
     call = ops.four_bit_attention if kind is FourBitBatch else ops.window_attention
-    near(call(b.q, *b.arrays, window, sinks, cap=cap, slopes=slopes), want, bound)
+    near(call(b.q, *b.arrays, window or (0 if kind is FourBitBatch else 1 << 20), sinks, cap=cap, slopes=slopes), want, bound)
 
 
 @pytest.mark.parametrize("count", [1, 40])
