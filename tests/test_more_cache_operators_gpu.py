@@ -715,3 +715,36 @@ def test_as_many_sequences_as_a_call_can_have(ops, kind):
             near(vals.view(b.rows, 1, 64), kept, 2.0 ** -11 * kept.abs() + 2.0 ** -25)
         else:
             assert torch.equal(kept, v)
+
+
+@pytest.mark.parametrize("kind", [Batch, FourBitBatch])
+@pytest.mark.parametrize("counts", [[1, 1, 1, 0], [1, 2, 0, 30]])
+@pytest.mark.parametrize("heads", [2, 24, 80, 256])  # one to 128 query heads of a key/value head
+def test_bad_pages_and_lengths_within_a_window(ops, lib, kind, counts, heads):
+    contexts, window, sinks = [100, 250, 300, 40], 100, 60  # the bad page is one of the first, behind it one that none sees
+    b = kind(contexts, counts, heads, 2, 64, 16, extra_rows=3)
+    want, bound = four.attention(b, window, sinks)
+    zeros = kind(contexts, counts, heads, 2, 64, 16, extra_rows=3)
+    for cache in (zeros.k_cache, zeros.v_cache):
+        cache[zeros.page_table[1, 3].long()] = 0
+    by_zeros, zero_bound = four.attention(zeros, window, sinks)
+    call = ops.four_bit_attention if kind is FourBitBatch else ops.window_attention
+    lo, hi, last = b.cut[1], b.cut[2], b.cut[-1]
+    for bad in (-1, b.k_cache.shape[0], 2 ** 31 - 1):
+        table = b.page_table.clone()
+        table[1, 3] = bad
+        got = call(b.q, b.k_cache, b.v_cache, b.cu_tokens, b.context, table, window, sinks)
+        assert lib.consume_status() == BAD_CACHE
+        near(got[:lo], want[:lo], bound[:lo])
+        near(got[hi:last], want[hi:last], bound[hi:last])
+        near(got[lo:hi], by_zeros[lo:hi], zero_bound[lo:hi])
+    for context in (-1, b.page_table.shape[1] * 16, 2 ** 31 - 1):
+        lengths = b.context.clone()
+        lengths[1] = context
+        got = call(b.q, b.k_cache, b.v_cache, b.cu_tokens, lengths, b.page_table, window, sinks)
+        assert lib.consume_status() == BAD_CACHE
+        near(got[:lo], want[:lo], bound[:lo])
+        near(got[hi:last], want[hi:last], bound[hi:last])
+        assert bool((got[lo:hi] == 0).all())
+    near(call(b.q, *b.arrays, window, sinks)[:last], want[:last], bound[:last])
+    assert lib.consume_status() == 0
