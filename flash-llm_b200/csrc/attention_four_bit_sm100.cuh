@@ -908,7 +908,7 @@ __global__ void __launch_bounds__(four_warps(TILES) * 32, 1) four_bit_attention_
                         if (__half_as_ushort(__float2half_rn(largest)) > limit_v) {
                             const int   exponent = min((__float_as_int(largest) >> 23) - 127, 15);  // NaN has not become the largest
                             const float unit     = __int_as_float((127 + 5 - exponent) << 23);
-                            keep_v               = limit_v > 0 ? unit / unit_v : 1.0f;
+                            keep_v               = unit / unit_v;  // (of lowest values there are sums before the first step)
                             unit_v               = unit;
                             limit_v              = __half_as_ushort(__float2half_rn(128.0f / unit));
                         }

@@ -1,0 +1,101 @@
+"""What the running sums of the attention over 4 bits can lose, on the GPU against the definition in 64 bits."""
+import math
+
+import pytest
+import torch
+
+import four_bit_cache as four
+from four_bit_cache import FourBitBatch
+from test_more_cache_operators_gpu import healthy, near, ops  # noqa: F401  (fixtures)
+
+pytestmark = pytest.mark.gpu
+
+
+def few_rows(batch, window=0, sinks=0, scale=None):
+    """(output, bound on the error of the kernel of few rows) of every row, [rows][heads * dim] in 64 bits.
+
+    Scores: codes times queries are exact, sums of `dim` products in 32 bits, truncated at each addition of the tensor core (2^-20 of
+    the sizes of steps times codes and lowest values); an error d of them is one of 2 d of the weights, numerator and denominator
+    together, and 2^-20 holds exponentials and sums.  A weight times its step is rounded to fp16, 2^-11 of it at most, which is
+    multiplied by a code less 7.5: b = 2^-11 x 7.5 p step.  The roundings of n keys are independent, so their sum passes 6 times the
+    root of the sum of b^2 once in 3e7 (Hoeffding).  Products below fp16's normal numbers are off by 2^-25 of units in which the
+    largest step is at least 2^5, for each key by 2^-27 of the largest step in the output (the weights' sum is 1 at least).  The output
+    is rounded to fp16, 2^-11 of it or 2^-25."""
+    dim, share = batch.dim, batch.heads // batch.kv_heads
+    scale = dim ** -0.5 if scale is None else scale
+    out = torch.zeros((batch.rows, batch.heads, dim), dtype=torch.float64, device=batch.device)
+    bound = torch.zeros_like(out)
+    for b, (context, count) in enumerate(zip(batch.contexts, batch.counts)):
+        lo, hi = batch.cut[b], batch.cut[b + 1]
+        away = torch.arange(context + count, device=batch.device)[None] - (context + torch.arange(count, device=batch.device)[:, None])
+        seen = away <= 0
+        if window:
+            seen &= (away > -window) | (away + context + torch.arange(count, device=batch.device)[:, None] < sinks)
+        (k, k_step, k_low), (v, v_step, v_low) = batch.parts_of(batch.k_cache, b), batch.parts_of(batch.v_cache, b)
+        q = batch.q[lo:hi].double().view(count, batch.kv_heads, share, dim)
+        score = scale * torch.einsum("tgsd,jgd->gstj", q, k)
+        off = 2.0 ** -20 * scale * torch.einsum("tgsd,jgd->gstj", q.abs(), 15 * k_step + k_low.abs())
+        p = torch.softmax(torch.where(seen, score, torch.full_like(score, -math.inf)), -1)
+        error = torch.where(seen, off, torch.zeros_like(off)).amax(-1)
+        mix = lambda w, x: torch.einsum("gstj,jgd->tgsd", w, x).reshape(count, batch.heads, dim)  # noqa: E731
+        out[lo:hi] = mix(p, v)
+        size = (2 * error.permute(2, 0, 1).reshape(count, batch.heads, 1) + 2.0 ** -20) * mix(p, 15 * v_step + v_low.abs())
+        bound[lo:hi] = (2.0 ** -11 * out[lo:hi].abs() + 6 * 2.0 ** -11 * mix(p.square(), (7.5 * v_step).square()).sqrt() + size
+                        + 2.0 ** -27 * (context + count) * v_step.amax() + 2.0 ** -25)
+    return out.view(batch.rows, -1), bound.view(batch.rows, -1)
+
+
+# --------------------------------------------------------------------------------------------------- steps of zero
+
+def flat_values(b, s, keys, size=1.0):
+    """Makes each 64 values of sequence s at the positions `keys` one value: a step of zero, and a lowest value that is not."""
+    g = torch.Generator().manual_seed(11)
+    x = (size * (1.0 + torch.rand((len(keys), b.kv_heads, b.dim // four.GROUP), generator=g))).half().float().to(b.device)
+    where, place = b.pages_of(s, keys)
+    four.put(b.v_cache, b.dim, (where, slice(None), place), x.repeat_interleave(four.GROUP, -1))
+    assert bool((four.parts(b.v_cache, b.dim)[1][where, :, place, :, 0] == 0).all())
+
+
+# Pieces of several blocks of 32 keys, or of 16 where a sequence has more than eight rows.
+LONG = [([30000], [1], 4, 1, 128, 64), ([30000], [1], 1, 1, 64, 16), ([30000], [1], 12, 1, 64, 32), ([30000, 9000], [3, 1], 4, 1, 128, 64)]
+
+
+@pytest.mark.parametrize("size,later", [(1.0, 1.0), (512.0, 1.0), (60.0, 2.0 ** -9), (1.0, 2.0 ** 9)])
+@pytest.mark.parametrize("period,flat", [(32, 16), (64, 32), (96, 40), (1024, 512), (1024, 1023)])
+@pytest.mark.parametrize("contexts,counts,heads,kv_heads,dim,page", LONG)
+def test_values_without_a_step_keep_their_weight(ops, contexts, counts, heads, kv_heads, dim, page, period, flat, size, later):  # noqa: F811
+    """The first `flat` of each `period` positions have values without a step, the others steps `later` times as large as usual."""
+    b = FourBitBatch(contexts, counts, heads, kv_heads, dim, page)
+    four.parts(b.v_cache, dim)[1][:] *= later
+    for s, (c, t) in enumerate(zip(contexts, counts)):
+        place = torch.arange(c + t, device="cuda")
+        flat_values(b, s, place[place % period < flat], size)
+    near(ops.four_bit_attention(b.q, *b.arrays), *few_rows(b))
+
+
+@pytest.mark.parametrize("window,sinks", [(0, 0), (200, 4), (200, 40)])
+@pytest.mark.parametrize("flat", [1, 4, 16, 32, 40, 100, 300, -1, -40])
+@pytest.mark.parametrize("kv_heads,dim,page", [(2, 128, 16), (2, 64, 64)])
+def test_values_without_a_step_in_many_sequences(ops, kv_heads, dim, page, flat, window, sinks):  # noqa: F811
+    """The first `flat` positions of every sequence, the last for a negative number."""
+    n = 320
+    b = FourBitBatch([300] * n, [1] * n, kv_heads, kv_heads, dim, page)
+    place = torch.arange(301, device="cuda")
+    for s in range(n):
+        flat_values(b, s, place[:flat] if flat > 0 else place[flat:])
+    near(ops.four_bit_attention(b.q, *b.arrays, window, sinks), *few_rows(b, window, sinks))
+
+
+@pytest.mark.parametrize("count,heads", [(1, 4), (3, 4)])
+def test_appended_rows_without_a_step_keep_their_weight(ops, count, heads):  # noqa: F811
+    """As a program has them: rows of one value each through the append, others behind them, then attention of them all."""
+    dim, total = 128, 20000
+    b = FourBitBatch([0], [total], heads, 1, dim, 16)
+    qkv = torch.randn((total, (heads + 2) * dim), device="cuda").half()
+    flat = torch.arange(total, device="cuda") % 256 < 128
+    qkv[flat, -dim:] = torch.linspace(0.5, 2.0, int(flat.sum()), device="cuda").half()[:, None]
+    q = ops.four_bit_append(qkv, *b.arrays)
+    cu = torch.tensor([0, count], dtype=torch.int32, device="cuda")
+    context = torch.tensor([total - count], dtype=torch.int32, device="cuda")
+    b.contexts, b.counts, b.cut, b.rows, b.q = [total - count], [count], [0, count], count, q[total - count:].contiguous()
+    near(ops.four_bit_attention(b.q, b.k_cache, b.v_cache, cu, context, b.page_table), *few_rows(b))
