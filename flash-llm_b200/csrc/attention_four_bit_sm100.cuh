@@ -49,6 +49,7 @@ struct FourBitParams {
     int                  most_rows;  // sequences with more rows (tokens x share) are somebody else's
     float                scale;
     float                cap;  // 0: none
+    float                unit;  // times a difference of the maxima that parts leave: the exponent of a power of two
 };
 
 constexpr int kFourKeys = 16;  // keys of a product: a page holds whole sixteens
@@ -248,9 +249,9 @@ __device__ __forceinline__ uint32_t four_transpose(uint32_t a)
     return d;
 }
 
-__device__ __forceinline__ float four_weight(float top, float newtop)
+__device__ __forceinline__ float four_weight(float top, float newtop, float unit = 1.0f)
 {
-    return top == newtop ? 1.0f : ptx::exp2_approx(top - newtop);
+    return top == newtop ? 1.0f : ptx::exp2_approx((top - newtop) * unit);
 }
 
 // Place of a key's values among the 16 of a block: a thread's four keys, 2 t, 2 t + 1, 2 t + 8 and 2 t + 9, lie four places apart.
@@ -260,9 +261,9 @@ __device__ __forceinline__ int four_value_place(int key)
 }
 
 // Adds up four columns of a row of one item's parts, in key order: `stats(i)` is the i-th part's maximum and sum of the row, `sums(i)`
-// its outputs of these columns.  AT_ONCE parts' loads are under way at a time.
+// its outputs of these columns, `unit` FourBitParams'.  AT_ONCE parts' loads are under way at a time.
 template<int AT_ONCE, typename Stats, typename Sums>
-__device__ __forceinline__ float4 four_add_up(int count, Stats&& stats, Sums&& sums, float2& all)
+__device__ __forceinline__ float4 four_add_up(int count, float unit, Stats&& stats, Sums&& sums, float2& all)
 {
     float  top = -CUDART_INF_F, sum = 0.0f;
     float4 o   = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
@@ -284,13 +285,13 @@ __device__ __forceinline__ float4 four_add_up(int count, Stats&& stats, Sums&& s
         for (int i = 0; i < AT_ONCE; ++i)
             newtop = fmaxf(newtop, s[i].x);
         // (Never zero: a part's infinity stays one.)
-        const float before = fmaxf(four_weight(top, newtop), 0x1p-126f);
+        const float before = fmaxf(four_weight(top, newtop, unit), 0x1p-126f);
         sum *= before;
         o   = make_float4(o.x * before, o.y * before, o.z * before, o.w * before);
         top = newtop;
 #pragma unroll
         for (int i = 0; i < AT_ONCE; ++i) {
-            const float keep = fmaxf(four_weight(s[i].x, top), 0x1p-126f);
+            const float keep = fmaxf(four_weight(s[i].x, top, unit), 0x1p-126f);
             sum              = fmaf(s[i].y, keep, sum);
             o                = make_float4(fmaf(x[i].x, keep, o.x), fmaf(x[i].y, keep, o.y), fmaf(x[i].z, keep, o.z), fmaf(x[i].w, keep, o.w));
         }
@@ -524,7 +525,7 @@ __device__ __forceinline__ void four_finish(const FourBitParams& p, const FourSh
         if (row < from.rows) {
             float2       all;
             const float4 o = four_add_up<1>(
-                count, [&](int k) { return sh.stats[begin + k][k == 0 ? tail : 0][row]; },
+                count, p.unit, [&](int k) { return sh.stats[begin + k][k == 0 ? tail : 0][row]; },
                 [&](int k) {
                     const int            w  = begin + k;
                     const unsigned char* at = k == 0 && tail ? smem + w * ring_bytes : first_sums + w * four_rows_bytes(HEAD_DIM, ROWS / 8);
@@ -1101,7 +1102,7 @@ __global__ void __launch_bounds__(256) four_bit_join_kernel(const __grid_constan
         const int    row = u / (HEAD_DIM / 4), column = u % (HEAD_DIM / 4) * 4;
         float2       all;
         const float4 o = four_add_up<8>(
-            cta - begin + 1, [&](int i) { return stats[slot(i) * 16 + row]; },
+            cta - begin + 1, p.unit, [&](int i) { return stats[slot(i) * 16 + row]; },
             [&](int i) { return reinterpret_cast<const float4*>(sums + (slot(i) * 16 + row) * HEAD_DIM + column); }, all);
         *reinterpret_cast<uint2*>(four_out<HEAD_DIM>(p, last.first, last.head, last.row0 + row) + column) = four_outputs(o, all.y);
     }

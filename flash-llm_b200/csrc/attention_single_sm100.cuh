@@ -164,7 +164,7 @@ __global__ void __launch_bounds__(kSingleWarps * 32, 1) window_single_kernel(con
                         slope[e] = 2 * t + e < rows ? p.slopes[head * p.share + row0 - token * p.share + 2 * t + e] * CUDART_L2E_F : 0.0f;
                 // PLAIN: maxima are of products, `factor` makes powers of two of them (where both are large, a difference of products keeps
                 // what their multiples lose); otherwise of scores in units of log 2.
-                const float factor = PLAIN ? p.scale * CUDART_L2E_F : 1.0f, limit = 8.0f / factor;
+                const float factor = PLAIN ? p.unit : 1.0f, limit = 8.0f / factor;
                 const float cap_in = !PLAIN && p.cap > 0.0f ? p.scale / p.cap : 0.0f;
 
                 float acc[HEAD_DIM / 16][4] = {};  // elements 16 m + g and 16 m + 8 + g, rows 2 t and 2 t + 1
@@ -274,7 +274,7 @@ __global__ void __launch_bounds__(kSingleWarps * 32, 1) window_single_kernel(con
                             nan = nan || (sum[e] == sum[e] && (acc[m][e] != acc[m][e] || acc[m][e + 2] != acc[m][e + 2]));
                         }
                         if (g == 0)
-                            sh.stats[warp][slot][row] = make_float2(top[e] * factor, sum[e]);
+                            sh.stats[warp][slot][row] = make_float2(top[e], sum[e]);
                     }
                 }
                 __syncwarp();

@@ -159,6 +159,7 @@ cudaError_t launch_single_tokens(cudaStream_t stream, const AttentionParams& a, 
     p.most_rows   = 0x7fffffff;
     p.scale       = a.scale;
     p.cap         = a.cap;
+    p.unit        = a.cap == 0.0f && a.slopes == nullptr ? a.scale * CUDART_L2E_F : 1.0f;  // (plain kernels' maxima are of products)
     return head_dim == 64 ? launch_single<64>(stream, p, sms) : launch_single<128>(stream, p, sms);
 }
 
@@ -267,6 +268,7 @@ int FlashLLM_FourBitAttention(void* stream, const void* Q, int ld_q, const void*
     p.most_rows     = many ? kFourMostRows : 0x7fffffff;
     p.scale     = scale;
     p.cap       = cap;
+    p.unit      = 1.0f;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     auto few = [&](auto dim, auto tiles) { return launch_four_bit<decltype(dim)::value, decltype(tiles)::value>(s, p, sms); };
     using Dim64 = std::integral_constant<int, 64>;

@@ -1,4 +1,5 @@
-"""What the running sums of the attention over 4 bits can lose, on the GPU against the definition in 64 bits."""
+"""What the running maxima and sums of the warps' attention kernels can lose, those over 4 bits and of single tokens through a window,
+on the GPU against the definitions in 64 bits."""
 import math
 
 import pytest
@@ -6,6 +7,7 @@ import torch
 
 import four_bit_cache as four
 from four_bit_cache import FourBitBatch
+from paged_cache import Batch
 from test_more_cache_operators_gpu import healthy, near, ops  # noqa: F401  (fixtures)
 
 pytestmark = pytest.mark.gpu
@@ -99,3 +101,53 @@ def test_appended_rows_without_a_step_keep_their_weight(ops, count, heads):  # n
     context = torch.tensor([total - count], dtype=torch.int32, device="cuda")
     b.contexts, b.counts, b.cut, b.rows, b.q = [total - count], [count], [0, count], count, q[total - count:].contiguous()
     near(ops.four_bit_attention(b.q, b.k_cache, b.v_cache, cu, context, b.page_table), *few_rows(b))
+
+
+# --------------------------------------------------------------------------------------------------- large scores
+
+def of_exact_scores(batch, score, window=0, sinks=0):
+    """(output, bound) of the rows of one sequence, whose scores [keys] in 64 bits are the same for all rows and exact in the kernels.
+
+    A weight is rounded to fp16, or its product with a step (see few_rows): b = 2^-11 p |v| or 2^-11 x 7.5 p step, 6 times the root of the
+    sum of b^2.  The scale times log2 e is off by 2^-23 of itself, exponents, which matter down to -30, by 2^-18 then; sums are of
+    sizes |v|, or 15 steps and the lowest value."""
+    (context,), (count,), share = batch.contexts, batch.counts, batch.heads // batch.kv_heads
+    away = torch.arange(context + count, device="cuda")[None] - (context + torch.arange(count, device="cuda")[:, None])
+    seen = away <= 0
+    if window:
+        seen &= (away > -window) | (torch.arange(context + count, device="cuda") < sinks)
+    p = torch.softmax(torch.where(seen, score, torch.full_like(score, -math.inf)), 1)
+    mix = lambda w, x: torch.einsum("tj,jgd->tgd", w, x).repeat_interleave(share, 1).reshape(count, -1)  # noqa: E731
+    if isinstance(batch, FourBitBatch):
+        v, step, low = batch.parts_of(batch.v_cache, 0)
+        each, size = 7.5 * step, 15 * step + low.abs()
+    else:
+        v = batch.rows_of(batch.v_cache, 0)
+        each = size = v.abs()
+    out = mix(p, v)
+    return out, (2.0 ** -11 * out.abs() + 6 * 2.0 ** -11 * mix(p.square(), each.square()).sqrt() + 2.0 ** -18 * mix(p, size)
+                 + 2.0 ** -25 * float(each.amax()))
+
+
+def large_scores(b, first, second, small):
+    """Queries and keys of a Batch of one sequence whose products are first x second + small, exactly."""
+    where, at = b.pages_of(0, torch.arange(len(small), device="cuda"))
+    b.k_cache[:] = 0
+    b.k_cache[where, :, at, 0] = second
+    b.k_cache[where, :, at, 1] = small.half()[:, None].expand(-1, b.kv_heads)
+    b.q[:] = 0
+    b.q.view(b.rows, b.heads, b.dim)[..., 0], b.q.view(b.rows, b.heads, b.dim)[..., 1] = first, 1.0
+
+
+LARGE = [(0.5, 1024.0, 32768.0, 4), (2.0 ** -5, 32768.0, 16384.0, 64)]  # 2^25 and 2^29, and a step of 32-bit numbers there
+
+
+@pytest.mark.parametrize("scale,first,second,step", LARGE)
+@pytest.mark.parametrize("dim,page,heads,kv_heads", [(64, 16, 4, 1), (128, 64, 12, 2)])
+def test_parts_of_large_scores_keep_their_weight_through_a_window(ops, dim, page, heads, kv_heads, scale, first, second, step):  # noqa: F811
+    """Some positions' scores are one or two steps of 32-bit numbers above the others', long runs of them, so that an item's parts have
+    other maxima: e^2 apart."""
+    b = Batch([20000], [1], heads, kv_heads, dim, page)
+    small = step * (torch.arange(20001, device="cuda") // 300 % 3).double()
+    large_scores(b, first, second, small)
+    near(ops.window_attention(b.q, *b.arrays, 15000, 5, scale=scale), *of_exact_scores(b, scale * small, 15000, 5))
