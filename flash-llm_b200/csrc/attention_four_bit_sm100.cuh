@@ -891,7 +891,7 @@ __global__ void __launch_bounds__(four_warps(TILES) * 32, 1) four_bit_attention_
                             most.x = fmaxf(most.x, fmaxf(s[j][n][0].x, s[j][n][1].x));
                             most.y = fmaxf(most.y, fmaxf(s[j][n][0].y, s[j][n][1].y));
                         }
-                        grown = grown || most.x > top[n][0] + 8.0f || most.y > top[n][1] + 8.0f;
+                        grown = grown || most.x - top[n][0] > 8.0f || most.y - top[n][1] > 8.0f;  // (a sum with 8 may be rounded to the next number)
                     }
                     if (__any_sync(0xffffffffu, grown)) {
                         float largest = 0.0f;

@@ -163,8 +163,9 @@ __global__ void __launch_bounds__(kSingleWarps * 32, 1) window_single_kernel(con
                     for (int e = 0; e < 2; ++e)
                         slope[e] = 2 * t + e < rows ? p.slopes[head * p.share + row0 - token * p.share + 2 * t + e] * CUDART_L2E_F : 0.0f;
                 // PLAIN: maxima are of products, `factor` makes powers of two of them (where both are large, a difference of products keeps
-                // what their multiples lose); otherwise of scores in units of log 2.
-                const float factor = PLAIN ? p.unit : 1.0f, limit = 8.0f / factor;
+                // what their multiples lose); otherwise of scores in units of log 2.  A maximum lags by `limit` at most: compared are
+                // differences, since a large maximum's sum with it may be rounded to the next number.
+                const float factor = PLAIN ? p.unit : 1.0f, limit = fminf(8.0f / factor, CUDART_MAX_NORMAL_F);
                 const float cap_in = !PLAIN && p.cap > 0.0f ? p.scale / p.cap : 0.0f;
 
                 float acc[HEAD_DIM / 16][4] = {};  // elements 16 m + g and 16 m + 8 + g, rows 2 t and 2 t + 1
@@ -213,7 +214,7 @@ __global__ void __launch_bounds__(kSingleWarps * 32, 1) window_single_kernel(con
                             if (!sees(key0 + g + 8 * k))
                                 s[2 * k] = s[2 * k + 1] = -CUDART_INF_F;
                     }
-                    if (__any_sync(0xffffffffu, fmaxf(s[0], s[2]) > top[0] + limit || fmaxf(s[1], s[3]) > top[1] + limit)) {
+                    if (__any_sync(0xffffffffu, fmaxf(s[0], s[2]) - top[0] > limit || fmaxf(s[1], s[3]) - top[1] > limit)) {
 #pragma unroll
                         for (int e = 0; e < 2; ++e) {
                             float newtop = fmaxf(top[e], fmaxf(s[e], s[e + 2]));

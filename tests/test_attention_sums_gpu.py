@@ -151,3 +151,41 @@ def test_parts_of_large_scores_keep_their_weight_through_a_window(ops, dim, page
     small = step * (torch.arange(20001, device="cuda") // 300 % 3).double()
     large_scores(b, first, second, small)
     near(ops.window_attention(b.q, *b.arrays, 15000, 5, scale=scale), *of_exact_scores(b, scale * small, 15000, 5))
+
+
+ONE = 0.6931471824645996  # times log2 e, in 32 bits: 1
+
+
+@pytest.mark.parametrize("dim,page,heads,kv_heads", [(64, 16, 4, 1), (128, 64, 12, 2)])
+@pytest.mark.parametrize("scale,first,second,step,slope", [
+    (2.0, 1024.0, 32768.0, 4, False),       # 2^25 and one step of 32-bit numbers more: 2^11.5 times the weight
+    (0.125, 32768.0, 16384.0, 64, False),   # 2^29
+    (ONE, 32768.0, 4096.0, 16, True),       # 2^27, in units of log 2
+])
+@pytest.mark.parametrize("base", [0, 1])
+def test_a_maximum_grows_by_a_step_of_32_bits_through_a_window(ops, scale, first, second, step, slope, base, dim, page, heads, kv_heads):  # noqa: F811
+    """One key in 128 has a score that is one step of 32-bit numbers above the others', which are even (base 0) or odd (1)."""
+    b = Batch([20000], [1], heads, kv_heads, dim, page)
+    small = step * (base + (torch.arange(20001, device="cuda") % 128 == 127).double())
+    large_scores(b, first, second, small)
+    slopes = torch.zeros(heads, device="cuda") if slope else None
+    near(ops.window_attention(b.q, *b.arrays, 15000, 5, scale=scale, slopes=slopes), *of_exact_scores(b, scale * small, 15000, 5))
+
+
+@pytest.mark.parametrize("slope", [False, True])
+@pytest.mark.parametrize("base", [0, 1])
+@pytest.mark.parametrize("heads,page", [(4, 64), (4, 16), (12, 32)])
+def test_a_maximum_grows_by_a_step_of_32_bits_over_four_bits(ops, heads, page, base, slope):  # noqa: F811
+    """The same over 4 bits: keys' lowest values alone make scores of 2^27 and 16 or 32 more."""
+    b = FourBitBatch([20000], [1], heads, 1, 128, page)
+    place = torch.arange(20001, device="cuda")
+    small = 16.0 * (base + (place % 128 == 127).double())
+    where, at = b.pages_of(0, place)
+    codes, scales = four.parts(b.k_cache, 128)
+    codes[where, :, at], scales[where, :, at] = 0, 0.0
+    scales[where, :, at, 0, 1] = 4096.0
+    scales[where, :, at, 1, 1] = small.half()[:, None]
+    b.q[:] = 0
+    b.q.view(heads, 128)[:, 0], b.q.view(heads, 128)[:, 64] = 32768.0, 1.0
+    slopes = torch.zeros(heads, device="cuda") if slope else None
+    near(ops.four_bit_attention(b.q, *b.arrays, scale=ONE, slopes=slopes), *of_exact_scores(b, ONE * small))
