@@ -440,7 +440,8 @@ __device__ __forceinline__ unsigned long long attn_sequence_units(const Attentio
 }
 
 // Units of every sequence; all threads, ends with a barrier.  The rows of a sequence that does not fit into the page table are
-// cleared here, by one CTA.
+// cleared here, by one CTA.  Each sequence is one thread's, then one warp's: what stands in sh.units tells a warp whether it is to be
+// counted and is overwritten with the count (kernels differ in their threads).
 template<bool WINDOW>
 __device__ __forceinline__ void attn_count_units(const AttentionParams& p, AttnSharedOf<WINDOW>& sh, int head_dim)
 {
@@ -448,7 +449,7 @@ __device__ __forceinline__ void attn_count_units(const AttentionParams& p, AttnS
     const int item_rows = 2 * p.tile_rows;
     bool      several   = false;
 #pragma unroll 1
-    for (int b = threadIdx.x; b < B; b += kAttnThreads) {
+    for (int b = threadIdx.x; b < B; b += blockDim.x) {
         const AttnSequence a = attn_sequence<WINDOW>(p, b);
         if (b < kAttnKnown)
             sh.known[b] = make_int4(a.s.first, a.s.count, a.s.context, a.prefix);
@@ -461,7 +462,7 @@ __device__ __forceinline__ void attn_count_units(const AttentionParams& p, AttnS
     }
     if (__syncthreads_or(several ? 1 : 0)) {
 #pragma unroll 1
-        for (int b = warp; b < B; b += kAttnThreads / 32) {
+        for (int b = warp; b < B; b += blockDim.x / 32) {
             if (sh.units[b] < kAttnLostRows)
                 continue;
             const AttnSequence a = attn_sequence<WINDOW>(p, b);
