@@ -1776,7 +1776,7 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
             if (ok && !whole && valid && column0 == 0 && (!fourfold || thread < 32))
                 reinterpret_cast<float2*>(p.workspace + attn_stats_offset(gridDim.x))[static_cast<size_t>(2 * blockIdx.x + slot) * kAttnSlotRows
                                                                                       + tile_row * kAttnRows + thread] =
-                    make_float2(st.top * st.factor, st.sum);
+                    make_float2(st.top, st.sum);  // (times the factor it would lose what it differs by from others')
             if (kind != kPartNone) {
                 written[slot] = true;
                 const bool all = !ptx::named_barrier_any(1, 256, !ok);  // a part is there for all rows or for none
@@ -2050,8 +2050,10 @@ __global__ void __launch_bounds__(256) attention_join_kernel(const AttentionPara
     } while (true);
     if (begin < 0 || parts[2 * begin + 1].kind != kPartBegins)
         return;  // a CTA gave up
-    auto  slot = [&](int c) { return static_cast<size_t>(2 * c + (c == begin ? 1 : 0)); };
-    float top  = -CUDART_INF_F;
+    // Maxima are of products where scores are plain, else of scores in units of log 2.
+    const float unit = p.cap == 0.0f && p.slopes == nullptr ? p.scale * CUDART_L2E_F : 1.0f;
+    auto        slot = [&](int c) { return static_cast<size_t>(2 * c + (c == begin ? 1 : 0)); };
+    float       top  = -CUDART_INF_F;
     for (int c = begin; c <= cta; ++c)
         top = fmaxf(top, stats[slot(c) * kAttnSlotRows + place].x);
     constexpr int kPer = HEAD_DIM / 4 / 8;  // float4 columns of a warp
@@ -2063,7 +2065,7 @@ __global__ void __launch_bounds__(256) attention_join_kernel(const AttentionPara
     for (int c = begin; c <= cta; ++c) {
         const float2 stat = stats[slot(c) * kAttnSlotRows + place];
         // Never zero: a part's infinity stays one.
-        const float  keep = stat.x == top ? 1.0f : fmaxf(ptx::exp2_approx(stat.x - top), 0x1p-126f);
+        const float  keep = stat.x == top ? 1.0f : fmaxf(ptx::exp2_approx((stat.x - top) * unit), 0x1p-126f);
         sum += stat.y * keep;
         const float4* src = sums + ((slot(c) * 2 + place / kAttnRows) * (HEAD_DIM / 4) + warp * kPer) * kAttnRows + place % kAttnRows;
 #pragma unroll

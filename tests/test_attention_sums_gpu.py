@@ -1,5 +1,5 @@
-"""What the running maxima and sums of the warps' attention kernels can lose, those over 4 bits and of single tokens through a window,
-on the GPU against the definitions in 64 bits."""
+"""What the running maxima and sums of the attention kernels can lose, on the GPU against the definitions in 64 bits: those of the
+warps' kernels, over 4 bits and of single tokens through a window, and the joining of parts."""
 import math
 
 import pytest
@@ -151,6 +151,18 @@ def test_parts_of_large_scores_keep_their_weight_through_a_window(ops, dim, page
     small = step * (torch.arange(20001, device="cuda") // 300 % 3).double()
     large_scores(b, first, second, small)
     near(ops.window_attention(b.q, *b.arrays, 15000, 5, scale=scale), *of_exact_scores(b, scale * small, 15000, 5))
+
+
+@pytest.mark.parametrize("scale,first,second,step", LARGE)
+@pytest.mark.parametrize("count,heads,kv_heads,dim,page", [(1, 4, 1, 64, 16), (3, 8, 2, 128, 64), (140, 2, 1, 64, 128)])
+@pytest.mark.parametrize("window", [0, 17000])
+def test_parts_of_large_scores_of_many_rows_keep_their_weight(ops, count, heads, kv_heads, dim, page, window, scale, first, second, step):  # noqa: F811
+    """The same for the tensor core's kernel, whose parts are those of other CTAs."""
+    b = Batch([20000], [count + (window > 0)], heads, kv_heads, dim, page)  # (a single token through a window is the warps')
+    small = step * (torch.arange(20000 + b.rows, device="cuda") // 600 % 3).double()
+    large_scores(b, first, second, small)
+    got = ops.window_attention(b.q, *b.arrays, window, 5, scale=scale) if window else ops.prompt_attention(b.q, *b.arrays, scale=scale)
+    near(got, *of_exact_scores(b, scale * small, window, 5))
 
 
 ONE = 0.6931471824645996  # times log2 e, in 32 bits: 1
