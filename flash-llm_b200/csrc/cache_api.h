@@ -72,7 +72,9 @@ inline cudaError_t multiprocessors_once(std::atomic<int> (&known)[64], int* coun
 inline bool scores_fit(float scale, float cap)
 {
     return scale > 0.0f && std::isfinite(scale) && cap >= 0.0f && std::isfinite(cap) && std::isfinite(scale * 8e11f)
-           && std::isfinite(cap * 1.45f) && (cap == 0.0f || std::isfinite(scale / cap * 3.0f));
+           && std::isfinite(cap * 1.45f) && (cap == 0.0f || std::isfinite(scale / cap * 3.0f))
+           // (scores of three quarters of the cap take twice the cap times log2 e)
+           && (std::isfinite(cap * 2.9f) || scale * 8e11f < 0.7f * cap);
 }
 
 }  // namespace flashllm
