@@ -29,6 +29,8 @@ def few_rows(batch, window=0, sinks=0, scale=None):
     bound = torch.zeros_like(out)
     for b, (context, count) in enumerate(zip(batch.contexts, batch.counts)):
         lo, hi = batch.cut[b], batch.cut[b + 1]
+        if count == 0:
+            continue
         away = torch.arange(context + count, device=batch.device)[None] - (context + torch.arange(count, device=batch.device)[:, None])
         seen = away <= 0
         if window:
@@ -45,6 +47,63 @@ def few_rows(batch, window=0, sinks=0, scale=None):
         bound[lo:hi] = (2.0 ** -11 * out[lo:hi].abs() + 6 * 2.0 ** -11 * mix(p.square(), (7.5 * v_step).square()).sqrt() + size
                         + 2.0 ** -27 * (context + count) * v_step.amax() + 2.0 ** -25)
     return out.view(batch.rows, -1), bound.view(batch.rows, -1)
+
+
+def many_rows(batch, window=0, sinks=0, scale=None):
+    """(output, bound on the error of the kernel of many rows) as few_rows has them.
+
+    Elements are rounded to fp16, 2^-11 of each at most, and multiplied.  A value's rounding adds p 2^-11 |v| to the output, its
+    weight's as much, an element of a key's p |v - output| scale |q| 2^-11 |k|: all independent, so 6 times the root of the sum of their
+    squares.  An error d of the scores has a second order, 2 d^2 of the weights: d is 6 times the root of the sum of (scale q 2^-11 k)^2
+    at most.  Sums are of the elements' sizes, 2^-20 of them as there, and of weights below fp16's normal numbers 2^-25 each."""
+    dim, share = batch.dim, batch.heads // batch.kv_heads
+    scale = dim ** -0.5 if scale is None else scale
+    out = torch.zeros((batch.rows, batch.heads, dim), dtype=torch.float64, device=batch.device)
+    bound = torch.zeros_like(out)
+    for b, (context, count) in enumerate(zip(batch.contexts, batch.counts)):
+        lo, hi = batch.cut[b], batch.cut[b + 1]
+        if count == 0:
+            continue
+        place = torch.arange(context + count, device=batch.device)
+        away = place[None] - (context + torch.arange(count, device=batch.device)[:, None])
+        seen = away <= 0
+        if window:
+            seen &= (away > -window) | (place < sinks)
+        k, v = batch.rows_of(batch.k_cache, b), batch.rows_of(batch.v_cache, b)
+        for h in range(batch.heads):
+            q, kh, vh = batch.q[lo:hi, h * dim:(h + 1) * dim].double(), k[:, h // share], v[:, h // share]
+            score = scale * q @ kh.T
+            p = torch.softmax(torch.where(seen, score, torch.full_like(score, -math.inf)), 1)
+            o = p @ vh
+            keys = (scale * 2.0 ** -11) ** 2 * (q.square() @ kh.square().T)  # the square of a score's error, a key's
+            p2 = p.square()
+            spread = (p2 * keys) @ vh.square() - 2 * o * ((p2 * keys) @ vh) + o.square() * (p2 * keys).sum(1, keepdim=True)
+            off = torch.where(seen, 2.0 ** -20 * scale * (q.abs() @ kh.abs().T), torch.zeros_like(p)).amax(1, keepdim=True)
+            second = 2 * 36 * torch.where(seen, keys, torch.zeros_like(keys)).amax(1, keepdim=True)
+            out[lo:hi, h] = o
+            bound[lo:hi, h] = (2.0 ** -11 * o.abs() + 6 * (2.0 ** -21 * (p2 @ vh.square()) + spread).sqrt()
+                               + (2 * off + second + 2.0 ** -20) * (p @ vh.abs()) + 2.0 ** -25 * (seen.double() @ vh.abs() * 2.0 ** -7 + 1))
+    return out.view(batch.rows, -1), bound.view(batch.rows, -1)
+
+
+# --------------------------------------------------------------------------------------------------- what each kernel rounds
+
+@pytest.mark.parametrize("window,sinks", [(0, 0), (150, 5)])
+@pytest.mark.parametrize("contexts,counts,heads,kv_heads,dim,page,gain", [
+    ([0], [1], 1, 1, 64, 16, 1.0), ([210], [1], 16, 16, 64, 16, 1.0), ([5000, 31, 900], [1, 1, 1], 8, 2, 128, 64, 2.0),
+    ([3000, 17], [1, 1], 20, 1, 128, 32, 0.3), ([900, 100], [3, 2], 12, 4, 128, 16, 2.0), ([20000], [8], 4, 1, 64, 128, 4.0)])
+def test_few_rows_over_four_bits_round_no_more_than_they_say(ops, contexts, counts, heads, kv_heads, dim, page, gain, window, sinks):  # noqa: F811
+    b = FourBitBatch(contexts, counts, heads, kv_heads, dim, page, gain=gain)
+    near(ops.four_bit_attention(b.q, *b.arrays, window, sinks), *few_rows(b, window, sinks))
+
+
+@pytest.mark.parametrize("window,sinks", [(0, 0), (150, 5)])
+@pytest.mark.parametrize("contexts,counts,heads,kv_heads,dim,page,gain", [
+    ([0], [200], 2, 2, 64, 16, 1.0), ([130, 0, 77], [300, 40, 129], 8, 2, 128, 128, 2.0), ([3000], [65], 4, 1, 128, 32, 0.3),
+    ([2000, 9], [1, 1], 40, 1, 64, 64, 1.0), ([20000], [12], 4, 1, 64, 128, 4.0)])
+def test_many_rows_over_four_bits_round_no_more_than_they_say(ops, contexts, counts, heads, kv_heads, dim, page, gain, window, sinks):  # noqa: F811
+    b = FourBitBatch(contexts, counts, heads, kv_heads, dim, page, gain=gain)
+    near(ops.four_bit_attention(b.q, *b.arrays, window, sinks), *many_rows(b, window, sinks))
 
 
 # --------------------------------------------------------------------------------------------------- steps of zero
