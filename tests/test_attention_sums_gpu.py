@@ -260,3 +260,22 @@ def test_a_maximum_grows_by_a_step_of_32_bits_over_four_bits(ops, heads, page, b
     b.q.view(heads, 128)[:, 0], b.q.view(heads, 128)[:, 64] = 32768.0, 1.0
     slopes = torch.zeros(heads, device="cuda") if slope else None
     near(ops.four_bit_attention(b.q, *b.arrays, scale=ONE, slopes=slopes), *of_exact_scores(b, ONE * small))
+
+
+@pytest.mark.parametrize("count,heads,page", [(140, 2, 64), (12, 4, 16), (1, 40, 32)])
+def test_large_scores_of_many_rows_over_four_bits_keep_their_weight(ops, count, heads, page):  # noqa: F811
+    """Scores of 2^24, 2 or 4 more for long runs of keys; elements are exact in fp16, values' roundings as large as their weights'."""
+    b = FourBitBatch([20000], [count], heads, 1, 128, page)
+    place = torch.arange(20000 + count, device="cuda")
+    small = 16.0 * (place // 600 % 3).double()
+    where, at = b.pages_of(0, place)
+    codes, scales = four.parts(b.k_cache, 128)
+    codes[where, :, at], scales[where, :, at] = 0, 0.0
+    scales[where, :, at, 0, 1] = 4096.0
+    scales[where, :, at, 1, 1] = small.half()[:, None]
+    b.q[:] = 0
+    b.q.view(count, heads, 128)[..., 0], b.q.view(count, heads, 128)[..., 64] = 32768.0, 1.0
+    values = Batch([20000], [count], heads, 1, 128, page)  # of 16 bits, of which the bound is
+    values.rows_of = lambda cache, s: 2.0 ** 0.5 * b.rows_of(b.v_cache, s)
+    want, bound = of_exact_scores(values, 0.125 * small)
+    near(ops.four_bit_attention(b.q, *b.arrays, scale=0.125), want / 2.0 ** 0.5, bound)
