@@ -93,8 +93,8 @@ constexpr int kAppendRows = 16;  // of a CTA, at most
 // Bound by memory for prompts, by a chain of dependent loads for a few tokens (sequence, page, row).  A CTA of many calls takes several
 // tokens: their places and angles are found side by side, and the loads of the next 32 bytes are under way while these are worked on.
 // 6612 tokens of 56 heads of 128: 47.4 us with a CTA for each, 43.6 so, 41.5 with eights of neighbouring threads side by side in
-// memory (wavefronts of the L1 74 to 49 % of what it can), 37.7 in two even rounds, 36.0 in one (up to 16 tokens a CTA): 5.3 TB/s,
-// 0.80 of the measured copy bandwidth.  What
+// memory (wavefronts of the L1 74 to 49 % of what it can), 37.7 in two even rounds, 36.0 to 36.8 in one (up to 16 tokens a CTA), all
+// replayed from a graph: 5.2 TB/s, 0.79 of the measured copy bandwidth; a call among others 38.5, 0.75.  What
 // is left is the work on registers, 260 operations for a thread's 16 elements.
 template<int HEAD_DIM, bool INTERLEAVED, bool FOUR_BIT>
 __global__ void __launch_bounds__(kRotaryThreads) norm_append_kernel(const __grid_constant__ AppendParams p)

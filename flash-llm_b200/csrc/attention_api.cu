@@ -166,8 +166,13 @@ static cudaError_t attend(cudaStream_t stream, AttentionParams p, const void* Q,
     p.workspace = static_cast<unsigned char*>(workspace);
     attn_set_heads(&p, heads, kv_heads);
     // With a window and no more tokens than sequences these are single tokens (or few; the kernel takes any).  Of many query heads to a
-    // key/value head it reads keys once for every eight (64 sequences of two key/value heads, 1000 to 4000 positions, window 1024: 16
-    // query heads each 52 us, the kernel of many rows 55; 32 41 and 35; 128 121 and 46; 8 sequences: 32 15 and 20, 64 17 and 20).
+    // key/value head it reads keys once for every eight.  Us by warps / by the kernel of many rows, replayed from a graph, two key/value
+    // heads, 1000 to 8000 positions, windows of 256, 1024 and 4096:
+    //   64 sequences, heads of 128: 9 query heads each 16/24, 28/34, 52/52; 16 16/24, 28/35, 53/51; 32 20/25, 41/35, 96/51; 64 29/24, 68/35, 160/52
+    //   64 sequences, heads of 64:  9 12/17, 18/21, 33/31; 16 12/17, 18/21, 33/31; 32 15/17, 27/22, 56/31; 64 21/18, 44/24, 98/37
+    //   8 sequences, heads of 128:  16 13/17, 14/19, 16/23; 32 14/18, 15/20, 20/23; 64 14/18, 17/19, 29/23 (of 64 all but 21/17 for 64 and 4096)
+    // (With short windows of many sequences the warps would stay ahead up to 32.)  Sequences without a token are counted as well: the
+    // host does not know them.
     const bool warps = p.share <= 16 || (p.share <= 64 && static_cast<long long>(sequences) * kv_heads <= 32);
     if (p.window > 0 && tokens <= sequences && warps)
         return launch_single_tokens(stream, p, head_dim);

@@ -19,9 +19,9 @@
 // all sequences, tiles of rows and heads, is one linear sequence dealt out evenly over all warps; warps that share an item leave sums, which their CTA adds up in key
 // order, and CTAs that do leave theirs in the workspace for four_bit_join_kernel.
 //
-// Bound by the issue of operations, 320 for 16 keys, next to memory (9/16 of a byte per element): 16 sequences of 4000 to 40000 positions
-// in 8 heads of 128, 274 MB, 67 us of which 50 are the loop over the keys (42 at the measured copy bandwidth); 64 sequences of 100 to
-// 9000 positions, 138 MB, 41 us.
+// Bound by the issue of operations next to memory (9/16 of a byte per element): 310 for 16 keys in the loop, with all that is before
+// and behind it 322 in 16 sequences of 4000 to 40000 positions in 8 heads of 128, and 352 in 64 of 100 to 9000.  The former, 274 MB, are
+// 72 us a call, 67 replayed from a graph, of which 50 are the loop (42 at the measured copy bandwidth), the latter, 138 MB, 42 and 41.
 #pragma once
 #include <math_constants.h>
 
@@ -719,6 +719,8 @@ __global__ void __launch_bounds__(four_warps(TILES) * 32, 1) four_bit_attention_
                             slope[n][e] = p.slopes && r < rows ? p.slopes[head * p.share + row0 + r - tok * p.share] * CUDART_L2E_F : 0.0f;
                     }
                 }
+                // Scores are sums in units of log 2 at once: rounded as their terms are, so that of scores of 2^24 and more, where sums of
+                // 32 bits lose a power of two, no more is lost than there.
                 const float factor = PLAIN ? p.scale * CUDART_L2E_F : p.cap > 0.0f ? 1.0f : p.scale * CUDART_L2E_F;
                 const float cap_in = !PLAIN && p.cap > 0.0f ? p.scale / p.cap : 0.0f;
 #pragma unroll

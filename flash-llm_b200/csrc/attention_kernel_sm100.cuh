@@ -1281,7 +1281,9 @@ __device__ __forceinline__ void attn_softmax(AttnState& st, const AttnRowOf<WIND
 
 // Warps 12 to 15 over a cache of 4 bits: a tile's codes to elements of fp16 in the stages of K and V, as the tensor copies would lay
 // them.  Codes are read straight into registers, those of the next tile while this one's wait for its room: a thread has 32 elements
-// of a key, neighbours have the rest of it and the keys behind.  Elements are rounded to fp16 once, as four_bit_read gives them.
+// of a key, neighbours have the rest of it and the keys behind.  Elements are rounded to fp16 once, as four_bit_read gives them: both
+// operands of a product are of one type, and queries are fp16 (5.5e-4 of the output; 3e-4 where codes are multiplied as they are, which
+// takes a product and a pass over its scores for each 64 elements and was not tried here).
 template<int HEAD_DIM, bool WINDOW>
 __device__ __forceinline__ void attn_turn_codes(const AttentionParams& p, AttnSharedOf<WINDOW>& sh, unsigned char* k_stages, unsigned char* v_stages)
 {

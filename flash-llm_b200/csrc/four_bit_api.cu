@@ -88,7 +88,7 @@ static cudaError_t append(cudaStream_t stream, bool four_bit, const void* QKV, i
     if (const cudaError_t err = four_multiprocessors(&sms))
         return err;
     // As few rounds of CTAs over the multiprocessors, which hold four at a time, as kAppendRows allow, and tokens dealt out evenly over
-    // them (6612 tokens: 41.5 us with 8 each, 1.4 rounds, 37.7 with 6, 36.0 with 12, all at once).
+    // them (6612 tokens, replayed from a graph: 41.5 us with 8 each, 1.4 rounds, 37.7 with 6, 36.0 to 36.8 with 12, all at once).
     const long long places = 4ll * sms, rounds = (tokens + kAppendRows * places - 1) / (kAppendRows * places);
     p.rows                 = static_cast<int>((tokens + rounds * places - 1) / (rounds * places));
     auto launch            = [&](auto kernel) {
@@ -259,7 +259,7 @@ int FlashLLM_FourBitAttention(void* stream, const void* Q, int ld_q, const void*
     p.window    = window > 0 ? window : 0x7fffffff;
     p.sinks     = window > 0 ? sinks : 0;
     // Sequences of more than kFourMostRows rows are the other kernel's.  The host does not know the rows of each: where one token has
-    // more, all are (64 sequences of 1000 to 4000 positions, two key/value heads of 64 query heads each: 67 us, by warps 81); where
+    // more, all are (64 sequences of 1000 to 4000 positions, two key/value heads of 64 query heads of 128 each: 67 us, by warps 81); where
     // there is no more than a token for each sequence, or so many rows in all, none are (and rows that are more are right, if slower),
     // since the other kernel's launch and its join's are some 8 us though they find nothing to do.  Two tokens to a sequence are not
     // told from a long piece of one prompt among single tokens, which by warps would take as long as a sequence for every 16 rows.

@@ -6,7 +6,9 @@
 //
 //   element = lowest + step x code
 //
-// lowest = fp16(min), step = fp16((max - lowest) / 15), code = (x - lowest) / step to the nearest, all from 32 bits.  64 elements and
+// lowest = fp16(min), step = fp16((max - lowest) / 15), code = (x - lowest) / step to the nearest, all from 32 bits: what a turned key is
+// off there, some 2^-22 of it, makes the neighbouring code of some two in a million, no further from the element but a step from what
+// 64 bits would have kept.  64 elements and
 // not all 128 of a head: steps are 0.9 of what they would be for normally distributed elements, much less where few channels are
 // large, for 0.25 bits an element.  A group that holds a value which is not finite, or beyond fp16's range, has a step of NaN, and so
 // have its elements.
