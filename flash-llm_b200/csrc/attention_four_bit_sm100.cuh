@@ -719,8 +719,8 @@ __global__ void __launch_bounds__(four_warps(TILES) * 32, 1) four_bit_attention_
                             slope[n][e] = p.slopes && r < rows ? p.slopes[head * p.share + row0 + r - tok * p.share] * CUDART_L2E_F : 0.0f;
                     }
                 }
-                // Scores are sums in units of log 2 at once: rounded as their terms are, so that of scores of 2^24 and more, where sums of
-                // 32 bits lose a power of two, no more is lost than there.
+                // Scores are sums in units of log 2 at once, an operation less for each: steps and sums of queries times the factor are off by
+                // 2^-24 of a score, about as much as its sum in 32 bits is (of scores of 2^24 and more that is a power of two).
                 const float factor = PLAIN ? p.scale * CUDART_L2E_F : p.cap > 0.0f ? 1.0f : p.scale * CUDART_L2E_F;
                 const float cap_in = !PLAIN && p.cap > 0.0f ? p.scale / p.cap : 0.0f;
 #pragma unroll
